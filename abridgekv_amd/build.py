@@ -16,7 +16,7 @@ PROBE_LIB = PKG / "libabridgekv_probes.so"      # measurement probes, loaded by 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 DEVICE_SOURCES = ["decode_attn.hip", "kv_cache.hip", "prefill_attn.hip", "prefill_bwd.hip", "paged_prefill.hip",
-                  "attn_f32.hip"]
+                  "attn_f32.hip", "window_attn.hip", "window_bwd.hip"]
 HOST_SOURCES = ["planner.cpp", "paged_plan.cpp"]
 PROBE_SOURCES = ["probes.hip"]
 
@@ -28,7 +28,7 @@ DEVICE_FLAGS = ["--offload-arch=gfx950", "-Xclang", "-target-feature", "-Xclang"
 # waves per SIMD); the AMDGPU scheduler's own register-pressure trackers give the backward a better schedule
 # (same-process A/B on the B=4, 16 x (512 + 128)-row training launch: 4.58 -> 4.46 ms per backward, outputs
 # bit-identical), while the forward is fastest with the default (1275 vs 1297 us).
-SOURCE_FLAGS = {"prefill_bwd.hip": ["-mllvm", "-amdgpu-use-amdgpu-trackers"]}
+SOURCE_FLAGS = {name: ["-mllvm", "-amdgpu-use-amdgpu-trackers"] for name in ("prefill_bwd.hip", "window_bwd.hip")}
 
 
 def _run(cmd):

@@ -33,6 +33,7 @@ from dataclasses import dataclass
 import torch
 import torch.nn.functional as F
 from torch import nn
+from torch.autograd.function import once_differentiable
 
 from . import ops
 from .config import bitrev_offsets
@@ -101,21 +102,64 @@ class _MaskedPrefill(torch.autograd.Function):
         return dq, dk, dv, None, None, None
 
 
+@dataclass(frozen=True)
+class WindowMask:
+    """Causal attention under a sliding window with sinks: row i sees row j when j <= i and (i - j < ``window`` or
+    j < ``sinks``); ``seq_lens`` [B] int32 on the GPU: rows past a sequence's length are padding (None: none)."""
+    window: int
+    sinks: int = 0
+    seq_lens: torch.Tensor | None = None
+
+
+class _WindowAttention(torch.autograd.Function):
+    """The sliding-window kernels and their backward (abkv_window_attn / _bwd)."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, mask: WindowMask, scale: float):
+        lse = None
+        if any(ctx.needs_input_grad[:3]):
+            if q.dtype != torch.bfloat16:
+                raise NotImplementedError("the sliding-window backward runs bf16 inputs")
+            lse = torch.empty((q.shape[0], ops.HEADS_Q, q.shape[1]), dtype=torch.float32, device=q.device)
+        out, _ = ops.window_attention(q, k, v, mask.window, mask.sinks, seq_lens=mask.seq_lens, scale=scale, lse=lse)
+        if lse is not None:
+            ctx.save_for_backward(q, k, v, out, lse, mask.seq_lens)
+            ctx.window, ctx.sinks, ctx.scale = mask.window, mask.sinks, scale
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        q, k, v, out, lse, seq_lens = ctx.saved_tensors
+        g = grad_out
+        if g.stride(-1) != 1 or any(x % 8 for x in g.stride()[:-1]) or g.data_ptr() % 16:
+            g = g.contiguous()
+        dq, dk, dv = ops.window_attention_backward(q, k, v, out, lse, g, ctx.window, ctx.sinks, seq_lens=seq_lens,
+                                                   scale=ctx.scale)
+        return dq, dk, dv, None, None
+
+
 def masked_attention_forward(module, query, key, value, attention_mask, scaling=None, dropout=0.0, **kwargs):
     """HuggingFace attention function: query [B, 32, S, 128], key/value [B, 8, S, 128] bf16 ->
-    (out [B, S, 32, 128], None). ``attention_mask`` is a :class:`CompressMask`, or None for a plain causal forward
-    of the model (the full-context baseline and teacher, compress_forward.py:952-956, 1095-1105), which runs the
-    same kernel without code rows."""
-    if attention_mask is None:
-        attention_mask = CompressMask(query.shape[2], 0, 1)
-    if not isinstance(attention_mask, CompressMask):
-        raise TypeError(f"{ATTN_IMPLEMENTATION} attention needs a CompressMask or None, got "
-                        f"{type(attention_mask).__name__}")
+    (out [B, S, 32, 128], None). ``attention_mask`` is a :class:`CompressMask`, a :class:`WindowMask`, or None for a
+    plain causal forward of the model (the full-context baseline and teacher, compress_forward.py:952-956, 1095-1105),
+    which runs the compression mask's kernel without code rows, or, in a layer with a ``sliding_window``, the
+    sliding-window kernels."""
     if dropout:
         raise NotImplementedError("attention dropout is not supported")
-    if kwargs.get("sliding_window"):
-        raise NotImplementedError("sliding-window attention is not supported")
+    window = kwargs.get("sliding_window")
+    if attention_mask is None:
+        attention_mask = WindowMask(int(window)) if window else CompressMask(query.shape[2], 0, 1)
+    elif window:
+        raise NotImplementedError("a sliding-window layer takes no other mask")
     scale = ops.default_scale() if scaling is None else float(scaling)
+    if isinstance(attention_mask, WindowMask):
+        out = _WindowAttention.apply(query.transpose(1, 2), key.transpose(1, 2), value.transpose(1, 2), attention_mask,
+                                     scale)
+        return out, None
+    if not isinstance(attention_mask, CompressMask):
+        raise TypeError(f"{ATTN_IMPLEMENTATION} attention needs a CompressMask, a WindowMask or None, got "
+                        f"{type(attention_mask).__name__}")
     out = _MaskedPrefill.apply(query.transpose(1, 2), key.transpose(1, 2), value.transpose(1, 2), attention_mask,
                                int(module.layer_idx), scale)
     return out, None

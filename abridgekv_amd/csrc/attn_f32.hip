@@ -9,6 +9,7 @@
 #include <cstring>
 
 #include "common.h"
+#include "window_walk.h"
 
 namespace abkv {
 
@@ -49,6 +50,7 @@ struct F32Args {
   int replay_exclude;          // the codes do not see the block's last replay_rows content rows
   int num_tokens;
   int windows, window_parts;   // paged: 16-token windows, workgroups per window and KV head
+  int slide, sinks;            // sliding window: the rows i - slide + 1 .. i and the first `sinks` rows
   float scale;
   float* out;
   long o_sb, o_st, o_sh;
@@ -196,6 +198,36 @@ struct MaskedStages {
     return true;
   }
   // K and V rows of half h (rows 16h .. 16h + 15) of a stage
+  struct Half {
+    const float* k;
+    const float* v;
+    long k_ss, v_ss;
+  };
+  __device__ __forceinline__ Half half(const F32Stage& st, int) const {
+    return Half{k + (long)st.k0 * k_ss, v + (long)st.k0 * v_ss, k_ss, v_ss};
+  }
+  __device__ __forceinline__ static int row_of(const F32Stage& st, int row) { return min(row, st.end - 1 - st.k0); }
+};
+
+// Stages of kKeys keys that 16 rows see under a sliding window with sinks: the sinks before the first row's window, then the
+// windows, from their first key on (not cut at tiles).
+template <int kKeys>
+struct WindowStages {
+  const float* k;
+  const float* v;
+  long k_ss, v_ss;
+  int k0, seg_end, win_begin, end;     // next key, the end of its run; the windows' first key and last + 1
+  F32Span span;
+  __device__ __forceinline__ bool next(F32Stage& st) {
+    if (k0 >= seg_end && seg_end < end) {                    // the sinks are done
+      k0 = win_begin;
+      seg_end = end;
+    }
+    if (k0 >= seg_end) return false;
+    st = F32Stage{k0, min(k0 + kKeys, seg_end), span};
+    k0 += kKeys;
+    return true;
+  }
   struct Half {
     const float* k;
     const float* v;
@@ -579,6 +611,40 @@ __global__ __launch_bounds__(256, kKeys == 16 ? 3 : 2) void attn_f32_rows_kernel
   }
 }
 
+// Attention under a sliding window with sinks over whole prompts: the row kernel's workgroup, 16 query rows of a KV head,
+// over the stages its rows see.
+template <int kKeys>
+__global__ __launch_bounds__(256, 2) void attn_f32_window_kernel(F32Args a) {
+  __shared__ __attribute__((aligned(16))) float lds[4 * kKeys * kHeadDim];
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, m16 = lane & 15, g = lane >> 4;
+  const int kvh = blockIdx.x % kHeadsKV, tile = blockIdx.x / kHeadsKV;
+  const int head = kvh * kGroup + w;
+  const int b = tile % a.batch;
+  const int q0 = ((a.seq_len + kF32Rows - 1) / kF32Rows - 1 - tile / a.batch) * kF32Rows;
+  const int n = a.seq_lens ? min(max(a.seq_lens[b], 0), a.seq_len) : a.seq_len;
+  const int qrow = q0 + m16;
+  const bool seen = qrow < n, row = qrow < a.seq_len;
+  floatx4 q[8], o[8];
+  float m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+  float* out = a.out + (long)b * a.o_sb + (long)qrow * a.o_st + (long)head * a.o_sh;
+  bool add = false;
+  if (q0 < n) {                                              // (uniform)
+    f32_load_q(a.q + (long)b * a.q_sb + (long)min(qrow, n - 1) * a.q_st + (long)head * a.q_sh, g, seen, q);
+    const int lo = max(qrow + 1 - a.slide, 0), win_begin = max(q0 + 1 - a.slide, 0);
+    const int end = min(q0 + kF32Rows, n), sink_end = min(a.sinks, win_begin);
+    const F32Span span{seen ? min(a.sinks, qrow + 1) : 0, lo, seen ? (unsigned)(qrow + 1 - lo) : 0u};
+    WindowStages<kKeys> src{a.k + (long)b * a.k_sb + (long)kvh * a.k_sh, a.v + (long)b * a.v_sb + (long)kvh * a.v_sh,
+                            a.k_ss, a.v_ss, 0, sink_end, win_begin, end, span};
+    add = f32_attend<kKeys>(src, lds, q, a.scale, row ? out + 16 * g : nullptr, m, l, o);
+  }
+  if (!row) return;
+  f32_store(out, g, l, o, add);
+  if (a.lse != nullptr && g == 0) a.lse[((long)b * kHeadsQ + head) * a.seq_len + qrow] = f32_lse(m, l);
+}
+
 // Decode: a workgroup of 8 waves per (sequence, KV head); the waves share the pages (f32_pages) and their partial results
 // meet in LDS. The four heads fill the 16 columns four times over: the path is bound by memory, not by the matrix rate. 32
 // sequences of 900 .. 9500 rows 7014 -> 286 us (4.8 TB/s), one of 5000 rows 2102 -> 108 us, against the VALU form of one
@@ -771,6 +837,37 @@ int abkv_prefill_masked_attn_f32(const float* q, long q_sb, long q_ss, long q_sh
   // 6 x (200 + 2 x 40) 107 / 133; causal 1337 rows 209 / 181, and a paged code step over 4000 keys 7 % slower with 16.
   if (codes_k > 0) hipLaunchKernelGGL((attn_f32_rows_kernel<true, 16>), dim3(grid), dim3(256), 0, stream, a);
   else hipLaunchKernelGGL((attn_f32_rows_kernel<true, 32>), dim3(grid), dim3(256), 0, stream, a);
+  return (int)hipGetLastError();
+}
+
+int abkv_window_attn_f32(const float* q, long q_stride_b, long q_stride_s, long q_stride_h, const float* k, long k_stride_b,
+                         long k_stride_s, long k_stride_h, const float* v, long v_stride_b, long v_stride_s,
+                         long v_stride_h, int batch, int seq_len, const int32_t* seq_lens, int window, int sinks,
+                         float scale, float* out, long out_stride_b, long out_stride_s, long out_stride_h, float* lse,
+                         hipStream_t stream) {
+  using namespace abkv;
+  if (batch <= 0 || seq_len <= 0) return 0;
+  if (q == nullptr || k == nullptr || v == nullptr || out == nullptr || window <= 0 || sinks < 0)
+    return (int)hipErrorInvalidValue;
+  F32Args a = f32_defaults();
+  a.q = q;
+  a.q_sb = q_stride_b; a.q_st = q_stride_s; a.q_sh = q_stride_h;
+  a.k = k;
+  a.k_sb = k_stride_b; a.k_ss = k_stride_s; a.k_sh = k_stride_h;
+  a.v = v;
+  a.v_sb = v_stride_b; a.v_ss = v_stride_s; a.v_sh = v_stride_h;
+  a.batch = batch;
+  a.seq_len = seq_len;
+  a.seq_lens = seq_lens;
+  a.slide = window;
+  a.sinks = sinks;
+  a.scale = scale;
+  a.out = out;
+  a.o_sb = out_stride_b; a.o_st = out_stride_s; a.o_sh = out_stride_h;
+  a.lse = lse;
+  const unsigned grid = f32_grid(((long)seq_len + kF32Rows - 1) / kF32Rows * batch);
+  if (grid == 0) return (int)hipErrorInvalidValue;
+  hipLaunchKernelGGL((attn_f32_window_kernel<32>), dim3(grid), dim3(256), 0, stream, a);
   return (int)hipGetLastError();
 }
 

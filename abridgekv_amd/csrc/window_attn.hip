@@ -1,0 +1,167 @@
+// Attention under a sliding window with sinks (gfx950): whole prompts and prompt chunks over the paged cache.
+//
+//   row i sees key j when j <= i and (i - j < window or j < sinks), both inside the sequence;
+//   out_i = sum_j softmax_j(scale q_i . k_j) v_j, rows that see nothing (padding) are 0 with lse -inf.
+//
+// The mask is evaluated from (window, sinks, the sequence's length): a query tile of 64 rows walks the tiles of the sinks,
+// then the ceil((window + 63) / 64) (+ 1) tiles its rows' windows reach, and only tiles on an edge of a range are masked per
+// element. The work of a row is bounded by the window, not by its position. Tiles, softmax and the K/V pipeline are the
+// compression mask's (attn_tile.h): a workgroup of 8 waves per (sequence, KV head, query tile), a wave 16 rows x 2 heads.
+#include "window_tile.h"
+
+namespace abkv {
+
+// Prompt chunks: request r's queries are rows q_start[r] .. q_start[r + 1] - 1 at positions kv_start[r] + i.
+struct ChunkArgs {
+  const __bf16* kv; int num_pages;             // [pages, 2, 16, 8, 128]
+  const int32_t* block_table; long bt_stride; int bt_width;
+  const int32_t* q_start;                      // [B + 1]
+  const int32_t* kv_start;                     // [B]
+  const int32_t* tile_req;                     // [tiles] request of each 64-row query tile
+  const int32_t* tile_q0;                      // [tiles] its first query row within the request
+};
+
+template <bool kPaged>
+__global__ __launch_bounds__(512, 1) void window_attn_kernel(WindowArgs a, ChunkArgs c) {
+  constexpr int H = 2, kWaves = 8;
+  __shared__ __attribute__((aligned(16))) __bf16 K0[kTileElems], K1[kTileElems], K2[kTileElems];
+  __shared__ __attribute__((aligned(16))) __bf16 V0[kTileElems], V1[kTileElems], V2[kTileElems];
+  __bf16* const Kbuf[kStages] = {K0, K1, K2};
+  __bf16* const Vbuf[kStages] = {V0, V1, V2};
+  // KV head fastest: workgroups go to the 8 XCDs round-robin, so one XCD's L2 serves a head's rows to all its tiles
+  const int kvh = blockIdx.x % kHeadsKV;
+  const int tile = blockIdx.x / kHeadsKV;
+  int b, q0, kv0 = 0, t0 = 0, n, n_q;                        // n: keys; n_q: query rows of the sequence
+  if constexpr (kPaged) {
+    b = c.tile_req[tile];
+    q0 = c.tile_q0[tile];
+    t0 = c.q_start[b];
+    n_q = c.q_start[b + 1] - t0;
+    kv0 = c.kv_start[b];
+    n = kv0 + n_q;
+  } else {
+    b = tile % a.B;
+    q0 = (a.num_q_tiles - 1 - tile / a.B) * kBM;
+    n = n_q = window_rows(a, b);
+  }
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int m16 = lane & 15, j = lane >> 4;
+  const int hbase = H * (w & 1);                             // first of this wave's heads in the GQA group
+  const int qi = q0 + 16 * (w >> 1) + m16;                   // this lane's query row (MFMA column)
+  const bool seen = qi < n_q;
+
+  const long q_row = kPaged ? (long)(t0 + min(qi, n_q - 1)) * a.q_ss : (long)b * a.q_sb + (long)min(qi, a.S - 1) * a.q_ss;
+  bf16x8 qop[H][4];
+#pragma unroll
+  for (int u = 0; u < H; ++u)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      u32x4 x = ld16g(a.q + q_row + (long)(kvh * kGroup + hbase + u) * a.q_sh + 8 * (4 * i + j));
+      if (!seen) x = u32x4{0, 0, 0, 0};
+      qop[u][i] = __builtin_bit_cast(bf16x8, x);
+    }
+  floatx4 o[8][H];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int u = 0; u < H; ++u) o[i][u] = floatx4{0.f, 0.f, 0.f, 0.f};
+  float m_run[H], l_run[H];
+#pragma unroll
+  for (int u = 0; u < H; ++u) {
+    m_run[u] = -INFINITY;
+    l_run[u] = 0.f;
+  }
+  WindowWalk walk(kv0 + q0, kv0 + min(q0 + kBM, n_q) - 1, a.window, a.sinks);
+  const WindowLane lm(kv0 + qi, seen, a.window, a.sinks);
+  if (q0 < n_q) {                                            // (uniform)
+    if constexpr (kPaged) {
+      const PagedRows rows{c.kv + kvh * kHeadDim, c.block_table + (long)b * c.bt_stride, c.bt_width, c.num_pages};
+      attend_tiles<H, kWaves>(rows, walk, n, Kbuf, Vbuf, qop, o, m_run, l_run, lm, a.scale_log2, w, lane);
+    } else {
+      const DenseRows<false> rows{a.k + (long)b * a.k_sb + (long)kvh * a.k_sh, a.v + (long)b * a.v_sb + (long)kvh * a.v_sh,
+                                  a.k_ss, a.v_ss};
+      attend_tiles<H, kWaves>(rows, walk, n, Kbuf, Vbuf, qop, o, m_run, l_run, lm, a.scale_log2, w, lane);
+    }
+  }
+  if (qi >= (kPaged ? n_q : a.S)) return;
+  const long o_row = kPaged ? (long)(t0 + qi) * a.o_ss : (long)b * a.o_sb + (long)qi * a.o_ss;
+#pragma unroll
+  for (int u = 0; u < H; ++u) {
+    // padding rows (o = 0, and an l of unmasked tiles): 0, lse -inf. A row that sees keys has l > 0, or NaN scores.
+    const float l = seen ? l_run[u] : 0.f;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int head = kvh * kGroup + hbase + u;
+    __bf16* oh = a.out + o_row + (long)head * a.o_sh + 32 * j;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) store_acc_bf16x8(oh + 8 * p, o[2 * p][u], o[2 * p + 1][u], j, inv);
+    if (a.lse != nullptr && j == 0)
+      a.lse[kPaged ? (long)(t0 + qi) * kHeadsQ + head : ((long)b * kHeadsQ + head) * a.S + qi] =
+          l == 0.f ? -INFINITY : (m_run[u] + __log2f(l)) * 0.69314718055994531f;
+  }
+}
+
+}  // namespace abkv
+
+extern "C" {
+
+int abkv_window_attn(const void* q, long q_stride_b, long q_stride_s, long q_stride_h, const void* k, long k_stride_b,
+                     long k_stride_s, long k_stride_h, const void* v, long v_stride_b, long v_stride_s, long v_stride_h,
+                     int batch, int seq_len, const int32_t* seq_lens, int window, int sinks, float scale, void* out,
+                     long out_stride_b, long out_stride_s, long out_stride_h, float* lse, hipStream_t stream) {
+  using namespace abkv;
+  if (batch <= 0 || seq_len <= 0) return 0;
+  if (q == nullptr || k == nullptr || v == nullptr || out == nullptr || window <= 0 || sinks < 0)
+    return (int)hipErrorInvalidValue;
+  WindowArgs a;
+  a.q = static_cast<const __bf16*>(q);
+  a.q_sb = q_stride_b; a.q_ss = q_stride_s; a.q_sh = q_stride_h;
+  a.k = static_cast<const __bf16*>(k);
+  a.k_sb = k_stride_b; a.k_ss = k_stride_s; a.k_sh = k_stride_h;
+  a.v = static_cast<const __bf16*>(v);
+  a.v_sb = v_stride_b; a.v_ss = v_stride_s; a.v_sh = v_stride_h;
+  a.B = batch;
+  a.S = seq_len;
+  a.seq_lens = seq_lens;
+  a.window = window;
+  a.sinks = sinks;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.out = static_cast<__bf16*>(out);
+  a.o_sb = out_stride_b; a.o_ss = out_stride_s; a.o_sh = out_stride_h;
+  a.lse = lse;
+  a.num_q_tiles = (seq_len - 1) / kBM + 1;
+  const long grid = (long)a.num_q_tiles * batch * kHeadsKV;
+  if (grid * 512 > 0xFFFFFFFFL) return (int)hipErrorInvalidValue;
+  hipLaunchKernelGGL(window_attn_kernel<false>, dim3((unsigned)grid), dim3(512), 0, stream, a, ChunkArgs{});
+  return (int)hipGetLastError();
+}
+
+int abkv_paged_prefill_attn_window(const void* q, long q_stride_tok, long q_stride_head, const void* kv_cache,
+                                   int num_pages, const int32_t* block_table, long block_table_stride, int table_width,
+                                   const int32_t* q_start, const int32_t* kv_start, const int32_t* tile_req,
+                                   const int32_t* tile_q0, int num_tiles, int window, int sinks, float scale, void* out,
+                                   long out_stride_tok, long out_stride_head, float* lse, hipStream_t stream) {
+  using namespace abkv;
+  if (num_tiles <= 0) return 0;
+  if (q == nullptr || kv_cache == nullptr || block_table == nullptr || q_start == nullptr || kv_start == nullptr ||
+      tile_req == nullptr || tile_q0 == nullptr || out == nullptr || num_pages <= 0 || table_width <= 0 || window <= 0 ||
+      sinks < 0)
+    return (int)hipErrorInvalidValue;
+  WindowArgs a{};
+  a.q = static_cast<const __bf16*>(q);
+  a.q_ss = q_stride_tok; a.q_sh = q_stride_head;
+  a.window = window;
+  a.sinks = sinks;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.out = static_cast<__bf16*>(out);
+  a.o_ss = out_stride_tok; a.o_sh = out_stride_head;
+  a.lse = lse;
+  const ChunkArgs c{static_cast<const __bf16*>(kv_cache), num_pages, block_table, block_table_stride, table_width,
+                    q_start, kv_start, tile_req, tile_q0};
+  const long grid = (long)num_tiles * kHeadsKV;
+  if (grid * 512 > 0xFFFFFFFFL) return (int)hipErrorInvalidValue;
+  hipLaunchKernelGGL(window_attn_kernel<true>, dim3((unsigned)grid), dim3(512), 0, stream, a, c);
+  return (int)hipGetLastError();
+}
+
+}  // extern "C"

@@ -972,5 +972,174 @@ def paged_prefill_attention_packed(q: torch.Tensor, kv_cache: torch.Tensor, bloc
     return out, lse
 
 
+# -- attention under a sliding window with sinks ---------------------------------------------------------------------
+_MAX_INT = (1 << 31) - 1
+
+
+def _check_device(*tensors) -> None:
+    """All on the current GPU: the launch goes to its current stream."""
+    for t in tensors:
+        if t is not None and not (t.is_cuda and t.device.index == torch._C._cuda_getDevice()):
+            raise ValueError(f"tensors must be on the current GPU, got one on {t.device}")
+
+
+def _check_rows(name: str, t: torch.Tensor, dtype, shape) -> None:
+    """Dense [B, S, H, 128] or [T, H, 128] rows as the tile loads take them: 16-byte aligned, and a row stride that keeps
+    64 rows' offsets in 32 bits."""
+    if t.dtype != dtype or tuple(t.shape) != shape:
+        raise ValueError(f"{name} must be {dtype} {list(shape)}, got {t.dtype} {list(t.shape)}")
+    st, per = t.stride(), 16 // t.element_size()
+    if st[-1] != 1 or t.data_ptr() % 16 or any(x % per or x < 0 for x in st[:-1]) or st[-3] >= 1 << 24:
+        raise ValueError(f"{name} must have contiguous, 16-byte aligned rows, got strides {st}")
+
+
+def _check_window(window, sinks) -> tuple[int, int]:
+    _require(int(window) == window and 1 <= window <= _MAX_INT, "window must be an integer >= 1")
+    _require(int(sinks) == sinks and 0 <= sinks <= _MAX_INT, "sinks must be an integer >= 0")
+    return int(window), int(sinks)
+
+
+def _reach(window: int, sinks: int, rows: int) -> tuple[int, int]:
+    """The same mask of sequences of at most ``rows`` rows, told shorter: a window over every row is plain causal, and so
+    is a sink at every row."""
+    return (rows, 0) if rows and (window >= rows or sinks >= rows) else (window, sinks)
+
+
+def _check_lens(seq_lens, B) -> None:
+    _require(seq_lens is None or (seq_lens.dtype == torch.int32 and tuple(seq_lens.shape) == (B,)
+                                  and seq_lens.is_contiguous()), "seq_lens must be contiguous int32 [B]")
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, sinks: int = 0,
+                     seq_lens: torch.Tensor | None = None, scale: float | None = None, out: torch.Tensor | None = None,
+                     lse: torch.Tensor | None = None):
+    """Causal attention of whole prompts under a sliding window with sinks: row i sees row j when j <= i and
+    (i - j < ``window`` or j < ``sinks``).
+
+    q [B, S, 32, 128], k/v [B, S, 8, 128] bf16 (any strides with contiguous, 16-byte aligned rows); ``seq_lens`` [B] int32
+    on the GPU: rows past a sequence's length are padding, not read as keys, with out 0 and lse -inf (None: no padding).
+    Rows inside a sequence should hold finite values (one that does not can reach other rows of its 64-row tile).
+    Returns (out [B, S, 32, 128], lse [B, 32, S] fp32 natural log or None). The weights are rounded to bf16 for their
+    product with v and summed rounded, so lse is good to about 2^-9 / sqrt(visible rows). fp32 q/k/v select the fp32 mode
+    (out fp32, exact to fp32 rounding; no backward).
+    """
+    _require(q.dim() == 4, "q must be [B, S, 32, 128]")
+    B, S = q.shape[0], q.shape[1]
+    window, sinks = _check_window(window, sinks)
+    dt = torch.float32 if q.dtype == torch.float32 else torch.bfloat16
+    for name, t, h in (("q", q, HEADS_Q), ("k", k, HEADS_KV), ("v", v, HEADS_KV)):
+        _check_rows(name, t, dt, (B, S, h, HEAD_DIM))
+    _check_lens(seq_lens, B)
+    if out is not None:
+        _check_rows("out", out, dt, (B, S, HEADS_Q, HEAD_DIM))
+    _require(lse is None or (lse.dtype == torch.float32 and lse.is_contiguous() and tuple(lse.shape) == (B, HEADS_Q, S)),
+             "lse must be contiguous fp32 [B, 32, S]")
+    _check_device(q, k, v, seq_lens, out, lse)
+    window, sinks = _reach(window, sinks, S)
+    if out is None:
+        out = torch.empty((B, S, HEADS_Q, HEAD_DIM), dtype=dt, device=q.device)
+    scale = default_scale() if scale is None else float(scale)
+    fn = lib().abkv_window_attn_f32 if dt == torch.float32 else lib().abkv_window_attn
+    rc = fn(_ptr(q), q.stride(0), q.stride(1), q.stride(2), _ptr(k), k.stride(0), k.stride(1), k.stride(2), _ptr(v),
+            v.stride(0), v.stride(1), v.stride(2), B, S, _ptr(seq_lens), window, sinks, scale, _ptr(out), out.stride(0),
+            out.stride(1), out.stride(2), _ptr(lse), _stream())
+    check(rc, "abkv_window_attn")
+    return out, lse
+
+
+def window_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, lse: torch.Tensor,
+                              dout: torch.Tensor, window: int, sinks: int = 0, seq_lens: torch.Tensor | None = None,
+                              scale: float | None = None):
+    """Gradients (dq [B, S, 32, 128], dk, dv [B, S, 8, 128], bf16) of sum(dout * out) for :func:`window_attention` under
+    the same window, from its out and lse. Padding rows get 0, whatever dout holds there (bf16 only)."""
+    _require(q.dim() == 4, "q must be [B, S, 32, 128]")
+    B, S = q.shape[0], q.shape[1]
+    window, sinks = _check_window(window, sinks)
+    for name, t, h in (("q", q, HEADS_Q), ("k", k, HEADS_KV), ("v", v, HEADS_KV), ("out", out, HEADS_Q),
+                       ("dout", dout, HEADS_Q)):
+        _check_rows(name, t, torch.bfloat16, (B, S, h, HEAD_DIM))
+    _check_lens(seq_lens, B)
+    _require(lse.dtype == torch.float32 and lse.is_contiguous() and tuple(lse.shape) == (B, HEADS_Q, S),
+             "lse must be contiguous fp32 [B, 32, S]")
+    _check_device(q, k, v, out, lse, dout, seq_lens)
+    window, sinks = _reach(window, sinks, S)
+    scale = default_scale() if scale is None else float(scale)
+    dq = torch.empty((B, S, HEADS_Q, HEAD_DIM), dtype=torch.bfloat16, device=q.device)
+    dk = torch.empty((B, S, HEADS_KV, HEAD_DIM), dtype=torch.bfloat16, device=q.device)
+    dv = torch.empty_like(dk)
+    ws = torch.empty(lib().abkv_window_bwd_workspace_size(B, S, window, sinks), dtype=torch.uint8, device=q.device)
+    args = []
+    for t in (q, k, v, out, dout):
+        args += [_ptr(t), t.stride(0), t.stride(1), t.stride(2)]
+    args += [_ptr(lse), B, S, _ptr(seq_lens), window, sinks, scale]
+    for t in (dq, dk, dv):
+        args += [_ptr(t), t.stride(0), t.stride(1), t.stride(2)]
+    rc = lib().abkv_window_attn_bwd(*args, _ptr(ws), ws.numel(), _stream())
+    check(rc, "abkv_window_attn_bwd")
+    return dq, dk, dv
+
+
+def _check_paged(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor) -> None:
+    """bf16 query rows [T, 32, 128], a layer cache and its page table, on the current GPU."""
+    _require(q.dim() == 3, "q must be [T, 32, 128]")
+    _check_rows("q", q, torch.bfloat16, (q.shape[0], HEADS_Q, HEAD_DIM))
+    _require(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[1] > 0
+             and block_table.stride(1) == 1, "block_table must be int32 [B, W] with contiguous rows")
+    _require(kv_cache.dim() == 5 and kv_cache.shape[0] > 0, "kv_cache must hold at least one page")
+    _check_device(q, kv_cache, block_table)
+    _check_cache(kv_cache)
+
+
+def _chunk_plan(q, block_table, q_start, kv_start, head_tiles):
+    """Host checks of a causal chunk batch, and its device metadata: (query tokens, tiles, base address of int32
+    q_start [R + 1] | kv_start [R] | tile requests | tile starts, the tensor that holds them). ``head_tiles``
+    (query rows, rows before them) -> the tiles a request takes, as first rows."""
+    qs, ks = np.asarray(q_start, dtype=np.int64), np.asarray(kv_start, dtype=np.int64)
+    _require(qs.ndim == ks.ndim == 1 and qs.size == ks.size + 1 and ks.size <= block_table.shape[0],
+             "q_start [R + 1] and kv_start [R] must be flat sequences, R at most the table's rows")
+    _require(qs[0] == 0 and (qs[1:] >= qs[:-1]).all() and qs[-1] <= q.shape[0], "q_start must be a prefix sum <= T")
+    nq = qs[1:] - qs[:-1]
+    _require(ks.size == 0 or (ks.min() >= 0 and (ks + nq).max() <= block_table.shape[1] * PAGE),
+             "the chunks' rows must lie in [0, block_table width * 16)")
+    per = [head_tiles(int(n), int(p)) for n, p in zip(nq, ks)]
+    req = np.repeat(np.arange(ks.size), [len(t) for t in per])
+    if req.size == 0:
+        return 0, 0, None
+    meta = _upload([qs, ks, req, np.concatenate(per)], q.device)
+    return int(qs[-1]), req.size, meta
+
+
+def paged_prefill_attention_window(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, q_start, kv_start,
+                                   window: int, sinks: int = 0, scale: float | None = None,
+                                   out: torch.Tensor | None = None, lse: torch.Tensor | None = None):
+    """Prompt chunks over the paged cache under a sliding window with sinks: request r's queries are tokens
+    q_start[r]..q_start[r+1]-1 of q [T, 32, 128] bf16 at physical positions kv_start[r] + i (host sequences, as
+    :func:`paged_prefill_attention`), and a query at position p sees rows j <= p with p - j < ``window`` or j < ``sinks``.
+    The chunk's own rows must be in the cache. Returns (out [T, 32, 128] bf16, lse [T, 32] fp32 or None); rows past
+    q_start[-1] are left alone."""
+    window, sinks = _check_window(window, sinks)
+    _check_paged(q, kv_cache, block_table)
+    T = q.shape[0]
+    if out is not None:
+        _check_rows("out", out, torch.bfloat16, (T, HEADS_Q, HEAD_DIM))
+    _require(lse is None or (lse.dtype == torch.float32 and lse.is_contiguous() and tuple(lse.shape) == (T, HEADS_Q)),
+             "lse must be contiguous fp32 [T, 32]")
+    _check_device(out, lse)
+    if out is None:
+        out = torch.empty((T, HEADS_Q, HEAD_DIM), dtype=torch.bfloat16, device=q.device)
+    _, tiles, meta = _chunk_plan(q, block_table, q_start, kv_start, lambda n, _: np.arange(0, n, 64))
+    if tiles == 0:
+        return out, lse
+    R, at = len(kv_start), meta.data_ptr()
+    scale = default_scale() if scale is None else float(scale)
+    rc = lib().abkv_paged_prefill_attn_window(_ptr(q), q.stride(0), q.stride(1), _ptr(kv_cache), kv_cache.shape[0],
+                                              _ptr(block_table), _row_stride(block_table), block_table.shape[1], at,
+                                              at + 4 * (R + 1), at + 4 * (2 * R + 1), at + 4 * (2 * R + 1 + tiles), tiles,
+                                              window, sinks, scale, _ptr(out), out.stride(0), out.stride(1), _ptr(lse),
+                                              _stream())
+    check(rc, "abkv_paged_prefill_attn_window")
+    return out, lse
+
+
 def default_scale() -> float:
     return 1.0 / math.sqrt(HEAD_DIM)

@@ -429,6 +429,47 @@ int abkv_planner_is_token_active(void* planner, int64_t rid, int group, int64_t 
  * group_mask (< 0: all), 3 free, 4 drop step outputs. Returns n, or -(failing index + 1). */
 int64_t abkv_planner_apply_events(void* planner, const int64_t* events, int64_t n);
 
+/* ---------------------------------------------------------------------------------------------------------------
+ * Attention under a sliding window with sinks: row i sees key j when j <= i and (i - j < window or j < sinks), both below
+ * the sequence's length. The reference has no windowed attention; a window is what a compressed context is compared with,
+ * and its decoder layers may ask for one (abridgekv/compress_forward.py:1095-1132 is the full-context baseline).
+ * window >= 1, sinks >= 0.
+ *
+ * Whole prompts: q, out [batch, seq_len, 32, 128], k, v [batch, seq_len, 8, 128] bf16, any element strides that keep rows
+ * 16-byte aligned. seq_lens (device, [batch], or NULL: seq_len everywhere; clamped to [0, seq_len]): rows past it are
+ * padding, never read as keys, with out 0 and lse -inf. lse [batch, 32, seq_len] fp32 natural log, or NULL. Values of rows
+ * inside a sequence should be finite: a row that is not can reach rows of its 64-row tile that do not see it. */
+int abkv_window_attn(const void* q, long q_stride_b, long q_stride_s, long q_stride_h, const void* k, long k_stride_b,
+                     long k_stride_s, long k_stride_h, const void* v, long v_stride_b, long v_stride_s, long v_stride_h,
+                     int batch, int seq_len, const int32_t* seq_lens, int window, int sinks, float scale, void* out,
+                     long out_stride_b, long out_stride_s, long out_stride_h, float* lse, abkv_stream_t stream);
+/* The same in fp32 (inputs, outputs, sums); rows that are not finite reach only the rows that see them. */
+int abkv_window_attn_f32(const float* q, long q_stride_b, long q_stride_s, long q_stride_h, const float* k,
+                         long k_stride_b, long k_stride_s, long k_stride_h, const float* v, long v_stride_b,
+                         long v_stride_s, long v_stride_h, int batch, int seq_len, const int32_t* seq_lens, int window,
+                         int sinks, float scale, float* out, long out_stride_b, long out_stride_s, long out_stride_h,
+                         float* lse, abkv_stream_t stream);
+/* Gradients of abkv_window_attn (bf16) from its out and lse: dq [batch, seq_len, 32, 128], dk, dv [batch, seq_len, 8, 128],
+ * padding rows 0. workspace: abkv_window_bwd_workspace_size bytes, not shared by calls that may overlap. */
+size_t abkv_window_bwd_workspace_size(int batch, int seq_len, int window, int sinks);
+int abkv_window_attn_bwd(const void* q, long q_stride_b, long q_stride_s, long q_stride_h, const void* k, long k_stride_b,
+                         long k_stride_s, long k_stride_h, const void* v, long v_stride_b, long v_stride_s,
+                         long v_stride_h, const void* out, long out_stride_b, long out_stride_s, long out_stride_h,
+                         const void* dout, long dout_stride_b, long dout_stride_s, long dout_stride_h, const float* lse,
+                         int batch, int seq_len, const int32_t* seq_lens, int window, int sinks, float scale, void* dq,
+                         long dq_stride_b, long dq_stride_s, long dq_stride_h, void* dk, long dk_stride_b,
+                         long dk_stride_s, long dk_stride_h, void* dv, long dv_stride_b, long dv_stride_s,
+                         long dv_stride_h, void* workspace, size_t workspace_bytes, abkv_stream_t stream);
+/* Prompt chunks over the paged cache: request r's queries are rows q_start[r] .. q_start[r + 1] - 1 of q [T, 32, 128] bf16,
+ * at physical positions kv_start[r] + i, causal. q_start [requests + 1], kv_start [requests], tile_req / tile_q0 [num_tiles]
+ * (request and first query row of every 64-row query tile) on the device; every key position must lie inside the table row
+ * (page ids are clamped into the cache). out [T, 32, 128], lse [T, 32] or NULL; rows of no request are left alone. */
+int abkv_paged_prefill_attn_window(const void* q, long q_stride_tok, long q_stride_head, const void* kv_cache,
+                                   int num_pages, const int32_t* block_table, long block_table_stride, int table_width,
+                                   const int32_t* q_start, const int32_t* kv_start, const int32_t* tile_req,
+                                   const int32_t* tile_q0, int num_tiles, int window, int sinks, float scale, void* out,
+                                   long out_stride_tok, long out_stride_head, float* lse, abkv_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
