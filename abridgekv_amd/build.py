@@ -16,7 +16,7 @@ PROBE_LIB = PKG / "libabridgekv_probes.so"      # measurement probes, loaded by 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 DEVICE_SOURCES = ["decode_attn.hip", "kv_cache.hip", "prefill_attn.hip", "prefill_bwd.hip", "paged_prefill.hip",
-                  "attn_f32.hip", "window_attn.hip", "window_bwd.hip"]
+                  "attn_f32.hip", "window_attn.hip", "window_bwd.hip", "evict.hip"]
 HOST_SOURCES = ["planner.cpp", "paged_plan.cpp"]
 PROBE_SOURCES = ["probes.hip"]
 

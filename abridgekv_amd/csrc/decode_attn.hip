@@ -59,7 +59,50 @@ struct DecodeArgs {
   int side_max_pages;        // bound on side_count
   int side_split_rows;       // side rows per split and head (multiple of 32, <= 63 * min quota)
   int side_q[kHeadsKV], side_o[kHeadsKV];
+  // kWindow: rows [seq_len - window, seq_len) and the first `sinks` rows are seen
+  int window, sinks;
+  // kScored: the weights of every row are added to scores[b][KV head][row] after the merge
+  float* raw;                // [B, 32, raw_stride] scores of this step in log2 units
+  long raw_stride;
+  float* scores;
+  long s_sb, s_sh;
 };
+
+// What a launch of the decode kernel attends and leaves.
+constexpr int kPlain = 0;    // every row of the sequence
+constexpr int kWindow = 1;   // the sinks and the window
+constexpr int kScored = 2;   // every row, and each row's score for the weights to be added up (partials always)
+
+// The rows of a sequence that the step reads, as whole pages one after the other: pages below `sink_pages`, then pages
+// shifted by `shift`. In rows of that order (virtual rows), [0, sink_end) and [win_begin, end) are seen.
+struct DecodeRows {
+  int pages, sink_pages, shift;
+  int sink_end, win_begin, end;
+  __device__ __forceinline__ int page(int v) const { return v < sink_pages ? v : v + shift; }
+  __device__ __forceinline__ bool sees(int row) const { return row < end && (row < sink_end || row >= win_begin); }
+  // some of the 32 rows from `row` on are not seen
+  __device__ __forceinline__ bool partial(int row) const {
+    return row + 2 * kPage > end || (row < win_begin && row + 2 * kPage > sink_end);
+  }
+};
+template <int kMode>
+__device__ __forceinline__ DecodeRows decode_rows(const DecodeArgs& a, int b) {
+  DecodeRows r;
+  r.end = max(min(a.seq_lens[b], a.max_pages * kPage), 0);
+  r.pages = (r.end + kPage - 1) / kPage;
+  r.sink_pages = r.pages;
+  r.shift = r.sink_end = r.win_begin = 0;
+  if constexpr (kMode == kWindow) {
+    r.win_begin = max(r.end - a.window, 0);
+    r.sink_end = min(a.sinks, r.win_begin);
+    r.sink_pages = (r.sink_end + kPage - 1) / kPage;
+    r.shift = max(r.win_begin / kPage - r.sink_pages, 0);
+    r.pages -= r.shift;
+    r.win_begin -= r.shift * kPage;
+    r.end -= r.shift * kPage;
+  }
+  return r;
+}
 
 __device__ __forceinline__ u32x4 ld16(const __bf16* p) {
   return *reinterpret_cast<const u32x4*>(p);
@@ -142,7 +185,7 @@ __device__ __forceinline__ void combine_subs(const DecodeArgs& a, const float (&
   if (lane == 0) *reinterpret_cast<floatx4*>(a.part_ml + at * 4) = floatx4{m, l, range.scale, 0.f};
 }
 
-template <int kW, int kSub>
+template <int kW, int kSub, int kMode>
 __global__ __launch_bounds__(64 * kW * kSub) void decode_attn_kernel(DecodeArgs a) {
   // Grid (max_splits * 8 / kW, B): kW KV heads per workgroup, a wave each (kSub == 1); the 8 / kW workgroups of a split
   // are adjacent in x. Split fastest (dispatch order: the splits of sequence 0, then of sequence 1, ...), measured faster
@@ -159,13 +202,13 @@ __global__ __launch_bounds__(64 * kW * kSub) void decode_attn_kernel(DecodeArgs 
   const int m16 = lane & 15;                  // MFMA row/col index of this lane
   const int j = lane >> 4;                    // lane group (k-chunk index)
 
-  const int seq_len = max(min(a.seq_lens[b], a.max_pages * kPage), 0);
-  const int n_pages = (seq_len + kPage - 1) / kPage;
+  const DecodeRows rows = decode_rows<kMode>(a, b);
+  const int n_pages = rows.pages;
   const int n_splits = max(1, (n_pages + a.split_pages - 1) / a.split_pages);
   if (split >= n_splits) return;
   const int pg_begin = split * a.split_pages;
   const int pg_end = min(n_pages, pg_begin + a.split_pages);
-  const int row_end = seq_len;                                       // rows of this split: [pg_begin*16, row_end)
+  const int row_end = rows.end;                                      // rows of this split: [pg_begin*16, row_end)
   const int32_t* bt = a.block_table + (long)b * a.bt_stride;
 
   // Q^T operand: lane supplies q[head m16][dims 8*(4i+j) .. +8] for MFMA i (zero for the 12 padding columns).
@@ -189,7 +232,10 @@ __global__ __launch_bounds__(64 * kW * kSub) void decode_attn_kernel(DecodeArgs 
   // Page ids of the split, fetched once: lane l holds page pg_begin + l (clamped into the cache); the loop reads them
   // with readlane, so no page-table load sits between one chunk's compute and the next chunk's K/V loads.
   int pid_l = 0;
-  if (lane < pg_end - pg_begin) pid_l = min(max(bt[pg_begin + lane], 0), a.num_pages - 1);
+  if (lane < pg_end - pg_begin) {
+    const int pg = kMode == kWindow ? rows.page(pg_begin + lane) : pg_begin + lane;
+    pid_l = min(max(bt[pg], 0), a.num_pages - 1);
+  }
   const __bf16* kv_h = a.kv + kvh * kHeadDim;
   for (int pg = pg_begin + 2 * sub; pg < pg_end; pg += 2 * kSub) {
     const int p0 = __builtin_amdgcn_readlane(pid_l, pg - pg_begin);
@@ -220,7 +266,7 @@ __global__ __launch_bounds__(64 * kW * kSub) void decode_attn_kernel(DecodeArgs 
       for (int i = 0; i < 4; ++i) s[t] = mfma16x16x32(__builtin_bit_cast(bf16x8, kr[t][i]), qop[i], s[t]);
     }
     // s[t][r] = score of slot pg*16 + 16t + 4j + r for head m16.
-    const bool tail = (pg + 2) * kPage > row_end;
+    const bool tail = kMode == kWindow ? rows.partial(pg * kPage) : (pg + 2) * kPage > row_end;
     float sv[8];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -229,7 +275,7 @@ __global__ __launch_bounds__(64 * kW * kSub) void decode_attn_kernel(DecodeArgs 
         float x = s[t][r] * a.scale_log2;
         if (tail) {
           const int slot = pg * kPage + 16 * t + 4 * j + r;
-          x = slot < row_end ? x : -INFINITY;
+          x = (kMode == kWindow ? rows.sees(slot) : slot < row_end) ? x : -INFINITY;
         }
         sv[4 * t + r] = x;
       }
@@ -238,7 +284,16 @@ __global__ __launch_bounds__(64 * kW * kSub) void decode_attn_kernel(DecodeArgs 
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int slot = pg * kPage + (e < 4 ? 0 : 16) + 4 * j + (e & 3);
-        if (slot >= row_end) vr[e] = u32x4{0, 0, 0, 0};
+        if (kMode == kWindow ? !rows.sees(slot) : slot >= row_end) vr[e] = u32x4{0, 0, 0, 0};
+      }
+    }
+    if constexpr (kMode == kScored) {
+      // raw scores of the wave's four heads, four rows a lane (a row buffer of whole page pairs: raw_stride)
+      if (m16 < kGroup) {
+        float* raw = a.raw + ((long)b * kHeadsQ + kvh * kGroup + m16) * a.raw_stride + pg * kPage + 4 * j;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          *reinterpret_cast<floatx4*>(raw + 16 * t) = floatx4{sv[4 * t], sv[4 * t + 1], sv[4 * t + 2], sv[4 * t + 3]};
       }
     }
     float mx = sv[0];
@@ -375,13 +430,8 @@ __device__ __forceinline__ void merge_pair(MergeState& st) {
 // at [max_splits, max_splits + n_side)). Workgroup (sequence, group of 4 heads), one wave per head; the wave's four
 // 16-lane groups g take the splits k = g, g + 4, ... (lane c of a group: dims 8c .. 8c + 7, one 16-byte load per
 // split), each keeping a running max, and the four states are combined with two cross-lane swaps.
-__global__ __launch_bounds__(256) void decode_merge_kernel(DecodeArgs a) {
-  const int b = blockIdx.x;
-  const int seq_len = max(min(a.seq_lens[b], a.max_pages * kPage), 0);
-  const int n_pages = (seq_len + kPage - 1) / kPage;
-  const int n_main = max(1, (n_pages + a.split_pages - 1) / a.split_pages);
-  if (!a.force_partials && n_main <= 1) return;
-  const int head = 4 * blockIdx.y + (threadIdx.x >> 6);
+// This wave's head `head`, n_main main splits.
+__device__ __forceinline__ void merge_head(const DecodeArgs& a, int b, int head, int n_main) {
   const int lane = threadIdx.x & 63;
   const int g = lane >> 4, c = lane & 15;
   const int n_side = side_splits(a, b, head / kGroup);
@@ -420,6 +470,69 @@ __global__ __launch_bounds__(256) void decode_merge_kernel(DecodeArgs a) {
   *reinterpret_cast<u32x4*>(a.out + (long)b * a.o_sb + (long)head * a.o_sh + 8 * c) = wv;
   if (a.lse != nullptr && c == 0)
     a.lse[(long)b * kHeadsQ + head] = st.L > 0.f ? (st.M + __log2f(st.L)) * 0.69314718055994531f : -INFINITY;
+}
+
+template <int kMode>
+__global__ __launch_bounds__(256) void decode_merge_kernel(DecodeArgs a) {
+  const int b = blockIdx.x;
+  const int n_main = max(1, (decode_rows<kMode>(a, b).pages + a.split_pages - 1) / a.split_pages);
+  if (!a.force_partials && n_main <= 1) return;
+  merge_head(a, b, 4 * blockIdx.y + (threadIdx.x >> 6), n_main);
+}
+
+// The end of a scored step: the merge (the first 8 workgroups of a sequence, four heads each), and beside it the rows'
+// scores, workgroup (sequence, KV head, 1024 rows): scores[row] += sum over the group's heads u of exp2(raw_u - M_u) / L_u,
+// with (M_u, L_u) from the splits' records, which every workgroup combines for itself. One owner per score: no atomics, the
+// same bits every time. The raw scores cost 128 B written and read a row beside its 4 KiB of K and V.
+constexpr int kScoreRows = 1024;
+__global__ __launch_bounds__(256) void decode_score_kernel(DecodeArgs a) {
+  const int b = blockIdx.y;
+  const DecodeRows rows = decode_rows<kScored>(a, b);
+  const int n_main = max(1, (rows.pages + a.split_pages - 1) / a.split_pages);
+  const int lane = threadIdx.x & 63, u = threadIdx.x >> 6;
+  constexpr int kMerges = kHeadsQ / 4;
+  if ((int)blockIdx.x < kMerges) return merge_head(a, b, 4 * blockIdx.x + u, n_main);
+  const int kvh = (blockIdx.x - kMerges) % kHeadsKV;
+  const int row0 = (int)(blockIdx.x - kMerges) / kHeadsKV * kScoreRows;
+  if (row0 >= rows.end) return;                              // (uniform)
+  __shared__ float sm[kGroup], si[kGroup];
+  {
+    const float* rec = a.part_ml + ((long)b * a.part_stride * kHeadsQ + kvh * kGroup + u) * 4;
+    float m = -INFINITY, l = 0.f;
+    for (int k = lane; k < n_main; k += 64) {
+      const float2 ml = *reinterpret_cast<const float2*>(rec + (long)k * kHeadsQ * 4);
+      const float mn = fmaxf(m, ml.x);
+      l = mn == -INFINITY ? l + ml.y : l * fast_exp2(m - mn) + ml.y * fast_exp2(ml.x - mn);
+      m = mn;
+    }
+    float M = m;
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) M = fmaxf(M, __shfl_xor(M, k, 64));
+    l = m == -INFINITY ? l : l * fast_exp2(m - M);           // (a lane without splits: 0)
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) l += __shfl_xor(l, k, 64);
+    if (lane == 0) {
+      sm[u] = M;
+      si[u] = 1.f / l;
+    }
+  }
+  __syncthreads();
+  const int row = row0 + 4 * threadIdx.x;
+  if (row >= rows.end) return;
+  floatx4 w = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int h = 0; h < kGroup; ++h) {
+    const floatx4 x = *reinterpret_cast<const floatx4*>(a.raw + ((long)b * kHeadsQ + kvh * kGroup + h) * a.raw_stride + row);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) w[r] += fast_exp2(x[r] - sm[h]) * si[h];
+  }
+  typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+  float* to = a.scores + (long)b * a.s_sb + (long)kvh * a.s_sh + row;
+  if (row + 4 <= rows.end) {
+    *reinterpret_cast<f32x4u*>(to) = *reinterpret_cast<const f32x4u*>(to) + w;
+  } else {
+    for (int r = 0; row + r < rows.end; ++r) to[r] += r == 0 ? w[0] : r == 1 ? w[1] : w[2];
+  }
 }
 
 // Attention of each sequence's 32 query heads over its side rows (per-head packed code pages; the reference keeps
@@ -571,14 +684,15 @@ inline bool share_splits(int max_splits, int num_seqs) {
   const long splits = (long)max_splits * num_seqs;
   return splits <= 64 || (num_seqs <= 32 && (splits <= 96 || (splits > 128 && splits <= 160)));
 }
+template <int kMode>
 inline void launch_decode(const DecodeArgs& a, int max_splits, int num_seqs, hipStream_t stream) {
   if (share_splits(max_splits, num_seqs)) {
-    hipLaunchKernelGGL((decode_attn_kernel<1, kGroup>), dim3(max_splits * kHeadsKV, num_seqs), dim3(64 * kGroup), 0,
+    hipLaunchKernelGGL((decode_attn_kernel<1, kGroup, kMode>), dim3(max_splits * kHeadsKV, num_seqs), dim3(64 * kGroup), 0,
                        stream, a);
     return;
   }
   constexpr int kW = 2;
-  hipLaunchKernelGGL((decode_attn_kernel<kW, 1>), dim3(max_splits * (kHeadsKV / kW), num_seqs), dim3(64 * kW), 0, stream,
+  hipLaunchKernelGGL((decode_attn_kernel<kW, 1, kMode>), dim3(max_splits * (kHeadsKV / kW), num_seqs), dim3(64 * kW), 0, stream,
                      a);
 }
 
@@ -659,11 +773,11 @@ int abkv_decode_attn(const void* q, long q_stride_seq, long q_stride_head,
   a.part_stride = max_splits;
   a.force_partials = 0;
   a.side_count = nullptr;
-  launch_decode(a, max_splits, num_seqs, stream);
+  launch_decode<kPlain>(a, max_splits, num_seqs, stream);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return (int)err;
   if (max_splits > 1) {
-    hipLaunchKernelGGL(decode_merge_kernel, dim3(num_seqs, kHeadsQ / 4), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(decode_merge_kernel<kPlain>, dim3(num_seqs, kHeadsQ / 4), dim3(256), 0, stream, a);
     err = hipGetLastError();
   }
   return (int)err;
@@ -776,7 +890,7 @@ int abkv_decode_attn_packed(const void* q, long q_stride_seq, long q_stride_head
   a.side_count = packed_count;
   a.side_max_pages = max_packed_per_seq;
   a.side_split_rows = side_split_rows;
-  launch_decode(a, max_splits, num_seqs, stream);
+  launch_decode<kPlain>(a, max_splits, num_seqs, stream);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return (int)err;
   if (side_max > 0) {
@@ -784,7 +898,124 @@ int abkv_decode_attn_packed(const void* q, long q_stride_seq, long q_stride_head
     err = hipGetLastError();
     if (err != hipSuccess) return (int)err;
   }
-  hipLaunchKernelGGL(decode_merge_kernel, dim3(num_seqs, kHeadsQ / 4), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL(decode_merge_kernel<kPlain>, dim3(num_seqs, kHeadsQ / 4), dim3(256), 0, stream, a);
+  return (int)hipGetLastError();
+}
+
+// Splits of a sequence's visible pages: the sinks' pages, and one page more than the window fills.
+static int window_splits(int max_pages_per_seq, int split_pages, int window, int sinks) {
+  const long pages = ((long)sinks + abkv::kPage - 1) / abkv::kPage + ((long)window + abkv::kPage - 1) / abkv::kPage + 1;
+  const int most = pages < max_pages_per_seq ? (int)pages : max_pages_per_seq;
+  return (most + split_pages - 1) / split_pages;
+}
+
+static bool decode_call_ok(const void* q, const void* kv_cache, int num_pages, const int32_t* block_table,
+                           long block_table_stride, const int32_t* seq_lens, int num_seqs, int max_pages_per_seq,
+                           int split_pages, const void* out) {
+  return split_pages > 0 && !(split_pages & 1) && split_pages <= 64 && max_pages_per_seq > 0 &&
+         max_pages_per_seq <= (1 << 26) && num_pages > 0 && block_table_stride >= max_pages_per_seq && num_seqs <= 65535 &&
+         q != nullptr && kv_cache != nullptr && block_table != nullptr && seq_lens != nullptr && out != nullptr;
+}
+
+size_t abkv_decode_window_workspace_size(int num_seqs, int max_pages_per_seq, int split_pages, int window, int sinks) {
+  if (num_seqs <= 0 || max_pages_per_seq <= 0 || split_pages <= 0 || window <= 0 || sinks < 0) return 0;
+  const int splits = window_splits(max_pages_per_seq, split_pages, window, sinks);
+  return splits > 1 ? abkv_decode_workspace_size(num_seqs, splits) : 0;
+}
+
+int abkv_decode_attn_window(const void* q, long q_stride_seq, long q_stride_head, const void* kv_cache, int num_pages,
+                            const int32_t* block_table, long block_table_stride, const int32_t* seq_lens, int num_seqs,
+                            int max_pages_per_seq, int split_pages, int window, int sinks, float scale, void* out,
+                            long out_stride_seq, long out_stride_head, float* lse, void* workspace,
+                            size_t workspace_bytes, hipStream_t stream) {
+  using namespace abkv;
+  if (num_seqs <= 0) return 0;
+  if (window <= 0 || sinks < 0 || !decode_call_ok(q, kv_cache, num_pages, block_table, block_table_stride, seq_lens, num_seqs,
+                                                  max_pages_per_seq, split_pages, out))
+    return (int)hipErrorInvalidValue;
+  const int max_splits = window_splits(max_pages_per_seq, split_pages, window, sinks);
+  if (max_splits > 1 && (workspace == nullptr || workspace_bytes < abkv_decode_workspace_size(num_seqs, max_splits)))
+    return (int)hipErrorInvalidValue;
+  DecodeArgs a{};
+  a.q = static_cast<const __bf16*>(q);
+  a.q_sb = q_stride_seq;
+  a.q_sh = q_stride_head;
+  a.kv = static_cast<const __bf16*>(kv_cache);
+  a.block_table = block_table;
+  a.bt_stride = block_table_stride;
+  a.seq_lens = seq_lens;
+  a.split_pages = split_pages;
+  a.max_splits = a.part_stride = max_splits;
+  a.max_pages = max_pages_per_seq;
+  a.num_pages = num_pages;
+  a.window = window;
+  a.sinks = sinks;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.out = static_cast<__bf16*>(out);
+  a.o_sb = out_stride_seq;
+  a.o_sh = out_stride_head;
+  a.lse = lse;
+  a.part_o = static_cast<_Float16*>(workspace);
+  a.part_ml = reinterpret_cast<float*>(a.part_o + (size_t)num_seqs * max_splits * kHeadsQ * kHeadDim);
+  launch_decode<kWindow>(a, max_splits, num_seqs, stream);
+  hipError_t err = hipGetLastError();
+  if (err != hipSuccess || max_splits <= 1) return (int)err;
+  hipLaunchKernelGGL(decode_merge_kernel<kWindow>, dim3(num_seqs, kHeadsQ / 4), dim3(256), 0, stream, a);
+  return (int)hipGetLastError();
+}
+
+// Partials of every split, then the raw scores: rows in whole page pairs per query head.
+size_t abkv_decode_scored_workspace_size(int num_seqs, int max_pages_per_seq, int split_pages) {
+  if (num_seqs <= 0 || max_pages_per_seq <= 0 || split_pages <= 0) return 0;
+  const size_t rows = ((size_t)max_pages_per_seq + 1) / 2 * 2 * abkv::kPage;
+  return abkv_decode_workspace_size(num_seqs, (max_pages_per_seq + split_pages - 1) / split_pages) +
+         (size_t)num_seqs * abkv::kHeadsQ * rows * sizeof(float);
+}
+
+int abkv_decode_attn_scored(const void* q, long q_stride_seq, long q_stride_head, const void* kv_cache, int num_pages,
+                            const int32_t* block_table, long block_table_stride, const int32_t* seq_lens, int num_seqs,
+                            int max_pages_per_seq, int split_pages, float scale, float* scores, long scores_stride_seq,
+                            long scores_stride_head, void* out, long out_stride_seq, long out_stride_head, float* lse,
+                            void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  using namespace abkv;
+  if (num_seqs <= 0) return 0;
+  if (scores == nullptr || !decode_call_ok(q, kv_cache, num_pages, block_table, block_table_stride, seq_lens, num_seqs,
+                                           max_pages_per_seq, split_pages, out))
+    return (int)hipErrorInvalidValue;
+  if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
+      workspace_bytes < abkv_decode_scored_workspace_size(num_seqs, max_pages_per_seq, split_pages))
+    return (int)hipErrorInvalidValue;
+  const int max_splits = (max_pages_per_seq + split_pages - 1) / split_pages;
+  DecodeArgs a{};
+  a.q = static_cast<const __bf16*>(q);
+  a.q_sb = q_stride_seq;
+  a.q_sh = q_stride_head;
+  a.kv = static_cast<const __bf16*>(kv_cache);
+  a.block_table = block_table;
+  a.bt_stride = block_table_stride;
+  a.seq_lens = seq_lens;
+  a.split_pages = split_pages;
+  a.max_splits = a.part_stride = max_splits;
+  a.max_pages = max_pages_per_seq;
+  a.num_pages = num_pages;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.out = static_cast<__bf16*>(out);
+  a.o_sb = out_stride_seq;
+  a.o_sh = out_stride_head;
+  a.lse = lse;
+  a.part_o = static_cast<_Float16*>(workspace);
+  a.part_ml = reinterpret_cast<float*>(a.part_o + (size_t)num_seqs * max_splits * kHeadsQ * kHeadDim);
+  a.force_partials = 1;
+  a.raw = reinterpret_cast<float*>(static_cast<char*>(workspace) + abkv_decode_workspace_size(num_seqs, max_splits));
+  a.raw_stride = (long)(max_pages_per_seq + 1) / 2 * 2 * kPage;
+  a.scores = scores;
+  a.s_sb = scores_stride_seq;
+  a.s_sh = scores_stride_head;
+  launch_decode<kScored>(a, max_splits, num_seqs, stream);
+  hipError_t err = hipGetLastError();
+  if (err != hipSuccess) return (int)err;
+  const int chunks = (max_pages_per_seq * kPage + kScoreRows - 1) / kScoreRows;
+  hipLaunchKernelGGL(decode_score_kernel, dim3(kHeadsQ / 4 + chunks * kHeadsKV, num_seqs), dim3(256), 0, stream, a);
   return (int)hipGetLastError();
 }
 

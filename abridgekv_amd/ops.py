@@ -1080,33 +1080,29 @@ def window_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
 
 
 def _check_paged(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor) -> None:
-    """bf16 query rows [T, 32, 128], a layer cache and its page table, on the current GPU."""
+    """bf16 query rows [T, 32, 128], a layer cache and its page table."""
     _require(q.dim() == 3, "q must be [T, 32, 128]")
     _check_rows("q", q, torch.bfloat16, (q.shape[0], HEADS_Q, HEAD_DIM))
     _require(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[1] > 0
              and block_table.stride(1) == 1, "block_table must be int32 [B, W] with contiguous rows")
-    _require(kv_cache.dim() == 5 and kv_cache.shape[0] > 0, "kv_cache must hold at least one page")
-    _check_device(q, kv_cache, block_table)
-    _check_cache(kv_cache)
+    _require(kv_cache.dtype == torch.bfloat16 and kv_cache.dim() == 5 and kv_cache.shape[1:] == _PAGE_SHAPE
+             and kv_cache.shape[0] > 0 and kv_cache.is_contiguous(),
+             f"kv_cache must be contiguous bf16 [P, 2, {PAGE}, {HEADS_KV}, {HEAD_DIM}]")
 
 
-def _chunk_plan(q, block_table, q_start, kv_start, head_tiles):
-    """Host checks of a causal chunk batch, and its device metadata: (query tokens, tiles, base address of int32
-    q_start [R + 1] | kv_start [R] | tile requests | tile starts, the tensor that holds them). ``head_tiles``
-    (query rows, rows before them) -> the tiles a request takes, as first rows."""
+def _chunk_plan(q, block_table, q_start, kv_start, tiles_of):
+    """Host checks of a causal chunk batch, and its metadata [q_start [R + 1] | kv_start [R] | the tiles' requests | their
+    first rows]; ``tiles_of`` (query rows, rows before them) -> the first rows of a request's tiles. None: no tile."""
     qs, ks = np.asarray(q_start, dtype=np.int64), np.asarray(kv_start, dtype=np.int64)
     _require(qs.ndim == ks.ndim == 1 and qs.size == ks.size + 1 and ks.size <= block_table.shape[0],
              "q_start [R + 1] and kv_start [R] must be flat sequences, R at most the table's rows")
-    _require(qs[0] == 0 and (qs[1:] >= qs[:-1]).all() and qs[-1] <= q.shape[0], "q_start must be a prefix sum <= T")
     nq = qs[1:] - qs[:-1]
+    _require(qs[0] == 0 and (nq >= 0).all() and qs[-1] <= q.shape[0], "q_start must be a prefix sum <= T")
     _require(ks.size == 0 or (ks.min() >= 0 and (ks + nq).max() <= block_table.shape[1] * PAGE),
              "the chunks' rows must lie in [0, block_table width * 16)")
-    per = [head_tiles(int(n), int(p)) for n, p in zip(nq, ks)]
+    per = [tiles_of(int(n), int(p)) for n, p in zip(nq, ks)]
     req = np.repeat(np.arange(ks.size), [len(t) for t in per])
-    if req.size == 0:
-        return 0, 0, None
-    meta = _upload([qs, ks, req, np.concatenate(per)], q.device)
-    return int(qs[-1]), req.size, meta
+    return [qs, ks, req, np.concatenate(per)] if req.size else None
 
 
 def paged_prefill_attention_window(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, q_start, kv_start,
@@ -1124,13 +1120,15 @@ def paged_prefill_attention_window(q: torch.Tensor, kv_cache: torch.Tensor, bloc
         _check_rows("out", out, torch.bfloat16, (T, HEADS_Q, HEAD_DIM))
     _require(lse is None or (lse.dtype == torch.float32 and lse.is_contiguous() and tuple(lse.shape) == (T, HEADS_Q)),
              "lse must be contiguous fp32 [T, 32]")
-    _check_device(out, lse)
+    plan = _chunk_plan(q, block_table, q_start, kv_start, lambda n, _: np.arange(0, n, 64))
+    _check_device(q, kv_cache, block_table, out, lse)
     if out is None:
         out = torch.empty((T, HEADS_Q, HEAD_DIM), dtype=torch.bfloat16, device=q.device)
-    _, tiles, meta = _chunk_plan(q, block_table, q_start, kv_start, lambda n, _: np.arange(0, n, 64))
-    if tiles == 0:
+    if plan is None:
         return out, lse
-    R, at = len(kv_start), meta.data_ptr()
+    tiles, R = plan[2].size, len(kv_start)
+    meta = _upload(plan, q.device)
+    at = meta.data_ptr()
     scale = default_scale() if scale is None else float(scale)
     rc = lib().abkv_paged_prefill_attn_window(_ptr(q), q.stride(0), q.stride(1), _ptr(kv_cache), kv_cache.shape[0],
                                               _ptr(block_table), _row_stride(block_table), block_table.shape[1], at,
@@ -1139,6 +1137,188 @@ def paged_prefill_attention_window(q: torch.Tensor, kv_cache: torch.Tensor, bloc
                                               _stream())
     check(rc, "abkv_paged_prefill_attn_window")
     return out, lse
+
+
+def _check_step(q, kv_cache, block_table, seq_lens, max_pages, split_pages, out, lse):
+    """Checks of a decode step's arguments but their device; (sequences, bound on their pages)."""
+    _check_paged(q, kv_cache, block_table)
+    B, W = q.shape[0], block_table.shape[1]
+    _require(block_table.shape[0] >= B and B <= 65535, "block_table must have a row per sequence (at most 65535)")
+    _require(seq_lens.dtype == torch.int32 and seq_lens.dim() == 1 and seq_lens.numel() >= B and seq_lens.is_contiguous(),
+             "seq_lens must be contiguous int32 [B]")
+    _require(0 < split_pages <= 64 and split_pages % 2 == 0, "split_pages must be an even number in [2, 64]")
+    max_pages = W if max_pages is None else int(max_pages)
+    _require(0 < max_pages <= W, "max_pages must be in [1, block_table width]")
+    if out is not None:
+        _check_rows("out", out, torch.bfloat16, (B, HEADS_Q, HEAD_DIM))
+    _require(lse is None or (lse.dtype == torch.float32 and lse.is_contiguous() and lse.numel() >= B * HEADS_Q),
+             "lse must be contiguous fp32 [B, 32]")
+    return B, max_pages
+
+
+def _take_workspace(workspace, need: int, device):
+    """(workspace, its bytes): the caller's, or one for this call."""
+    if need == 0:
+        return None, 0
+    if workspace is None:
+        return torch.empty(need, dtype=torch.uint8, device=device), need
+    nbytes = workspace.numel() * workspace.element_size()
+    _require(nbytes >= need and workspace.is_contiguous() and workspace.data_ptr() % 16 == 0,
+             f"workspace must be {need} contiguous, 16-byte aligned bytes")
+    _check_device(workspace)
+    return workspace, nbytes
+
+
+def decode_window_workspace(num_seqs: int, max_pages: int, window: int, sinks: int = 0,
+                            split_pages: int = DEFAULT_SPLIT_PAGES, device=None) -> torch.Tensor | None:
+    """Workspace for :func:`decode_attention_window` (None when no sequence can need a second split)."""
+    n = lib().abkv_decode_window_workspace_size(num_seqs, max_pages, split_pages, *_check_window(window, sinks))
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+
+
+def decode_attention_window(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                            window: int, sinks: int = 0, scale: float | None = None, max_pages: int | None = None,
+                            out: torch.Tensor | None = None, lse: torch.Tensor | None = None,
+                            split_pages: int = DEFAULT_SPLIT_PAGES, workspace: torch.Tensor | None = None):
+    """Decode attention of one layer under a sliding window with sinks: a sequence's token sees rows
+    [n - ``window``, n) and [0, ``sinks``) of its n = seq_lens[b] rows, and only their pages are read.
+
+    Arguments and results as :func:`decode_attention` (bf16 only): (out [B, 32, 128] bf16, lse [B, 32] fp32 or None).
+    """
+    window, sinks = _check_window(window, sinks)
+    B, max_pages = _check_step(q, kv_cache, block_table, seq_lens, max_pages, split_pages, out, lse)
+    _check_device(q, kv_cache, block_table, seq_lens, out, lse)
+    if out is None:
+        out = torch.empty((B, HEADS_Q, HEAD_DIM), dtype=torch.bfloat16, device=q.device)
+    need = lib().abkv_decode_window_workspace_size(B, max_pages, split_pages, window, sinks)
+    workspace, ws_bytes = _take_workspace(workspace, need, q.device)
+    scale = default_scale() if scale is None else float(scale)
+    rc = lib().abkv_decode_attn_window(_ptr(q), q.stride(0), q.stride(1), _ptr(kv_cache), kv_cache.shape[0],
+                                       _ptr(block_table), _row_stride(block_table), _ptr(seq_lens), B, max_pages,
+                                       split_pages, window, sinks, scale, _ptr(out), out.stride(0), out.stride(1), _ptr(lse),
+                                       _ptr(workspace), ws_bytes, _stream())
+    check(rc, "abkv_decode_attn_window")
+    return out, lse
+
+
+# -- a cache bounded by weight: scores and eviction ----------------------------------------------------------------------
+def _check_scores(scores: torch.Tensor, B: int, rows: int) -> None:
+    _require(scores.dtype == torch.float32 and scores.dim() == 3 and scores.shape[0] >= B and scores.shape[1] == HEADS_KV
+             and scores.shape[2] >= rows and scores.stride(2) == 1,
+             f"scores must be fp32 [B, {HEADS_KV}, rows] with contiguous rows, a row for each of the {rows} slots")
+    sb, sh = scores.stride()[:2]
+    _require(sh >= rows and (scores.shape[0] <= 1 or sb >= 7 * sh + rows or (sb >= rows and sh >= (scores.shape[0] - 1) * sb
+                                                                             + rows)), "scores must not share memory")
+
+
+def decode_scored_workspace(num_seqs: int, max_pages: int, split_pages: int = DEFAULT_SPLIT_PAGES,
+                            device=None) -> torch.Tensor:
+    """Workspace for :func:`decode_attention_scored`."""
+    return torch.empty(lib().abkv_decode_scored_workspace_size(num_seqs, max_pages, split_pages), dtype=torch.uint8,
+                       device=device)
+
+
+def decode_attention_scored(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                            scores: torch.Tensor, scale: float | None = None, max_pages: int | None = None,
+                            out: torch.Tensor | None = None, lse: torch.Tensor | None = None,
+                            split_pages: int = DEFAULT_SPLIT_PAGES, workspace: torch.Tensor | None = None):
+    """:func:`decode_attention` (bf16 only) that also adds the step's attention weights to the rows' scores:
+    scores[b, h, row] += the weights of KV head h's four query heads, for rows below seq_lens[b].
+
+    ``scores`` [B, 8, rows] fp32, a row for each of the 16 * ``max_pages`` slots (zero for a new sequence), is updated in
+    place; each score has one owner, so equal calls give equal bits. Returns (out [B, 32, 128] bf16, lse or None).
+    """
+    B, max_pages = _check_step(q, kv_cache, block_table, seq_lens, max_pages, split_pages, out, lse)
+    _check_scores(scores, B, max_pages * PAGE)
+    _check_device(q, kv_cache, block_table, seq_lens, scores, out, lse)
+    if out is None:
+        out = torch.empty((B, HEADS_Q, HEAD_DIM), dtype=torch.bfloat16, device=q.device)
+    need = lib().abkv_decode_scored_workspace_size(B, max_pages, split_pages)
+    workspace, ws_bytes = _take_workspace(workspace, need, q.device)
+    scale = default_scale() if scale is None else float(scale)
+    rc = lib().abkv_decode_attn_scored(_ptr(q), q.stride(0), q.stride(1), _ptr(kv_cache), kv_cache.shape[0],
+                                       _ptr(block_table), _row_stride(block_table), _ptr(seq_lens), B, max_pages,
+                                       split_pages, scale, _ptr(scores), scores.stride(0), scores.stride(1), _ptr(out),
+                                       out.stride(0), out.stride(1), _ptr(lse), _ptr(workspace), ws_bytes, _stream())
+    check(rc, "abkv_decode_attn_scored")
+    return out, lse
+
+
+def paged_prefill_scores(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, q_start, kv_start,
+                         lse: torch.Tensor, scores: torch.Tensor, scale: float | None = None) -> None:
+    """Add the attention weights of prompt queries to the rows' scores: scores[r, h, j] += sum over request r's queries that
+    see row j, and KV head h's four query heads, of exp(scale q.k - lse).
+
+    Queries as :func:`paged_prefill_attention` takes causal chunks (q [T, 32, 128] bf16, host q_start [R + 1] and kv_start
+    [R]); ``lse`` [T, 32] fp32: what that call left for them (rows with -inf add nothing). To weigh by a prompt's last
+    queries only, pass those alone with their kv_start. ``scores`` [R, 8, rows] fp32 is updated in place, one owner a score.
+    """
+    _check_paged(q, kv_cache, block_table)
+    _require(lse.dtype == torch.float32 and lse.is_contiguous() and tuple(lse.shape) == (q.shape[0], HEADS_Q),
+             "lse must be contiguous fp32 [T, 32]")
+    _check_scores(scores, len(kv_start), block_table.shape[1] * PAGE)
+    plan = _chunk_plan(q, block_table, q_start, kv_start, lambda n, p: np.arange(0, n + p if n else 0, 64))
+    _check_device(q, kv_cache, block_table, lse, scores)
+    if plan is None:
+        return
+    tiles, R = plan[2].size, len(kv_start)
+    meta = _upload(plan, q.device)
+    at = meta.data_ptr()
+    scale = default_scale() if scale is None else float(scale)
+    rc = lib().abkv_paged_prefill_scores(_ptr(q), q.stride(0), q.stride(1), _ptr(kv_cache), kv_cache.shape[0],
+                                         _ptr(block_table), _row_stride(block_table), block_table.shape[1], at,
+                                         at + 4 * (R + 1), at + 4 * (2 * R + 1), at + 4 * (2 * R + 1 + tiles), tiles,
+                                         _ptr(lse), _ptr(scores), scores.stride(0), scores.stride(1), scale, _stream())
+    check(rc, "abkv_paged_prefill_scores")
+
+
+def kv_evict(layer_caches, block_table: torch.Tensor, seq_lens: torch.Tensor, scores: torch.Tensor,
+             positions: torch.Tensor, num_tokens: torch.Tensor, budget: int, sinks: int = 0, recent: int = 0,
+             max_pages: int | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Evict the rows that weigh least from up to 16 layer caches, in place. Returns the new lengths [B] int32.
+
+    Per (layer, sequence, KV head) of n = seq_lens[b] rows, min(n, ``budget``) are kept: rows of the first ``sinks`` and the
+    last ``recent`` of the num_tokens[b] tokens, then the highest scores (ties: the lowest row; NaN below every number). Kept
+    rows past the new length move to the evicted rows below it, both in ascending order (the rows' order means nothing to
+    attention; at most as many rows move as are evicted), with their K and V, score and position; the rows behind get score 0
+    and position -1. Sequences within the budget are left as they are.
+
+    ``scores`` fp32 and ``positions`` int32 [L, B, 8, rows], contiguous, a row for each of the 16 * ``max_pages`` slots.
+    ``positions`` hold each row's token index; -1 (also what a new sequence starts with) marks rows appended since the last
+    eviction: their index is num_tokens[b] - (n - row). ``seq_lens`` and ``num_tokens`` [B] int32. The sequences' pages must
+    be their own. ``max_pages`` (default: the table's width, at most 16384) bounds ceil(seq_len / 16).
+    """
+    L, W = len(layer_caches), block_table.shape[1] if block_table.dim() == 2 else 0
+    budget, sinks, recent = int(budget), int(sinks), int(recent)
+    _require(1 <= budget <= _MAX_INT and sinks >= 0 and recent >= 0 and sinks + recent <= budget,
+             "budget must be >= 1 and hold the sinks and the recent rows")
+    _require(block_table.dtype == torch.int32 and W > 0 and block_table.stride(1) == 1,
+             "block_table must be int32 [B, W] with contiguous rows")
+    B = seq_lens.numel()
+    for name, t in (("seq_lens", seq_lens), ("num_tokens", num_tokens)):
+        _require(t.dtype == torch.int32 and tuple(t.shape) == (B,) and t.is_contiguous(), f"{name} must be contiguous int32 [B]")
+    _require(block_table.shape[0] >= B, "block_table must have a row per sequence")
+    max_pages = W if max_pages is None else int(max_pages)
+    _require(0 < max_pages <= min(W, 16384), "max_pages must be in [1, block_table width], at most 16384")
+    for name, t, dt in (("scores", scores, torch.float32), ("positions", positions, torch.int32)):
+        _require(t.dtype == dt and t.dim() == 4 and tuple(t.shape[:3]) == (L, B, HEADS_KV)
+                 and t.shape[3] >= max_pages * PAGE and t.is_contiguous(),
+                 f"{name} must be contiguous {dt} [{L}, {B}, {HEADS_KV}, rows] with a row for each of the "
+                 f"{max_pages * PAGE} slots")
+    _require(scores.shape == positions.shape, "scores and positions must have the same shape")
+    _require(len({c.data_ptr() for c in layer_caches}) == L, "a layer cache may be given once")
+    _check_device(block_table, seq_lens, num_tokens, scores, positions, *layer_caches)
+    arr, num_pages = _layer_ptrs(layer_caches)
+    _require(num_pages > 0, "the layer caches must hold at least one page")
+    out = torch.empty_like(seq_lens)
+    if B == 0:
+        return out
+    workspace, ws_bytes = _take_workspace(workspace, lib().abkv_kv_evict_workspace_size(L, B, max_pages), scores.device)
+    rc = lib().abkv_kv_evict(arr, L, num_pages, _ptr(block_table), _row_stride(block_table), _ptr(seq_lens), B, max_pages,
+                             _ptr(scores), _ptr(positions), scores.shape[3], _ptr(num_tokens), budget, sinks, recent,
+                             _ptr(out), _ptr(workspace), ws_bytes, _stream())
+    check(rc, "abkv_kv_evict")
+    return out
 
 
 def default_scale() -> float:

@@ -470,6 +470,56 @@ int abkv_paged_prefill_attn_window(const void* q, long q_stride_tok, long q_stri
                                    const int32_t* tile_q0, int num_tiles, int window, int sinks, float scale, void* out,
                                    long out_stride_tok, long out_stride_head, float* lse, abkv_stream_t stream);
 
+/* One new token per sequence over the paged cache under the window: as abkv_decode_attn, but of a sequence of n rows only
+ * the pages of rows [n - window, n) and [0, sinks) are read. split_pages splits those pages; workspace:
+ * abkv_decode_window_workspace_size bytes (0: none needed). num_seqs <= 65535. */
+size_t abkv_decode_window_workspace_size(int num_seqs, int max_pages_per_seq, int split_pages, int window, int sinks);
+int abkv_decode_attn_window(const void* q, long q_stride_seq, long q_stride_head, const void* kv_cache, int num_pages,
+                            const int32_t* block_table, long block_table_stride, const int32_t* seq_lens, int num_seqs,
+                            int max_pages_per_seq, int split_pages, int window, int sinks, float scale, void* out,
+                            long out_stride_seq, long out_stride_head, float* lse, void* workspace,
+                            size_t workspace_bytes, abkv_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------------------------
+ * A cache bounded by weight: every row of a (sequence, KV head) carries the attention weight it has received, summed over
+ * queries and the head's four query heads, and the rows that weigh least are evicted. (An uncompressed baseline beside the
+ * code rows; the reference's generator has eviction baselines on a contiguous cache, abridgekv/gen_compress.py:611-646.)
+ *
+ * scores: fp32 [num_seqs, 8, rows] (element strides, rows contiguous, at least 16 * max_pages_per_seq of them), row = physical
+ * slot. Zero for a new sequence; abkv_kv_evict keeps them with the rows.
+ *
+ * abkv_decode_attn_scored: abkv_decode_attn, and scores[b][h][row] += sum of the step's weights for rows [0, seq_lens[b])
+ * (others are left alone). workspace: abkv_decode_scored_workspace_size bytes, 16-byte aligned; num_seqs <= 65535. */
+size_t abkv_decode_scored_workspace_size(int num_seqs, int max_pages_per_seq, int split_pages);
+int abkv_decode_attn_scored(const void* q, long q_stride_seq, long q_stride_head, const void* kv_cache, int num_pages,
+                            const int32_t* block_table, long block_table_stride, const int32_t* seq_lens, int num_seqs,
+                            int max_pages_per_seq, int split_pages, float scale, float* scores, long scores_stride_seq,
+                            long scores_stride_head, void* out, long out_stride_seq, long out_stride_head, float* lse,
+                            void* workspace, size_t workspace_bytes, abkv_stream_t stream);
+/* The weights of prompt queries: scores[r][h][j] += sum over request r's queries i (rows q_start[r] .. q_start[r + 1] - 1 of
+ * q [T, 32, 128] bf16 at positions kv_start[r] + i) with j <= position, and h's query heads, of exp(scale q.k - lse).
+ * lse [T, 32]: what the queries' attention over the same rows left (a row with -inf adds nothing). tile_req / tile_k0
+ * [num_tiles]: request and first key (a multiple of 64) of every 64-key tile of rows [0, kv_start + queries). */
+int abkv_paged_prefill_scores(const void* q, long q_stride_tok, long q_stride_head, const void* kv_cache, int num_pages,
+                              const int32_t* block_table, long block_table_stride, int table_width, const int32_t* q_start,
+                              const int32_t* kv_start, const int32_t* tile_req, const int32_t* tile_k0, int num_tiles,
+                              const float* lse, float* scores, long scores_stride_req, long scores_stride_head, float scale,
+                              abkv_stream_t stream);
+/* Evict from up to 16 layer caches of one KV-cache group. Per (layer, sequence, KV head) of n = seq_lens[b] rows (clamped to
+ * 16 * max_pages_per_seq) m = min(n, budget) are kept: rows of tokens below `sinks` and from num_tokens[b] - recent on, then
+ * the highest scores (ties: the lowest row; NaN below every number). The kept rows at or past m move to the evicted rows below
+ * m, both in ascending order, with their K and V, score and position; rows m .. n - 1 get score 0 and position -1; out_lens[b]
+ * = m. scores, positions: [num_layers, num_seqs, 8, rows_stride]. positions hold each row's token index, or -1 for rows
+ * appended since the last eviction, whose index is num_tokens[b] - (n - row); kept rows get theirs written. A sequence within
+ * the budget is left as it is. The sequences' pages must be their own (a page shared by two sequences would be rewritten under
+ * the other). sinks + recent <= budget; at most 16384 pages a sequence. workspace: abkv_kv_evict_workspace_size bytes (0 up to
+ * 2048 pages). out_lens must not be seq_lens. */
+size_t abkv_kv_evict_workspace_size(int num_layers, int num_seqs, int max_pages_per_seq);
+int abkv_kv_evict(void* const* layer_caches, int num_layers, int num_pages, const int32_t* block_table,
+                  long block_table_stride, const int32_t* seq_lens, int num_seqs, int max_pages_per_seq, float* scores,
+                  int32_t* positions, long rows_stride, const int32_t* num_tokens, int budget, int sinks, int recent,
+                  int32_t* out_lens, void* workspace, size_t workspace_bytes, abkv_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
