@@ -112,10 +112,12 @@ class WindowMask:
 
 
 class _WindowAttention(torch.autograd.Function):
-    """The sliding-window kernels and their backward (abkv_window_attn / _bwd)."""
+    """The sliding-window kernels and their backward (abkv_window_attn / _bwd): query, key and value [B, heads, S, 128] as the
+    layers hand them, out [B, S, 32, 128]."""
 
     @staticmethod
-    def forward(ctx, q, k, v, mask: WindowMask, scale: float):
+    def forward(ctx, query, key, value, mask: WindowMask, scale: float):
+        q, k, v = query.transpose(1, 2), key.transpose(1, 2), value.transpose(1, 2)
         lse = None
         if any(ctx.needs_input_grad[:3]):
             if q.dtype != torch.bfloat16:
@@ -123,20 +125,21 @@ class _WindowAttention(torch.autograd.Function):
             lse = torch.empty((q.shape[0], ops.HEADS_Q, q.shape[1]), dtype=torch.float32, device=q.device)
         out, _ = ops.window_attention(q, k, v, mask.window, mask.sinks, seq_lens=mask.seq_lens, scale=scale, lse=lse)
         if lse is not None:
-            ctx.save_for_backward(q, k, v, out, lse, mask.seq_lens)
-            ctx.window, ctx.sinks, ctx.scale = mask.window, mask.sinks, scale
+            ctx.save_for_backward(query, key, value, out, lse, mask.seq_lens)
+            ctx.mask, ctx.scale = mask, scale
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out):
-        q, k, v, out, lse, seq_lens = ctx.saved_tensors
-        g = grad_out
-        if g.stride(-1) != 1 or any(x % 8 for x in g.stride()[:-1]) or g.data_ptr() % 16:
-            g = g.contiguous()
-        dq, dk, dv = ops.window_attention_backward(q, k, v, out, lse, g, ctx.window, ctx.sinks, seq_lens=seq_lens,
+        query, key, value, out, lse, seq_lens = ctx.saved_tensors
+        st = grad_out.stride()
+        if st[3] != 1 or (st[0] | st[1] | st[2]) % 8 or grad_out.data_ptr() % 16:
+            grad_out = grad_out.contiguous()
+        dq, dk, dv = ops.window_attention_backward(query.transpose(1, 2), key.transpose(1, 2), value.transpose(1, 2), out,
+                                                   lse, grad_out, ctx.mask.window, ctx.mask.sinks, seq_lens=seq_lens,
                                                    scale=ctx.scale)
-        return dq, dk, dv, None, None
+        return dq.transpose(1, 2), dk.transpose(1, 2), dv.transpose(1, 2), None, None
 
 
 def masked_attention_forward(module, query, key, value, attention_mask, scaling=None, dropout=0.0, **kwargs):
@@ -154,9 +157,7 @@ def masked_attention_forward(module, query, key, value, attention_mask, scaling=
         raise NotImplementedError("a sliding-window layer takes no other mask")
     scale = ops.default_scale() if scaling is None else float(scaling)
     if isinstance(attention_mask, WindowMask):
-        out = _WindowAttention.apply(query.transpose(1, 2), key.transpose(1, 2), value.transpose(1, 2), attention_mask,
-                                     scale)
-        return out, None
+        return _WindowAttention.apply(query, key, value, attention_mask, scale), None
     if not isinstance(attention_mask, CompressMask):
         raise TypeError(f"{ATTN_IMPLEMENTATION} attention needs a CompressMask, a WindowMask or None, got "
                         f"{type(attention_mask).__name__}")

@@ -614,7 +614,7 @@ __global__ __launch_bounds__(256, kKeys == 16 ? 3 : 2) void attn_f32_rows_kernel
 // Attention under a sliding window with sinks over whole prompts: the row kernel's workgroup, 16 query rows of a KV head,
 // over the stages its rows see.
 template <int kKeys>
-__global__ __launch_bounds__(256, 2) void attn_f32_window_kernel(F32Args a) {
+__global__ __launch_bounds__(256, kKeys == 16 ? 3 : 2) void attn_f32_window_kernel(F32Args a) {
   __shared__ __attribute__((aligned(16))) float lds[4 * kKeys * kHeadDim];
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, m16 = lane & 15, g = lane >> 4;
@@ -867,7 +867,7 @@ int abkv_window_attn_f32(const float* q, long q_stride_b, long q_stride_s, long 
   a.lse = lse;
   const unsigned grid = f32_grid(((long)seq_len + kF32Rows - 1) / kF32Rows * batch);
   if (grid == 0) return (int)hipErrorInvalidValue;
-  hipLaunchKernelGGL((attn_f32_window_kernel<32>), dim3(grid), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL((attn_f32_window_kernel<16>), dim3(grid), dim3(256), 0, stream, a);
   return (int)hipGetLastError();
 }
 

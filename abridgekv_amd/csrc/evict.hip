@@ -1,119 +1,172 @@
 // What a cache bounded by weight needs beside its attention (gfx950): the attention weights of a prompt's queries added up
 // per cached row, and the eviction of the rows that weigh least. (A decode step's weights: decode_attn.hip.)
-#include "common.h"
+#include "attn_tile.h"
 
 namespace abkv {
 
 // ---------------------------------------------------------------------------------------------------------------------
 // scores[r][KV head h][key j] += sum over h's four query heads u and the request's queries i >= j of
 //                                exp(scale q_iu . k_jh - lse_iu),      query i at position kv_start[r] + i.
-// A workgroup takes 64 keys of a KV head, a wave one of the four query heads (kPhases waves take its query rows in turn).
-// The wave keeps its 64 keys in registers as the MFMA's first operand (64 VGPRs), so a 16-row query operand, loaded from
-// global memory straight into operand registers, feeds 16 MFMAs: no LDS, no barrier in the loop. S^T = K . Q^T has a query
-// per lane column, so lse is one value a lane and the sums over queries stay in the 16 accumulator positions until the end.
-// One owner per score: no atomics, the same bits every time. Bound by the exponentials: per 16 x 64 pairs 256 cycles of
-// v_exp_f32 and 128 of FMAs and adds beside 256 of MFMA.
+// A wave keeps 32 keys of one query head in registers as the MFMA's first operand. S^T = K . Q^T has a query per lane column:
+// lse is one value a lane, and the sums over queries stay in the 8 accumulator positions until the end. A workgroup's 16 waves
+// are the KV head's four query heads by four groups of 32 keys (kTiles = 2), or by two groups at alternate steps (kTiles = 1,
+// where the longest workgroup would bound the launch). 32 query rows of the four heads at a time come into triple-buffered LDS
+// by DMA. One owner per score: no atomics, the same bits every time.
+// Bound by issue: a 16 x 64 step costs 419 cycles of MFMA, FMA, exponential and addition (measured alone, overlapped), here 640
+// with the operands' reads and the barriers. 1500 rows and 2048 behind 2048: 94 us a call, 650 TFLOP/s of visible pairs. Tried:
+// query rows straight into operand registers 166 us (64 bytes of each of 16 rows an instruction; without those loads 88); 64
+// keys a wave at two waves a SIMD, its three stages interleaved by hand, 95, with a step a barrier more 99.
 struct PromptScoreArgs {
   const __bf16* q;  long q_st, q_sh;           // [T, 32, 128]
   const __bf16* kv; int num_pages;             // [pages, 2, 16, 8, 128]
   const int32_t* block_table; long bt_stride; int bt_width;
   const int32_t* q_start;                      // [R + 1]
   const int32_t* kv_start;                     // [R]
-  const int32_t* tile_req;                     // [tiles] request of each 64-key tile
+  const int32_t* tile_req;                     // [tiles] request of each tile of 64 * kTiles keys
   const int32_t* tile_k0;                      // [tiles] its first key
   const float* lse;                            // [T, 32] natural log
   float* scores;  long s_sb, s_sh;             // [R, 8, rows]
   float scale_log2;
 };
 
-constexpr int kScorePhases = 2;
-__global__ __launch_bounds__(256 * kScorePhases) void prompt_scores_kernel(PromptScoreArgs a) {
-  __shared__ float sums[4 * kScorePhases][kBN];
+// Sum over a row of 16 lanes, in each of them (DPP: no LDS).
+__device__ __forceinline__ float sum16(float v) {
+  auto add = [](float x, int y) { return x + __int_as_float(y); };
+  v = add(v, __builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), 0xB1, 0xF, 0xF, false));   // quad_perm 1,0,3,2
+  v = add(v, __builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), 0x4E, 0xF, 0xF, false));   // quad_perm 2,3,0,1
+  v = add(v, __builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), 0x141, 0xF, 0xF, false));  // row_half_mirror
+  return add(v, __builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), 0x140, 0xF, 0xF, false));   // row_mirror
+}
+
+constexpr int kScoreQ = 32;                                  // query rows of an iteration
+constexpr int kScoreWaves = 16;
+template <int kTiles>
+__global__ __launch_bounds__(64 * kScoreWaves) void prompt_scores_kernel(PromptScoreArgs a) {
+  constexpr int kSubs = 2 * kTiles, kPhases = kScoreWaves / kGroup / kSubs;
+  constexpr int kElems = kGroup * kScoreQ * kHeadDim, kRows = kScoreQ * kGroup;
+  __shared__ __attribute__((aligned(16))) __bf16 Q0[kElems], Q1[kElems], Q2[kElems];
+  __shared__ __attribute__((aligned(16))) float L0[kRows], L1[kRows], L2[kRows];
+  __shared__ float sums[kScoreWaves][32];
+  __bf16* const Qb[3] = {Q0, Q1, Q2};
+  float* const Lb[3] = {L0, L1, L2};
   const int kvh = blockIdx.x % kHeadsKV, tile = blockIdx.x / kHeadsKV;
-  const int r = a.tile_req[tile], k0 = a.tile_k0[tile];
+  const int r = a.tile_req[tile], first_key = a.tile_k0[tile];
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, m16 = lane & 15, j = lane >> 4;
   const int t0 = a.q_start[r], nq = a.q_start[r + 1] - t0, kv0 = a.kv_start[r];
   const int n_keys = kv0 + nq;
-  const int head = kvh * kGroup + (w & 3);
+  const int u = w & 3, sub = w >> 2 & (kSubs - 1), phase = w / (kGroup * kSubs);
+  const int k0 = first_key + 32 * sub;                       // this wave's keys
 
-  bf16x8 kop[4][4];
+  // iteration n: query rows 32n .. 32n + 31 of head h in LDS rows 32h .. (a wave's two DMAs: eight rows), and their lse as
+  // [row][head] (eight waves write the same 16 rows' values). A lane's offset from the iteration's first row does not change,
+  // so an iteration costs scalar arithmetic only; the last one re-reads the request's last row past its end (weight 0), and
+  // so do the iterations issued past the last.
+  const int last_iter = (nq - 1) / kScoreQ;
+  const int half = w & 1, lrow = 16 * half + (lane >> 2);
+  auto offset = [&](int i, int limit) {                      // bytes to the lane's piece of DMA i, rows up to `limit`
+    const int row = 8 * w + 4 * i + j;                       // LDS row: head row / 32, query row % 32
+    return (unsigned)((min(row & (kScoreQ - 1), limit) * (int)a.q_st + row / kScoreQ * (int)a.q_sh + 8 * (m16 ^ (row & 15))) * 2);
+  };
+  unsigned off[2] = {offset(0, kScoreQ - 1), offset(1, kScoreQ - 1)}, off_l = (lrow * kHeadsQ + (lane & 3)) * 4;
+  const char* const q_base = reinterpret_cast<const char*>(a.q + (long)t0 * a.q_st + (long)kvh * kGroup * a.q_sh);
+  const char* const l_base = reinterpret_cast<const char*>(a.lse + (long)t0 * kHeadsQ + kvh * kGroup);
+  auto issue = [&](int n, __bf16* qb, float* lb) {
+    if (n >= last_iter) {                                    // (uniform, at the end of the walk)
+      n = last_iter;
+      const int limit = nq - 1 - kScoreQ * n;
+      off[0] = offset(0, limit);
+      off[1] = offset(1, limit);
+      off_l = (min(lrow, limit) * kHeadsQ + (lane & 3)) * 4;
+    }
+    const char* const qp = q_base + (long)n * kScoreQ * a.q_st * 2;
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const int key = k0 + 16 * t + m16;
-    const int pg = min((k0 >> 4) + t, a.bt_width - 1);
-    const int page = min(max(a.block_table[(long)r * a.bt_stride + pg], 0), a.num_pages - 1);
-    const __bf16* row = a.kv + (long)page * kPageElems + m16 * kSlotElems + kvh * kHeadDim;
+    for (int i = 0; i < 2; ++i)
+      __builtin_amdgcn_global_load_lds((const void*)(qp + off[i]), ABKV_LDS(qb + 4 * (2 * w + i) * kHeadDim), 16, 0, 0);
+    __builtin_amdgcn_global_load_lds((const void*)(l_base + (long)n * kScoreQ * kHeadsQ * 4 + off_l), ABKV_LDS(lb + 64 * half),
+                                     4, 0, 0);
+  };
+  bf16x8 kop[2][4];
+  floatx4 sum[2] = {floatx4{0.f, 0.f, 0.f, 0.f}, floatx4{0.f, 0.f, 0.f, 0.f}};
+  auto work = [&](int row0, const __bf16* qb, const float* lb) {
+    const int in = row0 & (kScoreQ - 1);                     // the step's first row in the iteration's rows
+    const float l = lb[(in + m16) * kGroup + u];
+    // rows past the request and rows that see nothing weigh 0
+    const float l2 = row0 + m16 < nq && l > -INFINITY ? l * 1.4426950408889634f : INFINITY;
+    floatx4 s[2] = {floatx4{0.f, 0.f, 0.f, 0.f}, floatx4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      u32x4 x = *reinterpret_cast<const u32x4*>(row + 8 * (4 * i + j));
-      if (key >= n_keys) x = u32x4{0, 0, 0, 0};              // stale bytes
-      kop[t][i] = __builtin_bit_cast(bf16x8, x);
+      const bf16x8 qop = __builtin_bit_cast(bf16x8, lds16(qb, kScoreQ * u + in + m16, 4 * i + j));
+#pragma unroll
+      for (int t = 0; t < 2; ++t) s[t] = mfma16x16x32(kop[t][i], qop, s[t]);
     }
-  }
-  floatx4 sum[4];
+    const int before = kv0 + row0 + m16 - k0;                // keys 0 .. before of the wave's are seen
+    if (kv0 + row0 >= k0 + 31) {                             // (uniform) all of them by all rows
 #pragma unroll
-  for (int t = 0; t < 4; ++t) sum[t] = floatx4{0.f, 0.f, 0.f, 0.f};
-
-  const int steps = (nq + 15) >> 4;
-  const int first = (max(k0 - kv0, 0) >> 4) + (w >> 2);      // the first query rows that see a key of the tile
-  const __bf16* qh = a.q + (long)head * a.q_sh + 8 * j;
-  u32x4 qn[4];
-  float ln = 0.f;
-  auto load = [&](int step) {
-    const int tok = t0 + min(16 * step + m16, nq - 1);
-    const __bf16* p = qh + (long)tok * a.q_st;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) qn[i] = *reinterpret_cast<const u32x4*>(p + 32 * i);
-    ln = a.lse[(long)tok * kHeadsQ + head];
-  };
-  if (first < steps) load(first);
-  for (int step = first; step < steps; step += kScorePhases) {
-    bf16x8 qop[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) qop[i] = __builtin_bit_cast(bf16x8, qn[i]);
-    const int qi = 16 * step + m16;
-    // rows past the request and rows that see nothing weigh 0
-    const float l2 = qi < nq && ln > -INFINITY ? ln * 1.4426950408889634f : INFINITY;
-    if (step + kScorePhases < steps) load(step + kScorePhases);
-    floatx4 s[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) s[t] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int t = 0; t < 4; ++t) s[t] = mfma16x16x32(kop[t][i], qop[i], s[t]);
-    const int before = kv0 + qi - k0;                        // keys 0 .. before of the tile are seen
-    if (kv0 + 16 * step >= k0 + kBN - 1) {                   // (uniform) all of them by all rows
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e) sum[t][e] += fast_exp2(fmaf(s[t][e], a.scale_log2, -l2));
     } else {
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float p = fast_exp2(fmaf(s[t][e], a.scale_log2, -l2));
           sum[t][e] += 16 * t + 4 * j + e <= before ? p : 0.f;
         }
     }
+  };
+  // the first query rows that see a key of the workgroup (a tile lies below n_keys, so some row does)
+  int n = max(first_key - kv0, 0) / kScoreQ;
+  const int end = last_iter + 1;
+  if (n < end) {                                             // (uniform)
+    // the keys through the third buffer: loaded straight into operand registers, the four heads' waves read them four times
+    const PagedRows rows{a.kv + kvh * kHeadDim, a.block_table + (long)r * a.bt_stride, a.bt_width, a.num_pages};
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+      issue_half<kScoreWaves, false>(rows, rows.template src<1>(min(first_key + kBN * t, n_keys - 1), w, n_keys), n_keys,
+                                     Q2 + t * kTileElems, w, lane);
+    issue(n, Q0, L0);
+    issue(n + 1, Q1, L1);
+    __asm__ volatile("s_waitcnt vmcnt(6)" ::: "memory");     // the keys; two iterations of three loads stay in flight
+    __builtin_amdgcn_s_barrier();
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) kop[t][i] = __builtin_bit_cast(bf16x8, lds16(Q2, 32 * sub + 16 * t + m16, 4 * i + j));
+    // Every iteration waits for this wave's three DMAs of it (the next one's stay in flight), then for the other waves', who
+    // are then also done reading the buffer that the iteration after next takes.
+    auto step = [&](auto slot_c) -> bool {
+      constexpr int sl = decltype(slot_c)::value;
+      __asm__ volatile("s_waitcnt vmcnt(3) lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      issue(n + 2, Qb[(sl + 2) % 3], Lb[(sl + 2) % 3]);
+#pragma unroll
+      for (int i = 0; i < 2; i += kPhases) work(kScoreQ * n + 16 * (phase + i), Qb[sl], Lb[sl]);
+      return ++n < end;
+    };
+    for (;;) {
+      if (!step(Slot<0>{})) break;
+      if (!step(Slot<1>{})) break;
+      if (!step(Slot<2>{})) break;
+    }
+    __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");     // no DMA may outlive the workgroup's LDS
   }
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
+  for (int t = 0; t < 2; ++t)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      float x = sum[t][e];
-#pragma unroll
-      for (int m = 1; m < 16; m <<= 1) x += __shfl_xor(x, m, 64);
+      const float x = sum16(sum[t][e]);                      // over the query columns
       if (m16 == 0) sums[w][16 * t + 4 * j + e] = x;
     }
   __syncthreads();
-  const int key = k0 + threadIdx.x;
-  if (threadIdx.x < kBN && key < n_keys) {
+  const int tid = threadIdx.x, key = first_key + tid;
+  if (tid < kBN * kTiles && key < n_keys) {
     float x = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4 * kScorePhases; ++i) x += sums[i][threadIdx.x];
+    for (int p = 0; p < kPhases; ++p)
+#pragma unroll
+      for (int h = 0; h < kGroup; ++h) x += sums[h + kGroup * (tid / 32 + kSubs * p)][tid & 31];
     a.scores[(long)r * a.s_sb + (long)kvh * a.s_sh + key] += x;
   }
 }
@@ -310,19 +363,21 @@ extern "C" {
 int abkv_paged_prefill_scores(const void* q, long q_stride_tok, long q_stride_head, const void* kv_cache, int num_pages,
                               const int32_t* block_table, long block_table_stride, int table_width, const int32_t* q_start,
                               const int32_t* kv_start, const int32_t* tile_req, const int32_t* tile_k0, int num_tiles,
-                              const float* lse, float* scores, long scores_stride_req, long scores_stride_head, float scale,
+                              int tile_keys, const float* lse, float* scores, long scores_stride_req, long scores_stride_head, float scale,
                               hipStream_t stream) {
   using namespace abkv;
   if (num_tiles <= 0) return 0;
   if (q == nullptr || kv_cache == nullptr || block_table == nullptr || q_start == nullptr || kv_start == nullptr ||
-      tile_req == nullptr || tile_k0 == nullptr || lse == nullptr || scores == nullptr || num_pages <= 0 || table_width <= 0)
+      tile_req == nullptr || tile_k0 == nullptr || lse == nullptr || scores == nullptr || num_pages <= 0 || table_width <= 0 ||
+      (tile_keys != kBN && tile_keys != 2 * kBN))
     return (int)hipErrorInvalidValue;
   const PromptScoreArgs a{static_cast<const __bf16*>(q), q_stride_tok, q_stride_head, static_cast<const __bf16*>(kv_cache),
                           num_pages, block_table, block_table_stride, table_width, q_start, kv_start, tile_req, tile_k0, lse,
                           scores, scores_stride_req, scores_stride_head, scale * 1.4426950408889634f};
   const long grid = (long)num_tiles * kHeadsKV;
-  if (grid * 256 * kScorePhases > 0xFFFFFFFFL) return (int)hipErrorInvalidValue;
-  hipLaunchKernelGGL(prompt_scores_kernel, dim3((unsigned)grid), dim3(256 * kScorePhases), 0, stream, a);
+  if (grid * 64 * kScoreWaves > 0xFFFFFFFFL) return (int)hipErrorInvalidValue;
+  if (tile_keys == kBN) hipLaunchKernelGGL(prompt_scores_kernel<1>, dim3((unsigned)grid), dim3(64 * kScoreWaves), 0, stream, a);
+  else hipLaunchKernelGGL(prompt_scores_kernel<2>, dim3((unsigned)grid), dim3(64 * kScoreWaves), 0, stream, a);
   return (int)hipGetLastError();
 }
 

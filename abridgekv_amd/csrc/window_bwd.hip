@@ -1,9 +1,9 @@
 // Backward of attention under a sliding window with sinks (gfx950): dq, dk, dv from the forward's output and lse, as
 // prefill_bwd.hip: P = exp2(S * scale * log2(e) - lse * log2(e)), dS = P o (dP - rowsum(dO o O)), dQ = scale * dS K,
 // dK = scale * dS^T Q, dV = P^T dO, dK and dV summed over the KV head's four query heads.
-//   window_bwd_prep_kernel  per (row, query head): lse2 = lse * log2(e) and D = sum_d dO * O, rows padded to whole tiles
-//                           (lse2 = +inf and D = 0 past the sequence, so that padding weighs 0)
-//   window_bwd_dq_kernel    the forward's query tiles and key walk; dQ^T += K^T dS^T
+//   window_bwd_dq_kernel    the forward's query tiles and key walk; dQ^T += K^T dS^T. Before it, each (row, query head)'s
+//                           lse2 = lse * log2(e) and D = sum_d dO * O, which it leaves for the next kernel in rows padded to
+//                           whole tiles (lse2 = +inf and D = 0 past the sequence, so that padding weighs 0)
 //   window_bwd_dkv_kernel   a workgroup per 64 keys of a KV head over the query tiles whose windows reach them: the same
 //                           count for every key tile. Keys among the sinks are seen by every later row as well: these far
 //                           query tiles are cut into parts with workgroups of their own (SinkPlan), which leave fp32 sums
@@ -32,32 +32,6 @@ struct WindowBwdArgs {
 
 constexpr int kWinSlotFloats = 2 * kBN * kHeadDim;          // dK and dV of a key tile, of one KV head
 
-__global__ __launch_bounds__(256) void window_bwd_prep_kernel(WindowBwdArgs a) {
-  // 16 lanes per (row, query head): lane c takes dims 8c .. 8c + 7 of O and dO
-  if (blockIdx.x == 0)
-    for (int i = threadIdx.x; i < a.plan.sink_tiles * a.f.B * kHeadsKV; i += 256) a.done[i] = 0;
-  const long idx = ((long)blockIdx.x * 256 + threadIdx.x) >> 4;
-  const int c = threadIdx.x & 15;
-  if (idx >= (long)a.f.B * kHeadsQ * a.Sp) return;          // uniform over the 16 lanes of a row
-  const int i = (int)(idx % a.Sp);
-  const long bh = idx / a.Sp;
-  const int h = (int)(bh % kHeadsQ), b = (int)(bh / kHeadsQ);
-  const bool in = i < window_rows(a.f, b);
-  float d = 0.f;
-  if (in) {
-    const __bf16* op = a.o + (long)b * a.o_sb + (long)i * a.o_ss + (long)h * a.o_sh;
-    const __bf16* gp = a.dout + (long)b * a.g_sb + (long)i * a.g_ss + (long)h * a.g_sh;
-    const u32x4 x = ld16g(op + 8 * c), y = ld16g(gp + 8 * c);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) d += bf16_lo(x[e]) * bf16_lo(y[e]) + bf16_hi(x[e]) * bf16_hi(y[e]);
-  }
-#pragma unroll
-  for (int m = 1; m < 16; m <<= 1) d += __shfl_xor(d, m, 64);
-  if (c != 0) return;
-  a.lse2[idx] = in ? a.lse[bh * a.f.S + i] * 1.4426950408889634f : INFINITY;
-  a.dvec[idx] = d;
-}
-
 __global__ __launch_bounds__(512, 1) void window_bwd_dq_kernel(WindowBwdArgs a) {
   constexpr int H = 2, kWaves = 8;
   __shared__ __attribute__((aligned(16))) __bf16 K0[kTileElems], K1[kTileElems], V0[kTileElems], V1[kTileElems];
@@ -75,6 +49,8 @@ __global__ __launch_bounds__(512, 1) void window_bwd_dq_kernel(WindowBwdArgs a) 
   const int hbase = H * (w & 1);
   const int qrow = q0 + 16 * (w >> 1) + m16;
   const bool seen = qrow < n;
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < a.plan.sink_tiles * f.B * kHeadsKV; i += 512) a.done[i] = 0;
   bf16x8 qop[H][4], gop[H][4];
   float l2[H], dd[H];
 #pragma unroll
@@ -82,16 +58,24 @@ __global__ __launch_bounds__(512, 1) void window_bwd_dq_kernel(WindowBwdArgs a) 
     const int head = kvh * kGroup + hbase + u, r = min(qrow, f.S - 1);
     const __bf16* qp = f.q + (long)b * f.q_sb + (long)r * f.q_ss + (long)head * f.q_sh;
     const __bf16* gp = a.dout + (long)b * a.g_sb + (long)r * a.g_ss + (long)head * a.g_sh;
+    const __bf16* op = a.o + (long)b * a.o_sb + (long)r * a.o_ss + (long)head * a.o_sh;
+    float d = 0.f;                                           // dims 8 * (4i + j) .. + 7 of the row's dot product
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      u32x4 x = ld16g(qp + 8 * (4 * i + j)), y = ld16g(gp + 8 * (4 * i + j));
-      if (!seen) x = y = u32x4{0, 0, 0, 0};
+      u32x4 x = ld16g(qp + 8 * (4 * i + j)), y = ld16g(gp + 8 * (4 * i + j)), z = ld16g(op + 8 * (4 * i + j));
+      if (!seen) x = y = z = u32x4{0, 0, 0, 0};
       qop[u][i] = __builtin_bit_cast(bf16x8, x);
       gop[u][i] = __builtin_bit_cast(bf16x8, y);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) d += bf16_lo(y[e]) * bf16_lo(z[e]) + bf16_hi(y[e]) * bf16_hi(z[e]);
     }
-    const long wi = ((long)b * kHeadsQ + head) * a.Sp + qrow;         // qrow < Sp
-    l2[u] = a.lse2[wi];
-    dd[u] = a.dvec[wi];
+    dd[u] = sum_xor32(sum_xor16(d));
+    l2[u] = seen ? a.lse[((long)b * kHeadsQ + head) * f.S + r] * 1.4426950408889634f : INFINITY;
+    if (j == 0) {
+      const long wi = ((long)b * kHeadsQ + head) * a.Sp + qrow;       // qrow < Sp
+      a.lse2[wi] = l2[u];
+      a.dvec[wi] = dd[u];
+    }
   }
   floatx4 dq[8][H];
 #pragma unroll
@@ -410,15 +394,11 @@ int abkv_window_attn_bwd(const void* q, long q_stride_b, long q_stride_s, long q
   a.dk_sb = dk_stride_b; a.dk_ss = dk_stride_s; a.dk_sh = dk_stride_h;
   a.dv = static_cast<__bf16*>(dv);
   a.dv_sb = dv_stride_b; a.dv_ss = dv_stride_s; a.dv_sh = dv_stride_h;
-  const long rows = (long)batch * kHeadsQ * a.Sp;
   const long gq = (long)f.num_q_tiles * batch * kHeadsKV;
   const long gk = (long)plan.items() * batch * kHeadsKV;
-  if (rows * 16 > 0xFFFFFFFFL - 256 || gq * 512 > 0xFFFFFFFFL || gk * 256 > 0xFFFFFFFFL) return (int)hipErrorInvalidValue;
-  hipLaunchKernelGGL(window_bwd_prep_kernel, dim3((unsigned)((rows * 16 + 255) / 256)), dim3(256), 0, stream, a);
-  hipError_t err = hipGetLastError();
-  if (err != hipSuccess) return (int)err;
+  if (gq * 512 > 0xFFFFFFFFL || gk * 256 > 0xFFFFFFFFL) return (int)hipErrorInvalidValue;
   hipLaunchKernelGGL(window_bwd_dq_kernel, dim3((unsigned)gq), dim3(512), 0, stream, a);
-  err = hipGetLastError();
+  const hipError_t err = hipGetLastError();
   if (err != hipSuccess) return (int)err;
   hipLaunchKernelGGL(window_bwd_dkv_kernel, dim3((unsigned)gk), dim3(256), 0, stream, a);
   return (int)hipGetLastError();

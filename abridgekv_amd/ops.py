@@ -978,25 +978,29 @@ _MAX_INT = (1 << 31) - 1
 
 def _check_device(*tensors) -> None:
     """All on the current GPU: the launch goes to its current stream."""
+    dev = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else None
     for t in tensors:
-        if t is not None and not (t.is_cuda and t.device.index == torch._C._cuda_getDevice()):
+        if t is not None and t.get_device() != dev:
             raise ValueError(f"tensors must be on the current GPU, got one on {t.device}")
 
 
 def _check_rows(name: str, t: torch.Tensor, dtype, shape) -> None:
     """Dense [B, S, H, 128] or [T, H, 128] rows as the tile loads take them: 16-byte aligned, and a row stride that keeps
     64 rows' offsets in 32 bits."""
-    if t.dtype != dtype or tuple(t.shape) != shape:
+    if t.dtype != dtype or t.shape != shape:
         raise ValueError(f"{name} must be {dtype} {list(shape)}, got {t.dtype} {list(t.shape)}")
-    st, per = t.stride(), 16 // t.element_size()
-    if st[-1] != 1 or t.data_ptr() % 16 or any(x % per or x < 0 for x in st[:-1]) or st[-3] >= 1 << 24:
+    st = t.stride()
+    steps = st[0] | st[1] | st[-2]
+    if st[-1] != 1 or steps % (16 // t.element_size()) or t.data_ptr() % 16 or st[-3] >= 1 << 24:
         raise ValueError(f"{name} must have contiguous, 16-byte aligned rows, got strides {st}")
 
 
 def _check_window(window, sinks) -> tuple[int, int]:
-    _require(int(window) == window and 1 <= window <= _MAX_INT, "window must be an integer >= 1")
-    _require(int(sinks) == sinks and 0 <= sinks <= _MAX_INT, "sinks must be an integer >= 0")
-    return int(window), int(sinks)
+    if type(window) is not int or type(sinks) is not int:
+        _require(int(window) == window and int(sinks) == sinks, "window and sinks must be integers")
+        window, sinks = int(window), int(sinks)
+    _require(1 <= window <= _MAX_INT and 0 <= sinks <= _MAX_INT, "window must be >= 1 and sinks >= 0")
+    return window, sinks
 
 
 def _reach(window: int, sinks: int, rows: int) -> tuple[int, int]:
@@ -1040,9 +1044,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
         out = torch.empty((B, S, HEADS_Q, HEAD_DIM), dtype=dt, device=q.device)
     scale = default_scale() if scale is None else float(scale)
     fn = lib().abkv_window_attn_f32 if dt == torch.float32 else lib().abkv_window_attn
-    rc = fn(_ptr(q), q.stride(0), q.stride(1), q.stride(2), _ptr(k), k.stride(0), k.stride(1), k.stride(2), _ptr(v),
-            v.stride(0), v.stride(1), v.stride(2), B, S, _ptr(seq_lens), window, sinks, scale, _ptr(out), out.stride(0),
-            out.stride(1), out.stride(2), _ptr(lse), _stream())
+    rc = fn(q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], B, S,
+            _ptr(seq_lens), window, sinks, scale, out.data_ptr(), *out.stride()[:3], _ptr(lse), _stream())
     check(rc, "abkv_window_attn")
     return out, lse
 
@@ -1062,19 +1065,25 @@ def window_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     _require(lse.dtype == torch.float32 and lse.is_contiguous() and tuple(lse.shape) == (B, HEADS_Q, S),
              "lse must be contiguous fp32 [B, 32, S]")
     _check_device(q, k, v, out, lse, dout, seq_lens)
-    window, sinks = _reach(window, sinks, S)
-    scale = default_scale() if scale is None else float(scale)
+    return _window_backward(q, k, v, out, lse, dout, *_reach(window, sinks, S), seq_lens,
+                            default_scale() if scale is None else float(scale))
+
+
+def _window_backward(q, k, v, out, lse, dout, window, sinks, seq_lens, scale):
+    """window_attention_backward of arguments that are checked."""
+    B, S = q.shape[:2]
     dq = torch.empty((B, S, HEADS_Q, HEAD_DIM), dtype=torch.bfloat16, device=q.device)
     dk = torch.empty((B, S, HEADS_KV, HEAD_DIM), dtype=torch.bfloat16, device=q.device)
     dv = torch.empty_like(dk)
-    ws = torch.empty(lib().abkv_window_bwd_workspace_size(B, S, window, sinks), dtype=torch.uint8, device=q.device)
+    ws_bytes = lib().abkv_window_bwd_workspace_size(B, S, window, sinks)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
     args = []
     for t in (q, k, v, out, dout):
-        args += [_ptr(t), t.stride(0), t.stride(1), t.stride(2)]
-    args += [_ptr(lse), B, S, _ptr(seq_lens), window, sinks, scale]
+        args += (t.data_ptr(), *t.stride()[:3])
+    args += (lse.data_ptr(), B, S, _ptr(seq_lens), window, sinks, scale)
     for t in (dq, dk, dv):
-        args += [_ptr(t), t.stride(0), t.stride(1), t.stride(2)]
-    rc = lib().abkv_window_attn_bwd(*args, _ptr(ws), ws.numel(), _stream())
+        args += (t.data_ptr(), *t.stride()[:3])
+    rc = lib().abkv_window_attn_bwd(*args, ws.data_ptr(), ws_bytes, _stream())
     check(rc, "abkv_window_attn_bwd")
     return dq, dk, dv
 
@@ -1090,19 +1099,23 @@ def _check_paged(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Ten
              f"kv_cache must be contiguous bf16 [P, 2, {PAGE}, {HEADS_KV}, {HEAD_DIM}]")
 
 
-def _chunk_plan(q, block_table, q_start, kv_start, tiles_of):
-    """Host checks of a causal chunk batch, and its metadata [q_start [R + 1] | kv_start [R] | the tiles' requests | their
-    first rows]; ``tiles_of`` (query rows, rows before them) -> the first rows of a request's tiles. None: no tile."""
+def _check_chunks(q, block_table, q_start, kv_start):
+    """Host checks of a causal chunk batch: (q_start [R + 1], kv_start [R], queries [R]) as int64 arrays."""
     qs, ks = np.asarray(q_start, dtype=np.int64), np.asarray(kv_start, dtype=np.int64)
     _require(qs.ndim == ks.ndim == 1 and qs.size == ks.size + 1 and ks.size <= block_table.shape[0],
              "q_start [R + 1] and kv_start [R] must be flat sequences, R at most the table's rows")
     nq = qs[1:] - qs[:-1]
-    _require(qs[0] == 0 and (nq >= 0).all() and qs[-1] <= q.shape[0], "q_start must be a prefix sum <= T")
+    _require(qs[0] == 0 and (ks.size == 0 or nq.min() >= 0) and qs[-1] <= q.shape[0], "q_start must be a prefix sum <= T")
     _require(ks.size == 0 or (ks.min() >= 0 and (ks + nq).max() <= block_table.shape[1] * PAGE),
              "the chunks' rows must lie in [0, block_table width * 16)")
-    per = [tiles_of(int(n), int(p)) for n, p in zip(nq, ks)]
-    req = np.repeat(np.arange(ks.size), [len(t) for t in per])
-    return [qs, ks, req, np.concatenate(per)] if req.size else None
+    return qs, ks, nq
+
+
+def _tiles(rows: np.ndarray, step: int):
+    """(request, first row) of every tile of ``step`` rows of requests of ``rows`` rows."""
+    n = -(-rows // step)
+    req = np.repeat(np.arange(rows.size), n)
+    return req, (np.arange(req.size) - np.repeat(np.cumsum(n) - n, n)) * step
 
 
 def paged_prefill_attention_window(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, q_start, kv_start,
@@ -1120,14 +1133,15 @@ def paged_prefill_attention_window(q: torch.Tensor, kv_cache: torch.Tensor, bloc
         _check_rows("out", out, torch.bfloat16, (T, HEADS_Q, HEAD_DIM))
     _require(lse is None or (lse.dtype == torch.float32 and lse.is_contiguous() and tuple(lse.shape) == (T, HEADS_Q)),
              "lse must be contiguous fp32 [T, 32]")
-    plan = _chunk_plan(q, block_table, q_start, kv_start, lambda n, _: np.arange(0, n, 64))
+    qs, ks, nq = _check_chunks(q, block_table, q_start, kv_start)
     _check_device(q, kv_cache, block_table, out, lse)
     if out is None:
         out = torch.empty((T, HEADS_Q, HEAD_DIM), dtype=torch.bfloat16, device=q.device)
-    if plan is None:
+    req, q0 = _tiles(nq, 64)
+    tiles, R = req.size, ks.size
+    if tiles == 0:
         return out, lse
-    tiles, R = plan[2].size, len(kv_start)
-    meta = _upload(plan, q.device)
+    meta = _upload([qs, ks, req, q0], q.device)
     at = meta.data_ptr()
     scale = default_scale() if scale is None else float(scale)
     rc = lib().abkv_paged_prefill_attn_window(_ptr(q), q.stride(0), q.stride(1), _ptr(kv_cache), kv_cache.shape[0],
@@ -1139,6 +1153,22 @@ def paged_prefill_attention_window(q: torch.Tensor, kv_cache: torch.Tensor, bloc
     return out, lse
 
 
+def _step_split_pages(num_seqs: int, pages: int) -> int:
+    """Pages per split of a step's launch over ``num_seqs`` sequences of up to ``pages`` pages: by all pages of the batch, then
+    evened over the splits that takes. Short splits end a small launch sooner, long ones write fewer partials. us a step of
+    8 / 16 / 32 / 64 pages a split: one sequence of 1024 window rows 8.5 / 9.1 / 10.3 / 12.0, of 2100 scored rows 8.0 / 9.3 /
+    11.5 / 14.4; 32 of 1024 33.3 / 34.4 / 30.6 / 31.1; 64 of 4096 211 / 192 / 191 / 176, of 2100 scored 126 / 130 / 121 / 120."""
+    total = num_seqs * pages
+    most = 8 if total < 128 else 12 if total < 1500 else 24 if total < 3000 else 40 if total < 12000 else 64
+    splits = -(-pages // most)
+    return -(-pages // (2 * splits)) * 2
+
+
+def _window_pages(max_pages: int, window: int, sinks: int) -> int:
+    """Pages of a sequence that a window step reads, at most."""
+    return min(max_pages, -(-sinks // PAGE) + -(-window // PAGE) + 1)
+
+
 def _check_step(q, kv_cache, block_table, seq_lens, max_pages, split_pages, out, lse):
     """Checks of a decode step's arguments but their device; (sequences, bound on their pages)."""
     _check_paged(q, kv_cache, block_table)
@@ -1146,7 +1176,8 @@ def _check_step(q, kv_cache, block_table, seq_lens, max_pages, split_pages, out,
     _require(block_table.shape[0] >= B and B <= 65535, "block_table must have a row per sequence (at most 65535)")
     _require(seq_lens.dtype == torch.int32 and seq_lens.dim() == 1 and seq_lens.numel() >= B and seq_lens.is_contiguous(),
              "seq_lens must be contiguous int32 [B]")
-    _require(0 < split_pages <= 64 and split_pages % 2 == 0, "split_pages must be an even number in [2, 64]")
+    _require(split_pages is None or (0 < split_pages <= 64 and split_pages % 2 == 0),
+             "split_pages must be an even number in [2, 64]")
     max_pages = W if max_pages is None else int(max_pages)
     _require(0 < max_pages <= W, "max_pages must be in [1, block_table width]")
     if out is not None:
@@ -1169,9 +1200,10 @@ def _take_workspace(workspace, need: int, device):
     return workspace, nbytes
 
 
-def decode_window_workspace(num_seqs: int, max_pages: int, window: int, sinks: int = 0,
-                            split_pages: int = DEFAULT_SPLIT_PAGES, device=None) -> torch.Tensor | None:
-    """Workspace for :func:`decode_attention_window` (None when no sequence can need a second split)."""
+def decode_window_workspace(num_seqs: int, max_pages: int, window: int, sinks: int = 0, split_pages: int | None = None,
+                            device=None) -> torch.Tensor | None:
+    """Workspace for :func:`decode_attention_window` of the same sizes (None when no sequence can need a second split)."""
+    split_pages = split_pages or _step_split_pages(num_seqs, _window_pages(max_pages, window, sinks))
     n = lib().abkv_decode_window_workspace_size(num_seqs, max_pages, split_pages, *_check_window(window, sinks))
     return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
@@ -1179,17 +1211,19 @@ def decode_window_workspace(num_seqs: int, max_pages: int, window: int, sinks: i
 def decode_attention_window(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
                             window: int, sinks: int = 0, scale: float | None = None, max_pages: int | None = None,
                             out: torch.Tensor | None = None, lse: torch.Tensor | None = None,
-                            split_pages: int = DEFAULT_SPLIT_PAGES, workspace: torch.Tensor | None = None):
+                            split_pages: int | None = None, workspace: torch.Tensor | None = None):
     """Decode attention of one layer under a sliding window with sinks: a sequence's token sees rows
     [n - ``window``, n) and [0, ``sinks``) of its n = seq_lens[b] rows, and only their pages are read.
 
     Arguments and results as :func:`decode_attention` (bf16 only): (out [B, 32, 128] bf16, lse [B, 32] fp32 or None).
+    ``split_pages`` None: chosen by the sizes.
     """
     window, sinks = _check_window(window, sinks)
     B, max_pages = _check_step(q, kv_cache, block_table, seq_lens, max_pages, split_pages, out, lse)
     _check_device(q, kv_cache, block_table, seq_lens, out, lse)
     if out is None:
         out = torch.empty((B, HEADS_Q, HEAD_DIM), dtype=torch.bfloat16, device=q.device)
+    split_pages = split_pages or _step_split_pages(B, _window_pages(max_pages, window, sinks))
     need = lib().abkv_decode_window_workspace_size(B, max_pages, split_pages, window, sinks)
     workspace, ws_bytes = _take_workspace(workspace, need, q.device)
     scale = default_scale() if scale is None else float(scale)
@@ -1211,9 +1245,9 @@ def _check_scores(scores: torch.Tensor, B: int, rows: int) -> None:
                                                                              + rows)), "scores must not share memory")
 
 
-def decode_scored_workspace(num_seqs: int, max_pages: int, split_pages: int = DEFAULT_SPLIT_PAGES,
-                            device=None) -> torch.Tensor:
-    """Workspace for :func:`decode_attention_scored`."""
+def decode_scored_workspace(num_seqs: int, max_pages: int, split_pages: int | None = None, device=None) -> torch.Tensor:
+    """Workspace for :func:`decode_attention_scored` of the same sizes."""
+    split_pages = split_pages or _step_split_pages(num_seqs, max_pages)
     return torch.empty(lib().abkv_decode_scored_workspace_size(num_seqs, max_pages, split_pages), dtype=torch.uint8,
                        device=device)
 
@@ -1221,18 +1255,19 @@ def decode_scored_workspace(num_seqs: int, max_pages: int, split_pages: int = DE
 def decode_attention_scored(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
                             scores: torch.Tensor, scale: float | None = None, max_pages: int | None = None,
                             out: torch.Tensor | None = None, lse: torch.Tensor | None = None,
-                            split_pages: int = DEFAULT_SPLIT_PAGES, workspace: torch.Tensor | None = None):
+                            split_pages: int | None = None, workspace: torch.Tensor | None = None):
     """:func:`decode_attention` (bf16 only) that also adds the step's attention weights to the rows' scores:
     scores[b, h, row] += the weights of KV head h's four query heads, for rows below seq_lens[b].
 
     ``scores`` [B, 8, rows] fp32, a row for each of the 16 * ``max_pages`` slots (zero for a new sequence), is updated in
-    place; each score has one owner, so equal calls give equal bits. Returns (out [B, 32, 128] bf16, lse or None).
+    place; each score has one owner, so equal calls give equal bits. ``split_pages`` None: chosen by the sizes. Returns (out [B, 32, 128] bf16, lse or None).
     """
     B, max_pages = _check_step(q, kv_cache, block_table, seq_lens, max_pages, split_pages, out, lse)
     _check_scores(scores, B, max_pages * PAGE)
     _check_device(q, kv_cache, block_table, seq_lens, scores, out, lse)
     if out is None:
         out = torch.empty((B, HEADS_Q, HEAD_DIM), dtype=torch.bfloat16, device=q.device)
+    split_pages = split_pages or _step_split_pages(B, max_pages)
     need = lib().abkv_decode_scored_workspace_size(B, max_pages, split_pages)
     workspace, ws_bytes = _take_workspace(workspace, need, q.device)
     scale = default_scale() if scale is None else float(scale)
@@ -1242,6 +1277,17 @@ def decode_attention_scored(q: torch.Tensor, kv_cache: torch.Tensor, block_table
                                        out.stride(0), out.stride(1), _ptr(lse), _ptr(workspace), ws_bytes, _stream())
     check(rc, "abkv_decode_attn_scored")
     return out, lse
+
+
+def _score_tile_keys(ks: np.ndarray, nq: np.ndarray, num_cus: int) -> int:
+    """Keys of a workgroup of the prompt scores, 64 or 128, from requests of nq queries behind ks rows. By the longest
+    workgroup (as many queries as a request has) and the sum over all, a workgroup a CU: a query row takes 21 ns against 64 keys
+    and 33 against 128, a workgroup 5 us beside. us a call with 64 / 128: one prompt of 512 rows 22 / 28, of 2048 57 / 81, of
+    4096 120 / 149; 64 queries behind 4000 rows 18 / 15; 2048 behind 2048 beside 1500 118 / 94; four of 512 behind 512 38 / 31."""
+    longest, total = int(nq.max()), int((nq * (2 * ks + nq)).sum()) / 128
+    groups = HEADS_KV * int((ks + nq).sum()) / 64 / num_cus
+    per = HEADS_KV * total / num_cus
+    return 64 if 21e-3 * max(longest, per) + 5 * groups < 33e-3 * max(longest, per / 2) + 2.5 * groups else 128
 
 
 def paged_prefill_scores(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, q_start, kv_start,
@@ -1257,17 +1303,20 @@ def paged_prefill_scores(q: torch.Tensor, kv_cache: torch.Tensor, block_table: t
     _require(lse.dtype == torch.float32 and lse.is_contiguous() and tuple(lse.shape) == (q.shape[0], HEADS_Q),
              "lse must be contiguous fp32 [T, 32]")
     _check_scores(scores, len(kv_start), block_table.shape[1] * PAGE)
-    plan = _chunk_plan(q, block_table, q_start, kv_start, lambda n, p: np.arange(0, n + p if n else 0, 64))
+    qs, ks, nq = _check_chunks(q, block_table, q_start, kv_start)
     _check_device(q, kv_cache, block_table, lse, scores)
-    if plan is None:
+    if qs[-1] == 0:
         return
-    tiles, R = plan[2].size, len(kv_start)
-    meta = _upload(plan, q.device)
+    keys = _score_tile_keys(ks, nq, _num_cus())
+    req, k0 = _tiles(np.where(nq > 0, ks + nq, 0), keys)
+    order = np.argsort(np.maximum(k0 - ks[req], 0) - nq[req], kind="stable")      # the tiles that most queries see first
+    tiles, R = req.size, ks.size
+    meta = _upload([qs, ks, req[order], k0[order]], q.device)
     at = meta.data_ptr()
     scale = default_scale() if scale is None else float(scale)
     rc = lib().abkv_paged_prefill_scores(_ptr(q), q.stride(0), q.stride(1), _ptr(kv_cache), kv_cache.shape[0],
                                          _ptr(block_table), _row_stride(block_table), block_table.shape[1], at,
-                                         at + 4 * (R + 1), at + 4 * (2 * R + 1), at + 4 * (2 * R + 1 + tiles), tiles,
+                                         at + 4 * (R + 1), at + 4 * (2 * R + 1), at + 4 * (2 * R + 1 + tiles), tiles, keys,
                                          _ptr(lse), _ptr(scores), scores.stride(0), scores.stride(1), scale, _stream())
     check(rc, "abkv_paged_prefill_scores")
 
@@ -1306,10 +1355,17 @@ def kv_evict(layer_caches, block_table: torch.Tensor, seq_lens: torch.Tensor, sc
                  f"{name} must be contiguous {dt} [{L}, {B}, {HEADS_KV}, rows] with a row for each of the "
                  f"{max_pages * PAGE} slots")
     _require(scores.shape == positions.shape, "scores and positions must have the same shape")
-    _require(len({c.data_ptr() for c in layer_caches}) == L, "a layer cache may be given once")
+    _require(1 <= L <= 16, "between 1 and 16 layer caches per launch")
+    shape = layer_caches[0].shape
+    for c in layer_caches:
+        if c.dtype != torch.bfloat16 or c.shape != shape or not c.is_contiguous():
+            raise ValueError("layer caches must be contiguous bf16 of one shape")
+    _require(len(shape) == 5 and shape[1:] == _PAGE_SHAPE and shape[0] > 0,
+             f"layer caches must be [P, 2, {PAGE}, {HEADS_KV}, {HEAD_DIM}], got {tuple(shape)}")
     _check_device(block_table, seq_lens, num_tokens, scores, positions, *layer_caches)
-    arr, num_pages = _layer_ptrs(layer_caches)
-    _require(num_pages > 0, "the layer caches must hold at least one page")
+    ptrs = [c.data_ptr() for c in layer_caches]
+    _require(len(set(ptrs)) == L, "a layer cache may be given once")
+    arr, num_pages = (C.c_void_p * L)(*ptrs), shape[0]
     out = torch.empty_like(seq_lens)
     if B == 0:
         return out
