@@ -33,7 +33,6 @@ from dataclasses import dataclass
 import torch
 import torch.nn.functional as F
 from torch import nn
-from torch.autograd.function import once_differentiable
 
 from . import ops
 from .config import bitrev_offsets
@@ -125,20 +124,19 @@ class _WindowAttention(torch.autograd.Function):
             lse = torch.empty((q.shape[0], ops.HEADS_Q, q.shape[1]), dtype=torch.float32, device=q.device)
         out, _ = ops.window_attention(q, k, v, mask.window, mask.sinks, seq_lens=mask.seq_lens, scale=scale, lse=lse)
         if lse is not None:
-            ctx.save_for_backward(query, key, value, out, lse, mask.seq_lens)
+            ctx.save_for_backward(q, k, v, out, lse, mask.seq_lens)
             ctx.mask, ctx.scale = mask, scale
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_out):
-        query, key, value, out, lse, seq_lens = ctx.saved_tensors
+        if torch.is_grad_enabled():
+            raise RuntimeError("sliding-window attention has no second derivative")
+        q, k, v, out, lse, seq_lens = ctx.saved_tensors
         st = grad_out.stride()
-        if st[3] != 1 or (st[0] | st[1] | st[2]) % 8 or grad_out.data_ptr() % 16:
+        if st[3] != 1 or (st[0] | st[1] | st[2]) % 8 or st[1] >= 1 << 24 or grad_out.data_ptr() % 16:
             grad_out = grad_out.contiguous()
-        dq, dk, dv = ops.window_attention_backward(query.transpose(1, 2), key.transpose(1, 2), value.transpose(1, 2), out,
-                                                   lse, grad_out, ctx.mask.window, ctx.mask.sinks, seq_lens=seq_lens,
-                                                   scale=ctx.scale)
+        dq, dk, dv = ops.window_backward(q, k, v, out, lse, grad_out, ctx.mask.window, ctx.mask.sinks, seq_lens, ctx.scale)
         return dq.transpose(1, 2), dk.transpose(1, 2), dv.transpose(1, 2), None, None
 
 

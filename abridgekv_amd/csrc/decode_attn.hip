@@ -191,7 +191,7 @@ __global__ __launch_bounds__(64 * kW * kSub) void decode_attn_kernel(DecodeArgs 
   // are adjacent in x. Split fastest (dispatch order: the splits of sequence 0, then of sequence 1, ...), measured faster
   // than sequence-fastest orders on the saturated workload. kSub > 1 (kW == 1): kSub waves share the split of one KV
   // head, wave s taking page pairs s, s + kSub, ..., and their results meet in LDS (see launch_decode).
-  static_assert(kSub == 1 || (kW == 1 && kSub == kGroup), "a shared split has one KV head and a wave per query head");
+  static_assert(kSub == 1 || (kW == 1 && kSub >= kGroup), "a shared split has one KV head and a wave per query head");
   const int b = blockIdx.y;
   constexpr int kParts = kHeadsKV / kW;
   const int split = blockIdx.x / kParts;
@@ -354,6 +354,7 @@ __global__ __launch_bounds__(64 * kW * kSub) void decode_attn_kernel(DecodeArgs 
       }
     }
     __syncthreads();
+    if (kSub > kGroup && wave >= kGroup) return;
     combine_subs<kSub>(a, so, sm, sl, b, split, kvh * kGroup + wave, wave, lane, partial);
     return;
   }
@@ -686,6 +687,12 @@ inline bool share_splits(int max_splits, int num_seqs) {
 }
 template <int kMode>
 inline void launch_decode(const DecodeArgs& a, int max_splits, int num_seqs, hipStream_t stream) {
+  // Sequences of one split: eight waves share it (the windows' short ones; see _step_split_pages)
+  if (kMode != kPlain && max_splits == 1) {
+    hipLaunchKernelGGL((decode_attn_kernel<1, 2 * kGroup, kMode>), dim3(kHeadsKV, num_seqs), dim3(128 * kGroup), 0, stream,
+                       a);
+    return;
+  }
   if (share_splits(max_splits, num_seqs)) {
     hipLaunchKernelGGL((decode_attn_kernel<1, kGroup, kMode>), dim3(max_splits * kHeadsKV, num_seqs), dim3(64 * kGroup), 0,
                        stream, a);

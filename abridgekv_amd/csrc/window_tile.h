@@ -16,7 +16,32 @@ struct WindowArgs {
   __bf16* out;      long o_sb, o_ss, o_sh;
   float* lse;                                // natural log, [B, 32, S]; chunks: [T, 32]; or nullptr
   int num_q_tiles;
+  int group;                                 // tiles of one XCD in a row (window_tile)
 };
+
+// Workgroup -> (64-row tile, KV head, sequence). Workgroups go to the 8 XCDs round-robin by linear id; XCD x takes the tile
+// groups x, x + 8, ..., of `group` consecutive tiles of a sequence with all KV heads each: neighbouring tiles read mostly the
+// same rows of the other side, which then stay in one XCD's L2, and all of the rows' bytes, not one head's, so that its
+// requests spread over all L2 channels. One KV head per XCD, as the compression mask's kernels place them (there every tile
+// reads all codes), against this: B=2, 8192 rows, window 1024: forward 322 -> 294 us.
+struct WindowTile {
+  int tile, kvh, b;
+};
+__device__ __forceinline__ WindowTile window_tile(int tiles, int batch, int group) {
+  const int total = tiles * batch, x = blockIdx.x % 8, i = blockIdx.x / 8;
+  const int whole = total / (8 * group) * (8 * group);       // in whole rounds of groups; the rest evenly
+  int t, kvh;
+  if (i < whole) {
+    const int in = i % (8 * group);
+    kvh = in % kHeadsKV;
+    t = (i / (8 * group) * 8 + x) * group + in / kHeadsKV;
+  } else {
+    const int rest = x * (total - whole) + (i - whole);
+    kvh = rest % kHeadsKV;
+    t = whole + rest / kHeadsKV;
+  }
+  return {t % tiles, kvh, t / tiles};
+}
 
 __device__ __forceinline__ int window_rows(const WindowArgs& a, int b) {
   return a.seq_lens ? min(max(a.seq_lens[b], 0), a.S) : a.S;

@@ -1065,13 +1065,14 @@ def window_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     _require(lse.dtype == torch.float32 and lse.is_contiguous() and tuple(lse.shape) == (B, HEADS_Q, S),
              "lse must be contiguous fp32 [B, 32, S]")
     _check_device(q, k, v, out, lse, dout, seq_lens)
-    return _window_backward(q, k, v, out, lse, dout, *_reach(window, sinks, S), seq_lens,
-                            default_scale() if scale is None else float(scale))
+    return window_backward(q, k, v, out, lse, dout, window, sinks, seq_lens,
+                           default_scale() if scale is None else float(scale))
 
 
-def _window_backward(q, k, v, out, lse, dout, window, sinks, seq_lens, scale):
-    """window_attention_backward of arguments that are checked."""
+def window_backward(q, k, v, out, lse, dout, window, sinks, seq_lens, scale):
+    """:func:`window_attention_backward` of arguments that are checked already (autograd's saved tensors)."""
     B, S = q.shape[:2]
+    window, sinks = _reach(window, sinks, S)
     dq = torch.empty((B, S, HEADS_Q, HEAD_DIM), dtype=torch.bfloat16, device=q.device)
     dk = torch.empty((B, S, HEADS_KV, HEAD_DIM), dtype=torch.bfloat16, device=q.device)
     dv = torch.empty_like(dk)
@@ -1088,15 +1089,18 @@ def _window_backward(q, k, v, out, lse, dout, window, sinks, seq_lens, scale):
     return dq, dk, dv
 
 
-def _check_paged(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor) -> None:
-    """bf16 query rows [T, 32, 128], a layer cache and its page table."""
-    _require(q.dim() == 3, "q must be [T, 32, 128]")
-    _check_rows("q", q, torch.bfloat16, (q.shape[0], HEADS_Q, HEAD_DIM))
-    _require(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[1] > 0
-             and block_table.stride(1) == 1, "block_table must be int32 [B, W] with contiguous rows")
-    _require(kv_cache.dtype == torch.bfloat16 and kv_cache.dim() == 5 and kv_cache.shape[1:] == _PAGE_SHAPE
-             and kv_cache.shape[0] > 0 and kv_cache.is_contiguous(),
-             f"kv_cache must be contiguous bf16 [P, 2, {PAGE}, {HEADS_KV}, {HEAD_DIM}]")
+def _check_paged(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor) -> tuple[int, int, int]:
+    """bf16 query rows [T, 32, 128], a layer cache and its page table; (T, the table's rows and width)."""
+    T = q.shape[0] if q.dim() else 0
+    _check_rows("q", q, torch.bfloat16, (T, HEADS_Q, HEAD_DIM))
+    shape = kv_cache.shape
+    if (kv_cache.dtype is not torch.bfloat16 or len(shape) != 5 or shape[1:] != _PAGE_SHAPE or shape[0] == 0
+            or not kv_cache.is_contiguous()):
+        raise ValueError(f"kv_cache must be contiguous bf16 [P, 2, {PAGE}, {HEADS_KV}, {HEAD_DIM}]")
+    shape = block_table.shape
+    if block_table.dtype is not torch.int32 or len(shape) != 2 or shape[1] == 0 or block_table.stride(1) != 1:
+        raise ValueError("block_table must be int32 [B, W] with contiguous rows")
+    return T, shape[0], shape[1]
 
 
 def _check_chunks(q, block_table, q_start, kv_start):
@@ -1169,21 +1173,30 @@ def _window_pages(max_pages: int, window: int, sinks: int) -> int:
     return min(max_pages, -(-sinks // PAGE) + -(-window // PAGE) + 1)
 
 
+def _window_split_pages(num_seqs: int, max_pages: int, window: int, sinks: int) -> int:
+    """Pages per split of a window step: up to 28 pages one split, which eight waves share and no merge follows (us for windows
+    of 250 rows, sequences 1 / 16 / 64: 6.9 / 7.0 / 18.4, split in shorter ones 7.3 / 8.9 / 19.7; of 500: 8.8 / 12.2 / 29.8
+    against 8.0 / 13.2 / 30.1)."""
+    pages = _window_pages(max_pages, window, sinks)
+    return -(-pages // 2) * 2 if pages <= 28 else _step_split_pages(num_seqs, pages)
+
+
 def _check_step(q, kv_cache, block_table, seq_lens, max_pages, split_pages, out, lse):
     """Checks of a decode step's arguments but their device; (sequences, bound on their pages)."""
-    _check_paged(q, kv_cache, block_table)
-    B, W = q.shape[0], block_table.shape[1]
-    _require(block_table.shape[0] >= B and B <= 65535, "block_table must have a row per sequence (at most 65535)")
-    _require(seq_lens.dtype == torch.int32 and seq_lens.dim() == 1 and seq_lens.numel() >= B and seq_lens.is_contiguous(),
-             "seq_lens must be contiguous int32 [B]")
-    _require(split_pages is None or (0 < split_pages <= 64 and split_pages % 2 == 0),
-             "split_pages must be an even number in [2, 64]")
+    B, rows, W = _check_paged(q, kv_cache, block_table)
+    if rows < B or B > 65535:
+        raise ValueError("block_table must have a row per sequence (at most 65535)")
+    if seq_lens.dtype is not torch.int32 or seq_lens.dim() != 1 or seq_lens.shape[0] < B or not seq_lens.is_contiguous():
+        raise ValueError("seq_lens must be contiguous int32 [B]")
+    if split_pages is not None and not (0 < split_pages <= 64 and split_pages % 2 == 0):
+        raise ValueError("split_pages must be an even number in [2, 64]")
     max_pages = W if max_pages is None else int(max_pages)
-    _require(0 < max_pages <= W, "max_pages must be in [1, block_table width]")
+    if not 0 < max_pages <= W:
+        raise ValueError("max_pages must be in [1, block_table width]")
     if out is not None:
         _check_rows("out", out, torch.bfloat16, (B, HEADS_Q, HEAD_DIM))
-    _require(lse is None or (lse.dtype == torch.float32 and lse.is_contiguous() and lse.numel() >= B * HEADS_Q),
-             "lse must be contiguous fp32 [B, 32]")
+    if lse is not None and (lse.dtype is not torch.float32 or not lse.is_contiguous() or lse.numel() < B * HEADS_Q):
+        raise ValueError("lse must be contiguous fp32 [B, 32]")
     return B, max_pages
 
 
@@ -1203,7 +1216,7 @@ def _take_workspace(workspace, need: int, device):
 def decode_window_workspace(num_seqs: int, max_pages: int, window: int, sinks: int = 0, split_pages: int | None = None,
                             device=None) -> torch.Tensor | None:
     """Workspace for :func:`decode_attention_window` of the same sizes (None when no sequence can need a second split)."""
-    split_pages = split_pages or _step_split_pages(num_seqs, _window_pages(max_pages, window, sinks))
+    split_pages = split_pages or _window_split_pages(num_seqs, max_pages, window, sinks)
     n = lib().abkv_decode_window_workspace_size(num_seqs, max_pages, split_pages, *_check_window(window, sinks))
     return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
@@ -1223,7 +1236,7 @@ def decode_attention_window(q: torch.Tensor, kv_cache: torch.Tensor, block_table
     _check_device(q, kv_cache, block_table, seq_lens, out, lse)
     if out is None:
         out = torch.empty((B, HEADS_Q, HEAD_DIM), dtype=torch.bfloat16, device=q.device)
-    split_pages = split_pages or _step_split_pages(B, _window_pages(max_pages, window, sinks))
+    split_pages = split_pages or _window_split_pages(B, max_pages, window, sinks)
     need = lib().abkv_decode_window_workspace_size(B, max_pages, split_pages, window, sinks)
     workspace, ws_bytes = _take_workspace(workspace, need, q.device)
     scale = default_scale() if scale is None else float(scale)
@@ -1237,12 +1250,13 @@ def decode_attention_window(q: torch.Tensor, kv_cache: torch.Tensor, block_table
 
 # -- a cache bounded by weight: scores and eviction ----------------------------------------------------------------------
 def _check_scores(scores: torch.Tensor, B: int, rows: int) -> None:
-    _require(scores.dtype == torch.float32 and scores.dim() == 3 and scores.shape[0] >= B and scores.shape[1] == HEADS_KV
-             and scores.shape[2] >= rows and scores.stride(2) == 1,
-             f"scores must be fp32 [B, {HEADS_KV}, rows] with contiguous rows, a row for each of the {rows} slots")
+    shape = scores.shape
+    if (scores.dtype is not torch.float32 or len(shape) != 3 or shape[0] < B or shape[1] != HEADS_KV or shape[2] < rows
+            or scores.stride(2) != 1):
+        raise ValueError(f"scores must be fp32 [B, {HEADS_KV}, rows] with contiguous rows, one for each of {rows} slots")
     sb, sh = scores.stride()[:2]
-    _require(sh >= rows and (scores.shape[0] <= 1 or sb >= 7 * sh + rows or (sb >= rows and sh >= (scores.shape[0] - 1) * sb
-                                                                             + rows)), "scores must not share memory")
+    if sh < rows or not (shape[0] <= 1 or sb >= 7 * sh + rows or (sb >= rows and sh >= (shape[0] - 1) * sb + rows)):
+        raise ValueError("scores must not share memory")
 
 
 def decode_scored_workspace(num_seqs: int, max_pages: int, split_pages: int | None = None, device=None) -> torch.Tensor:
@@ -1344,24 +1358,25 @@ def kv_evict(layer_caches, block_table: torch.Tensor, seq_lens: torch.Tensor, sc
     _require(block_table.dtype == torch.int32 and W > 0 and block_table.stride(1) == 1,
              "block_table must be int32 [B, W] with contiguous rows")
     B = seq_lens.numel()
-    for name, t in (("seq_lens", seq_lens), ("num_tokens", num_tokens)):
-        _require(t.dtype == torch.int32 and tuple(t.shape) == (B,) and t.is_contiguous(), f"{name} must be contiguous int32 [B]")
+    for t in (seq_lens, num_tokens):
+        if t.dtype is not torch.int32 or t.shape != (B,) or not t.is_contiguous():
+            raise ValueError("seq_lens and num_tokens must be contiguous int32 [B]")
     _require(block_table.shape[0] >= B, "block_table must have a row per sequence")
     max_pages = W if max_pages is None else int(max_pages)
     _require(0 < max_pages <= min(W, 16384), "max_pages must be in [1, block_table width], at most 16384")
-    for name, t, dt in (("scores", scores, torch.float32), ("positions", positions, torch.int32)):
-        _require(t.dtype == dt and t.dim() == 4 and tuple(t.shape[:3]) == (L, B, HEADS_KV)
-                 and t.shape[3] >= max_pages * PAGE and t.is_contiguous(),
-                 f"{name} must be contiguous {dt} [{L}, {B}, {HEADS_KV}, rows] with a row for each of the "
-                 f"{max_pages * PAGE} slots")
-    _require(scores.shape == positions.shape, "scores and positions must have the same shape")
+    shape = scores.shape
+    if (scores.dtype is not torch.float32 or positions.dtype is not torch.int32 or len(shape) != 4
+            or shape[:3] != (L, B, HEADS_KV) or shape[3] < max_pages * PAGE or positions.shape != shape
+            or not scores.is_contiguous() or not positions.is_contiguous()):
+        raise ValueError(f"scores and positions must be contiguous fp32 and int32 [{L}, {B}, {HEADS_KV}, rows] with a row for "
+                         f"each of {max_pages * PAGE} slots")
     _require(1 <= L <= 16, "between 1 and 16 layer caches per launch")
     shape = layer_caches[0].shape
     for c in layer_caches:
-        if c.dtype != torch.bfloat16 or c.shape != shape or not c.is_contiguous():
+        if c.dtype is not torch.bfloat16 or c.shape != shape or not c.is_contiguous():
             raise ValueError("layer caches must be contiguous bf16 of one shape")
-    _require(len(shape) == 5 and shape[1:] == _PAGE_SHAPE and shape[0] > 0,
-             f"layer caches must be [P, 2, {PAGE}, {HEADS_KV}, {HEAD_DIM}], got {tuple(shape)}")
+    if len(shape) != 5 or shape[1:] != _PAGE_SHAPE or shape[0] == 0:
+        raise ValueError(f"layer caches must be [P, 2, {PAGE}, {HEADS_KV}, {HEAD_DIM}], got {tuple(shape)}")
     _check_device(block_table, seq_lens, num_tokens, scores, positions, *layer_caches)
     ptrs = [c.data_ptr() for c in layer_caches]
     _require(len(set(ptrs)) == L, "a layer cache may be given once")
