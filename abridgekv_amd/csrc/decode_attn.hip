@@ -62,8 +62,8 @@ struct DecodeArgs {
   // kWindow: rows [seq_len - window, seq_len) and the first `sinks` rows are seen
   int window, sinks;
   // kScored: the weights of every row are added to scores[b][KV head][row] after the merge
-  float* raw;                // [B, 32, raw_stride] scores of this step in log2 units
-  long raw_stride;
+  float* raw;                // [B, 8, raw_pairs, 4 heads, 32 rows] scores of this step in log2 units, by page pairs
+  long raw_pairs;
   float* scores;
   long s_sb, s_sh;
 };
@@ -72,6 +72,7 @@ struct DecodeArgs {
 constexpr int kPlain = 0;    // every row of the sequence
 constexpr int kWindow = 1;   // the sinks and the window
 constexpr int kScored = 2;   // every row, and each row's score for the weights to be added up (partials always)
+constexpr int kWhole = 3;    // every row in one split, the scores in LDS, and the weights added up at the end
 
 // The rows of a sequence that the step reads, as whole pages one after the other: pages below `sink_pages`, then pages
 // shifted by `shift`. In rows of that order (virtual rows), [0, sink_end) and [win_begin, end) are seen.
@@ -185,8 +186,32 @@ __device__ __forceinline__ void combine_subs(const DecodeArgs& a, const float (&
   if (lane == 0) *reinterpret_cast<floatx4*>(a.part_ml + at * 4) = floatx4{m, l, range.scale, 0.f};
 }
 
+// scores[row .. row + 3] += sum over a KV head's query heads h of exp2(raw - m[h]) * inv_l[h], rows below `end`; raw: the four
+// rows' scores of head 0, the next head `stride` behind.
+__device__ __forceinline__ void add_weights(const DecodeArgs& a, int b, int kvh, int row, int end, const float* raw, int stride,
+                                            const float* m, const float* inv_l) {
+  floatx4 w = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int h = 0; h < kGroup; ++h) {
+    const floatx4 x = *reinterpret_cast<const floatx4*>(raw + h * stride);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) w[r] += fast_exp2(x[r] - m[h]) * inv_l[h];
+  }
+  typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+  float* to = a.scores + (long)b * a.s_sb + (long)kvh * a.s_sh + row;
+  if (row + 4 <= end) {
+    *reinterpret_cast<f32x4u*>(to) = *reinterpret_cast<const f32x4u*>(to) + w;
+  } else {
+    for (int r = 0; row + r < end; ++r) to[r] += r == 0 ? w[0] : r == 1 ? w[1] : w[2];
+  }
+}
+
+// kWhole: floats of a head's scores in LDS (whole page pairs, and four that spread the heads over the banks).
+constexpr int kWholeSub = 8, kWholePages = 256;
+__host__ __device__ __forceinline__ constexpr int whole_stride(int max_pages) { return (max_pages + 1) / 2 * 2 * kPage + 4; }
+
 template <int kW, int kSub, int kMode>
-__global__ __launch_bounds__(64 * kW * kSub) void decode_attn_kernel(DecodeArgs a) {
+__global__ __launch_bounds__(64 * kW * kSub, kMode == kWhole ? 4 : 1) void decode_attn_kernel(DecodeArgs a) {
   // Grid (max_splits * 8 / kW, B): kW KV heads per workgroup, a wave each (kSub == 1); the 8 / kW workgroups of a split
   // are adjacent in x. Split fastest (dispatch order: the splits of sequence 0, then of sequence 1, ...), measured faster
   // than sequence-fastest orders on the saturated workload. kSub > 1 (kW == 1): kSub waves share the split of one KV
@@ -232,14 +257,19 @@ __global__ __launch_bounds__(64 * kW * kSub) void decode_attn_kernel(DecodeArgs 
   // Page ids of the split, fetched once: lane l holds page pg_begin + l (clamped into the cache); the loop reads them
   // with readlane, so no page-table load sits between one chunk's compute and the next chunk's K/V loads.
   int pid_l = 0;
-  if (lane < pg_end - pg_begin) {
+  extern __shared__ __attribute__((aligned(16))) float lds_raw[];          // kWhole: [4 heads][whole_stride]
+  if constexpr (kMode == kWhole) {                           // this wave's pages: lane l its l-th
+    const int pg = 2 * (sub + kSub * (lane >> 1)) + (lane & 1);
+    if (pg < pg_end) pid_l = min(max(bt[pg], 0), a.num_pages - 1);
+  } else if (lane < pg_end - pg_begin) {
     const int pg = kMode == kWindow ? rows.page(pg_begin + lane) : pg_begin + lane;
     pid_l = min(max(bt[pg], 0), a.num_pages - 1);
   }
   const __bf16* kv_h = a.kv + kvh * kHeadDim;
   for (int pg = pg_begin + 2 * sub; pg < pg_end; pg += 2 * kSub) {
-    const int p0 = __builtin_amdgcn_readlane(pid_l, pg - pg_begin);
-    const int p1 = __builtin_amdgcn_readlane(pid_l, min(pg + 1, pg_end - 1) - pg_begin);
+    const int at = kMode == kWhole ? 2 * ((pg / 2 - sub) / kSub) : pg - pg_begin;
+    const int p0 = __builtin_amdgcn_readlane(pid_l, at);
+    const int p1 = __builtin_amdgcn_readlane(pid_l, pg + 1 < pg_end ? at + 1 : at);
     const __bf16* base0 = kv_h + (long)p0 * kPageElems;
     const __bf16* base1 = kv_h + (long)p1 * kPageElems;
 
@@ -288,9 +318,17 @@ __global__ __launch_bounds__(64 * kW * kSub) void decode_attn_kernel(DecodeArgs 
       }
     }
     if constexpr (kMode == kScored) {
-      // raw scores of the wave's four heads, four rows a lane (a row buffer of whole page pairs: raw_stride)
+      // the wave's four heads, four rows a lane: 512 bytes in a row
       if (m16 < kGroup) {
-        float* raw = a.raw + ((long)b * kHeadsQ + kvh * kGroup + m16) * a.raw_stride + pg * kPage + 4 * j;
+        float* raw = a.raw + ((((long)b * kHeadsKV + kvh) * a.raw_pairs + pg / 2) * kGroup + m16) * 32 + 4 * j;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          *reinterpret_cast<floatx4*>(raw + 16 * t) = floatx4{sv[4 * t], sv[4 * t + 1], sv[4 * t + 2], sv[4 * t + 3]};
+      }
+    }
+    if constexpr (kMode == kWhole) {
+      if (m16 < kGroup) {
+        float* raw = lds_raw + m16 * whole_stride(a.max_pages) + pg * kPage + 4 * j;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
           *reinterpret_cast<floatx4*>(raw + 16 * t) = floatx4{sv[4 * t], sv[4 * t + 1], sv[4 * t + 2], sv[4 * t + 3]};
@@ -354,8 +392,23 @@ __global__ __launch_bounds__(64 * kW * kSub) void decode_attn_kernel(DecodeArgs 
       }
     }
     __syncthreads();
-    if (kSub > kGroup && wave >= kGroup) return;
-    combine_subs<kSub>(a, so, sm, sl, b, split, kvh * kGroup + wave, wave, lane, partial);
+    if (kSub == kGroup || wave < kGroup)
+      combine_subs<kSub>(a, so, sm, sl, b, split, kvh * kGroup + wave, wave, lane, partial);
+    if constexpr (kMode == kWhole) {
+      float m[kGroup], inv_l[kGroup];
+#pragma unroll
+      for (int h = 0; h < kGroup; ++h) {
+        float l = 0.f;
+        m[h] = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kSub; ++i) m[h] = fmaxf(m[h], sm[i][h]);
+#pragma unroll
+        for (int i = 0; i < kSub; ++i) l += sm[i][h] == -INFINITY ? 0.f : sl[i][h] * fast_exp2(sm[i][h] - m[h]);
+        inv_l[h] = 1.f / l;
+      }
+      for (int row = 4 * threadIdx.x; row < rows.end; row += 4 * 64 * kSub)
+        add_weights(a, b, kvh, row, rows.end, lds_raw + row, whole_stride(a.max_pages), m, inv_l);
+    }
     return;
   }
   const float amax = partial ? column_absmax(o) : 0.f;    // (a uniform branch: all lanes take part in the shuffles)
@@ -481,7 +534,7 @@ __global__ __launch_bounds__(256) void decode_merge_kernel(DecodeArgs a) {
   merge_head(a, b, 4 * blockIdx.y + (threadIdx.x >> 6), n_main);
 }
 
-// The end of a scored step: the merge (the first 8 workgroups of a sequence, four heads each), and beside it the rows'
+// The end of a scored step in splits: the merge (the first 8 workgroups of a sequence, four heads each), and beside it the rows'
 // scores, workgroup (sequence, KV head, 1024 rows): scores[row] += sum over the group's heads u of exp2(raw_u - M_u) / L_u,
 // with (M_u, L_u) from the splits' records, which every workgroup combines for itself. One owner per score: no atomics, the
 // same bits every time. The raw scores cost 128 B written and read a row beside its 4 KiB of K and V.
@@ -520,20 +573,8 @@ __global__ __launch_bounds__(256) void decode_score_kernel(DecodeArgs a) {
   __syncthreads();
   const int row = row0 + 4 * threadIdx.x;
   if (row >= rows.end) return;
-  floatx4 w = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int h = 0; h < kGroup; ++h) {
-    const floatx4 x = *reinterpret_cast<const floatx4*>(a.raw + ((long)b * kHeadsQ + kvh * kGroup + h) * a.raw_stride + row);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) w[r] += fast_exp2(x[r] - sm[h]) * si[h];
-  }
-  typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
-  float* to = a.scores + (long)b * a.s_sb + (long)kvh * a.s_sh + row;
-  if (row + 4 <= rows.end) {
-    *reinterpret_cast<f32x4u*>(to) = *reinterpret_cast<const f32x4u*>(to) + w;
-  } else {
-    for (int r = 0; row + r < rows.end; ++r) to[r] += r == 0 ? w[0] : r == 1 ? w[1] : w[2];
-  }
+  add_weights(a, b, kvh, row, rows.end, a.raw + (((long)b * kHeadsKV + kvh) * a.raw_pairs + row / 32) * (kGroup * 32) + (row & 31),
+              32, sm, si);
 }
 
 // Attention of each sequence's 32 query heads over its side rows (per-head packed code pages; the reference keeps
@@ -971,9 +1012,18 @@ int abkv_decode_attn_window(const void* q, long q_stride_seq, long q_stride_head
   return (int)hipGetLastError();
 }
 
-// Partials of every split, then the raw scores: rows in whole page pairs per query head.
+// Whether a scored step takes a workgroup of eight waves per (sequence, KV head), which holds the rows' scores in LDS until it
+// knows their weights, instead of splits whose scores go through memory: 19 MB written among the reads of 64 sequences of 2304
+// rows cost 28 us of 138, and the partials, their merge and the second launch fall away too. us a step so / split, rows up to
+// 250, 1000 and 3000: 64 sequences 15.1 / 20.4, 49.8 / 59.0, 139 / 162; 24 7.6 / 10.3, 23.6 / 27.7, 63.4 / 67.2; 16 7.3 / 8.3,
+// 21.8 / 18.8 (500: 10.6 / 13.0); one 7.1 / 8.0, 13.7 / 8.0. Four to sixteen waves are within 5 %.
+static bool whole_sequences(int num_seqs, int max_pages_per_seq) {
+  return max_pages_per_seq <= abkv::kWholePages && (num_seqs >= 24 || max_pages_per_seq <= (num_seqs >= 16 ? 32 : 20));
+}
+
+// Partials of every split, then the raw scores: rows in whole page pairs.
 size_t abkv_decode_scored_workspace_size(int num_seqs, int max_pages_per_seq, int split_pages) {
-  if (num_seqs <= 0 || max_pages_per_seq <= 0 || split_pages <= 0) return 0;
+  if (num_seqs <= 0 || max_pages_per_seq <= 0 || split_pages <= 0 || whole_sequences(num_seqs, max_pages_per_seq)) return 0;
   const size_t rows = ((size_t)max_pages_per_seq + 1) / 2 * 2 * abkv::kPage;
   return abkv_decode_workspace_size(num_seqs, (max_pages_per_seq + split_pages - 1) / split_pages) +
          (size_t)num_seqs * abkv::kHeadsQ * rows * sizeof(float);
@@ -989,8 +1039,9 @@ int abkv_decode_attn_scored(const void* q, long q_stride_seq, long q_stride_head
   if (scores == nullptr || !decode_call_ok(q, kv_cache, num_pages, block_table, block_table_stride, seq_lens, num_seqs,
                                            max_pages_per_seq, split_pages, out))
     return (int)hipErrorInvalidValue;
-  if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
-      workspace_bytes < abkv_decode_scored_workspace_size(num_seqs, max_pages_per_seq, split_pages))
+  const bool whole = whole_sequences(num_seqs, max_pages_per_seq);
+  if (!whole && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
+                 workspace_bytes < abkv_decode_scored_workspace_size(num_seqs, max_pages_per_seq, split_pages)))
     return (int)hipErrorInvalidValue;
   const int max_splits = (max_pages_per_seq + split_pages - 1) / split_pages;
   DecodeArgs a{};
@@ -1014,10 +1065,18 @@ int abkv_decode_attn_scored(const void* q, long q_stride_seq, long q_stride_head
   a.part_ml = reinterpret_cast<float*>(a.part_o + (size_t)num_seqs * max_splits * kHeadsQ * kHeadDim);
   a.force_partials = 1;
   a.raw = reinterpret_cast<float*>(static_cast<char*>(workspace) + abkv_decode_workspace_size(num_seqs, max_splits));
-  a.raw_stride = (long)(max_pages_per_seq + 1) / 2 * 2 * kPage;
+  a.raw_pairs = (max_pages_per_seq + 1) / 2;
   a.scores = scores;
   a.s_sb = scores_stride_seq;
   a.s_sh = scores_stride_head;
+  if (whole) {
+    a.split_pages = max_pages_per_seq;
+    a.force_partials = 0;
+    const size_t lds = (size_t)kGroup * whole_stride(max_pages_per_seq) * sizeof(float);
+    hipLaunchKernelGGL((decode_attn_kernel<1, kWholeSub, kWhole>), dim3(kHeadsKV, num_seqs), dim3(64 * kWholeSub), lds, stream,
+                       a);
+    return (int)hipGetLastError();
+  }
   launch_decode<kScored>(a, max_splits, num_seqs, stream);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return (int)err;

@@ -1259,11 +1259,12 @@ def _check_scores(scores: torch.Tensor, B: int, rows: int) -> None:
         raise ValueError("scores must not share memory")
 
 
-def decode_scored_workspace(num_seqs: int, max_pages: int, split_pages: int | None = None, device=None) -> torch.Tensor:
-    """Workspace for :func:`decode_attention_scored` of the same sizes."""
+def decode_scored_workspace(num_seqs: int, max_pages: int, split_pages: int | None = None,
+                            device=None) -> torch.Tensor | None:
+    """Workspace for :func:`decode_attention_scored` of the same sizes (None when it takes none)."""
     split_pages = split_pages or _step_split_pages(num_seqs, max_pages)
-    return torch.empty(lib().abkv_decode_scored_workspace_size(num_seqs, max_pages, split_pages), dtype=torch.uint8,
-                       device=device)
+    n = lib().abkv_decode_scored_workspace_size(num_seqs, max_pages, split_pages)
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
 
 def decode_attention_scored(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -1274,7 +1275,8 @@ def decode_attention_scored(q: torch.Tensor, kv_cache: torch.Tensor, block_table
     scores[b, h, row] += the weights of KV head h's four query heads, for rows below seq_lens[b].
 
     ``scores`` [B, 8, rows] fp32, a row for each of the 16 * ``max_pages`` slots (zero for a new sequence), is updated in
-    place; each score has one owner, so equal calls give equal bits. ``split_pages`` None: chosen by the sizes. Returns (out [B, 32, 128] bf16, lse or None).
+    place; each score has one owner, so equal calls give equal bits. ``split_pages`` (None: chosen by the sizes): where
+    sequences are split at all. Returns (out [B, 32, 128] bf16, lse or None).
     """
     B, max_pages = _check_step(q, kv_cache, block_table, seq_lens, max_pages, split_pages, out, lse)
     _check_scores(scores, B, max_pages * PAGE)

@@ -489,7 +489,8 @@ int abkv_decode_attn_window(const void* q, long q_stride_seq, long q_stride_head
  * slot. Zero for a new sequence; abkv_kv_evict keeps them with the rows.
  *
  * abkv_decode_attn_scored: abkv_decode_attn, and scores[b][h][row] += sum of the step's weights for rows [0, seq_lens[b])
- * (others are left alone). workspace: abkv_decode_scored_workspace_size bytes, 16-byte aligned; num_seqs <= 65535. */
+ * (others are left alone). workspace: abkv_decode_scored_workspace_size bytes, 16-byte aligned (0: none needed, the step is
+ * not split); num_seqs <= 65535. */
 size_t abkv_decode_scored_workspace_size(int num_seqs, int max_pages_per_seq, int split_pages);
 int abkv_decode_attn_scored(const void* q, long q_stride_seq, long q_stride_head, const void* kv_cache, int num_pages,
                             const int32_t* block_table, long block_table_stride, const int32_t* seq_lens, int num_seqs,

@@ -105,6 +105,26 @@ def test_decode_more_sequences_than_share_splits():
         assert np.abs(scores[b, :, : lens[b]].double().cpu().numpy() - w).max() <= W_TOL
 
 
+@pytest.mark.parametrize("B,most", [(24, 4096), (30, 700), (16, 512), (17, 513), (5, 320), (5, 321), (1, 1), (26, 4097)])
+def test_decode_scored_whole_and_split(B, most):
+    """Sizes on both sides of the rule that picks a workgroup per sequence and head or splits."""
+    from abridgekv_amd import ops
+    rng = np.random.default_rng(B + most)
+    lens = [most] + [int(x) for x in rng.integers(0, min(most, 600), B - 1)] if B > 1 else [most]
+    q, k, v, cache, table, sl = _paged(lens, B)
+    M = table.shape[1] * 16
+    scores = torch.full((B, 8, M), 0.5, device="cuda")
+    lse = torch.empty((B, 32), device="cuda")
+    out, _ = ops.decode_attention_scored(q.cuda(), cache, table, sl, scores, lse=lse)
+    for b in {0, 1 % B, B // 2, B - 1}:
+        n = lens[b]
+        _close(out[b], lse[b], q[b], k[b], v[b], np.ones(n, bool))
+        assert (scores[b, :, n:] == 0.5).all()
+        if n:
+            w = oe.weights(q[b: b + 1].double().numpy(), k[b].double().numpy(), v[b].double().numpy(), [n - 1], SCALE)
+            assert np.abs(scores[b, :, :n].double().cpu().numpy() - 0.5 - w).max() <= W_TOL
+
+
 @pytest.mark.parametrize("split_pages", [2, 32])
 def test_decode_scored(split_pages):
     from abridgekv_amd import ops
