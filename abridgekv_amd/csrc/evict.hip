@@ -177,10 +177,10 @@ __global__ __launch_bounds__(64 * kScoreWaves) void prompt_scores_kernel(PromptS
 // evicted slots < m, both in ascending order, so a pass moves no more rows than it evicts and sources and destinations never
 // meet: attention does not depend on the order of rows, and the tokens' indices travel in `positions`.
 //
-// One workgroup of 16 waves per (layer, sequence, head) does it all: keys that order as (held, score) in LDS; the m-th
-// largest by four 8-bit digits of a histogram; each wave walks its own run of slots, so ranks among ties, holes and movers
-// are ballot counts plus one prefix over 16 waves; then rows, scores and positions move. Bound by the latency of these
-// phases for one sequence, by the moved rows for a batch.
+// One workgroup per (layer, sequence, head) does it all: keys that order as (held, score) in LDS; the m-th largest by up to
+// four 8-bit digits of a histogram (no further than the rows that share its digits are kept all); each wave walks its own run
+// of slots, so ranks among ties, holes and movers are ballot counts plus one prefix over the waves; then rows, scores and
+// positions move. Bound by the latency of these phases for one sequence, by the moved rows (256-byte pieces) for a batch.
 struct EvictArgs {
   __bf16* caches[16];
   int num_pages;
@@ -204,18 +204,17 @@ __device__ __forceinline__ uint32_t score_key(float x, bool held) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int kEvictWaves = 16;
 constexpr int kEvictMaxRows = 1 << 18;         // rows whose kept bits fit LDS beside the rest
 
-template <int kSlots>
-__global__ __launch_bounds__(64 * kEvictWaves) void evict_kernel(EvictArgs a) {
-  constexpr int kThreads = 64 * kEvictWaves;
+template <int kSlots, int kWaves>
+__global__ __launch_bounds__(64 * kWaves) void evict_kernel(EvictArgs a) {
+  constexpr int kThreads = 64 * kWaves;
   constexpr int kCopies = 8;                                 // of the histogram: most scores share their first digit
   __shared__ uint32_t lds_keys[kSlots > 0 ? kSlots : 1];
   __shared__ uint64_t kept_bits[(kSlots > 0 ? kSlots : kEvictMaxRows) / 64];
   __shared__ uint32_t hist[256 * kCopies];
-  __shared__ int counts[kEvictWaves][2];
-  __shared__ uint32_t pick[2];
+  __shared__ int counts[kWaves][2];
+  __shared__ int pick[3];
   const int h = blockIdx.x % kHeadsKV;
   const int lb = blockIdx.x / kHeadsKV;
   const int b = lb % a.batch, layer = lb / a.batch;
@@ -269,16 +268,18 @@ __global__ __launch_bounds__(64 * kEvictWaves) void evict_kernel(EvictArgs a) {
         while (i < 3 && want > above + c[i]) above += c[i++];
         pick[0] = 255 - 4 * lane - i;
         pick[1] = want - above;
+        pick[2] = i == 0 ? c[0] : i == 1 ? c[1] : i == 2 ? c[2] : c[3];
       }
     }
     __syncthreads();
-    prefix |= pick[0] << shift;
+    prefix |= (uint32_t)pick[0] << shift;
     mask |= 255u << shift;
     want = pick[1];
+    if (want == pick[2]) break;                              // (uniform) all keys with these digits are kept
   }
   // kept: keys above the prefix, and the first `want` that equal it
   int ties = 0;
-  for (int s = s0 + lane; s - lane < s1; s += 64) ties += __popcll(__ballot(s < s1 && keys[min(s, n - 1)] == prefix));
+  for (int s = s0 + lane; s - lane < s1; s += 64) ties += __popcll(__ballot(s < s1 && (keys[min(s, n - 1)] & mask) == prefix));
   if (lane == 0) counts[w][0] = ties;
   __syncthreads();
   int rank = 0;
@@ -287,7 +288,7 @@ __global__ __launch_bounds__(64 * kEvictWaves) void evict_kernel(EvictArgs a) {
   const uint64_t below = (1ull << lane) - 1;
   int holes = 0, movers = 0;
   for (int s = s0 + lane; s - lane < s1; s += 64) {
-    const uint32_t k = keys[min(s, n - 1)];
+    const uint32_t k = keys[min(s, n - 1)] & mask;
     const uint64_t eq = __ballot(s < s1 && k == prefix);
     const bool keep = s < s1 && (k > prefix || (k == prefix && rank + __popcll(eq & below) < want));
     rank += __popcll(eq);
@@ -302,7 +303,7 @@ __global__ __launch_bounds__(64 * kEvictWaves) void evict_kernel(EvictArgs a) {
   }
   __syncthreads();                                           // every wave is done with the keys: their place takes the lists
   int hole_at = 0, mover_at = 0, total = 0;
-  for (int i = 0; i < kEvictWaves; ++i) {
+  for (int i = 0; i < kWaves; ++i) {
     hole_at += i < w ? counts[i][0] : 0;
     mover_at += i < w ? counts[i][1] : 0;
     total += counts[i][0];
@@ -401,7 +402,7 @@ int abkv_kv_evict(void* const* layer_caches, int num_layers, int num_pages, cons
   const size_t need = abkv_kv_evict_workspace_size(num_layers, num_seqs, max_pages_per_seq);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return (int)hipErrorInvalidValue;
   const long grid = (long)num_layers * num_seqs * kHeadsKV;
-  if (grid * 64 * kEvictWaves > 0xFFFFFFFFL) return (int)hipErrorInvalidValue;
+  if (grid * 1024 > 0xFFFFFFFFL) return (int)hipErrorInvalidValue;
   EvictArgs a{};
   for (int l = 0; l < num_layers; ++l) {
     if (layer_caches[l] == nullptr) return (int)hipErrorInvalidValue;
@@ -422,11 +423,15 @@ int abkv_kv_evict(void* const* layer_caches, int num_layers, int num_pages, cons
   a.recent = recent;
   a.out_lens = out_lens;
   a.work = static_cast<uint32_t*>(workspace);
-  // by the LDS the keys take: two workgroups a CU up to 4096 rows (their 32 waves), one above
-  const dim3 g((unsigned)grid), t(64 * kEvictWaves);
-  if (a.max_rows <= 4096) hipLaunchKernelGGL(evict_kernel<4096>, g, t, 0, stream, a);
-  else if (a.max_rows <= 32768) hipLaunchKernelGGL(evict_kernel<32768>, g, t, 0, stream, a);
-  else hipLaunchKernelGGL(evict_kernel<0>, g, t, 0, stream, a);
+  // 16 waves end a launch that fills the GPU once soonest; more workgroups a CU overlap one's selection with another's moves. us
+  // with 16 / 8 / 4 waves (six layers): 1 sequence of 2560 rows 15.5 / 17.8 / 23.4, 8 29.7 / 32.3 / 38.3, 64 227 / 218 / 228; 64
+  // of 600 rows 82 / 65 / 59. Above 4096 rows LDS holds one workgroup a CU.
+  const dim3 g((unsigned)grid);
+  if (a.max_rows <= 1024 && grid >= 1024) hipLaunchKernelGGL((evict_kernel<1024, 4>), g, dim3(256), 0, stream, a);
+  else if (a.max_rows <= 4096 && grid >= 1024) hipLaunchKernelGGL((evict_kernel<4096, 8>), g, dim3(512), 0, stream, a);
+  else if (a.max_rows <= 4096) hipLaunchKernelGGL((evict_kernel<4096, 16>), g, dim3(1024), 0, stream, a);
+  else if (a.max_rows <= 32768) hipLaunchKernelGGL((evict_kernel<32768, 16>), g, dim3(1024), 0, stream, a);
+  else hipLaunchKernelGGL((evict_kernel<0, 16>), g, dim3(1024), 0, stream, a);
   return (int)hipGetLastError();
 }
 

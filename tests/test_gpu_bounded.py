@@ -230,6 +230,13 @@ def test_evict(budget, sinks, recent, levels, recorded):
     _check_evict(*_evict_case(lens, budget + (levels or 0), levels=levels, recorded=recorded), budget, sinks, recent)
 
 
+@pytest.mark.parametrize("most,budget", [(300, 100), (1024, 700), (1040, 999)])
+def test_evict_many_sequences(most, budget):
+    """Enough workgroups for the forms of fewer waves."""
+    lens = [most] + [int(x) for x in np.random.default_rng(most).integers(0, min(most, 320), 64)]
+    _check_evict(*_evict_case(lens, most, layers=2, levels=200), budget, 3, 40)
+
+
 def test_evict_odd_scores():
     """NaN, infinities, both zeros and negative scores; ties of all kinds."""
     case = list(_evict_case([200, 130], 9, layers=1))
