@@ -263,15 +263,24 @@ class AbridgeMetadataBuilder:
 
 
 class AbridgeAttentionImpl:
-    """Backend implementation for one attention layer (32 query heads, 8 KV heads, head size 128, bf16)."""
+    """Backend implementation for one attention layer (32 query heads, 8 KV heads, head size 128, bf16).
+
+    ``sliding_window`` W: a token sees the W rows up to its own and the first ``sinks`` rows of its sequence; decodes then
+    read only the window's and the sinks' pages. Code steps see their whole context, so a windowed layer refuses them."""
 
     def __init__(self, num_heads: int = ops.HEADS_Q, head_size: int = ops.HEAD_DIM, scale: float | None = None,
-                 num_kv_heads: int = ops.HEADS_KV, kv_cache_dtype: str = "auto"):
+                 num_kv_heads: int = ops.HEADS_KV, kv_cache_dtype: str = "auto", sliding_window: int | None = None,
+                 sinks: int = 0):
         if (num_heads, head_size, num_kv_heads) != (ops.HEADS_Q, ops.HEAD_DIM, ops.HEADS_KV):
             raise NotImplementedError(f"kernels are built for {ops.HEADS_Q} q heads, {ops.HEADS_KV} KV heads, "
                                       f"head size {ops.HEAD_DIM}")
         if kv_cache_dtype not in ("auto", "bfloat16"):
             raise NotImplementedError("kv cache dtype must be bf16")
+        if sliding_window is None and sinks:
+            raise ValueError("sinks need a sliding_window")
+        if sliding_window is not None and (sliding_window < 1 or sinks < 0):
+            raise ValueError("sliding_window must be >= 1 and sinks >= 0")
+        self.sliding_window, self.sinks = sliding_window, sinks
         self.num_heads, self.head_size, self.num_kv_heads = num_heads, head_size, num_kv_heads
         self.scale = ops.default_scale() if scale is None else float(scale)
 
@@ -298,6 +307,8 @@ class AbridgeAttentionImpl:
     def attend(self, q: torch.Tensor, kv_cache: torch.Tensor, md: AbridgeAttentionMetadata, out: torch.Tensor,
                lse: torch.Tensor | None = None) -> None:
         """Attention only (the cache already holds this step's rows): decodes, then chunks and code steps."""
+        if self.sliding_window is not None:
+            return self._attend_window(q, kv_cache, md, out, lse)
         nd, nd_tok, n_tok = md.num_decodes, md.num_decode_tokens, md.num_actual_tokens
         if nd:
             torch.ops.abridgekv.decode_attn(q[:nd_tok], kv_cache, md.block_table[:nd], md.seq_lens_dev[:nd],
@@ -318,6 +329,27 @@ class AbridgeAttentionImpl:
                                         np.where(code, lim, sl), causal, self.scale,
                                         out=out[nd_tok:n_tok], lse=None if lse is None else lse[nd_tok:n_tok],
                                         excluded=ex)
+
+    def _attend_window(self, q, kv_cache, md: AbridgeAttentionMetadata, out, lse) -> None:
+        """:meth:`attend` of a layer with a sliding window."""
+        nd, nd_tok, n_tok = md.num_decodes, md.num_decode_tokens, md.num_actual_tokens
+        if not md.causal or (md.code_key_limit != NOT_CODE).any():
+            raise NotImplementedError("a sliding-window layer takes causal requests only")
+        if nd:
+            # the builder's workspace holds splits of 32 pages of every row; shorter ones where they fit too
+            pages, held = md.max_decode_pages, md.workspace.numel() if md.workspace is not None else 0
+            split = ops.window_split_pages(nd, pages, self.sliding_window, self.sinks)
+            if ops.decode_window_bytes(nd, pages, self.sliding_window, self.sinks, split) > held:
+                split = ops.DEFAULT_SPLIT_PAGES
+            torch.ops.abridgekv.decode_attn_window(q[:nd_tok], kv_cache, md.block_table[:nd], md.seq_lens_dev[:nd],
+                                                   self.sliding_window, self.sinks, self.scale, pages, split,
+                                                   out[:nd_tok], None if lse is None else lse[:nd_tok], md.workspace)
+        if nd < md.num_reqs and n_tok > nd_tok:
+            qsl = md.query_start_loc[nd:] - nd_tok
+            ops.paged_prefill_attention_window(q[nd_tok:n_tok], kv_cache, md.block_table[nd:], qsl,
+                                               md.seq_lens[nd:] - np.diff(qsl), self.sliding_window, self.sinks,
+                                               scale=self.scale, out=out[nd_tok:n_tok],
+                                               lse=None if lse is None else lse[nd_tok:n_tok])
 
 
 class AbridgeAttentionBackend:

@@ -20,6 +20,9 @@ every decoder layer runs ``abkv_prefill_masked_attn`` through a HuggingFace atte
 is never materialised: the kernel evaluates it from (C, K, L, R, N, prompt_len, head quota, tail, xattn); layouts off
 the 64-row tile grid, L > 1, replay rows, the raw tail and non-full xattn take its walk over segments.
 
+A :class:`WindowMask` in place of the compression mask runs the sliding-window kernels (``baseline_loss(window=, sinks=)``,
+and any layer with a ``sliding_window`` of its own).
+
 The raw tail (``raw_tail`` = W, a training ablation the reference's serving refuses, compress_forward.py:89-96):
 content row i of the next block sees the block's last W - i content rows (the rolling window of a retained tail),
 and the block's codes see their whole block.
@@ -559,15 +562,21 @@ class CompressLM(nn.Module):
                           use_cache=False).logits
 
     def baseline_loss(self, content_ids, ce_chunk=0, ctx_blocks=0, block_ce=False, resp_mask=None, per_token=False,
-                      include_cross_block=False):
+                      include_cross_block=False, window=0, sinks=0):
         """Plain causal LM without compression on the same predict positions (compress_forward.py:1095-1132):
-        sequences of ``ctx_blocks`` contiguous blocks (0: all N, the full-context ceiling; 1: the floor)."""
+        sequences of ``ctx_blocks`` contiguous blocks (0: all N, the full-context ceiling; 1: the floor). ``window`` > 0:
+        attention under a sliding window of that many tokens with the first ``sinks`` visible, the context of bounded size
+        that a compressed one is compared with."""
+        if sinks and not window:
+            raise ValueError("sinks need a window")
         B, N, C = content_ids.shape
         G = ctx_blocks if ctx_blocks else N
         if N % G:
             raise ValueError(f"ctx_blocks={G} must divide N={N}")
         flat = content_ids.reshape(B * (N // G), G * C)
-        out = self.model.model(inputs_embeds=self._embed_for_plain_forward(flat), use_cache=False).last_hidden_state
+        mask = {"full_attention": WindowMask(int(window), int(sinks))} if window else None
+        out = self.model.model(inputs_embeds=self._embed_for_plain_forward(flat), attention_mask=mask,
+                               use_cache=False).last_hidden_state
         ar = torch.arange(G * C, device=flat.device)
         pos = ar[:-1] if include_cross_block else ar[(ar % C) != (C - 1)]
         hid = out[:, pos, :].reshape(-1, out.size(-1))
@@ -621,16 +630,21 @@ class CompressLM(nn.Module):
     def forward(self, content_ids, distill_lambda=0.0, copy_lambda=0.0, distill_temp=1.0, ce_chunk=0, baseline=False,
                 ctx_blocks=0, teacher_logits=None, teacher_hidden=None, block_ce=False, resp_mask=None,
                 raw_prompt=False, blockmask=None, per_token=False, include_cross_block=False,
-                boundary_recovery_width=0, boundary_recovery_weight=1.0, teacher_rows=None, teacher_head=None):
+                boundary_recovery_width=0, boundary_recovery_weight=1.0, teacher_rows=None, teacher_head=None,
+                window=0, sinks=0):
         """Losses of the compressed teacher-forced forward, same signature, control flow and return dicts as
         compress_forward.py:1134-1315: the full-context baseline, CE (masked by ``resp_mask``, per block, per
         token), self- or teacher distillation (KL at ``distill_temp``), the chunked frozen-teacher KD
         (``teacher_rows`` / ``teacher_head``), the copy loss (``copy_lambda``: the copy region reproduces the last
         block from its codes) and the representation loss (``teacher_hidden``). ``blockmask``: a prebuilt
-        :class:`CompressMask` (the analogue of the reference's prebuilt BlockMask)."""
+        :class:`CompressMask` (the analogue of the reference's prebuilt BlockMask). ``window``, ``sinks``: of the baseline
+        (:meth:`baseline_loss`)."""
         if baseline:
             return self.baseline_loss(content_ids, ce_chunk, ctx_blocks, block_ce=block_ce, resp_mask=resp_mask,
-                                      per_token=per_token, include_cross_block=include_cross_block)
+                                      per_token=per_token, include_cross_block=include_cross_block, window=window,
+                                      sinks=sinks)
+        if window or sinks:
+            raise ValueError("a window is an option of the baseline")
         B, N, C = content_ids.shape
         dev = content_ids.device
         with_copy = copy_lambda > 0

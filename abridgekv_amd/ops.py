@@ -1173,7 +1173,7 @@ def _window_pages(max_pages: int, window: int, sinks: int) -> int:
     return min(max_pages, -(-sinks // PAGE) + -(-window // PAGE) + 1)
 
 
-def _window_split_pages(num_seqs: int, max_pages: int, window: int, sinks: int) -> int:
+def window_split_pages(num_seqs: int, max_pages: int, window: int, sinks: int) -> int:
     """Pages per split of a window step: up to 28 pages one split, which eight waves share and no merge follows (us for windows
     of 250 rows, sequences 1 / 16 / 64: 6.9 / 7.0 / 18.4, split in shorter ones 7.3 / 8.9 / 19.7; of 500: 8.8 / 12.2 / 29.8
     against 8.0 / 13.2 / 30.1)."""
@@ -1213,11 +1213,16 @@ def _take_workspace(workspace, need: int, device):
     return workspace, nbytes
 
 
+def decode_window_bytes(num_seqs: int, max_pages: int, window: int, sinks: int, split_pages: int) -> int:
+    """Workspace bytes that :func:`decode_attention_window` takes with ``split_pages`` pages a split."""
+    return lib().abkv_decode_window_workspace_size(num_seqs, max_pages, split_pages, window, sinks)
+
+
 def decode_window_workspace(num_seqs: int, max_pages: int, window: int, sinks: int = 0, split_pages: int | None = None,
                             device=None) -> torch.Tensor | None:
     """Workspace for :func:`decode_attention_window` of the same sizes (None when no sequence can need a second split)."""
-    split_pages = split_pages or _window_split_pages(num_seqs, max_pages, window, sinks)
-    n = lib().abkv_decode_window_workspace_size(num_seqs, max_pages, split_pages, *_check_window(window, sinks))
+    split_pages = split_pages or window_split_pages(num_seqs, max_pages, window, sinks)
+    n = decode_window_bytes(num_seqs, max_pages, *_check_window(window, sinks), split_pages)
     return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
 
@@ -1236,7 +1241,7 @@ def decode_attention_window(q: torch.Tensor, kv_cache: torch.Tensor, block_table
     _check_device(q, kv_cache, block_table, seq_lens, out, lse)
     if out is None:
         out = torch.empty((B, HEADS_Q, HEAD_DIM), dtype=torch.bfloat16, device=q.device)
-    split_pages = split_pages or _window_split_pages(B, max_pages, window, sinks)
+    split_pages = split_pages or window_split_pages(B, max_pages, window, sinks)
     need = lib().abkv_decode_window_workspace_size(B, max_pages, split_pages, window, sinks)
     workspace, ws_bytes = _take_workspace(workspace, need, q.device)
     scale = default_scale() if scale is None else float(scale)
@@ -1339,7 +1344,8 @@ def paged_prefill_scores(q: torch.Tensor, kv_cache: torch.Tensor, block_table: t
 
 def kv_evict(layer_caches, block_table: torch.Tensor, seq_lens: torch.Tensor, scores: torch.Tensor,
              positions: torch.Tensor, num_tokens: torch.Tensor, budget: int, sinks: int = 0, recent: int = 0,
-             max_pages: int | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+             max_pages: int | None = None, out: torch.Tensor | None = None,
+             workspace: torch.Tensor | None = None) -> torch.Tensor:
     """Evict the rows that weigh least from up to 16 layer caches, in place. Returns the new lengths [B] int32.
 
     Per (layer, sequence, KV head) of n = seq_lens[b] rows, min(n, ``budget``) are kept: rows of the first ``sinks`` and the
@@ -1351,7 +1357,8 @@ def kv_evict(layer_caches, block_table: torch.Tensor, seq_lens: torch.Tensor, sc
     ``scores`` fp32 and ``positions`` int32 [L, B, 8, rows], contiguous, a row for each of the 16 * ``max_pages`` slots.
     ``positions`` hold each row's token index; -1 (also what a new sequence starts with) marks rows appended since the last
     eviction: their index is num_tokens[b] - (n - row). ``seq_lens`` and ``num_tokens`` [B] int32. The sequences' pages must
-    be their own. ``max_pages`` (default: the table's width, at most 16384) bounds ceil(seq_len / 16).
+    be their own. ``max_pages`` (default: the table's width, at most 16384) bounds ceil(seq_len / 16). ``out`` [B] int32 (not
+    ``seq_lens``): where the new lengths go.
     """
     L, W = len(layer_caches), block_table.shape[1] if block_table.dim() == 2 else 0
     budget, sinks, recent = int(budget), int(sinks), int(recent)
@@ -1379,11 +1386,15 @@ def kv_evict(layer_caches, block_table: torch.Tensor, seq_lens: torch.Tensor, sc
             raise ValueError("layer caches must be contiguous bf16 of one shape")
     if len(shape) != 5 or shape[1:] != _PAGE_SHAPE or shape[0] == 0:
         raise ValueError(f"layer caches must be [P, 2, {PAGE}, {HEADS_KV}, {HEAD_DIM}], got {tuple(shape)}")
-    _check_device(block_table, seq_lens, num_tokens, scores, positions, *layer_caches)
+    if out is None:
+        out = torch.empty_like(seq_lens)
+    elif (out.dtype is not torch.int32 or out.shape != (B,) or not out.is_contiguous()
+          or (B and out.data_ptr() == seq_lens.data_ptr())):
+        raise ValueError("out must be contiguous int32 [B] apart from seq_lens")
+    _check_device(block_table, seq_lens, num_tokens, scores, positions, out, *layer_caches)
     ptrs = [c.data_ptr() for c in layer_caches]
     _require(len(set(ptrs)) == L, "a layer cache may be given once")
     arr, num_pages = (C.c_void_p * L)(*ptrs), shape[0]
-    out = torch.empty_like(seq_lens)
     if B == 0:
         return out
     workspace, ws_bytes = _take_workspace(workspace, lib().abkv_kv_evict_workspace_size(L, B, max_pages), scores.device)

@@ -252,3 +252,93 @@ def _prefill_masked_attn_bwd_fake(q, k, v, out, lse, dout, block_c, codes_k, num
 
 OPS = ("decode_attn", "kv_append", "rope_kv_append", "slot_mapping", "kv_move_segments", "kv_move_mixed",
        "moves_expand", "paged_prefill_attn", "prefill_masked_attn", "prefill_masked_attn_bwd")
+
+
+# -- contexts of bounded size: sliding window with sinks, accumulated weights, eviction -------------------------------
+def _step_checks(q, kv_cache, out):
+    _need(q.dim() == 3 and tuple(q.shape[1:]) == (_ops.HEADS_Q, _ops.HEAD_DIM), "q must be [B, 32, 128]")
+    _need(tuple(out.shape) == tuple(q.shape), "out must be [B, 32, 128]")
+    _need(kv_cache.dim() == 5, "kv_cache must be [P, 2, 16, 8, 128]")
+
+
+@torch.library.custom_op(f"{_NS}::decode_attn_window", mutates_args=("out", "lse", "workspace"))
+def decode_attn_window(q: Tensor, kv_cache: Tensor, block_table: Tensor, seq_lens: Tensor, window: int, sinks: int,
+                       scale: float, max_pages: int, split_pages: int, out: Tensor, lse: Optional[Tensor],
+                       workspace: Optional[Tensor]) -> None:
+    """abkv_decode_attn_window: decode under a sliding window with sinks. A batch that needs more than one split must
+    bring ``workspace`` (ops.decode_window_workspace): the op never allocates."""
+    if lib().abkv_decode_window_workspace_size(q.shape[0], max_pages, split_pages, window, sinks):
+        _need(workspace is not None, "decode_attn_window: the batch needs a workspace (ops.decode_window_workspace)")
+    _ops.decode_attention_window(q, kv_cache, block_table, seq_lens, window, sinks, scale, max_pages=max_pages, out=out,
+                                 lse=lse, split_pages=split_pages, workspace=workspace)
+
+
+@decode_attn_window.register_fake
+def _decode_attn_window_fake(q, kv_cache, block_table, seq_lens, window, sinks, scale, max_pages, split_pages, out, lse,
+                             workspace):
+    _step_checks(q, kv_cache, out)
+
+
+@torch.library.custom_op(f"{_NS}::decode_attn_scored", mutates_args=("scores", "out", "lse", "workspace"))
+def decode_attn_scored(q: Tensor, kv_cache: Tensor, block_table: Tensor, seq_lens: Tensor, scores: Tensor, scale: float,
+                       max_pages: int, split_pages: int, out: Tensor, lse: Optional[Tensor],
+                       workspace: Optional[Tensor]) -> None:
+    """abkv_decode_attn_scored: decode that adds its weights to the rows' scores. Sizes that need one must bring
+    ``workspace`` (ops.decode_scored_workspace): the op never allocates."""
+    if lib().abkv_decode_scored_workspace_size(q.shape[0], max_pages, split_pages):
+        _need(workspace is not None, "decode_attn_scored: the batch needs a workspace (ops.decode_scored_workspace)")
+    _ops.decode_attention_scored(q, kv_cache, block_table, seq_lens, scores, scale, max_pages=max_pages, out=out, lse=lse,
+                                 split_pages=split_pages, workspace=workspace)
+
+
+@decode_attn_scored.register_fake
+def _decode_attn_scored_fake(q, kv_cache, block_table, seq_lens, scores, scale, max_pages, split_pages, out, lse,
+                             workspace):
+    _step_checks(q, kv_cache, out)
+    _need(scores.dim() == 3 and scores.shape[1] == _ops.HEADS_KV, "scores must be [B, 8, rows]")
+
+
+@torch.library.custom_op(f"{_NS}::kv_evict", mutates_args=("layer_caches", "scores", "positions", "out_lens", "workspace"))
+def kv_evict(layer_caches: list[Tensor], block_table: Tensor, seq_lens: Tensor, scores: Tensor, positions: Tensor,
+             num_tokens: Tensor, budget: int, sinks: int, recent: int, max_pages: int, out_lens: Tensor,
+             workspace: Optional[Tensor]) -> None:
+    """abkv_kv_evict: the rows that weigh least leave up to 16 layer caches, the new lengths go to out_lens [B]. More than
+    2048 pages a sequence need ``workspace``."""
+    if lib().abkv_kv_evict_workspace_size(len(layer_caches), seq_lens.numel(), max_pages):
+        _need(workspace is not None, "kv_evict: the batch needs a workspace")
+    _ops.kv_evict(layer_caches, block_table, seq_lens, scores, positions, num_tokens, budget, sinks, recent,
+                  max_pages=max_pages, out=out_lens, workspace=workspace)
+
+
+@kv_evict.register_fake
+def _kv_evict_fake(layer_caches, block_table, seq_lens, scores, positions, num_tokens, budget, sinks, recent, max_pages,
+                   out_lens, workspace):
+    _need(0 < len(layer_caches) <= 16, "between 1 and 16 layer caches per call")
+    _need(scores.shape == positions.shape and out_lens.shape == seq_lens.shape, "scores / positions, out_lens / seq_lens")
+
+
+@torch.library.custom_op(f"{_NS}::window_attn", mutates_args=("out", "lse"))
+def window_attn(q: Tensor, k: Tensor, v: Tensor, window: int, sinks: int, seq_lens: Optional[Tensor], scale: float,
+                out: Tensor, lse: Optional[Tensor]) -> None:
+    """abkv_window_attn: attention of whole prompts under a sliding window with sinks, q [B, S, 32, 128]."""
+    _ops.window_attention(q, k, v, window, sinks, seq_lens=seq_lens, scale=scale, out=out, lse=lse)
+
+
+@window_attn.register_fake
+def _window_attn_fake(q, k, v, window, sinks, seq_lens, scale, out, lse):
+    _need(tuple(out.shape) == tuple(q.shape), "out must be [B, S, 32, 128]")
+
+
+@torch.library.custom_op(f"{_NS}::window_attn_bwd", mutates_args=())
+def window_attn_bwd(q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor, dout: Tensor, window: int, sinks: int,
+                    seq_lens: Optional[Tensor], scale: float) -> tuple[Tensor, Tensor, Tensor]:
+    """abkv_window_attn_bwd: (dq, dk, dv) of sum(dout * out) under the same window (new tensors)."""
+    return _ops.window_attention_backward(q, k, v, out, lse, dout, window, sinks, seq_lens=seq_lens, scale=scale)
+
+
+@window_attn_bwd.register_fake
+def _window_attn_bwd_fake(q, k, v, out, lse, dout, window, sinks, seq_lens, scale):
+    return (q.new_empty(q.shape), k.new_empty(k.shape), k.new_empty(k.shape))
+
+
+BOUNDED_OPS = ("decode_attn_window", "decode_attn_scored", "kv_evict", "window_attn", "window_attn_bwd")
