@@ -26,6 +26,7 @@ __global__ __launch_bounds__(512, 1) void window_attn_kernel(WindowArgs a, Chunk
   constexpr int H = 2, kWaves = 8;
   __shared__ __attribute__((aligned(16))) __bf16 K0[kTileElems], K1[kTileElems], K2[kTileElems];
   __shared__ __attribute__((aligned(16))) __bf16 V0[kTileElems], V1[kTileElems], V2[kTileElems];
+  __shared__ __attribute__((aligned(16))) __bf16 Ks[kTileElems];           // the sinks, where they are few
   __bf16* const Kbuf[kStages] = {K0, K1, K2};
   __bf16* const Vbuf[kStages] = {V0, V1, V2};
   // KV head fastest: workgroups go to the 8 XCDs round-robin, so one XCD's L2 serves a head's rows to all its tiles. Then the
@@ -75,17 +76,31 @@ __global__ __launch_bounds__(512, 1) void window_attn_kernel(WindowArgs a, Chunk
     m_run[u] = -INFINITY;
     l_run[u] = 0.f;
   }
-  WindowWalk walk(kv0 + q0, kv0 + min(q0 + kBM, n_q) - 1, a.window, a.sinks);
-  const WindowLane lm(kv0 + qi, seen, a.window, a.sinks);
   if (q0 < n_q) {                                            // (uniform)
-    if constexpr (kPaged) {
-      const PagedRows rows{c.kv + kvh * kHeadDim, c.block_table + (long)b * c.bt_stride, c.bt_width, c.num_pages};
+    const bool few = short_sinks(kv0 + q0, a.window, a.sinks);
+    const int sinks = few ? 0 : a.sinks;                     // the walk's
+    WindowWalk walk(kv0 + q0, kv0 + min(q0 + kBM, n_q) - 1, a.window, sinks);
+    const WindowLane lm(kv0 + qi, seen, a.window, sinks);
+    float m0[H], l0[H];                                      // the sinks' own
+    auto attend = [&](const auto& rows) {
+      if (few) {
+        issue_sinks(rows, n, Ks, w, lane);
+        __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        attend_sinks<H>(Ks, a.sinks, qop, o, m_run, l0, a.scale_log2, lane);
+#pragma unroll
+        for (int u = 0; u < H; ++u) m0[u] = m_run[u];
+      }
       attend_tiles<H, kWaves>(rows, walk, n, Kbuf, Vbuf, qop, o, m_run, l_run, lm, a.scale_log2, w, lane);
-    } else {
-      const DenseRows<false> rows{a.k + (long)b * a.k_sb + (long)kvh * a.k_sh, a.v + (long)b * a.v_sb + (long)kvh * a.v_sh,
-                                  a.k_ss, a.v_ss};
-      attend_tiles<H, kWaves>(rows, walk, n, Kbuf, Vbuf, qop, o, m_run, l_run, lm, a.scale_log2, w, lane);
-    }
+#pragma unroll
+      for (int u = 0; u < H; ++u)
+        if (few) l_run[u] += l0[u] * fast_exp2(m0[u] - m_run[u]);
+    };
+    if constexpr (kPaged)
+      attend(PagedRows{c.kv + kvh * kHeadDim, c.block_table + (long)b * c.bt_stride, c.bt_width, c.num_pages});
+    else
+      attend(DenseRows<false>{a.k + (long)b * a.k_sb + (long)kvh * a.k_sh, a.v + (long)b * a.v_sb + (long)kvh * a.v_sh,
+                              a.k_ss, a.v_ss});
   }
   if (qi >= (kPaged ? n_q : a.S)) return;
   const long o_row = kPaged ? (long)(t0 + qi) * a.o_ss : (long)b * a.o_sb + (long)qi * a.o_ss;
