@@ -107,15 +107,16 @@ class _MaskedPrefill(torch.autograd.Function):
 @dataclass(frozen=True)
 class WindowMask:
     """Causal attention under a sliding window with sinks: row i sees row j when j <= i and (i - j < ``window`` or
-    j < ``sinks``); ``seq_lens`` [B] int32 on the GPU: rows past a sequence's length are padding (None: none)."""
+    j < ``sinks``); ``seq_lens`` [B] int32 on the GPU: rows past a sequence's length are padding (None: none). As with any
+    autograd function, a backward pass is captured into a graph only when no eager graph of the same leaves is alive."""
     window: int
     sinks: int = 0
     seq_lens: torch.Tensor | None = None
 
 
 class _WindowAttention(torch.autograd.Function):
-    """The sliding-window kernels and their backward (abkv_window_attn / _bwd): query, key and value [B, heads, S, 128] as the
-    layers hand them, out [B, S, 32, 128]."""
+    """The sliding-window kernels and their backward (abkv_window_attn / _bwd): query, key and value [B, heads, S, 128] as
+    the layers hand them, out [B, S, 32, 128]."""
 
     @staticmethod
     def forward(ctx, query, key, value, mask: WindowMask, scale: float):

@@ -847,7 +847,8 @@ int abkv_window_attn_f32(const float* q, long q_stride_b, long q_stride_s, long 
                          hipStream_t stream) {
   using namespace abkv;
   if (batch <= 0 || seq_len <= 0) return 0;
-  if (q == nullptr || k == nullptr || v == nullptr || out == nullptr || window <= 0 || sinks < 0)
+  if (q == nullptr || k == nullptr || v == nullptr || out == nullptr || window <= 0 || sinks < 0 ||
+      !softmax_scale_ok(scale) || !row_strides_ok(q_stride_s, k_stride_s, v_stride_s))
     return (int)hipErrorInvalidValue;
   F32Args a = f32_defaults();
   a.q = q;

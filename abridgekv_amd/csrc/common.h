@@ -7,6 +7,11 @@
 
 namespace abkv {
 
+// Arguments of the sliding-window and weight entries: scores are masked before they are scaled, so a scale is positive and
+// finite; the tile loads keep 64 rows' offsets in 32 bits.
+inline bool softmax_scale_ok(float scale) { return scale > 0.f && scale < INFINITY; }
+inline bool row_strides_ok(long a, long b = 0, long c = 0, long d = 0, long e = 0) { return ((a | b | c | d | e) >> 24) == 0; }
+
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));

@@ -978,8 +978,9 @@ int abkv_decode_attn_window(const void* q, long q_stride_seq, long q_stride_head
                             size_t workspace_bytes, hipStream_t stream) {
   using namespace abkv;
   if (num_seqs <= 0) return 0;
-  if (window <= 0 || sinks < 0 || !decode_call_ok(q, kv_cache, num_pages, block_table, block_table_stride, seq_lens, num_seqs,
-                                                  max_pages_per_seq, split_pages, out))
+  if (window <= 0 || sinks < 0 || !softmax_scale_ok(scale) ||
+      !decode_call_ok(q, kv_cache, num_pages, block_table, block_table_stride, seq_lens, num_seqs, max_pages_per_seq,
+                      split_pages, out))
     return (int)hipErrorInvalidValue;
   const int max_splits = window_splits(max_pages_per_seq, split_pages, window, sinks);
   if (max_splits > 1 && (workspace == nullptr || workspace_bytes < abkv_decode_workspace_size(num_seqs, max_splits)))
@@ -1036,8 +1037,9 @@ int abkv_decode_attn_scored(const void* q, long q_stride_seq, long q_stride_head
                             void* workspace, size_t workspace_bytes, hipStream_t stream) {
   using namespace abkv;
   if (num_seqs <= 0) return 0;
-  if (scores == nullptr || !decode_call_ok(q, kv_cache, num_pages, block_table, block_table_stride, seq_lens, num_seqs,
-                                           max_pages_per_seq, split_pages, out))
+  if (scores == nullptr || !softmax_scale_ok(scale) ||
+      !decode_call_ok(q, kv_cache, num_pages, block_table, block_table_stride, seq_lens, num_seqs, max_pages_per_seq,
+                      split_pages, out))
     return (int)hipErrorInvalidValue;
   const bool whole = whole_sequences(num_seqs, max_pages_per_seq);
   if (!whole && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) ||

@@ -91,8 +91,9 @@ __global__ __launch_bounds__(64 * kScoreWaves) void prompt_scores_kernel(PromptS
   auto work = [&](int row0, const __bf16* qb, const float* lb) {
     const int in = row0 & (kScoreQ - 1);                     // the step's first row in the iteration's rows
     const float l = lb[(in + m16) * kGroup + u];
-    // rows past the request and rows that see nothing weigh 0
+    // rows past the request and rows that see nothing weigh 0, the latter (seldom there) whatever their scores
     const float l2 = row0 + m16 < nq && l > -INFINITY ? l * 1.4426950408889634f : INFINITY;
+    const bool all = __all(l != -INFINITY);
     floatx4 s[2] = {floatx4{0.f, 0.f, 0.f, 0.f}, floatx4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -100,8 +101,8 @@ __global__ __launch_bounds__(64 * kScoreWaves) void prompt_scores_kernel(PromptS
 #pragma unroll
       for (int t = 0; t < 2; ++t) s[t] = mfma16x16x32(kop[t][i], qop, s[t]);
     }
-    const int before = kv0 + row0 + m16 - k0;                // keys 0 .. before of the wave's are seen
-    if (kv0 + row0 >= k0 + 31) {                             // (uniform) all of them by all rows
+    const int before = l == -INFINITY ? -1 : kv0 + row0 + m16 - k0;          // keys 0 .. before of the wave's are seen
+    if (all && kv0 + row0 >= k0 + 31) {                      // (uniform) all of them by all rows
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -370,7 +371,7 @@ int abkv_paged_prefill_scores(const void* q, long q_stride_tok, long q_stride_he
   if (num_tiles <= 0) return 0;
   if (q == nullptr || kv_cache == nullptr || block_table == nullptr || q_start == nullptr || kv_start == nullptr ||
       tile_req == nullptr || tile_k0 == nullptr || lse == nullptr || scores == nullptr || num_pages <= 0 || table_width <= 0 ||
-      (tile_keys != kBN && tile_keys != 2 * kBN))
+      (tile_keys != kBN && tile_keys != 2 * kBN) || !row_strides_ok(q_stride_tok) || q_stride_head >= 1L << 28 || !softmax_scale_ok(scale))
     return (int)hipErrorInvalidValue;
   const PromptScoreArgs a{static_cast<const __bf16*>(q), q_stride_tok, q_stride_head, static_cast<const __bf16*>(kv_cache),
                           num_pages, block_table, block_table_stride, table_width, q_start, kv_start, tile_req, tile_k0, lse,

@@ -129,7 +129,8 @@ int abkv_window_attn(const void* q, long q_stride_b, long q_stride_s, long q_str
                      long out_stride_b, long out_stride_s, long out_stride_h, float* lse, hipStream_t stream) {
   using namespace abkv;
   if (batch <= 0 || seq_len <= 0) return 0;
-  if (q == nullptr || k == nullptr || v == nullptr || out == nullptr || window <= 0 || sinks < 0)
+  if (q == nullptr || k == nullptr || v == nullptr || out == nullptr || window <= 0 || sinks < 0 ||
+      !softmax_scale_ok(scale) || !row_strides_ok(q_stride_s, k_stride_s, v_stride_s))
     return (int)hipErrorInvalidValue;
   WindowArgs a;
   a.q = static_cast<const __bf16*>(q);
@@ -163,7 +164,7 @@ int abkv_paged_prefill_attn_window(const void* q, long q_stride_tok, long q_stri
   if (num_tiles <= 0) return 0;
   if (q == nullptr || kv_cache == nullptr || block_table == nullptr || q_start == nullptr || kv_start == nullptr ||
       tile_req == nullptr || tile_q0 == nullptr || out == nullptr || num_pages <= 0 || table_width <= 0 || window <= 0 ||
-      sinks < 0)
+      sinks < 0 || !softmax_scale_ok(scale) || !row_strides_ok(q_stride_tok))
     return (int)hipErrorInvalidValue;
   WindowArgs a{};
   a.q = static_cast<const __bf16*>(q);

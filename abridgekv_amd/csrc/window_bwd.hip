@@ -355,7 +355,8 @@ int abkv_window_attn_bwd(const void* q, long q_stride_b, long q_stride_s, long q
   using namespace abkv;
   if (batch <= 0 || seq_len <= 0) return 0;
   if (q == nullptr || k == nullptr || v == nullptr || out == nullptr || dout == nullptr || lse == nullptr ||
-      dq == nullptr || dk == nullptr || dv == nullptr || window <= 0 || sinks < 0)
+      dq == nullptr || dk == nullptr || dv == nullptr || window <= 0 || sinks < 0 ||
+      !softmax_scale_ok(scale) || !row_strides_ok(q_stride_s, k_stride_s, v_stride_s, out_stride_s, dout_stride_s))
     return (int)hipErrorInvalidValue;
   const SinkPlan plan(seq_len, batch, window, sinks);
   const WindowBwdLayout lay(batch, seq_len, plan);

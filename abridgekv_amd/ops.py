@@ -995,6 +995,24 @@ def _check_rows(name: str, t: torch.Tensor, dtype, shape) -> None:
         raise ValueError(f"{name} must have contiguous, 16-byte aligned rows, got strides {st}")
 
 
+def _check_out(out: torch.Tensor, dtype, shape) -> None:
+    """Rows that are written: as :func:`_check_rows`, and no two of them in one place."""
+    _check_rows("out", out, dtype, shape)
+    if not out.is_contiguous():
+        span = 0
+        for st, n in sorted((st, n) for st, n in zip(out.stride(), out.shape) if n > 1):
+            _require(st > span, "out must not share memory between its rows")
+            span += st * (n - 1)
+
+
+def _softmax_scale(scale) -> float:
+    if scale is None:
+        return default_scale()
+    scale = float(scale)
+    _require(0 < scale < math.inf, "scale must be positive and finite")
+    return scale
+
+
 def _check_window(window, sinks) -> tuple[int, int]:
     if type(window) is not int or type(sinks) is not int:
         _require(int(window) == window and int(sinks) == sinks, "window and sinks must be integers")
@@ -1030,19 +1048,19 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     _require(q.dim() == 4, "q must be [B, S, 32, 128]")
     B, S = q.shape[0], q.shape[1]
     window, sinks = _check_window(window, sinks)
+    scale = _softmax_scale(scale)
     dt = torch.float32 if q.dtype == torch.float32 else torch.bfloat16
     for name, t, h in (("q", q, HEADS_Q), ("k", k, HEADS_KV), ("v", v, HEADS_KV)):
         _check_rows(name, t, dt, (B, S, h, HEAD_DIM))
     _check_lens(seq_lens, B)
     if out is not None:
-        _check_rows("out", out, dt, (B, S, HEADS_Q, HEAD_DIM))
+        _check_out(out, dt, (B, S, HEADS_Q, HEAD_DIM))
     _require(lse is None or (lse.dtype == torch.float32 and lse.is_contiguous() and tuple(lse.shape) == (B, HEADS_Q, S)),
              "lse must be contiguous fp32 [B, 32, S]")
     _check_device(q, k, v, seq_lens, out, lse)
     window, sinks = _reach(window, sinks, S)
     if out is None:
         out = torch.empty((B, S, HEADS_Q, HEAD_DIM), dtype=dt, device=q.device)
-    scale = default_scale() if scale is None else float(scale)
     fn = lib().abkv_window_attn_f32 if dt == torch.float32 else lib().abkv_window_attn
     rc = fn(q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], B, S,
             _ptr(seq_lens), window, sinks, scale, out.data_ptr(), *out.stride()[:3], _ptr(lse), _stream())
@@ -1058,6 +1076,7 @@ def window_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     _require(q.dim() == 4, "q must be [B, S, 32, 128]")
     B, S = q.shape[0], q.shape[1]
     window, sinks = _check_window(window, sinks)
+    scale = _softmax_scale(scale)
     for name, t, h in (("q", q, HEADS_Q), ("k", k, HEADS_KV), ("v", v, HEADS_KV), ("out", out, HEADS_Q),
                        ("dout", dout, HEADS_Q)):
         _check_rows(name, t, torch.bfloat16, (B, S, h, HEAD_DIM))
@@ -1065,8 +1084,7 @@ def window_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     _require(lse.dtype == torch.float32 and lse.is_contiguous() and tuple(lse.shape) == (B, HEADS_Q, S),
              "lse must be contiguous fp32 [B, 32, S]")
     _check_device(q, k, v, out, lse, dout, seq_lens)
-    return window_backward(q, k, v, out, lse, dout, window, sinks, seq_lens,
-                           default_scale() if scale is None else float(scale))
+    return window_backward(q, k, v, out, lse, dout, window, sinks, seq_lens, scale)
 
 
 def window_backward(q, k, v, out, lse, dout, window, sinks, seq_lens, scale):
@@ -1131,14 +1149,16 @@ def paged_prefill_attention_window(q: torch.Tensor, kv_cache: torch.Tensor, bloc
     The chunk's own rows must be in the cache. Returns (out [T, 32, 128] bf16, lse [T, 32] fp32 or None); rows past
     q_start[-1] are left alone."""
     window, sinks = _check_window(window, sinks)
+    scale = _softmax_scale(scale)
     _check_paged(q, kv_cache, block_table)
     T = q.shape[0]
     if out is not None:
-        _check_rows("out", out, torch.bfloat16, (T, HEADS_Q, HEAD_DIM))
+        _check_out(out, torch.bfloat16, (T, HEADS_Q, HEAD_DIM))
     _require(lse is None or (lse.dtype == torch.float32 and lse.is_contiguous() and tuple(lse.shape) == (T, HEADS_Q)),
              "lse must be contiguous fp32 [T, 32]")
     qs, ks, nq = _check_chunks(q, block_table, q_start, kv_start)
     _check_device(q, kv_cache, block_table, out, lse)
+    _require(not torch.cuda.is_current_stream_capturing(), "a chunk batch is uploaded from the host: not in a captured graph")
     if out is None:
         out = torch.empty((T, HEADS_Q, HEAD_DIM), dtype=torch.bfloat16, device=q.device)
     req, q0 = _tiles(nq, 64)
@@ -1147,7 +1167,6 @@ def paged_prefill_attention_window(q: torch.Tensor, kv_cache: torch.Tensor, bloc
         return out, lse
     meta = _upload([qs, ks, req, q0], q.device)
     at = meta.data_ptr()
-    scale = default_scale() if scale is None else float(scale)
     rc = lib().abkv_paged_prefill_attn_window(_ptr(q), q.stride(0), q.stride(1), _ptr(kv_cache), kv_cache.shape[0],
                                               _ptr(block_table), _row_stride(block_table), block_table.shape[1], at,
                                               at + 4 * (R + 1), at + 4 * (2 * R + 1), at + 4 * (2 * R + 1 + tiles), tiles,
@@ -1194,7 +1213,7 @@ def _check_step(q, kv_cache, block_table, seq_lens, max_pages, split_pages, out,
     if not 0 < max_pages <= W:
         raise ValueError("max_pages must be in [1, block_table width]")
     if out is not None:
-        _check_rows("out", out, torch.bfloat16, (B, HEADS_Q, HEAD_DIM))
+        _check_out(out, torch.bfloat16, (B, HEADS_Q, HEAD_DIM))
     if lse is not None and (lse.dtype is not torch.float32 or not lse.is_contiguous() or lse.numel() < B * HEADS_Q):
         raise ValueError("lse must be contiguous fp32 [B, 32]")
     return B, max_pages
@@ -1231,12 +1250,14 @@ def decode_attention_window(q: torch.Tensor, kv_cache: torch.Tensor, block_table
                             out: torch.Tensor | None = None, lse: torch.Tensor | None = None,
                             split_pages: int | None = None, workspace: torch.Tensor | None = None):
     """Decode attention of one layer under a sliding window with sinks: a sequence's token sees rows
-    [n - ``window``, n) and [0, ``sinks``) of its n = seq_lens[b] rows, and only their pages are read.
+    [n - ``window``, n) and [0, ``sinks``) of its n = seq_lens[b] rows, and only their pages are read. Rows count as the cache
+    holds them (an eviction by weight leaves them out of the tokens' order).
 
     Arguments and results as :func:`decode_attention` (bf16 only): (out [B, 32, 128] bf16, lse [B, 32] fp32 or None).
     ``split_pages`` None: chosen by the sizes.
     """
     window, sinks = _check_window(window, sinks)
+    scale = _softmax_scale(scale)
     B, max_pages = _check_step(q, kv_cache, block_table, seq_lens, max_pages, split_pages, out, lse)
     _check_device(q, kv_cache, block_table, seq_lens, out, lse)
     if out is None:
@@ -1244,7 +1265,6 @@ def decode_attention_window(q: torch.Tensor, kv_cache: torch.Tensor, block_table
     split_pages = split_pages or window_split_pages(B, max_pages, window, sinks)
     need = lib().abkv_decode_window_workspace_size(B, max_pages, split_pages, window, sinks)
     workspace, ws_bytes = _take_workspace(workspace, need, q.device)
-    scale = default_scale() if scale is None else float(scale)
     rc = lib().abkv_decode_attn_window(_ptr(q), q.stride(0), q.stride(1), _ptr(kv_cache), kv_cache.shape[0],
                                        _ptr(block_table), _row_stride(block_table), _ptr(seq_lens), B, max_pages,
                                        split_pages, window, sinks, scale, _ptr(out), out.stride(0), out.stride(1), _ptr(lse),
@@ -1283,6 +1303,7 @@ def decode_attention_scored(q: torch.Tensor, kv_cache: torch.Tensor, block_table
     place; each score has one owner, so equal calls give equal bits. ``split_pages`` (None: chosen by the sizes): where
     sequences are split at all. Returns (out [B, 32, 128] bf16, lse or None).
     """
+    scale = _softmax_scale(scale)
     B, max_pages = _check_step(q, kv_cache, block_table, seq_lens, max_pages, split_pages, out, lse)
     _check_scores(scores, B, max_pages * PAGE)
     _check_device(q, kv_cache, block_table, seq_lens, scores, out, lse)
@@ -1291,7 +1312,6 @@ def decode_attention_scored(q: torch.Tensor, kv_cache: torch.Tensor, block_table
     split_pages = split_pages or _step_split_pages(B, max_pages)
     need = lib().abkv_decode_scored_workspace_size(B, max_pages, split_pages)
     workspace, ws_bytes = _take_workspace(workspace, need, q.device)
-    scale = default_scale() if scale is None else float(scale)
     rc = lib().abkv_decode_attn_scored(_ptr(q), q.stride(0), q.stride(1), _ptr(kv_cache), kv_cache.shape[0],
                                        _ptr(block_table), _row_stride(block_table), _ptr(seq_lens), B, max_pages,
                                        split_pages, scale, _ptr(scores), scores.stride(0), scores.stride(1), _ptr(out),
@@ -1317,15 +1337,18 @@ def paged_prefill_scores(q: torch.Tensor, kv_cache: torch.Tensor, block_table: t
     see row j, and KV head h's four query heads, of exp(scale q.k - lse).
 
     Queries as :func:`paged_prefill_attention` takes causal chunks (q [T, 32, 128] bf16, host q_start [R + 1] and kv_start
-    [R]); ``lse`` [T, 32] fp32: what that call left for them (rows with -inf add nothing). To weigh by a prompt's last
-    queries only, pass those alone with their kv_start. ``scores`` [R, 8, rows] fp32 is updated in place, one owner a score.
+    [R]); ``lse`` [T, 32] fp32: what that call left for them (rows with -inf add nothing, whatever they hold). To weigh by a
+    prompt's last queries only, pass those alone with their kv_start. ``scores`` [R, 8, rows] fp32 is updated in place, one owner a score.
     """
+    scale = _softmax_scale(scale)
     _check_paged(q, kv_cache, block_table)
+    _require(q.stride(1) < 1 << 28, f"q must have heads less than 2^28 elements apart, got strides {q.stride()}")
     _require(lse.dtype == torch.float32 and lse.is_contiguous() and tuple(lse.shape) == (q.shape[0], HEADS_Q),
              "lse must be contiguous fp32 [T, 32]")
     _check_scores(scores, len(kv_start), block_table.shape[1] * PAGE)
     qs, ks, nq = _check_chunks(q, block_table, q_start, kv_start)
     _check_device(q, kv_cache, block_table, lse, scores)
+    _require(not torch.cuda.is_current_stream_capturing(), "a chunk batch is uploaded from the host: not in a captured graph")
     if qs[-1] == 0:
         return
     keys = _score_tile_keys(ks, nq, _num_cus())
@@ -1334,7 +1357,6 @@ def paged_prefill_scores(q: torch.Tensor, kv_cache: torch.Tensor, block_table: t
     tiles, R = req.size, ks.size
     meta = _upload([qs, ks, req[order], k0[order]], q.device)
     at = meta.data_ptr()
-    scale = default_scale() if scale is None else float(scale)
     rc = lib().abkv_paged_prefill_scores(_ptr(q), q.stride(0), q.stride(1), _ptr(kv_cache), kv_cache.shape[0],
                                          _ptr(block_table), _row_stride(block_table), block_table.shape[1], at,
                                          at + 4 * (R + 1), at + 4 * (2 * R + 1), at + 4 * (2 * R + 1 + tiles), tiles, keys,
@@ -1357,8 +1379,8 @@ def kv_evict(layer_caches, block_table: torch.Tensor, seq_lens: torch.Tensor, sc
     ``scores`` fp32 and ``positions`` int32 [L, B, 8, rows], contiguous, a row for each of the 16 * ``max_pages`` slots.
     ``positions`` hold each row's token index; -1 (also what a new sequence starts with) marks rows appended since the last
     eviction: their index is num_tokens[b] - (n - row). ``seq_lens`` and ``num_tokens`` [B] int32. The sequences' pages must
-    be their own. ``max_pages`` (default: the table's width, at most 16384) bounds ceil(seq_len / 16). ``out`` [B] int32 (not
-    ``seq_lens``): where the new lengths go.
+    be their own. ``max_pages`` (default: the table's width, at most 16384) bounds ceil(seq_len / 16). ``out`` [B] int32,
+    apart from the others: where the new lengths go.
     """
     L, W = len(layer_caches), block_table.shape[1] if block_table.dim() == 2 else 0
     budget, sinks, recent = int(budget), int(sinks), int(recent)
@@ -1389,11 +1411,15 @@ def kv_evict(layer_caches, block_table: torch.Tensor, seq_lens: torch.Tensor, sc
     if out is None:
         out = torch.empty_like(seq_lens)
     elif (out.dtype is not torch.int32 or out.shape != (B,) or not out.is_contiguous()
-          or (B and out.data_ptr() == seq_lens.data_ptr())):
-        raise ValueError("out must be contiguous int32 [B] apart from seq_lens")
+          or any(abs(out.data_ptr() - t.data_ptr()) < 4 * B for t in (seq_lens, num_tokens))):
+        raise ValueError("out must be contiguous int32 [B] apart from seq_lens and num_tokens")
+    _require(scores.numel() == 0 or abs(scores.data_ptr() - positions.data_ptr()) >= 4 * scores.numel(),
+             "scores and positions must not share memory")
     _check_device(block_table, seq_lens, num_tokens, scores, positions, out, *layer_caches)
     ptrs = [c.data_ptr() for c in layer_caches]
-    _require(len(set(ptrs)) == L, "a layer cache may be given once")
+    at = sorted(ptrs)
+    nbytes = 2 * layer_caches[0].numel()
+    _require(all(y - x >= nbytes for x, y in zip(at, at[1:])), "layer caches must not share memory")
     arr, num_pages = (C.c_void_p * L)(*ptrs), shape[0]
     if B == 0:
         return out

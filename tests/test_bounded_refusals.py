@@ -49,6 +49,41 @@ def test_window_attention():
     _bad(on_gpu, ops.window_attention_backward, q, k, v, q, torch.zeros(2, 32, 9), q, 4)
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.1, float("inf"), float("nan")])
+def test_scales(scale):
+    """Scores are masked before they are scaled."""
+    q, k, v = _dense()
+    lse = torch.zeros(2, 32, 9)
+    _bad("scale", ops.window_attention, q, k, v, 4, scale=scale)
+    _bad("scale", ops.window_attention_backward, q, k, v, q, lse, q, 4, scale=scale)
+    q, cache, table, lens = _paged()
+    _bad("scale", ops.decode_attention_window, q, cache, table, lens, 4, scale=scale)
+    _bad("scale", ops.decode_attention_scored, q, cache, table, lens, torch.zeros((2, 8, 64)), scale=scale)
+    _bad("scale", ops.paged_prefill_attention_window, q, cache, table, [0, 2], [0], 4, scale=scale)
+    _bad("scale", ops.paged_prefill_scores, q, cache, table, [0, 2], [0], torch.zeros(2, 32), torch.zeros((1, 8, 64)), scale=scale)
+
+
+def test_outputs_that_share_memory():
+    q, k, v = _dense()
+    for out in (q[:1].expand(2, -1, -1, -1), q[:, :1].expand(-1, 9, -1, -1), q[:, :, :1].expand(-1, -1, 32, -1),
+                torch.zeros(1 << 18, dtype=BF).as_strided((2, 9, 32, 128), (9 * 4096 - 128, 4096, 128, 1))):
+        _bad("out must not share", ops.window_attention, q, k, v, 4, out=out)
+    order = torch.zeros((32, 9, 2, 128), dtype=BF).permute(2, 1, 0, 3)                 # any order of its own rows
+    _bad("current GPU", ops.window_attention, q, k, v, 4, out=order)
+    q, cache, table, lens = _paged()
+    _bad("out must not share", ops.decode_attention_window, q, cache, table, lens, 4, out=q[:1].expand(2, -1, -1))
+    _bad("out must not share", ops.paged_prefill_attention_window, q, cache, table, [0, 2], [0], 4, out=q[:1].expand(2, -1, -1))
+    scores, positions = torch.zeros((1, 2, 8, 64)), torch.zeros((1, 2, 8, 64), dtype=I32)
+    many = torch.zeros(5, dtype=I32)
+    for tokens, out in ((lens.clone(), lens), (many[:2], many[1:3]), (many[1:3], many[:2]), (many[:2], many[:2])):
+        _bad("out must be contiguous int32", ops.kv_evict, [cache], table, lens, scores, positions, tokens, 4, out=out)
+    _bad("current GPU", ops.kv_evict, [cache], table, lens, scores, positions, many[:2], 4, out=many[2:4])
+    _bad("share memory", ops.kv_evict, [cache], table, lens, scores, scores.view(I32), lens.clone(), 4)
+    pool = torch.zeros((15, 2, 16, 8, 128), dtype=BF)
+    two = dict(scores=torch.zeros((2, 2, 8, 64)), positions=torch.zeros((2, 2, 8, 64), dtype=I32))
+    _bad("current GPU", ops.kv_evict, [pool[5:10], pool[:5]], table, lens, num_tokens=lens.clone(), budget=4, **two)
+
+
 def _paged(B=2, W=4, P=10):
     return (torch.zeros((B, 32, 128), dtype=BF), torch.zeros((P, 2, 16, 8, 128), dtype=BF), torch.zeros((B, W), dtype=I32),
             torch.ones(B, dtype=I32))
@@ -157,6 +192,16 @@ def test_c_entry_points_return_errors():
     def win(window=4, sinks=0, q=one):
         return L.abkv_window_attn(q, 1, 1, 1, one, 1, 1, 1, one, 1, 1, 1, 1, 8, None, window, sinks, 1.0, one, 1, 1, 1, None, 0)
 
+    def scaled(scale, stride=1):
+        return (L.abkv_window_attn(one, 1, stride, 1, one, 1, 1, 1, one, 1, 1, 1, 1, 8, None, 4, 0, scale, one, 1, 1, 1, None, 0),
+                L.abkv_window_attn_f32(one, 1, stride, 1, one, 1, 1, 1, one, 1, 1, 1, 1, 8, None, 4, 0, scale, one, 1, 1, 1, None,
+                                       0),
+                L.abkv_window_attn_bwd(one, 1, stride, 1, *[one, 1, 1, 1] * 4, one, 1, 8, None, 4, 0, scale, *[one, 1, 1, 1] * 3,
+                                       one, 1 << 30, 0),
+                L.abkv_paged_prefill_attn_window(one, stride, 1, one, 4, one, 4, 4, *n, 1, 4, 0, scale, one, 1, 1, None, 0),
+                L.abkv_paged_prefill_scores(one, stride, 1, one, 4, one, 4, 4, *n, 1, 64, one, one, 64, 64, scale, 0))
+
+    assert set(scaled(0.0) + scaled(-1.0) + scaled(float("nan")) + scaled(float("inf")) + scaled(1.0, 1 << 24)) == {bad}
     assert win(0) == win(4, -1) == win(q=0) == bad
     assert L.abkv_window_attn(one, 1, 1, 1, one, 1, 1, 1, one, 1, 1, 1, 0, 8, None, 4, 0, 1.0, one, 1, 1, 1, None, 0) == 0
     args = [one, 1, 1, 1] * 5 + [one, 1, 8, None, 4, 0, 1.0] + [one, 1, 1, 1] * 3
@@ -167,6 +212,9 @@ def test_c_entry_points_return_errors():
         return L.abkv_decode_attn_window(one, 1, 1, one, 4, one, stride, one, seqs, pages, split, window, sinks, 1.0, one, 1, 1,
                                          None, ws, size, 0)
 
+    assert L.abkv_decode_attn_window(one, 1, 1, one, 4, one, 4, one, 1, 4, 2, 4, 0, 0.0, one, 1, 1, None, one, 1 << 30, 0) == bad
+    assert L.abkv_decode_attn_scored(one, 1, 1, one, 4, one, 4, one, 1, 4, 2, -1.0, one, 64, 64, one, 1, 1, None, one, 1 << 30,
+                                     0) == bad
     assert dec(0) == dec(4, -1) == dec(split=3) == dec(split=66) == dec(pages=0) == dec(seqs=65536) == dec(stride=3) == bad
     assert dec(window=64, size=8) == dec(window=64, ws=0) == bad
     assert dec(seqs=0) == 0

@@ -180,6 +180,43 @@ def test_prefill_scores(chunk, past):
             assert (np.abs(got[:, :n] - want[r]) <= W_TOL * (1 + want[r])).all(), np.abs(got[:, :n] - want[r]).max()
 
 
+@pytest.mark.parametrize("held", [1.0, float("inf"), float("nan")])
+def test_prefill_scores_of_rows_that_see_nothing(held):
+    """Rows with lse -inf, whatever they hold, among others and at a request's end, add nothing."""
+    from abridgekv_amd import ops
+    q, k, v, cache, table, _ = _paged([300], 8)
+    q = torch.randn((200, 32, 128), generator=torch.Generator().manual_seed(5)).to(torch.bfloat16).cuda()
+    lse = torch.full((200, 32), 6.0, device="cuda")
+    want = torch.zeros((1, 8, table.shape[1] * 16), device="cuda")
+    got = want.clone()
+    dead = torch.zeros(200, dtype=torch.bool)
+    dead[[0, 3, 17, 64, 65, 130, 199]] = True
+    for at in range(200):                                    # each live row alone, behind its own rows
+        if not dead[at]:
+            ops.paged_prefill_scores(q[at: at + 1], cache, table, [0, 1], [100 + at], lse[at: at + 1].contiguous(), want)
+    q[dead], lse[dead] = held, -float("inf")
+    ops.paged_prefill_scores(q, cache, table, [0, 200], [100], lse, got)
+    # the same terms added up in other orders: at most 4 x 193 of them
+    assert (got - want).abs().max() <= 772 * 2.0 ** -24 * want.max()
+
+
+def test_chunks_in_a_capture_are_refused():
+    """Their tiles are uploaded from the host: a replay would read what is no longer there."""
+    from abridgekv_amd import ops
+    q, k, v, cache, table, _ = _paged([30], 8)
+    q = q.cuda()
+    lse, scores = torch.zeros((1, 32), device="cuda"), torch.zeros((1, 8, 32), device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x = q * 2
+        with pytest.raises(ValueError, match="captured"):
+            ops.paged_prefill_attention_window(q[:1], cache, table, [0, 1], [0], 4)
+        with pytest.raises(ValueError, match="captured"):
+            ops.paged_prefill_scores(q[:1], cache, table, [0, 1], [0], lse, scores)
+    graph.replay()
+    assert torch.equal(x, q * 2)
+
+
 def _evict_case(lens, seed, layers=2, levels=None, recorded=False):
     """Caches of rows that name themselves, scores (``levels``: few different ones) and positions."""
     q, k, v, cache, table, sl = _paged(lens, seed, garbage=3.0)
