@@ -145,6 +145,44 @@ __device__ __forceinline__ void store_acc_bf16x8(__bf16* dst, const floatx4& a, 
   store_bf16x8(dst, lo, hi, inv);
 }
 
+// The whole 128-dim rows of a wave's accumulator columns (head u) times inv, dst the lane's row: a 4 x 4 transpose of
+// 16-byte pieces over the lane groups first, so that an instruction writes 16 whole 64-byte runs and not a quarter of 64
+// (window attention of two sequences of 4096 rows, window 64: 66 -> 58 us). Lanes of a row are active together.
+template <int H>
+__device__ __forceinline__ void store_acc_rows(__bf16* dst, const floatx4 (&o)[8][H], int u, int j, float inv) {
+  const bool odd = j & 1;
+  uint32_t x[4][4];                                          // [p]: dims 32j + 8p .. + 7
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const floatx4 a = o[2 * p][u] * inv, b = o[2 * p + 1][u] * inv;
+    const uint32_t a0 = pack_bf16x2(a[0], a[1]), a1 = pack_bf16x2(a[2], a[3]);
+    const uint32_t b0 = pack_bf16x2(b[0], b[1]), b1 = pack_bf16x2(b[2], b[3]);
+    x[p][0] = odd ? b0 : a0;
+    x[p][1] = odd ? b1 : a1;
+    x[p][2] = odd ? a0 : b0;
+    x[p][3] = odd ? a1 : b1;
+  }
+#pragma unroll
+  for (int p = 0; p < 2; ++p)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const auto r = __builtin_amdgcn_permlane32_swap(x[p][e], x[p + 2][e], false, false);
+      x[p][e] = r[0];
+      x[p + 2][e] = r[1];
+    }
+#pragma unroll
+  for (int p = 0; p < 4; p += 2)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const auto r = __builtin_amdgcn_permlane16_swap(x[p][e], x[p + 1][e], false, false);
+      x[p][e] = r[0];
+      x[p + 1][e] = r[1];
+    }
+#pragma unroll
+  for (int p = 0; p < 4; ++p)                                // [p]: dims 32p + 8j .. + 7
+    *reinterpret_cast<u32x4*>(dst + 32 * p + 8 * j) = u32x4{x[p][0], x[p][1], x[p][2], x[p][3]};
+}
+
 __device__ __forceinline__ bf16x8 vt_operand(const __bf16* Vbuf, int kb, int t, int lane) {
   typedef short s4 __attribute__((ext_vector_type(4)));
   const int g = lane >> 4, i = lane & 15;

@@ -4,9 +4,16 @@
 //   out_i = sum_j softmax_j(scale q_i . k_j) v_j, rows that see nothing (padding) are 0 with lse -inf.
 //
 // The mask is evaluated from (window, sinks, the sequence's length): a query tile of 64 rows walks the tiles of the sinks,
-// then the ceil((window + 63) / 64) (+ 1) tiles its rows' windows reach, and only tiles on an edge of a range are masked per
-// element. The work of a row is bounded by the window, not by its position. Tiles, softmax and the K/V pipeline are the
-// compression mask's (attn_tile.h): a workgroup of 8 waves per (sequence, KV head, query tile), a wave 16 rows x 2 heads.
+// then the ceil((window + 63) / 64) (+ 1) tiles its rows' windows reach, and only tiles on an edge of a range are masked
+// per element. The work of a row is bounded by the window, not by its position.
+//
+// A workgroup of 4 waves takes a query tile of two of a KV head's four query heads, a wave 16 rows x 2 heads (tiles and softmax
+// as the compression mask's, attn_tile.h). Query rows and outputs are most of the bytes under a short window, and workgroups
+// of one length all load, compute and store at the same times: two of them share a CU (two buffers each of K and V, 80 KiB), so
+// that one's loads and stores run beside the other's products. Against one workgroup of 8 waves for all four heads, three
+// buffers each, us a call of two sequences of 4096 rows under windows of 64 / 128 / 512 / 1024: 58 / 66 / 105 / 156 -> 48 / 57 /
+// 99 / 147 (copies of the query rows and outputs alone: 27). Outputs in whole 64-byte runs (store_acc_rows) before it 66 / 73 /
+// 112 / 160 -> 58 / 66 / 105 / 156. Bound by issue within a tile (as the masked prefill) and the edge tiles under long windows.
 #include "window_tile.h"
 
 namespace abkv {
@@ -22,19 +29,18 @@ struct ChunkArgs {
 };
 
 template <bool kPaged>
-__global__ __launch_bounds__(512, 1) void window_attn_kernel(WindowArgs a, ChunkArgs c) {
-  constexpr int H = 2, kWaves = 8;
-  __shared__ __attribute__((aligned(16))) __bf16 K0[kTileElems], K1[kTileElems], K2[kTileElems];
-  __shared__ __attribute__((aligned(16))) __bf16 V0[kTileElems], V1[kTileElems], V2[kTileElems];
+__global__ __launch_bounds__(256, 2) void window_attn_kernel(WindowArgs a, ChunkArgs c) {
+  constexpr int H = 2, kWaves = 4;
+  __shared__ __attribute__((aligned(16))) __bf16 K0[kTileElems], K1[kTileElems], V0[kTileElems], V1[kTileElems];
   __shared__ __attribute__((aligned(16))) __bf16 Ks[kTileElems];           // the sinks, where they are few
-  __bf16* const Kbuf[kStages] = {K0, K1, K2};
-  __bf16* const Vbuf[kStages] = {V0, V1, V2};
-  // KV head fastest: workgroups go to the 8 XCDs round-robin, so one XCD's L2 serves a head's rows to all its tiles. Then the
-  // query tile, the sequence last: with the sequence before it, a padded batch of two gives every other workgroup little to
-  // do, and the dispatch, in turn over an XCD's parts as well, leaves half of them idle (8192 and 5000 rows, window 1024: 321
-  // us, this order 280).
+  __bf16* const Kbuf[2] = {K0, K1};
+  __bf16* const Vbuf[2] = {V0, V1};
+  // KV head fastest: workgroups go to the 8 XCDs round-robin, so one XCD's L2 serves a head's rows to all its tiles. Then
+  // the pair of heads and the query tile, the sequence last: with the sequence before them, a padded batch of two gives
+  // every other workgroup little to do, and the dispatch, in turn over an XCD's parts as well, leaves half of them idle
+  // (8192 and 5000 rows, window 1024: 321 us, this order 280, both with 8 waves).
   const int kvh = blockIdx.x % kHeadsKV;
-  const int tile = blockIdx.x / kHeadsKV;
+  const int tile = blockIdx.x / (2 * kHeadsKV);
   int b, q0, kv0 = 0, t0 = 0, n, n_q;                        // n: keys; n_q: query rows of the sequence
   if constexpr (kPaged) {
     b = c.tile_req[tile];
@@ -51,19 +57,19 @@ __global__ __launch_bounds__(512, 1) void window_attn_kernel(WindowArgs a, Chunk
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int m16 = lane & 15, j = lane >> 4;
-  const int hbase = H * (w & 1);                             // first of this wave's heads in the GQA group
-  const int qi = q0 + 16 * (w >> 1) + m16;                   // this lane's query row (MFMA column)
+  const int hbase = H * (blockIdx.x / kHeadsKV & 1);         // first of the workgroup's heads in the GQA group
+  const int qi = q0 + 16 * w + m16;                          // this lane's query row (MFMA column)
   const bool seen = qi < n_q;
 
-  const long q_row = kPaged ? (long)(t0 + min(qi, n_q - 1)) * a.q_ss : (long)b * a.q_sb + (long)min(qi, a.S - 1) * a.q_ss;
+  // (rows past the sequence: its last one, not stored)
+  const long q_row = (kPaged ? (long)t0 * a.q_ss : (long)b * a.q_sb) + (long)min(qi, max(n_q - 1, 0)) * a.q_ss;
   bf16x8 qop[H][4];
 #pragma unroll
   for (int u = 0; u < H; ++u)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      u32x4 x = ld16g(a.q + q_row + (long)(kvh * kGroup + hbase + u) * a.q_sh + 8 * (4 * i + j));
-      if (!seen) x = u32x4{0, 0, 0, 0};
-      qop[u][i] = __builtin_bit_cast(bf16x8, x);
+      const __bf16* x = a.q + q_row + (long)(kvh * kGroup + hbase + u) * a.q_sh + 8 * (4 * i + j);
+      qop[u][i] = __builtin_bit_cast(bf16x8, ld16g(x));
     }
   floatx4 o[8][H];
 #pragma unroll
@@ -83,15 +89,16 @@ __global__ __launch_bounds__(512, 1) void window_attn_kernel(WindowArgs a, Chunk
     const WindowLane lm(kv0 + qi, seen, a.window, sinks);
     float m0[H], l0[H];                                      // the sinks' own
     auto attend = [&](const auto& rows) {
+      if (few) issue_sinks(rows, n, Ks, w, lane);
+      start_pair<kWaves>(rows, walk, n, Kbuf, Vbuf, w, lane);
       if (few) {
-        issue_sinks(rows, n, Ks, w, lane);
-        __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __asm__ volatile("s_waitcnt vmcnt(12)" ::: "memory");    // (all but the first tiles')
         __builtin_amdgcn_s_barrier();
         attend_sinks<H>(Ks, a.sinks, qop, o, m_run, l0, a.scale_log2, lane);
 #pragma unroll
         for (int u = 0; u < H; ++u) m0[u] = m_run[u];
       }
-      attend_tiles<H, kWaves>(rows, walk, n, Kbuf, Vbuf, qop, o, m_run, l_run, lm, a.scale_log2, w, lane);
+      attend_pair<H, kWaves>(rows, walk, n, Kbuf, Vbuf, qop, o, m_run, l_run, lm, a.scale_log2, w, lane);
 #pragma unroll
       for (int u = 0; u < H; ++u)
         if (few) l_run[u] += l0[u] * fast_exp2(m0[u] - m_run[u]);
@@ -106,13 +113,14 @@ __global__ __launch_bounds__(512, 1) void window_attn_kernel(WindowArgs a, Chunk
   const long o_row = kPaged ? (long)(t0 + qi) * a.o_ss : (long)b * a.o_sb + (long)qi * a.o_ss;
 #pragma unroll
   for (int u = 0; u < H; ++u) {
-    // padding rows (o = 0, and an l of unmasked tiles): 0, lse -inf. A row that sees keys has l > 0, or NaN scores.
+    // padding rows (with o and l of unmasked tiles): 0, lse -inf. A row that sees keys has l > 0, or NaN scores.
     const float l = seen ? l_run[u] : 0.f;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const int head = kvh * kGroup + hbase + u;
-    __bf16* oh = a.out + o_row + (long)head * a.o_sh + 32 * j;
+    if (!seen)
 #pragma unroll
-    for (int p = 0; p < 4; ++p) store_acc_bf16x8(oh + 8 * p, o[2 * p][u], o[2 * p + 1][u], j, inv);
+      for (int e = 0; e < 8; ++e) o[e][u] = floatx4{0.f, 0.f, 0.f, 0.f};
+    store_acc_rows<H>(a.out + o_row + (long)head * a.o_sh, o, u, j, inv);
     if (a.lse != nullptr && j == 0)
       a.lse[kPaged ? (long)(t0 + qi) * kHeadsQ + head : ((long)b * kHeadsQ + head) * a.S + qi] =
           l == 0.f ? -INFINITY : (m_run[u] + __log2f(l)) * 0.69314718055994531f;
@@ -149,9 +157,9 @@ int abkv_window_attn(const void* q, long q_stride_b, long q_stride_s, long q_str
   a.o_sb = out_stride_b; a.o_ss = out_stride_s; a.o_sh = out_stride_h;
   a.lse = lse;
   a.num_q_tiles = (seq_len - 1) / kBM + 1;
-  const long grid = (long)a.num_q_tiles * batch * kHeadsKV;
-  if (grid * 512 > 0xFFFFFFFFL) return (int)hipErrorInvalidValue;
-  hipLaunchKernelGGL(window_attn_kernel<false>, dim3((unsigned)grid), dim3(512), 0, stream, a, ChunkArgs{});
+  const long grid = 2L * a.num_q_tiles * batch * kHeadsKV;
+  if (grid * 256 > 0xFFFFFFFFL) return (int)hipErrorInvalidValue;
+  hipLaunchKernelGGL(window_attn_kernel<false>, dim3((unsigned)grid), dim3(256), 0, stream, a, ChunkArgs{});
   return (int)hipGetLastError();
 }
 
@@ -177,9 +185,9 @@ int abkv_paged_prefill_attn_window(const void* q, long q_stride_tok, long q_stri
   a.lse = lse;
   const ChunkArgs c{static_cast<const __bf16*>(kv_cache), num_pages, block_table, block_table_stride, table_width,
                     q_start, kv_start, tile_req, tile_q0};
-  const long grid = (long)num_tiles * kHeadsKV;
-  if (grid * 512 > 0xFFFFFFFFL) return (int)hipErrorInvalidValue;
-  hipLaunchKernelGGL(window_attn_kernel<true>, dim3((unsigned)grid), dim3(512), 0, stream, a, c);
+  const long grid = 2L * num_tiles * kHeadsKV;
+  if (grid * 256 > 0xFFFFFFFFL) return (int)hipErrorInvalidValue;
+  hipLaunchKernelGGL(window_attn_kernel<true>, dim3((unsigned)grid), dim3(256), 0, stream, a, c);
   return (int)hipGetLastError();
 }
 

@@ -51,6 +51,17 @@ __global__ __launch_bounds__(512, 1) void window_bwd_dq_kernel(WindowBwdArgs a) 
   const bool seen = qrow < n;
   if (blockIdx.x == 0)
     for (int i = threadIdx.x; i < a.plan.sink_tiles * f.B * kHeadsKV; i += 512) a.done[i] = 0;
+  const DenseRows<false> rows{f.k + (long)b * f.k_sb + (long)kvh * f.k_sh, f.v + (long)b * f.v_sb + (long)kvh * f.v_sh,
+                              f.k_ss, f.v_ss};
+  WindowWalk walk(q0, min(q0 + kBM, n) - 1, f.window, f.sinks);
+  int tc = 0;
+  TileMask mc;
+  const bool any = q0 < n && walk.next(tc, mc, true);        // (uniform)
+  if (any) {                                                 // the first tile comes in beside the rows
+    const auto s0 = rows.template src<2>(tc, w, n);
+    issue_half<kWaves, false>(rows, s0, n, Kb[0], w, lane);
+    issue_half<kWaves, true>(rows, s0, n, Vb[0], w, lane);
+  }
   bf16x8 qop[H][4], gop[H][4];
   float l2[H], dd[H];
 #pragma unroll
@@ -83,18 +94,8 @@ __global__ __launch_bounds__(512, 1) void window_bwd_dq_kernel(WindowBwdArgs a) 
 #pragma unroll
     for (int u = 0; u < H; ++u) dq[i][u] = floatx4{0.f, 0.f, 0.f, 0.f};
 
-  const DenseRows<false> rows{f.k + (long)b * f.k_sb + (long)kvh * f.k_sh, f.v + (long)b * f.v_sb + (long)kvh * f.v_sh,
-                              f.k_ss, f.v_ss};
-  WindowWalk walk(q0, min(q0 + kBM, n) - 1, f.window, f.sinks);
   const WindowLane lm(qrow, seen, f.window, f.sinks);
-  int tc = 0;
-  TileMask mc;
-  if (q0 < n && walk.next(tc, mc, true)) {                   // (uniform)
-    {
-      const auto s0 = rows.template src<2>(tc, w, n);
-      issue_half<kWaves, false>(rows, s0, n, Kb[0], w, lane);
-      issue_half<kWaves, true>(rows, s0, n, Vb[0], w, lane);
-    }
+  if (any) {
     // Double buffer as the masked prefill's dQ: wait for tile i, issue tile i + 1 (or re-load tile i past the end) into
     // the other buffer, compute tile i.
     auto step = [&](auto buf_c) -> bool {
@@ -139,10 +140,8 @@ __global__ __launch_bounds__(512, 1) void window_bwd_dq_kernel(WindowBwdArgs a) 
   if (qrow >= f.S) return;
 #pragma unroll
   for (int u = 0; u < H; ++u) {
-    __bf16* dp = a.dq + (long)b * a.dq_sb + (long)qrow * a.dq_ss + (long)(kvh * kGroup + hbase + u) * a.dq_sh + 32 * j;
-    const float f_out = seen ? a.scale : 0.f;
-#pragma unroll
-    for (int p = 0; p < 4; ++p) store_acc_bf16x8(dp + 8 * p, dq[2 * p][u], dq[2 * p + 1][u], j, f_out);
+    __bf16* dp = a.dq + (long)b * a.dq_sb + (long)qrow * a.dq_ss + (long)(kvh * kGroup + hbase + u) * a.dq_sh;
+    store_acc_rows<H>(dp, dq, u, j, seen ? a.scale : 0.f);
   }
 }
 
@@ -173,19 +172,6 @@ __global__ __launch_bounds__(256, 2) void window_bwd_dkv_kernel(WindowBwdArgs a)
   const int key = k0 + 16 * w + m16;                         // this lane's column
   const bool in = key < n;
 
-  bf16x8 kop[4], vop[4];
-  {
-    const int r = min(key, f.S - 1);
-    const __bf16* kp = f.k + (long)b * f.k_sb + (long)r * f.k_ss + (long)kvh * f.k_sh;
-    const __bf16* vp = f.v + (long)b * f.v_sb + (long)r * f.v_ss + (long)kvh * f.v_sh;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      u32x4 x = ld16g(kp + 8 * (4 * e + j)), y = ld16g(vp + 8 * (4 * e + j));
-      if (!in) x = y = u32x4{0, 0, 0, 0};
-      kop[e] = __builtin_bit_cast(bf16x8, x);
-      vop[e] = __builtin_bit_cast(bf16x8, y);
-    }
-  }
   floatx4 dk[8][1], dv[8][1];
 #pragma unroll
   for (int e = 0; e < 8; ++e) dk[e][0] = dv[e][0] = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -218,8 +204,22 @@ __global__ __launch_bounds__(256, 2) void window_bwd_dkv_kernel(WindowBwdArgs a)
     if (w == 0) __builtin_amdgcn_global_load_lds((const void*)(a.lse2 + wi), ABKV_LDS(Lb[sl_dst]), 4, 0, 0);
     if (w == 1) __builtin_amdgcn_global_load_lds((const void*)(a.dvec + wi), ABKV_LDS(Eb[sl_dst]), 4, 0, 0);
   };
-  if (next_pair()) {
-    issue(qt, h, 0);
+  const bool any = next_pair();
+  if (any) issue(qt, h, 0);                                  // the first rows come in beside the keys
+  bf16x8 kop[4], vop[4];
+  {
+    const int r = min(key, f.S - 1);
+    const __bf16* kp = f.k + (long)b * f.k_sb + (long)r * f.k_ss + (long)kvh * f.k_sh;
+    const __bf16* vp = f.v + (long)b * f.v_sb + (long)r * f.v_ss + (long)kvh * f.v_sh;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      u32x4 x = ld16g(kp + 8 * (4 * e + j)), y = ld16g(vp + 8 * (4 * e + j));
+      if (!in) x = y = u32x4{0, 0, 0, 0};
+      kop[e] = __builtin_bit_cast(bf16x8, x);
+      vop[e] = __builtin_bit_cast(bf16x8, y);
+    }
+  }
+  if (any) {
     auto step = [&](auto buf_c) -> bool {
       constexpr int sl = decltype(buf_c)::value;
       const int q0 = qt * kBM;
@@ -313,13 +313,10 @@ __global__ __launch_bounds__(256, 2) void window_bwd_dkv_kernel(WindowBwdArgs a)
     }
   }
   if (key >= f.S) return;                                    // (padding keys: sums of 0)
-  __bf16* kp = a.dk + (long)b * a.dk_sb + (long)key * a.dk_ss + (long)kvh * a.dk_sh + 32 * j;
-  __bf16* vp = a.dv + (long)b * a.dv_sb + (long)key * a.dv_ss + (long)kvh * a.dv_sh + 32 * j;
-#pragma unroll
-  for (int p = 0; p < 4; ++p) {
-    store_acc_bf16x8(kp + 8 * p, dk[2 * p][0], dk[2 * p + 1][0], j, in ? a.scale : 0.f);
-    store_acc_bf16x8(vp + 8 * p, dv[2 * p][0], dv[2 * p + 1][0], j, in ? 1.f : 0.f);
-  }
+  __bf16* kp = a.dk + (long)b * a.dk_sb + (long)key * a.dk_ss + (long)kvh * a.dk_sh;
+  __bf16* vp = a.dv + (long)b * a.dv_sb + (long)key * a.dv_ss + (long)kvh * a.dv_sh;
+  store_acc_rows<1>(kp, dk, 0, j, in ? a.scale : 0.f);
+  store_acc_rows<1>(vp, dv, 0, j, in ? 1.f : 0.f);
 }
 
 // Workspace: lse2, D (fp32 [B, 32, Sp] each), the counters, then the slots on a 16-byte boundary.

@@ -16,32 +16,7 @@ struct WindowArgs {
   __bf16* out;      long o_sb, o_ss, o_sh;
   float* lse;                                // natural log, [B, 32, S]; chunks: [T, 32]; or nullptr
   int num_q_tiles;
-  int group;                                 // tiles of one XCD in a row (window_tile)
 };
-
-// Workgroup -> (64-row tile, KV head, sequence). Workgroups go to the 8 XCDs round-robin by linear id; XCD x takes the tile
-// groups x, x + 8, ..., of `group` consecutive tiles of a sequence with all KV heads each: neighbouring tiles read mostly the
-// same rows of the other side, which then stay in one XCD's L2, and all of the rows' bytes, not one head's, so that its
-// requests spread over all L2 channels. One KV head per XCD, as the compression mask's kernels place them (there every tile
-// reads all codes), against this: B=2, 8192 rows, window 1024: forward 322 -> 294 us.
-struct WindowTile {
-  int tile, kvh, b;
-};
-__device__ __forceinline__ WindowTile window_tile(int tiles, int batch, int group) {
-  const int total = tiles * batch, x = blockIdx.x % 8, i = blockIdx.x / 8;
-  const int whole = total / (8 * group) * (8 * group);       // in whole rounds of groups; the rest evenly
-  int t, kvh;
-  if (i < whole) {
-    const int in = i % (8 * group);
-    kvh = in % kHeadsKV;
-    t = (i / (8 * group) * 8 + x) * group + in / kHeadsKV;
-  } else {
-    const int rest = x * (total - whole) + (i - whole);
-    kvh = rest % kHeadsKV;
-    t = whole + rest / kHeadsKV;
-  }
-  return {t % tiles, kvh, t / tiles};
-}
 
 __device__ __forceinline__ int window_rows(const WindowArgs& a, int b) {
   return a.seq_lens ? min(max(a.seq_lens[b], 0), a.S) : a.S;
@@ -75,32 +50,32 @@ __device__ __forceinline__ void tile_mask(floatx4 (&s)[2][2][H], int k0, const T
       }
 }
 
-// Up to 32 sinks before a query tile's windows take half a tile of their own, outside the walk (a whole one costs a tenth of
-// a query tile under a window of 512): 32 K rows and 32 V rows in one LDS tile. Sinks that the windows reach, or more of them,
-// stay with the walk.
+// Up to 32 sinks before a query tile's windows take half a tile of their own, outside the walk (a whole one costs a tenth
+// of a query tile under a window of 512; 4 sinks: windows of 128 / 512 / 1024 81 / 121 / 269 -> 74 / 114 / 262 us): 32 K
+// rows and 32 V rows in one LDS tile. Sinks that the windows reach, or more of them, stay with the walk.
 constexpr int kShortSinks = 32;
 __device__ __forceinline__ bool short_sinks(int q0, int window, int sinks) {
   return sinks > 0 && sinks <= kShortSinks && q0 + 1 - window >= kBN;
 }
 
-// DMA of the sinks' rows (keys 0 .. 31, fewer than n_keys >= 64): K in rows 0 .. 31 of buf, V in rows 32 .. 63, by 8 waves.
+// DMA of the sinks' rows (keys 0 .. 31, fewer than n_keys >= 64): K in rows 0 .. 31 of buf, V in rows 32 .. 63, by 4 waves.
 template <class Rows>
 __device__ __forceinline__ void issue_sinks(const Rows& rows, int n_keys, __bf16* buf, int w, int lane) {
-  const auto src = rows.template src<2>(0, w & 3, n_keys);   // waves 4 .. 7: the V rows of the same keys
+  const auto src = rows.template src<4>(0, w & 1, n_keys);   // waves 2 and 3: the V rows of the same keys
 #pragma unroll
-  for (int n = 0; n < 2; ++n) {
-    const int row = 8 * (w & 3) + 4 * n + (lane >> 4);
+  for (int n = 0; n < 4; ++n) {
+    const int row = 16 * (w & 1) + 4 * n + (lane >> 4);
     const int chunk = (lane & 15) ^ (row & 15);              // (row + 32 swizzles alike)
-    const __bf16* p = w < 4 ? rows.template addr<false>(src, row, chunk, n_keys)
+    const __bf16* p = w < 2 ? rows.template addr<false>(src, row, chunk, n_keys)
                             : rows.template addr<true>(src, row, chunk, n_keys);
-    __builtin_amdgcn_global_load_lds((const void*)p, ABKV_LDS(buf + (4 * (2 * w + n)) * kHeadDim), 16, 0, 0);
+    __builtin_amdgcn_global_load_lds((const void*)p, ABKV_LDS(buf + (4 * (4 * w + n)) * kHeadDim), 16, 0, 0);
   }
 }
 
 // Scores of the 32 rows from row `first` of an LDS tile (tile_scores' first half).
 template <int H>
-__device__ __forceinline__ void half_scores(const __bf16* buf, int first, const bf16x8 (&qop)[H][4], floatx4 (&s)[2][H], int m16,
-                                            int j) {
+__device__ __forceinline__ void half_scores(const __bf16* buf, int first, const bf16x8 (&qop)[H][4], floatx4 (&s)[2][H],
+                                            int m16, int j) {
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -162,6 +137,72 @@ __device__ __forceinline__ void attend_sinks(const __bf16* buf, int sinks, const
   }
 #pragma unroll
   for (int u = 0; u < H; ++u) l[u] = mfma16x16x32(ones, pop[u], floatx4{0.f, 0.f, 0.f, 0.f})[0];
+}
+
+// The first DMAs of a walk of at least one tile: K and V of tile 0, K of tile 1 (the first again where there is none).
+template <int kWaves, class Rows, class Walk>
+__device__ __forceinline__ void start_pair(const Rows& rows, Walk walk, int n_keys, __bf16* const (&K)[2],
+                                           __bf16* const (&V)[2], int w, int lane) {
+  int t = 0;
+  TileMask m;
+  walk.next(t, m, true);
+  const auto s0 = rows.template src<16 / kWaves>(t, w, n_keys);
+  issue_half<kWaves, false>(rows, s0, n_keys, K[0], w, lane);
+  issue_half<kWaves, true>(rows, s0, n_keys, V[0], w, lane);
+  walk.next(t, m, false);                                    // (t stays past the end)
+  issue_half<kWaves, false>(rows, rows.template src<16 / kWaves>(t, w, n_keys), n_keys, K[1], w, lane);
+}
+
+// attend_tiles with two buffers each of K and V, tile m in K[m % 2] and V[m % 2], started by start_pair. Iteration n: wait for
+// the DMAs of iteration n - 1 (K(n+1), V(n)), barrier, DMA K(n+2) and V(n+1) into the buffers that were read last, softmax of
+// tile n beside the scores of tile n + 1, O += V(n) . P(n). The wait is the other workgroup's time: two share a CU.
+template <int H, int kWaves, class Rows, class Walk, class Lane>
+__device__ __forceinline__ void attend_pair(const Rows& rows, Walk& walk, int n_keys, __bf16* const (&K)[2],
+                                            __bf16* const (&V)[2], const bf16x8 (&qop)[H][4], floatx4 (&o)[8][H],
+                                            float (&m_run)[H], float (&l_run)[H], const Lane& lane_mask, float scale_log2,
+                                            int w, int lane) {
+  constexpr int kPerWave = 16 / kWaves;
+  const int m16 = lane & 15, j = lane >> 4;
+  int t0 = 0, t1 = 0;                              // first keys of tiles n, n+1
+  TileMask m0, m1;
+  if (!walk.next(t0, m0, true)) return;
+  t1 = t0;
+  bool h1 = walk.next(t1, m1, false);
+  static_assert(kWaves == 4, "the count that start_pair leaves behind K(0)");
+  __asm__ volatile("s_waitcnt vmcnt(8)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  floatx4 sa[2][2][H], sb[2][2][H], lsum[H];
+#pragma unroll
+  for (int u = 0; u < H; ++u) lsum[u] = floatx4{0.f, 0.f, 0.f, 0.f};
+  tile_scores<H>(K[0], qop, sa, m16, j);
+  auto step = [&](floatx4 (&s_cur)[2][2][H], floatx4 (&s_nxt)[2][2][H], auto slot_c) -> bool {
+    constexpr int slot = decltype(slot_c)::value;
+    int t2 = t1;
+    TileMask m2;
+    const bool h2 = h1 && walk.next(t2, m2, false);
+    const auto src_k = rows.template src<kPerWave>(h2 ? t2 : t0, w, n_keys);
+    const auto src_v = rows.template src<kPerWave>(h1 ? t1 : t0, w, n_keys);
+    __asm__ volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    issue_half<kWaves, false>(rows, src_k, n_keys, K[slot], w, lane);
+    issue_half<kWaves, true>(rows, src_v, n_keys, V[1 - slot], w, lane);
+    tile_mask<H, Walk>(s_cur, t0, m0, lane_mask, j);
+    bf16x8 pop[2][H];
+    tile_softmax<H>(s_cur, o, m_run, lsum, scale_log2, pop);
+    tile_scores<H>(K[1 - slot], qop, s_nxt, m16, j);         // (discarded after the last tile)
+    tile_pv<H>(V[slot], pop, o, lsum, lane);
+    if (!h1) return false;
+    t0 = t1; m0 = m1;
+    t1 = t2; m1 = m2; h1 = h2;
+    return true;
+  };
+  for (;;) {
+    if (!step(sa, sb, Slot<0>{})) break;
+    if (!step(sb, sa, Slot<1>{})) break;
+  }
+  __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");       // no DMA may outlive the workgroup's LDS
+#pragma unroll
+  for (int u = 0; u < H; ++u) l_run[u] = lsum[u][0];
 }
 
 }  // namespace abkv

@@ -47,7 +47,9 @@ struct WindowSpan {
 
 // Work of the window's dK/dV launch: one item per key tile for its near query tiles, and for each tile that holds sinks
 // `parts` more for the far ones, `part` query tiles each. The items of a sink tile leave fp32 sums in slots.
-constexpr int kSinkPartMin = 4;      // query tiles (x 4 heads) a far part is worth starting for
+// Query tiles (x 4 heads) a far part is worth starting for: with 8, us a forward and backward of three of up to 777 rows, window
+// 129, 17 sinks 120 (with 4: 99), of 2048 rows, window 64 117 (96), of 1000 rows, 100 sinks 107 (86).
+constexpr int kSinkPartMin = 4;
 constexpr int kSinkSlots = 384;      // bound on the far parts of a launch (64 KiB of sums each, per KV head)
 struct SinkPlan {
   int tiles, sink_tiles, part, parts;          // key tiles; those that hold sinks; query tiles per far part; parts a tile
