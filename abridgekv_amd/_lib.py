@@ -114,7 +114,7 @@ SIGNATURES = {
                              + [_vp, C.c_int, C.c_int, _vp, C.c_int, C.c_int, C.c_float]
                              + [_vp, C.c_long, C.c_long, C.c_long] * 3 + [_vp, C.c_size_t, _vp]),
     "abkv_paged_prefill_attn_window": (C.c_int, [_vp, C.c_long, C.c_long, _vp, C.c_int, _vp, C.c_long, C.c_int, _vp,
-                                                 _vp, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_float, _vp, C.c_long,
+                                                 _vp, C.c_int, C.c_int, C.c_int, C.c_float, _vp, C.c_long,
                                                  C.c_long, _vp, _vp]),
     "abkv_decode_window_workspace_size": (C.c_size_t, [C.c_int] * 5),
     "abkv_decode_attn_window": (C.c_int, [_vp, C.c_long, C.c_long, _vp, C.c_int, _vp, C.c_long, _vp, C.c_int, C.c_int,

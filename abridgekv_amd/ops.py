@@ -1146,7 +1146,7 @@ def paged_prefill_attention_window(q: torch.Tensor, kv_cache: torch.Tensor, bloc
     """Prompt chunks over the paged cache under a sliding window with sinks: request r's queries are tokens
     q_start[r]..q_start[r+1]-1 of q [T, 32, 128] bf16 at physical positions kv_start[r] + i (host sequences, as
     :func:`paged_prefill_attention`), and a query at position p sees rows j <= p with p - j < ``window`` or j < ``sinks``.
-    The chunk's own rows must be in the cache. Returns (out [T, 32, 128] bf16, lse [T, 32] fp32 or None); rows past
+    The chunk's own rows must be in the cache. The starts go with the launch (a captured one keeps them). Returns (out [T, 32, 128] bf16, lse [T, 32] fp32 or None); rows past
     q_start[-1] are left alone."""
     window, sinks = _check_window(window, sinks)
     scale = _softmax_scale(scale)
@@ -1156,22 +1156,18 @@ def paged_prefill_attention_window(q: torch.Tensor, kv_cache: torch.Tensor, bloc
         _check_out(out, torch.bfloat16, (T, HEADS_Q, HEAD_DIM))
     _require(lse is None or (lse.dtype == torch.float32 and lse.is_contiguous() and tuple(lse.shape) == (T, HEADS_Q)),
              "lse must be contiguous fp32 [T, 32]")
-    qs, ks, nq = _check_chunks(q, block_table, q_start, kv_start)
+    qs, ks, _ = _check_chunks(q, block_table, q_start, kv_start)
     _check_device(q, kv_cache, block_table, out, lse)
-    _require(not torch.cuda.is_current_stream_capturing(), "a chunk batch is uploaded from the host: not in a captured graph")
     if out is None:
         out = torch.empty((T, HEADS_Q, HEAD_DIM), dtype=torch.bfloat16, device=q.device)
-    req, q0 = _tiles(nq, 64)
-    tiles, R = req.size, ks.size
-    if tiles == 0:
+    if qs[-1] == 0:
         return out, lse
-    meta = _upload([qs, ks, req, q0], q.device)
-    at = meta.data_ptr()
+    starts = np.concatenate((qs, ks), dtype=np.int32, casting="unsafe")
+    at, R = starts.ctypes.data, ks.size
     rc = lib().abkv_paged_prefill_attn_window(_ptr(q), q.stride(0), q.stride(1), _ptr(kv_cache), kv_cache.shape[0],
                                               _ptr(block_table), _row_stride(block_table), block_table.shape[1], at,
-                                              at + 4 * (R + 1), at + 4 * (2 * R + 1), at + 4 * (2 * R + 1 + tiles), tiles,
-                                              window, sinks, scale, _ptr(out), out.stride(0), out.stride(1), _ptr(lse),
-                                              _stream())
+                                              at + 4 * (R + 1), R, window, sinks, scale, _ptr(out), out.stride(0),
+                                              out.stride(1), _ptr(lse), _stream())
     check(rc, "abkv_paged_prefill_attn_window")
     return out, lse
 

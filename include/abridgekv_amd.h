@@ -461,14 +461,14 @@ int abkv_window_attn_bwd(const void* q, long q_stride_b, long q_stride_s, long q
                          long dk_stride_s, long dk_stride_h, void* dv, long dv_stride_b, long dv_stride_s,
                          long dv_stride_h, void* workspace, size_t workspace_bytes, abkv_stream_t stream);
 /* Prompt chunks over the paged cache: request r's queries are rows q_start[r] .. q_start[r + 1] - 1 of q [T, 32, 128] bf16,
- * at physical positions kv_start[r] + i, causal. q_start [requests + 1], kv_start [requests], tile_req / tile_q0 [num_tiles]
- * (request and first query row of every 64-row query tile) on the device; every key position must lie inside the table row
- * (page ids are clamped into the cache). out [T, 32, 128], lse [T, 32] or NULL; rows of no request are left alone. */
+ * at physical positions kv_start[r] + i, causal. q_start [num_requests + 1] and kv_start [num_requests] are on the HOST and
+ * go with the launch (one for every 64 requests); every key position must lie inside the table row (page ids are clamped
+ * into the cache). out [T, 32, 128], lse [T, 32] or NULL; rows of no request are left alone. */
 int abkv_paged_prefill_attn_window(const void* q, long q_stride_tok, long q_stride_head, const void* kv_cache,
                                    int num_pages, const int32_t* block_table, long block_table_stride, int table_width,
-                                   const int32_t* q_start, const int32_t* kv_start, const int32_t* tile_req,
-                                   const int32_t* tile_q0, int num_tiles, int window, int sinks, float scale, void* out,
-                                   long out_stride_tok, long out_stride_head, float* lse, abkv_stream_t stream);
+                                   const int32_t* q_start, const int32_t* kv_start, int num_requests, int window, int sinks,
+                                   float scale, void* out, long out_stride_tok, long out_stride_head, float* lse,
+                                   abkv_stream_t stream);
 
 /* One new token per sequence over the paged cache under the window: as abkv_decode_attn, but of a sequence of n rows only
  * the pages of rows [n - window, n) and [0, sinks) are read. split_pages splits those pages; workspace:

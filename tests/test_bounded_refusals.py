@@ -198,7 +198,7 @@ def test_c_entry_points_return_errors():
                                        0),
                 L.abkv_window_attn_bwd(one, 1, stride, 1, *[one, 1, 1, 1] * 4, one, 1, 8, None, 4, 0, scale, *[one, 1, 1, 1] * 3,
                                        one, 1 << 30, 0),
-                L.abkv_paged_prefill_attn_window(one, stride, 1, one, 4, one, 4, 4, *n, 1, 4, 0, scale, one, 1, 1, None, 0),
+                L.abkv_paged_prefill_attn_window(one, stride, 1, one, 4, one, 4, 4, one, one, 1, 4, 0, scale, one, 1, 1, None, 0),
                 L.abkv_paged_prefill_scores(one, stride, 1, one, 4, one, 4, 4, *n, 1, 64, one, one, 64, 64, scale, 0))
 
     assert set(scaled(0.0) + scaled(-1.0) + scaled(float("nan")) + scaled(float("inf")) + scaled(1.0, 1 << 24)) == {bad}
@@ -223,6 +223,14 @@ def test_c_entry_points_return_errors():
     assert L.abkv_decode_attn_scored(one, 1, 1, one, 4, one, 40, one, 1, 40, 2, 1.0, 0, 640, 640, one, 1, 1, None, one,
                                      1 << 30, 0) == bad
     assert L.abkv_paged_prefill_scores(one, 1, 1, one, 4, one, 4, 4, *n, 1, 96, one, one, 64, 64, 1.0, 0) == bad
+
+    def chunk(starts, past, requests=None, width=4):
+        starts, past = (C.c_int32 * len(starts))(*starts), (C.c_int32 * len(past))(*past)
+        return L.abkv_paged_prefill_attn_window(one, 4096, 128, one, 4, one, width, width, C.addressof(starts), C.addressof(past),
+                                                len(past) if requests is None else requests, 4, 0, 1.0, one, 4096, 128, None, 0)
+
+    assert chunk([0, 1], [64]) == chunk([0, 65], [0]) == chunk([2, 1], [0]) == chunk([0, 1], [-1]) == chunk([-1, 0], [0]) == bad
+    assert chunk([0, 1, 2], [0, 64]) == bad and chunk([0, 5], [0], 0) == chunk([3, 3, 3], [0, 64]) == 0     # nothing to launch
     caches = (C.c_void_p * 1)(one)
 
     def ev(layers=1, budget=4, sinks=0, recent=0, pages=4, rows=64, arr=caches, ws=None):

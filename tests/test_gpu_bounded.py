@@ -200,7 +200,7 @@ def test_prefill_scores_of_rows_that_see_nothing(held):
     assert (got - want).abs().max() <= 772 * 2.0 ** -24 * want.max()
 
 
-def test_chunks_in_a_capture_are_refused():
+def test_prompt_scores_in_a_capture_are_refused():
     """Their tiles are uploaded from the host: a replay would read what is no longer there."""
     from abridgekv_amd import ops
     q, k, v, cache, table, _ = _paged([30], 8)
@@ -209,8 +209,6 @@ def test_chunks_in_a_capture_are_refused():
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         x = q * 2
-        with pytest.raises(ValueError, match="captured"):
-            ops.paged_prefill_attention_window(q[:1], cache, table, [0, 1], [0], 4)
         with pytest.raises(ValueError, match="captured"):
             ops.paged_prefill_scores(q[:1], cache, table, [0, 1], [0], lse, scores)
     graph.replay()

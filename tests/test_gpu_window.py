@@ -214,3 +214,43 @@ def test_paged_chunks(window, sinks):
                                            SCALE, bounds=True)
         assert (np.abs(out[a: a + c].double().cpu().numpy() - want) <= tol).all(), r
         assert np.abs(lse[a: a + c].double().cpu().numpy() - want_lse).max() <= ow.SLACK * ow.EPS + 1e-4, r
+
+
+def test_more_chunks_than_a_launch_takes():
+    """150 requests, some without queries, against each alone."""
+    from abridgekv_amd import ops
+    gen = torch.Generator().manual_seed(3)
+    rng = np.random.default_rng(3)
+    chunk, past = rng.integers(0, 4, 150) * rng.integers(1, 30, 150), rng.integers(0, 90, 150)
+    k = [torch.randn((c + p, 8, 128), generator=gen).to(torch.bfloat16) for c, p in zip(chunk, past)]
+    cache, table = _paged(k, k, 1400, 1, float("nan"))
+    q_start = np.concatenate([[0], np.cumsum(chunk)])
+    q = torch.randn((int(q_start[-1]), 32, 128), generator=gen).to(torch.bfloat16).cuda()
+    lse = torch.empty((q.shape[0], 32), device="cuda")
+    out, _ = ops.paged_prefill_attention_window(q, cache, table, q_start, past, 50, 3, lse=lse)
+    for r in range(150):
+        a, b = int(q_start[r]), int(q_start[r + 1])
+        if a < b:
+            one = torch.empty((b - a, 32), device="cuda")
+            alone, _ = ops.paged_prefill_attention_window(q[a:b], cache, table[r: r + 1], [0, b - a], [past[r]], 50, 3, lse=one)
+            assert torch.equal(out[a:b], alone) and torch.equal(lse[a:b], one), r
+
+
+def test_chunks_in_a_captured_graph():
+    """The requests' starts are the capture's, rows and tables are read by each replay."""
+    from abridgekv_amd import ops
+    gen = torch.Generator().manual_seed(9)
+    k = [torch.randn((n, 8, 128), generator=gen).to(torch.bfloat16) for n in (400, 90)]
+    cache, table = _paged(k, k, 60, 1, float("nan"))
+    q = torch.randn((130, 32, 128), generator=gen).to(torch.bfloat16).cuda()
+    args = ([0, 100, 130], [300, 60], 120, 4)
+    ops.paged_prefill_attention_window(q, cache, table, *args)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, _ = ops.paged_prefill_attention_window(q, cache, table, *args)
+    junk = [ops.paged_prefill_attention_window(q, cache, table, [0, 7], [50], 3)[0] for _ in range(3)]
+    for i in range(3):
+        q.copy_(torch.randn(q.shape, generator=gen).to(torch.bfloat16))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, ops.paged_prefill_attention_window(q, cache, table, *args)[0]), len(junk)
