@@ -124,8 +124,8 @@ SIGNATURES = {
     "abkv_decode_attn_scored": (C.c_int, [_vp, C.c_long, C.c_long, _vp, C.c_int, _vp, C.c_long, _vp, C.c_int, C.c_int,
                                           C.c_int, C.c_float, _vp, C.c_long, C.c_long, _vp, C.c_long, C.c_long, _vp, _vp,
                                           C.c_size_t, _vp]),
-    "abkv_paged_prefill_scores": (C.c_int, [_vp, C.c_long, C.c_long, _vp, C.c_int, _vp, C.c_long, C.c_int, _vp, _vp, _vp,
-                                            _vp, C.c_int, C.c_int, _vp, _vp, C.c_long, C.c_long, C.c_float, _vp]),
+    "abkv_paged_prefill_scores": (C.c_int, [_vp, C.c_long, C.c_long, _vp, C.c_int, _vp, C.c_long, C.c_int, _vp, _vp,
+                                            C.c_int, C.c_int, _vp, _vp, C.c_long, C.c_long, C.c_float, _vp]),
     "abkv_kv_evict_workspace_size": (C.c_size_t, [C.c_int] * 3),
     "abkv_kv_evict": (C.c_int, [C.POINTER(_vp), C.c_int, C.c_int, _vp, C.c_long, _vp, C.c_int, C.c_int, _vp, _vp,
                                 C.c_long, _vp, C.c_int, C.c_int, C.c_int, _vp, _vp, C.c_size_t, _vp]),

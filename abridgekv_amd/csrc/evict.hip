@@ -1,5 +1,7 @@
 // What a cache bounded by weight needs beside its attention (gfx950): the attention weights of a prompt's queries added up
 // per cached row, and the eviction of the rows that weigh least. (A decode step's weights: decode_attn.hip.)
+#include <algorithm>
+
 #include "attn_tile.h"
 
 namespace abkv {
@@ -16,17 +18,18 @@ namespace abkv {
 // with the operands' reads and the barriers. 1500 rows and 2048 behind 2048: 94 us a call, 650 TFLOP/s of visible pairs. Tried:
 // query rows straight into operand registers 166 us (64 bytes of each of 16 rows an instruction; without those loads 88); 64
 // keys a wave at two waves a SIMD, its three stages interleaved by hand, 95, with a step a barrier more 99.
+// The requests and the tiles' order go with the launch's arguments (uploaded before it, two prompts 88 us a call and 64 queries
+// behind 4000 rows 41, this 83 and 21).
+constexpr int kScoreRequests = 64, kScoreTiles = 640;        // of a launch (3.3 KiB of arguments)
 struct PromptScoreArgs {
   const __bf16* q;  long q_st, q_sh;           // [T, 32, 128]
   const __bf16* kv; int num_pages;             // [pages, 2, 16, 8, 128]
-  const int32_t* block_table; long bt_stride; int bt_width;
-  const int32_t* q_start;                      // [R + 1]
-  const int32_t* kv_start;                     // [R]
-  const int32_t* tile_req;                     // [tiles] request of each tile of 64 * kTiles keys
-  const int32_t* tile_k0;                      // [tiles] its first key
+  const int32_t* block_table; long bt_stride; int bt_width;      // (of the launch's first request)
   const float* lse;                            // [T, 32] natural log
-  float* scores;  long s_sb, s_sh;             // [R, 8, rows]
+  float* scores;  long s_sb, s_sh;             // [R, 8, rows] (of the launch's first request)
   float scale_log2;
+  int32_t q_start[kScoreRequests + 1], kv_start[kScoreRequests];
+  uint32_t tiles[kScoreTiles];                 // request << 24 | number of its tile of 64 * kTiles keys
 };
 
 // Sum over a row of 16 lanes, in each of them (DPP: no LDS).
@@ -50,7 +53,8 @@ __global__ __launch_bounds__(64 * kScoreWaves) void prompt_scores_kernel(PromptS
   __bf16* const Qb[3] = {Q0, Q1, Q2};
   float* const Lb[3] = {L0, L1, L2};
   const int kvh = blockIdx.x % kHeadsKV, tile = blockIdx.x / kHeadsKV;
-  const int r = a.tile_req[tile], first_key = a.tile_k0[tile];
+  const uint32_t code = a.tiles[tile];
+  const int r = code >> 24, first_key = (code & 0xffffffu) * (kBN * kTiles);
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, m16 = lane & 15, j = lane >> 4;
   const int t0 = a.q_start[r], nq = a.q_start[r + 1] - t0, kv0 = a.kv_start[r];
@@ -364,23 +368,69 @@ extern "C" {
 
 int abkv_paged_prefill_scores(const void* q, long q_stride_tok, long q_stride_head, const void* kv_cache, int num_pages,
                               const int32_t* block_table, long block_table_stride, int table_width, const int32_t* q_start,
-                              const int32_t* kv_start, const int32_t* tile_req, const int32_t* tile_k0, int num_tiles,
-                              int tile_keys, const float* lse, float* scores, long scores_stride_req, long scores_stride_head, float scale,
-                              hipStream_t stream) {
+                              const int32_t* kv_start, int num_requests, int tile_keys, const float* lse, float* scores,
+                              long scores_stride_req, long scores_stride_head, float scale, hipStream_t stream) {
   using namespace abkv;
-  if (num_tiles <= 0) return 0;
+  if (num_requests <= 0) return 0;
   if (q == nullptr || kv_cache == nullptr || block_table == nullptr || q_start == nullptr || kv_start == nullptr ||
-      tile_req == nullptr || tile_k0 == nullptr || lse == nullptr || scores == nullptr || num_pages <= 0 || table_width <= 0 ||
-      (tile_keys != kBN && tile_keys != 2 * kBN) || !row_strides_ok(q_stride_tok) || q_stride_head >= 1L << 28 || !softmax_scale_ok(scale))
+      lse == nullptr || scores == nullptr || num_pages <= 0 || table_width <= 0 ||
+      (tile_keys != kBN && tile_keys != 2 * kBN) || !row_strides_ok(q_stride_tok) || q_stride_head >= 1L << 28 ||
+      !softmax_scale_ok(scale))
     return (int)hipErrorInvalidValue;
-  const PromptScoreArgs a{static_cast<const __bf16*>(q), q_stride_tok, q_stride_head, static_cast<const __bf16*>(kv_cache),
-                          num_pages, block_table, block_table_stride, table_width, q_start, kv_start, tile_req, tile_k0, lse,
-                          scores, scores_stride_req, scores_stride_head, scale * 1.4426950408889634f};
-  const long grid = (long)num_tiles * kHeadsKV;
-  if (grid * 64 * kScoreWaves > 0xFFFFFFFFL) return (int)hipErrorInvalidValue;
-  if (tile_keys == kBN) hipLaunchKernelGGL(prompt_scores_kernel<1>, dim3((unsigned)grid), dim3(64 * kScoreWaves), 0, stream, a);
-  else hipLaunchKernelGGL(prompt_scores_kernel<2>, dim3((unsigned)grid), dim3(64 * kScoreWaves), 0, stream, a);
-  return (int)hipGetLastError();
+  const long slots = std::min((long)table_width * kPage, 1L << 30);              // (tile numbers: 24 bits)
+  for (int r = 0; r < num_requests; ++r)
+    if (q_start[0] < 0 || q_start[r + 1] < q_start[r] || kv_start[r] < 0 ||
+        (long)kv_start[r] + q_start[r + 1] - q_start[r] > slots)
+      return (int)hipErrorInvalidValue;
+  PromptScoreArgs a{};
+  a.q = static_cast<const __bf16*>(q);
+  a.q_st = q_stride_tok; a.q_sh = q_stride_head;
+  a.kv = static_cast<const __bf16*>(kv_cache);
+  a.num_pages = num_pages;
+  a.bt_stride = block_table_stride;
+  a.bt_width = table_width;
+  a.lse = lse;
+  a.s_sb = scores_stride_req; a.s_sh = scores_stride_head;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  int count = 0;
+  auto launch = [&]() -> hipError_t {
+    const dim3 grid((unsigned)(count * kHeadsKV)), block(64 * kScoreWaves);
+    count = 0;
+    if (grid.x == 0) return hipSuccess;
+    if (tile_keys == kBN) hipLaunchKernelGGL(prompt_scores_kernel<1>, grid, block, 0, stream, a);
+    else hipLaunchKernelGGL(prompt_scores_kernel<2>, grid, block, 0, stream, a);
+    return hipGetLastError();
+  };
+  for (int first = 0; first < num_requests; first += kScoreRequests) {
+    const int n = std::min(num_requests - first, kScoreRequests);
+    const int32_t* qs = q_start + first;
+    const int32_t* ks = kv_start + first;
+    a.block_table = block_table + (long)first * block_table_stride;
+    a.scores = scores + (long)first * scores_stride_req;
+    int most = 0, next[kScoreRequests] = {};
+    for (int r = 0; r < n; ++r) {
+      a.q_start[r] = qs[r];
+      a.kv_start[r] = ks[r];
+      most = std::max(most, qs[r + 1] - qs[r]);
+    }
+    a.q_start[n] = qs[n];
+    // the tiles that most queries see first, to within a tile's keys: workgroups that start last are short
+    for (long level = most; level > 0; level -= tile_keys)
+      for (int r = 0; r < n; ++r) {
+        const int rows = qs[r + 1] - qs[r];
+        for (;; ++next[r]) {
+          const long k0 = (long)next[r] * tile_keys;
+          if (rows == 0 || k0 >= (long)ks[r] + rows || rows - std::max(k0 - ks[r], 0L) <= level - tile_keys) break;
+          a.tiles[count++] = (uint32_t)r << 24 | (uint32_t)next[r];
+          if (count < kScoreTiles) continue;
+          const hipError_t err = launch();
+          if (err != hipSuccess) return (int)err;
+        }
+      }
+    const hipError_t err = launch();
+    if (err != hipSuccess) return (int)err;
+  }
+  return 0;
 }
 
 size_t abkv_kv_evict_workspace_size(int num_layers, int num_seqs, int max_pages_per_seq) {

@@ -18,8 +18,9 @@
 
 namespace abkv {
 
-// Prompt chunks: request r's queries are rows q_start[r] .. q_start[r + 1] - 1 at positions kv_start[r] + i. The requests come
-// with the launch's arguments (uploaded before it, four chunks of up to 512 cost 54 us a call, this 47.5), and a workgroup finds its own by bisection.
+// Prompt chunks: request r's queries are rows q_start[r] .. q_start[r + 1] - 1 at positions kv_start[r] + i. The requests
+// come with the launch's arguments (uploaded before it, four chunks of up to 512 cost 54 us a call, this 47.5), and a
+// workgroup finds its own by bisection.
 constexpr int kChunks = 64;                    // requests of a launch
 struct ChunkArgs {
   static constexpr bool kPaged = true;

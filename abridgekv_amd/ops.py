@@ -1133,13 +1133,6 @@ def _check_chunks(q, block_table, q_start, kv_start):
     return qs, ks, nq
 
 
-def _tiles(rows: np.ndarray, step: int):
-    """(request, first row) of every tile of ``step`` rows of requests of ``rows`` rows."""
-    n = -(-rows // step)
-    req = np.repeat(np.arange(rows.size), n)
-    return req, (np.arange(req.size) - np.repeat(np.cumsum(n) - n, n)) * step
-
-
 def paged_prefill_attention_window(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, q_start, kv_start,
                                    window: int, sinks: int = 0, scale: float | None = None,
                                    out: torch.Tensor | None = None, lse: torch.Tensor | None = None):
@@ -1335,6 +1328,7 @@ def paged_prefill_scores(q: torch.Tensor, kv_cache: torch.Tensor, block_table: t
     Queries as :func:`paged_prefill_attention` takes causal chunks (q [T, 32, 128] bf16, host q_start [R + 1] and kv_start
     [R]); ``lse`` [T, 32] fp32: what that call left for them (rows with -inf add nothing, whatever they hold). To weigh by a
     prompt's last queries only, pass those alone with their kv_start. ``scores`` [R, 8, rows] fp32 is updated in place, one owner a score.
+    The starts go with the launch (a captured one keeps them).
     """
     scale = _softmax_scale(scale)
     _check_paged(q, kv_cache, block_table)
@@ -1344,19 +1338,15 @@ def paged_prefill_scores(q: torch.Tensor, kv_cache: torch.Tensor, block_table: t
     _check_scores(scores, len(kv_start), block_table.shape[1] * PAGE)
     qs, ks, nq = _check_chunks(q, block_table, q_start, kv_start)
     _check_device(q, kv_cache, block_table, lse, scores)
-    _require(not torch.cuda.is_current_stream_capturing(), "a chunk batch is uploaded from the host: not in a captured graph")
     if qs[-1] == 0:
         return
     keys = _score_tile_keys(ks, nq, _num_cus())
-    req, k0 = _tiles(np.where(nq > 0, ks + nq, 0), keys)
-    order = np.argsort(np.maximum(k0 - ks[req], 0) - nq[req], kind="stable")      # the tiles that most queries see first
-    tiles, R = req.size, ks.size
-    meta = _upload([qs, ks, req[order], k0[order]], q.device)
-    at = meta.data_ptr()
+    starts = np.concatenate((qs, ks), dtype=np.int32, casting="unsafe")
+    at, R = starts.ctypes.data, ks.size
     rc = lib().abkv_paged_prefill_scores(_ptr(q), q.stride(0), q.stride(1), _ptr(kv_cache), kv_cache.shape[0],
                                          _ptr(block_table), _row_stride(block_table), block_table.shape[1], at,
-                                         at + 4 * (R + 1), at + 4 * (2 * R + 1), at + 4 * (2 * R + 1 + tiles), tiles, keys,
-                                         _ptr(lse), _ptr(scores), scores.stride(0), scores.stride(1), scale, _stream())
+                                         at + 4 * (R + 1), R, keys, _ptr(lse), _ptr(scores), scores.stride(0),
+                                         scores.stride(1), scale, _stream())
     check(rc, "abkv_paged_prefill_scores")
 
 

@@ -499,14 +499,13 @@ int abkv_decode_attn_scored(const void* q, long q_stride_seq, long q_stride_head
                             void* workspace, size_t workspace_bytes, abkv_stream_t stream);
 /* The weights of prompt queries: scores[r][h][j] += sum over request r's queries i (rows q_start[r] .. q_start[r + 1] - 1 of
  * q [T, 32, 128] bf16 at positions kv_start[r] + i) with j <= position, and h's query heads, of exp(scale q.k - lse).
- * lse [T, 32]: what the queries' attention over the same rows left (a row with -inf adds nothing). tile_req / tile_k0
- * [num_tiles]: request and first key of every tile of tile_keys (64 or 128; the first key a multiple of it) rows of
- * [0, kv_start + queries), the ones that most queries see first. */
+ * lse [T, 32]: what the queries' attention over the same rows left (a row with -inf adds nothing). q_start
+ * [num_requests + 1] and kv_start [num_requests] are on the HOST and go with the launch (one for every 64 requests and 640
+ * tiles of tile_keys keys, 64 or 128). */
 int abkv_paged_prefill_scores(const void* q, long q_stride_tok, long q_stride_head, const void* kv_cache, int num_pages,
                               const int32_t* block_table, long block_table_stride, int table_width, const int32_t* q_start,
-                              const int32_t* kv_start, const int32_t* tile_req, const int32_t* tile_k0, int num_tiles,
-                              int tile_keys, const float* lse, float* scores, long scores_stride_req, long scores_stride_head, float scale,
-                              abkv_stream_t stream);
+                              const int32_t* kv_start, int num_requests, int tile_keys, const float* lse, float* scores,
+                              long scores_stride_req, long scores_stride_head, float scale, abkv_stream_t stream);
 /* Evict from up to 16 layer caches of one KV-cache group. Per (layer, sequence, KV head) of n = seq_lens[b] rows (clamped to
  * 16 * max_pages_per_seq) m = min(n, budget) are kept: rows of tokens below `sinks` and from num_tokens[b] - recent on, then
  * the highest scores (ties: the lowest row; NaN below every number). The kept rows at or past m move to the evicted rows below

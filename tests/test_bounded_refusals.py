@@ -186,7 +186,6 @@ def test_evict():
 def test_c_entry_points_return_errors():
     """Bad arguments that get past no launch (the pointers are never followed)."""
     L, one = lib(), 1 << 12
-    n = [one] * 4
     bad = 1                                                  # hipErrorInvalidValue
 
     def win(window=4, sinks=0, q=one):
@@ -199,7 +198,7 @@ def test_c_entry_points_return_errors():
                 L.abkv_window_attn_bwd(one, 1, stride, 1, *[one, 1, 1, 1] * 4, one, 1, 8, None, 4, 0, scale, *[one, 1, 1, 1] * 3,
                                        one, 1 << 30, 0),
                 L.abkv_paged_prefill_attn_window(one, stride, 1, one, 4, one, 4, 4, one, one, 1, 4, 0, scale, one, 1, 1, None, 0),
-                L.abkv_paged_prefill_scores(one, stride, 1, one, 4, one, 4, 4, *n, 1, 64, one, one, 64, 64, scale, 0))
+                L.abkv_paged_prefill_scores(one, stride, 1, one, 4, one, 4, 4, one, one, 1, 64, one, one, 64, 64, scale, 0))
 
     assert set(scaled(0.0) + scaled(-1.0) + scaled(float("nan")) + scaled(float("inf")) + scaled(1.0, 1 << 24)) == {bad}
     assert win(0) == win(4, -1) == win(q=0) == bad
@@ -222,12 +221,15 @@ def test_c_entry_points_return_errors():
                                      0) == bad
     assert L.abkv_decode_attn_scored(one, 1, 1, one, 4, one, 40, one, 1, 40, 2, 1.0, 0, 640, 640, one, 1, 1, None, one,
                                      1 << 30, 0) == bad
-    assert L.abkv_paged_prefill_scores(one, 1, 1, one, 4, one, 4, 4, *n, 1, 96, one, one, 64, 64, 1.0, 0) == bad
+    assert L.abkv_paged_prefill_scores(one, 1, 1, one, 4, one, 4, 4, one, one, 1, 96, one, one, 64, 64, 1.0, 0) == bad
 
     def chunk(starts, past, requests=None, width=4):
         starts, past = (C.c_int32 * len(starts))(*starts), (C.c_int32 * len(past))(*past)
-        return L.abkv_paged_prefill_attn_window(one, 4096, 128, one, 4, one, width, width, C.addressof(starts), C.addressof(past),
-                                                len(past) if requests is None else requests, 4, 0, 1.0, one, 4096, 128, None, 0)
+        batch = (one, 4096, 128, one, 4, one, width, width, C.addressof(starts), C.addressof(past),
+                 len(past) if requests is None else requests)
+        rc = L.abkv_paged_prefill_attn_window(*batch, 4, 0, 1.0, one, 4096, 128, None, 0)
+        assert rc == L.abkv_paged_prefill_scores(*batch, 64, one, one, 512, 64, 1.0, 0)
+        return rc
 
     assert chunk([0, 1], [64]) == chunk([0, 65], [0]) == chunk([2, 1], [0]) == chunk([0, 1], [-1]) == chunk([-1, 0], [0]) == bad
     assert chunk([0, 1, 2], [0, 64]) == bad and chunk([0, 5], [0], 0) == chunk([3, 3, 3], [0, 64]) == 0     # nothing to launch
@@ -290,11 +292,5 @@ def test_step_splits():
 
 
 def test_score_tiles():
-    for ks, nq in (([0], [1]), ([0, 500], [2048, 3]), ([8000], [64])):
-        ks, nq = np.array(ks), np.array(nq)
-        assert ops._score_tile_keys(ks, nq, 256) in (64, 128)
-        req, first = ops._tiles(ks + nq, 64)
-        for r in range(ks.size):
-            assert first[req == r].tolist() == list(range(0, int(ks[r] + nq[r]), 64))
-    req, first = ops._tiles(np.array([0, 65, 0, 64]), 64)
-    assert req.tolist() == [1, 1, 3] and first.tolist() == [0, 64, 0]
+    for ks, nq in (([0], [1]), ([0, 500], [2048, 3]), ([8000], [64]), ([7, 0], [0, 2])):
+        assert ops._score_tile_keys(np.array(ks), np.array(nq), 256) in (64, 128)

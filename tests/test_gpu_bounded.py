@@ -200,19 +200,48 @@ def test_prefill_scores_of_rows_that_see_nothing(held):
     assert (got - want).abs().max() <= 772 * 2.0 ** -24 * want.max()
 
 
-def test_prompt_scores_in_a_capture_are_refused():
-    """Their tiles are uploaded from the host: a replay would read what is no longer there."""
+def test_prefill_scores_of_more_than_a_launch_takes():
+    """150 requests, and 12 of more tiles than one launch lists (over the same pages), against each alone."""
     from abridgekv_amd import ops
-    q, k, v, cache, table, _ = _paged([30], 8)
-    q = q.cuda()
-    lse, scores = torch.zeros((1, 32), device="cuda"), torch.zeros((1, 8, 32), device="cuda")
+    rng = np.random.default_rng(3)
+    short = (rng.integers(0, 4, 150) * rng.integers(1, 30, 150), rng.integers(0, 90, 150), 1)
+    for chunk, past, seed in (short, (rng.integers(1, 100, 12), rng.integers(8000, 8100, 12), 2)):
+        lens = [int(c + p) for c, p in zip(chunk, past)]
+        _, k, v, cache, table, _ = _paged(lens if seed == 1 else [8200], seed)
+        table = table.expand(len(lens), -1).contiguous()
+        q_start = np.concatenate([[0], np.cumsum(chunk)])
+        T = int(q_start[-1])
+        q = torch.randn((T, 32, 128), generator=torch.Generator().manual_seed(seed)).to(torch.bfloat16).cuda()
+        lse = torch.full((T, 32), 6.0, device="cuda")
+        scores = torch.rand((len(lens), 8, table.shape[1] * 16), device="cuda")
+        want = scores.clone()
+        ops.paged_prefill_scores(q, cache, table, q_start, past, lse, scores)
+        for r in range(len(lens)):
+            a, b = int(q_start[r]), int(q_start[r + 1])
+            ops.paged_prefill_scores(q[a:b], cache, table[r: r + 1], [0, b - a], [past[r]], lse[a:b], want[r: r + 1])
+        # tiles of 64 or 128 keys by the call's sizes: two orders of the same sums
+        assert ((scores - want).abs() <= 4 * chunk.max() * 2.0 ** -24 * want).all()
+
+
+def test_prefill_scores_in_a_captured_graph():
+    """The requests' starts are the capture's; queries, lse and scores are each replay's."""
+    from abridgekv_amd import ops
+    _, k, v, cache, table, _ = _paged([400, 90], 8)
+    gen = torch.Generator().manual_seed(2)
+    q = torch.randn((130, 32, 128), generator=gen).to(torch.bfloat16).cuda()
+    lse = torch.full((130, 32), 6.0, device="cuda")
+    scores = torch.zeros((2, 8, 400), device="cuda")
+    want = torch.zeros_like(scores)
+    ops.paged_prefill_scores(q, cache, table, [0, 100, 130], [300, 60], lse, scores.clone())
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        x = q * 2
-        with pytest.raises(ValueError, match="captured"):
-            ops.paged_prefill_scores(q[:1], cache, table, [0, 1], [0], lse, scores)
-    graph.replay()
-    assert torch.equal(x, q * 2)
+        ops.paged_prefill_scores(q, cache, table, [0, 100, 130], [300, 60], lse, scores)
+    for i in range(3):
+        q.copy_(torch.randn(q.shape, generator=gen).to(torch.bfloat16))
+        graph.replay()
+        torch.cuda.synchronize()
+        ops.paged_prefill_scores(q, cache, table, [0, 100, 130], [300, 60], lse, want)
+        assert torch.equal(scores, want)
 
 
 def _evict_case(lens, seed, layers=2, levels=None, recorded=False):
