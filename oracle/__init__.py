@@ -14,6 +14,8 @@ Modules (each function cites the reference file:line it restates):
                     gather-then-scatter semantics, block-table truncation and slot mapping.
 * ``prefill``    -- the teacher-forced compression mask in its two reference forms (role/block dense mask and the
                     closed-form arithmetic mask) and an fp64 masked attention.
+* ``window``     -- sliding-window attention with sinks and its gradients in fp64, with bounds on each rounding.
+* ``evict``      -- accumulated attention weights and the eviction of the lightest rows, one row at a time.
 * ``trace``      -- the block state machine that decides which spans are compacted when (processor semantics),
                     producing planner-agnostic event traces.
 
