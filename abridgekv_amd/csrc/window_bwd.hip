@@ -177,20 +177,29 @@ __global__ __launch_bounds__(256, 2) void window_bwd_dkv_kernel(WindowBwdArgs a)
   for (int e = 0; e < 8; ++e) dk[e][0] = dv[e][0] = floatx4{0.f, 0.f, 0.f, 0.f};
 
   const WindowSpan span(k0, n, f.window, f.sinks);
-  int qt = span.first, qt_end = span.near_end;
+  int qt_first = span.first, qt_end = span.near_end;
   if (z > 0) {
-    qt = min(span.near_end + (z - 1) * a.plan.part, span.far_end);
-    qt_end = min(qt + a.plan.part, span.far_end);
+    qt_first = min(span.near_end + (z - 1) * a.plan.part, span.far_end);
+    qt_end = min(qt_first + a.plan.part, span.far_end);
   }
+  // The near query tiles in cyclic order from a multiple of `reach`, their number for an inner key tile: the workgroups of
+  // neighbouring key tiles, which run at one time, then take the same query tile at the same step, and its rows come from
+  // their XCD's L2 (from its own first tile on, a workgroup reads what its neighbour read a step before, when the other 60 of
+  // the XCD have passed 8 MB: four times the fetches). us a forward and backward, two of 4096 rows, window 512: 463 -> 450;
+  // four, window 1024: 1346 -> 1307.
+  const int reach = (min(f.window, f.S) + kBN - 2) / kBM + 1;
+  int left = qt_end - qt_first, qt = (qt_first + reach - 1) / reach * reach;
+  if (z > 0 || qt >= qt_end) qt = qt_first;
   // rows that see this lane's key: from the key on, `rows` of them (past the sequence: none)
   const unsigned rows = !in ? 0u : (unsigned)(key < f.sinks ? n - key : min(f.window, n - key));
   int h = -1;
   auto next_pair = [&]() -> bool {                           // (query tile, head) pairs, head fastest
     if (++h == kGroup) {
       h = 0;
-      ++qt;
+      if (++qt == qt_end) qt = qt_first;
+      --left;
     }
-    return qt < qt_end;
+    return left > 0;
   };
   // Q / dO rows of (qt, head) as the tile rows, lse2 / D rows beside them (waves 0 and 1, 4 bytes per lane)
   auto issue = [&](int pq, int ph, int sl_dst) {
