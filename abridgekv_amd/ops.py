@@ -1139,8 +1139,8 @@ def paged_prefill_attention_window(q: torch.Tensor, kv_cache: torch.Tensor, bloc
     """Prompt chunks over the paged cache under a sliding window with sinks: request r's queries are tokens
     q_start[r]..q_start[r+1]-1 of q [T, 32, 128] bf16 at physical positions kv_start[r] + i (host sequences, as
     :func:`paged_prefill_attention`), and a query at position p sees rows j <= p with p - j < ``window`` or j < ``sinks``.
-    The chunk's own rows must be in the cache. The starts go with the launch (a captured one keeps them). Returns (out [T, 32, 128] bf16, lse [T, 32] fp32 or None); rows past
-    q_start[-1] are left alone."""
+    The chunk's own rows must be in the cache. The starts go with the launch (a captured one keeps them). Returns (out
+    [T, 32, 128] bf16, lse [T, 32] fp32 or None); rows past q_start[-1] are left alone."""
     window, sinks = _check_window(window, sinks)
     scale = _softmax_scale(scale)
     _check_paged(q, kv_cache, block_table)
@@ -1250,7 +1250,7 @@ def decode_attention_window(q: torch.Tensor, kv_cache: torch.Tensor, block_table
     B, max_pages = _check_step(q, kv_cache, block_table, seq_lens, max_pages, split_pages, out, lse)
     _check_device(q, kv_cache, block_table, seq_lens, out, lse)
     if out is None:
-        out = torch.empty((B, HEADS_Q, HEAD_DIM), dtype=torch.bfloat16, device=q.device)
+        out = q.new_empty((B, HEADS_Q, HEAD_DIM))
     split_pages = split_pages or window_split_pages(B, max_pages, window, sinks)
     need = lib().abkv_decode_window_workspace_size(B, max_pages, split_pages, window, sinks)
     workspace, ws_bytes = _take_workspace(workspace, need, q.device)
@@ -1297,7 +1297,7 @@ def decode_attention_scored(q: torch.Tensor, kv_cache: torch.Tensor, block_table
     _check_scores(scores, B, max_pages * PAGE)
     _check_device(q, kv_cache, block_table, seq_lens, scores, out, lse)
     if out is None:
-        out = torch.empty((B, HEADS_Q, HEAD_DIM), dtype=torch.bfloat16, device=q.device)
+        out = q.new_empty((B, HEADS_Q, HEAD_DIM))
     split_pages = split_pages or _step_split_pages(B, max_pages)
     need = lib().abkv_decode_scored_workspace_size(B, max_pages, split_pages)
     workspace, ws_bytes = _take_workspace(workspace, need, q.device)
@@ -1327,8 +1327,8 @@ def paged_prefill_scores(q: torch.Tensor, kv_cache: torch.Tensor, block_table: t
 
     Queries as :func:`paged_prefill_attention` takes causal chunks (q [T, 32, 128] bf16, host q_start [R + 1] and kv_start
     [R]); ``lse`` [T, 32] fp32: what that call left for them (rows with -inf add nothing, whatever they hold). To weigh by a
-    prompt's last queries only, pass those alone with their kv_start. ``scores`` [R, 8, rows] fp32 is updated in place, one owner a score.
-    The starts go with the launch (a captured one keeps them).
+    prompt's last queries only, pass those alone with their kv_start. ``scores`` [R, 8, rows] fp32 is updated in place, one
+    owner a score. The starts go with the launch (a captured one keeps them).
     """
     scale = _softmax_scale(scale)
     _check_paged(q, kv_cache, block_table)
