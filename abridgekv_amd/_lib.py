@@ -105,13 +105,13 @@ SIGNATURES = {
     "abkv_planner_apply_events": (C.c_int64, [_vp, _i64p, C.c_int64]),
     "abkv_window_attn": (C.c_int, [_vp, C.c_long, C.c_long, C.c_long] * 3
                          + [C.c_int, C.c_int, _vp, C.c_int, C.c_int, C.c_float, _vp, C.c_long, C.c_long, C.c_long,
-                            _vp, _vp]),
+                            _vp, _vp, _vp]),
     "abkv_window_attn_f32": (C.c_int, [_vp, C.c_long, C.c_long, C.c_long] * 3
                              + [C.c_int, C.c_int, _vp, C.c_int, C.c_int, C.c_float, _vp, C.c_long, C.c_long,
                                 C.c_long, _vp, _vp]),
     "abkv_window_bwd_workspace_size": (C.c_size_t, [C.c_int, C.c_int, C.c_int, C.c_int]),
     "abkv_window_attn_bwd": (C.c_int, [_vp, C.c_long, C.c_long, C.c_long] * 5
-                             + [_vp, C.c_int, C.c_int, _vp, C.c_int, C.c_int, C.c_float]
+                             + [_vp, _vp, C.c_int, C.c_int, _vp, C.c_int, C.c_int, C.c_float]
                              + [_vp, C.c_long, C.c_long, C.c_long] * 3 + [_vp, C.c_size_t, _vp]),
     "abkv_paged_prefill_attn_window": (C.c_int, [_vp, C.c_long, C.c_long, _vp, C.c_int, _vp, C.c_long, C.c_int, _vp,
                                                  _vp, C.c_int, C.c_int, C.c_int, C.c_float, _vp, C.c_long,

@@ -121,14 +121,16 @@ class _WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, query, key, value, mask: WindowMask, scale: float):
         q, k, v = query.transpose(1, 2), key.transpose(1, 2), value.transpose(1, 2)
-        lse = None
+        lse = low = None
         if any(ctx.needs_input_grad[:3]):
             if q.dtype != torch.bfloat16:
                 raise NotImplementedError("the sliding-window backward runs bf16 inputs")
             lse = torch.empty((q.shape[0], ops.HEADS_Q, q.shape[1]), dtype=torch.float32, device=q.device)
-        out, _ = ops.window_attention(q, k, v, mask.window, mask.sinks, seq_lens=mask.seq_lens, scale=scale, lse=lse)
+            low = torch.empty((*q.shape[:2], ops.HEADS_Q, ops.HEAD_DIM), dtype=torch.float8_e5m2, device=q.device)
+        out, _ = ops.window_attention(q, k, v, mask.window, mask.sinks, seq_lens=mask.seq_lens, scale=scale, lse=lse,
+                                      out_low=low)
         if lse is not None:
-            ctx.save_for_backward(q, k, v, out, lse, mask.seq_lens)
+            ctx.save_for_backward(q, k, v, out, lse, low, mask.seq_lens)
             ctx.mask, ctx.scale = mask, scale
         return out
 
@@ -136,11 +138,12 @@ class _WindowAttention(torch.autograd.Function):
     def backward(ctx, grad_out):
         if torch.is_grad_enabled():
             raise RuntimeError("sliding-window attention has no second derivative")
-        q, k, v, out, lse, seq_lens = ctx.saved_tensors
+        q, k, v, out, lse, low, seq_lens = ctx.saved_tensors
         st = grad_out.stride()
         if st[3] != 1 or (st[0] | st[1] | st[2]) % 8 or st[1] >= 1 << 24 or grad_out.data_ptr() % 16:
             grad_out = grad_out.contiguous()
-        dq, dk, dv = ops.window_backward(q, k, v, out, lse, grad_out, ctx.mask.window, ctx.mask.sinks, seq_lens, ctx.scale)
+        dq, dk, dv = ops.window_backward(q, k, v, out, lse, grad_out, ctx.mask.window, ctx.mask.sinks, seq_lens, ctx.scale,
+                                         low)
         return dq.transpose(1, 2), dk.transpose(1, 2), dv.transpose(1, 2), None, None
 
 

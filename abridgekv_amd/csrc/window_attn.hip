@@ -132,6 +132,8 @@ __global__ __launch_bounds__(256, 2) void window_attn_kernel(WindowArgs a, Chunk
 #pragma unroll
       for (int e = 0; e < 8; ++e) o[e][u] = floatx4{0.f, 0.f, 0.f, 0.f};
     store_acc_rows<H>(a.out + o_row + (long)head * a.o_sh, o, u, j, inv);
+    if constexpr (!kPaged)
+      if (a.low != nullptr) store_low<H>(a.low + (((long)b * a.S + qi) * kHeadsQ + head) * kHeadDim, o, u, j, inv);
     if (a.lse != nullptr && j == 0)
       a.lse[kPaged ? (long)(t0 + qi) * kHeadsQ + head : ((long)b * kHeadsQ + head) * a.S + qi] =
           l == 0.f ? -INFINITY : (m_run[u] + __log2f(l)) * 0.69314718055994531f;
@@ -145,7 +147,8 @@ extern "C" {
 int abkv_window_attn(const void* q, long q_stride_b, long q_stride_s, long q_stride_h, const void* k, long k_stride_b,
                      long k_stride_s, long k_stride_h, const void* v, long v_stride_b, long v_stride_s, long v_stride_h,
                      int batch, int seq_len, const int32_t* seq_lens, int window, int sinks, float scale, void* out,
-                     long out_stride_b, long out_stride_s, long out_stride_h, float* lse, hipStream_t stream) {
+                     long out_stride_b, long out_stride_s, long out_stride_h, float* lse, void* out_low,
+                     hipStream_t stream) {
   using namespace abkv;
   if (batch <= 0 || seq_len <= 0) return 0;
   if (q == nullptr || k == nullptr || v == nullptr || out == nullptr || window <= 0 || sinks < 0 ||
@@ -167,6 +170,7 @@ int abkv_window_attn(const void* q, long q_stride_b, long q_stride_s, long q_str
   a.out = static_cast<__bf16*>(out);
   a.o_sb = out_stride_b; a.o_ss = out_stride_s; a.o_sh = out_stride_h;
   a.lse = lse;
+  a.low = static_cast<uint8_t*>(out_low);
   a.num_q_tiles = (seq_len - 1) / kBM + 1;
   const long grid = 2L * a.num_q_tiles * batch * kHeadsKV;
   if (grid * 256 > 0xFFFFFFFFL) return (int)hipErrorInvalidValue;

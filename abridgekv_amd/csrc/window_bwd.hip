@@ -2,7 +2,8 @@
 // prefill_bwd.hip: P = exp2(S * scale * log2(e) - lse * log2(e)), dS = P o (dP - rowsum(dO o O)), dQ = scale * dS K,
 // dK = scale * dS^T Q, dV = P^T dO, dK and dV summed over the KV head's four query heads.
 //   window_bwd_dq_kernel    the forward's query tiles and key walk; dQ^T += K^T dS^T. Before it, each (row, query head)'s
-//                           lse2 = lse * log2(e) and D = sum_d dO * O, which it leaves for the next kernel in rows padded to
+//                           lse2 = lse * log2(e) and D = sum_d dO * O (O with the low part that its rounding left off,
+//                           where the caller has it), which it leaves for the next kernel in rows padded to
 //                           whole tiles (lse2 = +inf and D = 0 past the sequence, so that padding weighs 0)
 //   window_bwd_dkv_kernel   a workgroup per 64 keys of a KV head over the query tiles whose windows reach them: the same
 //                           count for every key tile. Keys among the sinks are seen by every later row as well: these far
@@ -62,6 +63,14 @@ __global__ __launch_bounds__(512, 1) void window_bwd_dq_kernel(WindowBwdArgs a) 
     issue_half<kWaves, false>(rows, s0, n, Kb[0], w, lane);
     issue_half<kWaves, true>(rows, s0, n, Vb[0], w, lane);
   }
+  uint2 t[H][4] = {};                                        // what the rounding of O left off, if the caller has it
+  if (f.low != nullptr) {
+    const uint8_t* lp = f.low + (((long)b * f.S + min(qrow, f.S - 1)) * kHeadsQ + kvh * kGroup + hbase) * kHeadDim + 8 * j;
+#pragma unroll
+    for (int u = 0; u < H; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t[u][i] = *reinterpret_cast<const uint2*>(lp + u * kHeadDim + 32 * i);
+  }
   bf16x8 qop[H][4], gop[H][4];
   float l2[H], dd[H];
 #pragma unroll
@@ -80,10 +89,30 @@ __global__ __launch_bounds__(512, 1) void window_bwd_dq_kernel(WindowBwdArgs a) 
 #pragma unroll
       for (int e = 0; e < 4; ++e) d += bf16_lo(y[e]) * bf16_lo(z[e]) + bf16_hi(y[e]) * bf16_hi(z[e]);
     }
-    dd[u] = sum_xor32(sum_xor16(d));
+    dd[u] = d;
     l2[u] = seen ? a.lse[((long)b * kHeadsQ + head) * f.S + r] * 1.4426950408889634f : INFINITY;
+  }
+  if (f.low != nullptr) {
+#pragma unroll
+    for (int u = 0; u < H; ++u) {
+      float d = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const u32x4 y = __builtin_bit_cast(u32x4, gop[u][i]);
+        const floatx4 t0 = load_low(t[u][i].x), t1 = load_low(t[u][i].y);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          d += bf16_lo(y[e]) * t0[2 * e] + bf16_hi(y[e]) * t0[2 * e + 1] + bf16_lo(y[2 + e]) * t1[2 * e] +
+               bf16_hi(y[2 + e]) * t1[2 * e + 1];
+      }
+      dd[u] += seen ? d * (1.f / 256) : 0.f;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < H; ++u) {
+    dd[u] = sum_xor32(sum_xor16(dd[u]));
     if (j == 0) {
-      const long wi = ((long)b * kHeadsQ + head) * a.Sp + qrow;       // qrow < Sp
+      const long wi = ((long)b * kHeadsQ + kvh * kGroup + hbase + u) * a.Sp + qrow;      // qrow < Sp
       a.lse2[wi] = l2[u];
       a.dvec[wi] = dd[u];
     }
@@ -354,7 +383,7 @@ int abkv_window_attn_bwd(const void* q, long q_stride_b, long q_stride_s, long q
                          long k_stride_s, long k_stride_h, const void* v, long v_stride_b, long v_stride_s,
                          long v_stride_h, const void* out, long out_stride_b, long out_stride_s, long out_stride_h,
                          const void* dout, long dout_stride_b, long dout_stride_s, long dout_stride_h, const float* lse,
-                         int batch, int seq_len, const int32_t* seq_lens, int window, int sinks, float scale, void* dq,
+                         const void* out_low, int batch, int seq_len, const int32_t* seq_lens, int window, int sinks, float scale, void* dq,
                          long dq_stride_b, long dq_stride_s, long dq_stride_h, void* dk, long dk_stride_b,
                          long dk_stride_s, long dk_stride_h, void* dv, long dv_stride_b, long dv_stride_s,
                          long dv_stride_h, void* workspace, size_t workspace_bytes, hipStream_t stream) {
@@ -383,6 +412,7 @@ int abkv_window_attn_bwd(const void* q, long q_stride_b, long q_stride_s, long q
   f.scale_log2 = scale * 1.4426950408889634f;
   f.out = nullptr; f.o_sb = f.o_ss = f.o_sh = 0;
   f.lse = nullptr;
+  f.low = static_cast<uint8_t*>(const_cast<void*>(out_low));
   f.num_q_tiles = plan.tiles;
   a.o = static_cast<const __bf16*>(out);
   a.o_sb = out_stride_b; a.o_ss = out_stride_s; a.o_sh = out_stride_h;

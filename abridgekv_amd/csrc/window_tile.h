@@ -15,6 +15,7 @@ struct WindowArgs {
   float scale_log2;
   __bf16* out;      long o_sb, o_ss, o_sh;
   float* lse;                                // natural log, [B, 32, S]; chunks: [T, 32]; or nullptr
+  uint8_t* low;                              // dense [B, S, 32, 128] or nullptr: what out's rounding left off (low_bytes)
   int num_q_tiles;
 };
 
@@ -203,6 +204,43 @@ __device__ __forceinline__ void attend_pair(const Rows& rows, Walk& walk, int n_
   __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");       // no DMA may outlive the workgroup's LDS
 #pragma unroll
   for (int u = 0; u < H; ++u) l_run[u] = lsum[u][0];
+}
+
+// What the bf16 rounding of an output leaves off, 256 times it in e5m2 (a lane's dims 32j .. 32j + 31 of head u). The backward's
+// D = sum_d dO O takes it: with O rounded, D is off by about 2^-9 of a sum of 128 products, and over few keys, where dP and D
+// nearly cancel, that is more than the rounding of dS: relative errors of dQ and dK (their own rounding gives 1.7e-3) of 2 rows
+// 3.9e-3, of 8 2.9e-3, of 777 under a window of 129 2.5e-3; with it 2.4e-3 each. e5m2 keeps all but an eighth of it down to
+// bf16's smallest values (beyond 57344 it saturates). Two of 4096 rows, window 512: 460 -> 477 us a forward and backward.
+template <int H>
+__device__ __forceinline__ void store_low(uint8_t* dst, const floatx4 (&o)[8][H], int u, int j, float inv) {
+  const bool odd = j & 1;
+  auto low = [](float x, uint32_t pair, bool hi) {
+    const float r = hi ? bf16_hi(pair) : bf16_lo(pair);
+    return fminf(fmaxf((x - r) * 256.f, -57344.f), 57344.f);
+  };
+  uint32_t w[8];                                             // [2p], [2p + 1]: dims 32j + 8p .. + 3, .. + 7
+#pragma unroll
+  for (int t = 0; t < 8; ++t) {
+    const floatx4 x = o[t][u] * inv;
+    const uint32_t p0 = pack_bf16x2(x[0], x[1]), p1 = pack_bf16x2(x[2], x[3]);
+    int b = __builtin_amdgcn_cvt_pk_bf8_f32(low(x[0], p0, false), low(x[1], p0, true), 0, false);
+    w[t] = __builtin_amdgcn_cvt_pk_bf8_f32(low(x[2], p1, false), low(x[3], p1, true), b, true);
+  }
+  // 16-byte piece 2j + h of the row is in half h of lane group j; after the swap half h holds pieces of its 64-byte run
+  u32x4 v[2];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const auto r = __builtin_amdgcn_permlane32_swap(odd ? w[e ^ 1] : w[e], odd ? w[(4 + e) ^ 1] : w[4 + e], false, false);
+    v[0][e] = r[0];
+    v[1][e] = r[1];
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) *reinterpret_cast<u32x4*>(dst + 64 * h + 16 * (2 * (j & 1) + (j >> 1))) = v[h];
+}
+// Four of them (a dword), unscaled.
+__device__ __forceinline__ floatx4 load_low(uint32_t w) {
+  const auto a = __builtin_amdgcn_cvt_pk_f32_bf8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_bf8((int)w, true);
+  return floatx4{a[0], a[1], b[0], b[1]};
 }
 
 }  // namespace abkv

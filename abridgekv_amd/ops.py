@@ -1032,9 +1032,15 @@ def _check_lens(seq_lens, B) -> None:
                                   and seq_lens.is_contiguous()), "seq_lens must be contiguous int32 [B]")
 
 
+def _check_low(out_low, B, S) -> None:
+    _require(out_low is None or (out_low.dtype == torch.float8_e5m2 and tuple(out_low.shape) == (B, S, HEADS_Q, HEAD_DIM)
+                                 and out_low.is_contiguous() and out_low.data_ptr() % 16 == 0),
+             "out_low must be contiguous float8_e5m2 [B, S, 32, 128]")
+
+
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, sinks: int = 0,
                      seq_lens: torch.Tensor | None = None, scale: float | None = None, out: torch.Tensor | None = None,
-                     lse: torch.Tensor | None = None):
+                     lse: torch.Tensor | None = None, out_low: torch.Tensor | None = None):
     """Causal attention of whole prompts under a sliding window with sinks: row i sees row j when j <= i and
     (i - j < ``window`` or j < ``sinks``).
 
@@ -1042,8 +1048,9 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     on the GPU: rows past a sequence's length are padding, not read as keys, with out 0 and lse -inf (None: no padding).
     Rows inside a sequence should hold finite values (one that does not can reach other rows of its 64-row tile).
     Returns (out [B, S, 32, 128], lse [B, 32, S] fp32 natural log or None). The weights are rounded to bf16 for their
-    product with v and summed rounded, so lse is good to about 2^-9 / sqrt(visible rows). fp32 q/k/v select the fp32 mode
-    (out fp32, exact to fp32 rounding; no backward).
+    product with v and summed rounded, so lse is good to about 2^-9 / sqrt(visible rows). ``out_low`` [B, S, 32, 128]
+    float8_e5m2 takes 256 times what out's rounding left off, for :func:`window_attention_backward`. fp32 q/k/v select the
+    fp32 mode (out fp32, exact to fp32 rounding; no backward).
     """
     _require(q.dim() == 4, "q must be [B, S, 32, 128]")
     B, S = q.shape[0], q.shape[1]
@@ -1057,22 +1064,28 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
         _check_out(out, dt, (B, S, HEADS_Q, HEAD_DIM))
     _require(lse is None or (lse.dtype == torch.float32 and lse.is_contiguous() and tuple(lse.shape) == (B, HEADS_Q, S)),
              "lse must be contiguous fp32 [B, 32, S]")
-    _check_device(q, k, v, seq_lens, out, lse)
+    _check_low(out_low, B, S)
+    _require(out_low is None or dt == torch.bfloat16, "out_low is for bf16 outputs")
+    _check_device(q, k, v, seq_lens, out, lse, out_low)
     window, sinks = _reach(window, sinks, S)
     if out is None:
         out = torch.empty((B, S, HEADS_Q, HEAD_DIM), dtype=dt, device=q.device)
-    fn = lib().abkv_window_attn_f32 if dt == torch.float32 else lib().abkv_window_attn
-    rc = fn(q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], B, S,
-            _ptr(seq_lens), window, sinks, scale, out.data_ptr(), *out.stride()[:3], _ptr(lse), _stream())
+    args = (q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], B, S,
+            _ptr(seq_lens), window, sinks, scale, out.data_ptr(), *out.stride()[:3], _ptr(lse))
+    if dt == torch.float32:
+        rc = lib().abkv_window_attn_f32(*args, _stream())
+    else:
+        rc = lib().abkv_window_attn(*args, _ptr(out_low), _stream())
     check(rc, "abkv_window_attn")
     return out, lse
 
 
 def window_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, lse: torch.Tensor,
                               dout: torch.Tensor, window: int, sinks: int = 0, seq_lens: torch.Tensor | None = None,
-                              scale: float | None = None):
+                              scale: float | None = None, out_low: torch.Tensor | None = None):
     """Gradients (dq [B, S, 32, 128], dk, dv [B, S, 8, 128], bf16) of sum(dout * out) for :func:`window_attention` under
-    the same window, from its out and lse. Padding rows get 0, whatever dout holds there (bf16 only)."""
+    the same window, from its out, lse and (without it dq and dk are less exact over few keys) out_low. Padding rows get 0,
+    whatever dout holds there (bf16 only)."""
     _require(q.dim() == 4, "q must be [B, S, 32, 128]")
     B, S = q.shape[0], q.shape[1]
     window, sinks = _check_window(window, sinks)
@@ -1083,11 +1096,12 @@ def window_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     _check_lens(seq_lens, B)
     _require(lse.dtype == torch.float32 and lse.is_contiguous() and tuple(lse.shape) == (B, HEADS_Q, S),
              "lse must be contiguous fp32 [B, 32, S]")
-    _check_device(q, k, v, out, lse, dout, seq_lens)
-    return window_backward(q, k, v, out, lse, dout, window, sinks, seq_lens, scale)
+    _check_low(out_low, B, S)
+    _check_device(q, k, v, out, lse, dout, seq_lens, out_low)
+    return window_backward(q, k, v, out, lse, dout, window, sinks, seq_lens, scale, out_low)
 
 
-def window_backward(q, k, v, out, lse, dout, window, sinks, seq_lens, scale):
+def window_backward(q, k, v, out, lse, dout, window, sinks, seq_lens, scale, out_low=None):
     """:func:`window_attention_backward` of arguments that are checked already (autograd's saved tensors)."""
     B, S = q.shape[:2]
     window, sinks = _reach(window, sinks, S)
@@ -1099,7 +1113,7 @@ def window_backward(q, k, v, out, lse, dout, window, sinks, seq_lens, scale):
     args = []
     for t in (q, k, v, out, dout):
         args += (t.data_ptr(), *t.stride()[:3])
-    args += (lse.data_ptr(), B, S, _ptr(seq_lens), window, sinks, scale)
+    args += (lse.data_ptr(), _ptr(out_low), B, S, _ptr(seq_lens), window, sinks, scale)
     for t in (dq, dk, dv):
         args += (t.data_ptr(), *t.stride()[:3])
     rc = lib().abkv_window_attn_bwd(*args, ws.data_ptr(), ws_bytes, _stream())

@@ -438,25 +438,27 @@ int64_t abkv_planner_apply_events(void* planner, const int64_t* events, int64_t 
  * Whole prompts: q, out [batch, seq_len, 32, 128], k, v [batch, seq_len, 8, 128] bf16, any element strides that keep rows
  * 16-byte aligned. seq_lens (device, [batch], or NULL: seq_len everywhere; clamped to [0, seq_len]): rows past it are
  * padding, never read as keys, with out 0 and lse -inf. lse [batch, 32, seq_len] fp32 natural log, or NULL. Values of rows
- * inside a sequence should be finite: a row that is not can reach rows of its 64-row tile that do not see it. */
+ * inside a sequence should be finite: a row that is not can reach rows of its 64-row tile that do not see it. out_low
+ * [batch, seq_len, 32, 128] dense, 16-byte aligned, or NULL: 256 times what out's rounding left off, e5m2, for the gradients. */
 int abkv_window_attn(const void* q, long q_stride_b, long q_stride_s, long q_stride_h, const void* k, long k_stride_b,
                      long k_stride_s, long k_stride_h, const void* v, long v_stride_b, long v_stride_s, long v_stride_h,
                      int batch, int seq_len, const int32_t* seq_lens, int window, int sinks, float scale, void* out,
-                     long out_stride_b, long out_stride_s, long out_stride_h, float* lse, abkv_stream_t stream);
+                     long out_stride_b, long out_stride_s, long out_stride_h, float* lse, void* out_low,
+                     abkv_stream_t stream);
 /* The same in fp32 (inputs, outputs, sums); rows that are not finite reach only the rows that see them. */
 int abkv_window_attn_f32(const float* q, long q_stride_b, long q_stride_s, long q_stride_h, const float* k,
                          long k_stride_b, long k_stride_s, long k_stride_h, const float* v, long v_stride_b,
                          long v_stride_s, long v_stride_h, int batch, int seq_len, const int32_t* seq_lens, int window,
                          int sinks, float scale, float* out, long out_stride_b, long out_stride_s, long out_stride_h,
                          float* lse, abkv_stream_t stream);
-/* Gradients of abkv_window_attn (bf16) from its out and lse: dq [batch, seq_len, 32, 128], dk, dv [batch, seq_len, 8, 128],
+/* Gradients of abkv_window_attn (bf16) from its out, lse and out_low (NULL: without it, and less exact): dq [batch, seq_len, 32, 128], dk, dv [batch, seq_len, 8, 128],
  * padding rows 0. workspace: abkv_window_bwd_workspace_size bytes, not shared by calls that may overlap. */
 size_t abkv_window_bwd_workspace_size(int batch, int seq_len, int window, int sinks);
 int abkv_window_attn_bwd(const void* q, long q_stride_b, long q_stride_s, long q_stride_h, const void* k, long k_stride_b,
                          long k_stride_s, long k_stride_h, const void* v, long v_stride_b, long v_stride_s,
                          long v_stride_h, const void* out, long out_stride_b, long out_stride_s, long out_stride_h,
                          const void* dout, long dout_stride_b, long dout_stride_s, long dout_stride_h, const float* lse,
-                         int batch, int seq_len, const int32_t* seq_lens, int window, int sinks, float scale, void* dq,
+                         const void* out_low, int batch, int seq_len, const int32_t* seq_lens, int window, int sinks, float scale, void* dq,
                          long dq_stride_b, long dq_stride_s, long dq_stride_h, void* dk, long dk_stride_b,
                          long dk_stride_s, long dk_stride_h, void* dv, long dv_stride_b, long dv_stride_s,
                          long dv_stride_h, void* workspace, size_t workspace_bytes, abkv_stream_t stream);

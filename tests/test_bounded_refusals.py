@@ -47,6 +47,12 @@ def test_window_attention():
     _bad("dout", ops.window_attention_backward, q, k, v, q, torch.zeros(2, 32, 9), q[:, :, :8], 4)
     _bad("out must be", ops.window_attention_backward, q, k, v, q.float(), torch.zeros(2, 32, 9), q, 4)
     _bad(on_gpu, ops.window_attention_backward, q, k, v, q, torch.zeros(2, 32, 9), q, 4)
+    low = torch.zeros((2, 9, 32, 128), dtype=torch.float8_e5m2)
+    _bad(on_gpu, ops.window_attention, q, k, v, 4, out_low=low)
+    for bad in (low[:1], low.view(torch.uint8), low.transpose(1, 2)):
+        _bad("out_low", ops.window_attention, q, k, v, 4, out_low=bad)
+        _bad("out_low", ops.window_attention_backward, q, k, v, q, torch.zeros(2, 32, 9), q, 4, out_low=bad)
+    _bad("out_low", ops.window_attention, q.float(), k.float(), v.float(), 4, out_low=low)
 
 
 @pytest.mark.parametrize("scale", [0.0, -0.1, float("inf"), float("nan")])
@@ -189,21 +195,23 @@ def test_c_entry_points_return_errors():
     bad = 1                                                  # hipErrorInvalidValue
 
     def win(window=4, sinks=0, q=one):
-        return L.abkv_window_attn(q, 1, 1, 1, one, 1, 1, 1, one, 1, 1, 1, 1, 8, None, window, sinks, 1.0, one, 1, 1, 1, None, 0)
+        return L.abkv_window_attn(q, 1, 1, 1, one, 1, 1, 1, one, 1, 1, 1, 1, 8, None, window, sinks, 1.0, one, 1, 1, 1, None, None, 0)
 
     def scaled(scale, stride=1):
-        return (L.abkv_window_attn(one, 1, stride, 1, one, 1, 1, 1, one, 1, 1, 1, 1, 8, None, 4, 0, scale, one, 1, 1, 1, None, 0),
+        return (L.abkv_window_attn(one, 1, stride, 1, one, 1, 1, 1, one, 1, 1, 1, 1, 8, None, 4, 0, scale, one, 1, 1, 1, None, None,
+                                   0),
                 L.abkv_window_attn_f32(one, 1, stride, 1, one, 1, 1, 1, one, 1, 1, 1, 1, 8, None, 4, 0, scale, one, 1, 1, 1, None,
                                        0),
-                L.abkv_window_attn_bwd(one, 1, stride, 1, *[one, 1, 1, 1] * 4, one, 1, 8, None, 4, 0, scale, *[one, 1, 1, 1] * 3,
+                L.abkv_window_attn_bwd(one, 1, stride, 1, *[one, 1, 1, 1] * 4, one, None, 1, 8, None, 4, 0, scale,
+                                       *[one, 1, 1, 1] * 3,
                                        one, 1 << 30, 0),
                 L.abkv_paged_prefill_attn_window(one, stride, 1, one, 4, one, 4, 4, one, one, 1, 4, 0, scale, one, 1, 1, None, 0),
                 L.abkv_paged_prefill_scores(one, stride, 1, one, 4, one, 4, 4, one, one, 1, 64, one, one, 64, 64, scale, 0))
 
     assert set(scaled(0.0) + scaled(-1.0) + scaled(float("nan")) + scaled(float("inf")) + scaled(1.0, 1 << 24)) == {bad}
     assert win(0) == win(4, -1) == win(q=0) == bad
-    assert L.abkv_window_attn(one, 1, 1, 1, one, 1, 1, 1, one, 1, 1, 1, 0, 8, None, 4, 0, 1.0, one, 1, 1, 1, None, 0) == 0
-    args = [one, 1, 1, 1] * 5 + [one, 1, 8, None, 4, 0, 1.0] + [one, 1, 1, 1] * 3
+    assert L.abkv_window_attn(one, 1, 1, 1, one, 1, 1, 1, one, 1, 1, 1, 0, 8, None, 4, 0, 1.0, one, 1, 1, 1, None, None, 0) == 0
+    args = [one, 1, 1, 1] * 5 + [one, None, 1, 8, None, 4, 0, 1.0] + [one, 1, 1, 1] * 3
     assert L.abkv_window_attn_bwd(*args, one, 16, 0) == bad                              # workspace too small
     assert L.abkv_window_attn_bwd(*args, 0, 1 << 30, 0) == bad
 

@@ -254,3 +254,55 @@ def test_chunks_in_a_captured_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, ops.paged_prefill_attention_window(q, cache, table, *args)[0]), len(junk)
+
+
+@pytest.mark.parametrize("B,S,lens,window,sinks", SHAPES)
+def test_low_part_of_the_outputs(B, S, lens, window, sinks):
+    """out + out_low / 256 is off by what the weights' rounding takes (the forward's bound) and by an eighth (half a step of
+    e5m2) of out's own rounding; padding 0; out and lse stay; the gradients keep their bounds."""
+    from abridgekv_amd import ops
+    (q, k, v, g), ref = _make(S + window % 97, B, S, lens)
+    lse, lse0 = (torch.empty((B, 32, S), device="cuda") for _ in range(2))
+    low = torch.full((B, S, 32, 128), 7.0, device="cuda").to(torch.float8_e5m2)
+    out, _ = ops.window_attention(q, k, v, window, sinks, seq_lens=_lens(lens), lse=lse, out_low=low)
+    plain, _ = ops.window_attention(q, k, v, window, sinks, seq_lens=_lens(lens), lse=lse0)
+    assert torch.equal(out, plain) and torch.equal(lse, lse0)
+    want, _, tol = ow.window_attention(*ref[:3], lens, window, sinks, SCALE, bounds=True)
+    left = low.float().double().cpu().numpy() / 256
+    err = np.abs(out.double().cpu().numpy() + left - want)
+    # (an output whose own rounding is below e5m2's smallest step, 2^-16 / 256, is off by half of that)
+    assert (err <= tol - (1 - 1 / 8 - 0.03) * ow.EPS * np.abs(want) + 2.0 ** -25).all(), err.max()
+    for b, n in enumerate(lens or []):
+        assert not left[b, n:].any()
+    got = ops.window_attention_backward(q, k, v, out, lse, g, window, sinks, seq_lens=_lens(lens), out_low=low)
+    grads = ow.window_backward(*ref, lens, window, sinks, SCALE, bounds=True)
+    for name, x, d, tol in zip(("dq", "dk", "dv"), got, grads[::2], grads[1::2]):
+        assert (np.abs(x.double().cpu().numpy() - d) <= tol).all(), name
+
+
+def test_backward_takes_its_row_sums_from_both_parts():
+    """A window of one row: P = 1, so dS = dO . V - dO . (out + out_low / 256) for any out and out_low that are given. dS and dQ
+    are rounded (two half steps), the products summed in fp32 (128 terms of each dot product)."""
+    from abridgekv_amd import ops
+    S, n = 150, 100
+    (q, k, v, g), ref = _make(11, 1, S, [n])
+    sl = _lens([n])
+    lse = torch.empty((1, 32, S), device="cuda")
+    ops.window_attention(q, k, v, 1, 0, seq_lens=sl, lse=lse)
+    gen = torch.Generator().manual_seed(1)
+    out = torch.randn((1, S, 32, 128), generator=gen).to(torch.bfloat16)
+    low = (300 * torch.randn((1, S, 32, 128), generator=gen)).to(torch.float8_e5m2)
+    out[:, n:], low[:, n:] = float("nan"), float("nan")
+    dq, dk, _ = ops.window_attention_backward(q, k, v, out.cuda(), lse, g, 1, 0, seq_lens=sl, out_low=low.cuda())
+    rq, rk, rv, rg = (x[0, :n] for x in ref)
+    rk, rv = np.repeat(rk, 4, 1), np.repeat(rv, 4, 1)
+    total = out.double().numpy()[0, :n] + low.float().double().numpy()[0, :n] / 256
+    ds = (rg * (rv - total)).sum(-1, keepdims=True)
+    fp32 = 256 * 2.0 ** -24 * (np.abs(rg) * (np.abs(rv) + np.abs(total))).sum(-1, keepdims=True) + ow.FP32 * np.abs(ds)
+    err = 2 * ow.SLACK * ow.EPS * np.abs(ds) + fp32
+    got = dq.double().cpu().numpy()[0]
+    assert (np.abs(got[:n] - SCALE * ds * rk) <= SCALE * err * np.abs(rk)).all() and not got[n:].any()
+    want, tol = (SCALE * x.reshape(n, 8, 4, 128).sum(2) for x in (ds * rq, err * np.abs(rq)))
+    got = dk.double().cpu().numpy()[0]
+    # (dK is rounded as the sum of four heads)
+    assert (np.abs(got[:n] - want) <= tol + ow.EPS * np.abs(want)).all() and not got[n:].any()
