@@ -115,7 +115,8 @@ __global__ __launch_bounds__(256, 2) void window_attn_kernel(WindowArgs a, Chunk
         if (few) l_run[u] += l0[u] * fast_exp2(m0[u] - m_run[u]);
     };
     if constexpr (kPaged)
-      attend(PagedRows{c.kv + kvh * kHeadDim, c.block_table + (long)b * c.bt_stride, c.bt_width, c.num_pages});
+      attend(PagedWindowRows{{c.kv + kvh * kHeadDim, c.block_table + (long)b * c.bt_stride, c.bt_width, c.num_pages},
+                             max(kv0 + q0 + 1 - a.window, 0), a.sinks});
     else
       attend(DenseRows<false>{a.k + (long)b * a.k_sb + (long)kvh * a.k_sh, a.v + (long)b * a.v_sb + (long)kvh * a.v_sh,
                               a.k_ss, a.v_ss});

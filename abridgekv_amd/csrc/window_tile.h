@@ -51,6 +51,20 @@ __device__ __forceinline__ void tile_mask(floatx4 (&s)[2][2][H], int k0, const T
       }
 }
 
+// Rows of a paged sequence that a query tile sees: keys below `sinks` and from `lo`, the first key of the tile's first row, on.
+// The others of the tiles that it walks (before the windows, behind the sinks) may hold anything, or lie on pages that are no
+// longer the sequence's: as the rows past its end they are not read, for a weight of 0 does not cancel a NaN.
+struct PagedWindowRows : PagedRows {
+  int lo, sinks;
+  template <bool kV>
+  __device__ __forceinline__ const __bf16* addr(const Src& t, int row, int chunk, int n_keys) const {
+    const int key = t.k0 + row;
+    const bool in = key < n_keys && (key >= lo || key < sinks);
+    const __bf16* base = in ? t.blk + (row & 15) * kSlotElems : t.last;
+    return base + ((kV ? kHalfElems : 0) + 8 * chunk);
+  }
+};
+
 // Up to 32 sinks before a query tile's windows take half a tile of their own, outside the walk (a whole one costs a tenth
 // of a query tile under a window of 512; 4 sinks: windows of 128 / 512 / 1024 81 / 121 / 269 -> 74 / 114 / 262 us): 32 K
 // rows and 32 V rows in one LDS tile. Sinks that the windows reach, or more of them, stay with the walk.
@@ -59,7 +73,7 @@ __device__ __forceinline__ bool short_sinks(int q0, int window, int sinks) {
   return sinks > 0 && sinks <= kShortSinks && q0 + 1 - window >= kBN;
 }
 
-// DMA of the sinks' rows (keys 0 .. 31, fewer than n_keys >= 64): K in rows 0 .. 31 of buf, V in rows 32 .. 63, by 4 waves.
+// DMA of the sinks' rows (keys 0 .. 31, fewer than n_keys >= 64; rows decides what stands for those past the sinks): K in rows 0 .. 31 of buf, V in rows 32 .. 63, by 4 waves.
 template <class Rows>
 __device__ __forceinline__ void issue_sinks(const Rows& rows, int n_keys, __bf16* buf, int w, int lane) {
   const auto src = rows.template src<4>(0, w & 1, n_keys);   // waves 2 and 3: the V rows of the same keys

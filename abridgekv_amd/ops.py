@@ -1153,7 +1153,8 @@ def paged_prefill_attention_window(q: torch.Tensor, kv_cache: torch.Tensor, bloc
     """Prompt chunks over the paged cache under a sliding window with sinks: request r's queries are tokens
     q_start[r]..q_start[r+1]-1 of q [T, 32, 128] bf16 at physical positions kv_start[r] + i (host sequences, as
     :func:`paged_prefill_attention`), and a query at position p sees rows j <= p with p - j < ``window`` or j < ``sinks``.
-    The chunk's own rows must be in the cache. The starts go with the launch (a captured one keeps them). Returns (out
+    The chunk's own rows must be in the cache. Rows that none of the request's queries sees may hold anything, and pages that hold
+    no other rows any table entry. The starts go with the launch (a captured one keeps them). Returns (out
     [T, 32, 128] bf16, lse [T, 32] fp32 or None); rows past q_start[-1] are left alone."""
     window, sinks = _check_window(window, sinks)
     scale = _softmax_scale(scale)

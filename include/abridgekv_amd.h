@@ -465,7 +465,8 @@ int abkv_window_attn_bwd(const void* q, long q_stride_b, long q_stride_s, long q
 /* Prompt chunks over the paged cache: request r's queries are rows q_start[r] .. q_start[r + 1] - 1 of q [T, 32, 128] bf16,
  * at physical positions kv_start[r] + i, causal. q_start [num_requests + 1] and kv_start [num_requests] are on the HOST and
  * go with the launch (one for every 64 requests); every key position must lie inside the table row (page ids are clamped
- * into the cache). out [T, 32, 128], lse [T, 32] or NULL; rows of no request are left alone. */
+ * into the cache). Rows that no query of the request sees are not read, nor are their pages' table entries used. out [T, 32, 128],
+ * lse [T, 32] or NULL; rows of no request are left alone. */
 int abkv_paged_prefill_attn_window(const void* q, long q_stride_tok, long q_stride_head, const void* kv_cache,
                                    int num_pages, const int32_t* block_table, long block_table_stride, int table_width,
                                    const int32_t* q_start, const int32_t* kv_start, int num_requests, int window, int sinks,
