@@ -302,9 +302,11 @@ __device__ __forceinline__ float lane_max(const floatx4 (&s)[2][2][H], int u) {
   return fmaxf(mx, s[1][1][u][3]);
 }
 
-template <int H>
+// `exact` (kExact): this lane's part of the column's weight sum before the weights are rounded.
+template <int H, bool kExact = false>
 __device__ __forceinline__ void tile_softmax(floatx4 (&s)[2][2][H], floatx4 (&o)[8][H], float (&m_run)[H],
-                                             floatx4 (&lsum)[H], float scale_log2, bf16x8 (&pop)[2][H]) {
+                                             floatx4 (&lsum)[H], float scale_log2, bf16x8 (&pop)[2][H],
+                                             float* exact = nullptr) {
   float neg_m[H];
   bool need = false;
 #pragma unroll
@@ -332,6 +334,7 @@ __device__ __forceinline__ void tile_softmax(floatx4 (&s)[2][2][H], floatx4 (&o)
       const float d = m_new == -INFINITY ? 0.f : m_new + neg_m[u];    // new max minus the offset t was taken at
       m_run[u] = m_new;
       lsum[u] *= alpha;
+      if constexpr (kExact) exact[u] *= alpha;
 #pragma unroll
       for (int i = 0; i < 8; ++i) o[i][u] *= alpha;
 #pragma unroll
@@ -347,8 +350,11 @@ __device__ __forceinline__ void tile_softmax(floatx4 (&s)[2][2][H], floatx4 (&o)
       u32x4 pw;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        pw[2 * t] = pack_bf16x2(fast_exp2(s[kk][t][u][0]), fast_exp2(s[kk][t][u][1]));
-        pw[2 * t + 1] = pack_bf16x2(fast_exp2(s[kk][t][u][2]), fast_exp2(s[kk][t][u][3]));
+        const float p0 = fast_exp2(s[kk][t][u][0]), p1 = fast_exp2(s[kk][t][u][1]);
+        const float p2 = fast_exp2(s[kk][t][u][2]), p3 = fast_exp2(s[kk][t][u][3]);
+        if constexpr (kExact) exact[u] += (p0 + p1) + (p2 + p3);
+        pw[2 * t] = pack_bf16x2(p0, p1);
+        pw[2 * t + 1] = pack_bf16x2(p2, p3);
       }
       pop[kk][u] = __builtin_bit_cast(bf16x8, pw);
     }

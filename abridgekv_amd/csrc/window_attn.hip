@@ -33,7 +33,11 @@ struct DenseArgs {
   static constexpr bool kPaged = false;
 };
 
-template <class Chunks>
+// kLse: the call wants lse. The output is divided by the sum of its rounded weights, but lse takes the unrounded ones, up to 2^8
+// under the running maximum's headroom: rounded, a few heavy keys would leave it up to 2^-8 off however many rows are visible (600 rows, one key 6 log2 units
+// above the others: 2.3e-3, this 2e-6). The additions cost 4 % (two sequences of 8192 and 5000 rows, window 1024: 244 -> 253 us),
+// so calls without lse leave them out.
+template <class Chunks, bool kLse>
 __global__ __launch_bounds__(256, 2) void window_attn_kernel(WindowArgs a, Chunks c) {
   constexpr bool kPaged = Chunks::kPaged;
   constexpr int H = 2, kWaves = 4;
@@ -87,11 +91,11 @@ __global__ __launch_bounds__(256, 2) void window_attn_kernel(WindowArgs a, Chunk
   for (int i = 0; i < 8; ++i)
 #pragma unroll
     for (int u = 0; u < H; ++u) o[i][u] = floatx4{0.f, 0.f, 0.f, 0.f};
-  float m_run[H], l_run[H];
+  float m_run[H], l_run[H], exact[H];
 #pragma unroll
   for (int u = 0; u < H; ++u) {
     m_run[u] = -INFINITY;
-    l_run[u] = 0.f;
+    l_run[u] = exact[u] = 0.f;
   }
   if (q0 < n_q) {                                            // (uniform)
     const bool few = short_sinks(kv0 + q0, a.window, a.sinks);
@@ -105,11 +109,11 @@ __global__ __launch_bounds__(256, 2) void window_attn_kernel(WindowArgs a, Chunk
       if (few) {
         __asm__ volatile("s_waitcnt vmcnt(12)" ::: "memory");    // (all but the first tiles')
         __builtin_amdgcn_s_barrier();
-        attend_sinks<H>(Ks, a.sinks, qop, o, m_run, l0, a.scale_log2, lane);
+        attend_sinks<H, kLse>(Ks, a.sinks, qop, o, m_run, l0, exact, a.scale_log2, lane);
 #pragma unroll
         for (int u = 0; u < H; ++u) m0[u] = m_run[u];
       }
-      attend_pair<H, kWaves>(rows, walk, n, Kbuf, Vbuf, qop, o, m_run, l_run, lm, a.scale_log2, w, lane);
+      attend_pair<H, kWaves, kLse>(rows, walk, n, Kbuf, Vbuf, qop, o, m_run, l_run, exact, lm, a.scale_log2, w, lane);
 #pragma unroll
       for (int u = 0; u < H; ++u)
         if (few) l_run[u] += l0[u] * fast_exp2(m0[u] - m_run[u]);
@@ -120,6 +124,10 @@ __global__ __launch_bounds__(256, 2) void window_attn_kernel(WindowArgs a, Chunk
     else
       attend(DenseRows<false>{a.k + (long)b * a.k_sb + (long)kvh * a.k_sh, a.v + (long)b * a.v_sb + (long)kvh * a.v_sh,
                               a.k_ss, a.v_ss});
+  }
+  if constexpr (kLse) {
+#pragma unroll
+    for (int u = 0; u < H; ++u) exact[u] = sum_xor32(sum_xor16(exact[u]));      // (before lanes leave)
   }
   if (qi >= (kPaged ? n_q : a.S)) return;
   const long o_row = kPaged ? (long)(t0 + qi) * a.o_ss : (long)b * a.o_sb + (long)qi * a.o_ss;
@@ -135,9 +143,9 @@ __global__ __launch_bounds__(256, 2) void window_attn_kernel(WindowArgs a, Chunk
     store_acc_rows<H>(a.out + o_row + (long)head * a.o_sh, o, u, j, inv);
     if constexpr (!kPaged)
       if (a.low != nullptr) store_low<H>(a.low + (((long)b * a.S + qi) * kHeadsQ + head) * kHeadDim, o, u, j, inv);
-    if (a.lse != nullptr && j == 0)
+    if (kLse && j == 0)
       a.lse[kPaged ? (long)(t0 + qi) * kHeadsQ + head : ((long)b * kHeadsQ + head) * a.S + qi] =
-          l == 0.f ? -INFINITY : (m_run[u] + __log2f(l)) * 0.69314718055994531f;
+          l == 0.f ? -INFINITY : (m_run[u] + __log2f(exact[u])) * 0.69314718055994531f;
   }
 }
 
@@ -175,7 +183,8 @@ int abkv_window_attn(const void* q, long q_stride_b, long q_stride_s, long q_str
   a.num_q_tiles = (seq_len - 1) / kBM + 1;
   const long grid = 2L * a.num_q_tiles * batch * kHeadsKV;
   if (grid * 256 > 0xFFFFFFFFL) return (int)hipErrorInvalidValue;
-  hipLaunchKernelGGL(window_attn_kernel<DenseArgs>, dim3((unsigned)grid), dim3(256), 0, stream, a, DenseArgs{});
+  const auto kernel = lse != nullptr ? window_attn_kernel<DenseArgs, true> : window_attn_kernel<DenseArgs, false>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, stream, a, DenseArgs{});
   return (int)hipGetLastError();
 }
 
@@ -223,7 +232,8 @@ int abkv_paged_prefill_attn_window(const void* q, long q_stride_tok, long q_stri
     const long grid = 2 * tiles * kHeadsKV;
     if (grid * 256 > 0xFFFFFFFFL) return (int)hipErrorInvalidValue;
     if (grid == 0) continue;
-    hipLaunchKernelGGL(window_attn_kernel<ChunkArgs>, dim3((unsigned)grid), dim3(256), 0, stream, a, c);
+    const auto kernel = lse != nullptr ? window_attn_kernel<ChunkArgs, true> : window_attn_kernel<ChunkArgs, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, stream, a, c);
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return (int)err;
   }

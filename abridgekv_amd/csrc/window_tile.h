@@ -116,10 +116,11 @@ __device__ __forceinline__ bf16x8 pack_half(const floatx4 (&x)[2][H], int u) {
   return __builtin_bit_cast(bf16x8, w);
 }
 
-// The sinks' share of a wave's columns as the start of its online softmax: o, m_run and the columns' weight sums l.
-template <int H>
+// The sinks' share of a wave's columns as the start of its online softmax: o, m_run and the columns' weight sums l (exact: this
+// lane's part of those before the weights are rounded).
+template <int H, bool kExact>
 __device__ __forceinline__ void attend_sinks(const __bf16* buf, int sinks, const bf16x8 (&qop)[H][4], floatx4 (&o)[8][H],
-                                             float (&m_run)[H], float (&l)[H], float scale_log2, int lane) {
+                                             float (&m_run)[H], float (&l)[H], float (&exact)[H], float scale_log2, int lane) {
   typedef short s8 __attribute__((ext_vector_type(8)));
   const bf16x8 ones = __builtin_bit_cast(bf16x8, s8{0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80, 0x3f80});
   const int m16 = lane & 15, j = lane >> 4;
@@ -141,7 +142,10 @@ __device__ __forceinline__ void attend_sinks(const __bf16* buf, int sinks, const
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) s[t][u][r] = fast_exp2(s[t][u][r] - m);
+      for (int r = 0; r < 4; ++r) {
+        s[t][u][r] = fast_exp2(s[t][u][r] - m);
+        if constexpr (kExact) exact[u] += s[t][u][r];
+      }
     pop[u] = pack_half<H>(s, u);
   }
 #pragma unroll
@@ -171,11 +175,12 @@ __device__ __forceinline__ void start_pair(const Rows& rows, Walk walk, int n_ke
 // attend_tiles with two buffers each of K and V, tile m in K[m % 2] and V[m % 2], started by start_pair. Iteration n: wait for
 // the DMAs of iteration n - 1 (K(n+1), V(n)), barrier, DMA K(n+2) and V(n+1) into the buffers that were read last, softmax of
 // tile n beside the scores of tile n + 1, O += V(n) . P(n). The wait is the other workgroup's time: two share a CU.
-template <int H, int kWaves, class Rows, class Walk, class Lane>
+// exact (kExact): this lane's part of the unrounded weight sums, rescaled from what it holds at the start.
+template <int H, int kWaves, bool kExact, class Rows, class Walk, class Lane>
 __device__ __forceinline__ void attend_pair(const Rows& rows, Walk& walk, int n_keys, __bf16* const (&K)[2],
                                             __bf16* const (&V)[2], const bf16x8 (&qop)[H][4], floatx4 (&o)[8][H],
-                                            float (&m_run)[H], float (&l_run)[H], const Lane& lane_mask, float scale_log2,
-                                            int w, int lane) {
+                                            float (&m_run)[H], float (&l_run)[H], float (&exact)[H], const Lane& lane_mask,
+                                            float scale_log2, int w, int lane) {
   constexpr int kPerWave = 16 / kWaves;
   const int m16 = lane & 15, j = lane >> 4;
   int t0 = 0, t1 = 0;                              // first keys of tiles n, n+1
@@ -203,7 +208,7 @@ __device__ __forceinline__ void attend_pair(const Rows& rows, Walk& walk, int n_
     issue_half<kWaves, true>(rows, src_v, n_keys, V[1 - slot], w, lane);
     tile_mask<H, Walk>(s_cur, t0, m0, lane_mask, j);
     bf16x8 pop[2][H];
-    tile_softmax<H>(s_cur, o, m_run, lsum, scale_log2, pop);
+    tile_softmax<H, kExact>(s_cur, o, m_run, lsum, scale_log2, pop, exact);
     tile_scores<H>(K[1 - slot], qop, s_nxt, m16, j);         // (discarded after the last tile)
     tile_pv<H>(V[slot], pop, o, lsum, lane);
     if (!h1) return false;

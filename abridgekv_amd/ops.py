@@ -1048,7 +1048,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     on the GPU: rows past a sequence's length are padding, not read as keys, with out 0 and lse -inf (None: no padding).
     Rows inside a sequence should hold finite values (one that does not can reach other rows of its 64-row tile).
     Returns (out [B, S, 32, 128], lse [B, 32, S] fp32 natural log or None). The weights are rounded to bf16 for their
-    product with v and summed rounded, so lse is good to about 2^-9 / sqrt(visible rows). ``out_low`` [B, S, 32, 128]
+    product with v, and out is divided by the sum of the rounded ones; lse is that of the weights before (fp32 sums).
+    ``out_low`` [B, S, 32, 128]
     float8_e5m2 takes 256 times what out's rounding left off, for :func:`window_attention_backward`. fp32 q/k/v select the
     fp32 mode (out fp32, exact to fp32 rounding; no backward).
     """
