@@ -114,6 +114,18 @@ class WindowMask:
     seq_lens: torch.Tensor | None = None
 
 
+class _FirstDerivatives(torch.autograd.Function):
+    """The window kernels' gradients, tied to what they were made from: a second derivative through any of it is refused."""
+
+    @staticmethod
+    def forward(ctx, dq, dk, dv, *sources):
+        return dq.view_as(dq), dk.view_as(dk), dv.view_as(dv)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("sliding-window attention has no second derivative")
+
+
 class _WindowAttention(torch.autograd.Function):
     """The sliding-window kernels and their backward (abkv_window_attn / _bwd): query, key and value [B, heads, S, 128] as
     the layers hand them, out [B, S, 32, 128]."""
@@ -130,20 +142,21 @@ class _WindowAttention(torch.autograd.Function):
         out, _ = ops.window_attention(q, k, v, mask.window, mask.sinks, seq_lens=mask.seq_lens, scale=scale, lse=lse,
                                       out_low=low)
         if lse is not None:
-            ctx.save_for_backward(q, k, v, out, lse, low, mask.seq_lens)
+            ctx.save_for_backward(query, key, value, out, lse, low, mask.seq_lens)
             ctx.mask, ctx.scale = mask, scale
         return out
 
     @staticmethod
     def backward(ctx, grad_out):
-        if torch.is_grad_enabled():
-            raise RuntimeError("sliding-window attention has no second derivative")
-        q, k, v, out, lse, low, seq_lens = ctx.saved_tensors
-        st = grad_out.stride()
-        if st[3] != 1 or (st[0] | st[1] | st[2]) % 8 or st[1] >= 1 << 24 or grad_out.data_ptr() % 16:
-            grad_out = grad_out.contiguous()
-        dq, dk, dv = ops.window_backward(q, k, v, out, lse, grad_out, ctx.mask.window, ctx.mask.sinks, seq_lens, ctx.scale,
-                                         low)
+        query, key, value, out, lse, low, seq_lens = ctx.saved_tensors
+        g, st = grad_out, grad_out.stride()
+        if st[3] != 1 or (st[0] | st[1] | st[2]) % 8 or st[1] >= 1 << 24 or g.data_ptr() % 16:
+            g = g.contiguous()
+        q, k, v = query.transpose(1, 2), key.transpose(1, 2), value.transpose(1, 2)
+        grads = ops.window_backward(q, k, v, out, lse, g, ctx.mask.window, ctx.mask.sinks, seq_lens, ctx.scale, low)
+        if torch.is_grad_enabled():                          # (create_graph)
+            grads = _FirstDerivatives.apply(*grads, query, key, value, grad_out)
+        dq, dk, dv = grads
         return dq.transpose(1, 2), dk.transpose(1, 2), dv.transpose(1, 2), None, None
 
 
