@@ -3,6 +3,7 @@
 #include <algorithm>
 
 #include "attn_tile.h"
+#include "score_rows.h"
 
 namespace abkv {
 
@@ -41,7 +42,6 @@ __device__ __forceinline__ float sum16(float v) {
   return add(v, __builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), 0x140, 0xF, 0xF, false));   // row_mirror
 }
 
-constexpr int kScoreQ = 32;                                  // query rows of an iteration
 constexpr int kScoreWaves = 16;
 template <int kTiles>
 __global__ __launch_bounds__(64 * kScoreWaves) void prompt_scores_kernel(PromptScoreArgs a) {
@@ -70,7 +70,7 @@ __global__ __launch_bounds__(64 * kScoreWaves) void prompt_scores_kernel(PromptS
   const int half = w & 1, lrow = 16 * half + (lane >> 2);
   auto offset = [&](int i, int limit) {                      // bytes to the lane's piece of DMA i, rows up to `limit`
     const int row = 8 * w + 4 * i + j;                       // LDS row: head row / 32, query row % 32
-    return (unsigned)((min(row & (kScoreQ - 1), limit) * (int)a.q_st + row / kScoreQ * (int)a.q_sh + 8 * (m16 ^ (row & 15))) * 2);
+    return score_piece(row, limit, (uint32_t)a.q_st, (uint32_t)a.q_sh, m16 ^ (row & 15));
   };
   unsigned off[2] = {offset(0, kScoreQ - 1), offset(1, kScoreQ - 1)}, off_l = (lrow * kHeadsQ + (lane & 3)) * 4;
   const char* const q_base = reinterpret_cast<const char*>(a.q + (long)t0 * a.q_st + (long)kvh * kGroup * a.q_sh);
@@ -374,7 +374,7 @@ int abkv_paged_prefill_scores(const void* q, long q_stride_tok, long q_stride_he
   if (num_requests <= 0) return 0;
   if (q == nullptr || kv_cache == nullptr || block_table == nullptr || q_start == nullptr || kv_start == nullptr ||
       lse == nullptr || scores == nullptr || num_pages <= 0 || table_width <= 0 ||
-      (tile_keys != kBN && tile_keys != 2 * kBN) || !row_strides_ok(q_stride_tok) || q_stride_head >= 1L << 28 ||
+      (tile_keys != kBN && tile_keys != 2 * kBN) || !row_strides_ok(q_stride_tok) || !score_head_stride_ok(q_stride_head) ||
       !softmax_scale_ok(scale))
     return (int)hipErrorInvalidValue;
   const long slots = std::min((long)table_width * kPage, 1L << 30);              // (tile numbers: 24 bits)

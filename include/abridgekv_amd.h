@@ -501,7 +501,8 @@ int abkv_decode_attn_scored(const void* q, long q_stride_seq, long q_stride_head
                             long scores_stride_head, void* out, long out_stride_seq, long out_stride_head, float* lse,
                             void* workspace, size_t workspace_bytes, abkv_stream_t stream);
 /* The weights of prompt queries: scores[r][h][j] += sum over request r's queries i (rows q_start[r] .. q_start[r + 1] - 1 of
- * q [T, 32, 128] bf16 at positions kv_start[r] + i) with j <= position, and h's query heads, of exp(scale q.k - lse).
+ * q [T, 32, 128] bf16 at positions kv_start[r] + i) with j <= position, and h's query heads, of exp(scale q.k - lse). Strides of
+ * q: 0 <= q_stride_tok < 2^24, 0 <= q_stride_head < 2^28.
  * lse [T, 32]: what the queries' attention over the same rows left (a row with -inf adds nothing). q_start
  * [num_requests + 1] and kv_start [num_requests] are on the HOST and go with the launch (one for every 64 requests and 640
  * tiles of tile_keys keys, 64 or 128). */
