@@ -8,7 +8,8 @@
 //   window_bwd_dkv_kernel   a workgroup per 64 keys of a KV head over the query tiles whose windows reach them: the same
 //                           count for every key tile. Keys among the sinks are seen by every later row as well: these far
 //                           query tiles are cut into parts with workgroups of their own (SinkPlan), which leave fp32 sums
-//                           in slots, and the last part of a tile to finish adds them up in part order.
+//                           in slots, and the last part of a tile to finish adds them up in part order. (Very many sink
+//                           tiles: no parts.)
 #include "bwd_tile.h"
 #include "window_tile.h"
 
@@ -206,11 +207,8 @@ __global__ __launch_bounds__(256, 2) void window_bwd_dkv_kernel(WindowBwdArgs a)
   for (int e = 0; e < 8; ++e) dk[e][0] = dv[e][0] = floatx4{0.f, 0.f, 0.f, 0.f};
 
   const WindowSpan span(k0, n, f.window, f.sinks);
-  int qt_first = span.first, qt_end = span.near_end;
-  if (z > 0) {
-    qt_first = min(span.near_end + (z - 1) * a.plan.part, span.far_end);
-    qt_end = min(qt_first + a.plan.part, span.far_end);
-  }
+  int qt_first, qt_end;
+  a.plan.range(span, z, qt_first, qt_end);
   // The near query tiles in cyclic order from a multiple of `reach`, their number for an inner key tile: the workgroups of
   // neighbouring key tiles, which run at one time, then take the same query tile at the same step, and its rows come from
   // their XCD's L2 (from its own first tile on, a workgroup reads what its neighbour read a step before, when the other 60 of

@@ -46,11 +46,13 @@ struct WindowSpan {
 };
 
 // Work of the window's dK/dV launch: one item per key tile for its near query tiles, and for each tile that holds sinks
-// `parts` more for the far ones, `part` query tiles each. The items of a sink tile leave fp32 sums in slots.
+// `parts` more for the far ones, `part` query tiles each. The items of a sink tile leave fp32 sums in slots. More sink tiles
+// than there are slots are enough items without parts: each then walks its near and far query tiles (sink_tiles 0).
 // Query tiles (x 4 heads) a far part is worth starting for: with 8, us a forward and backward of three of up to 777 rows, window
 // 129, 17 sinks 120 (with 4: 99), of 2048 rows, window 64 117 (96), of 1000 rows, 100 sinks 107 (86).
 constexpr int kSinkPartMin = 4;
-constexpr int kSinkSlots = 384;      // bound on the far parts of a launch (64 KiB of sums each, per KV head)
+constexpr int kSinkSlots = 384;      // far parts of a launch, and sink tiles that have some, at most (64 KiB of sums each, per
+                                     // KV head: slots for both, 384 MiB)
 struct SinkPlan {
   int tiles, sink_tiles, part, parts;          // key tiles; those that hold sinks; query tiles per far part; parts a tile
   SinkPlan() = default;
@@ -61,6 +63,7 @@ struct SinkPlan {
     sink_tiles = far > 0 ? imin((imin(sinks, seq_len) + kBN - 1) / kBN, tiles) : 0;
     part = imax(kSinkPartMin, near);
     parts = 0;
+    if ((long)sink_tiles * batch > kSinkSlots) sink_tiles = 0;
     if (sink_tiles == 0) return;
     const int most = imax(1, kSinkSlots / imax(1, sink_tiles * batch));          // parts of a tile, at most
     part = imax(part, (far + most - 1) / most);
@@ -68,6 +71,15 @@ struct SinkPlan {
   }
   ABKV_HD int items() const { return tiles + sink_tiles * parts; }               // per (KV head, sequence)
   ABKV_HD int slots() const { return sink_tiles * (parts + 1); }
+  // Query tiles [first, end) of item z of a key tile (0: the near ones, and the far ones where the launch has no parts).
+  ABKV_HD void range(const WindowSpan& span, int z, int& first, int& end) const {
+    first = span.first;
+    end = sink_tiles > 0 ? span.near_end : span.far_end;
+    if (z > 0) {
+      first = imin(span.near_end + (z - 1) * part, span.far_end);
+      end = imin(first + part, span.far_end);
+    }
+  }
 };
 
 }  // namespace abkv
