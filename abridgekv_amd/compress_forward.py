@@ -583,9 +583,12 @@ class CompressLM(nn.Module):
         """Plain causal LM without compression on the same predict positions (compress_forward.py:1095-1132):
         sequences of ``ctx_blocks`` contiguous blocks (0: all N, the full-context ceiling; 1: the floor). ``window`` > 0:
         attention under a sliding window of that many tokens with the first ``sinks`` visible, the context of bounded size
-        that a compressed one is compared with."""
+        that a compressed one is compared with (models whose layers all have full attention)."""
         if sinks and not window:
             raise ValueError("sinks need a window")
+        others = set(getattr(self.model.config, "layer_types", None) or ()) - {"full_attention"}
+        if window and others:
+            raise NotImplementedError(f"a windowed baseline takes full-attention layers only, the model has {sorted(others)}")
         B, N, C = content_ids.shape
         G = ctx_blocks if ctx_blocks else N
         if N % G:
