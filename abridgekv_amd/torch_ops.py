@@ -320,7 +320,8 @@ def _kv_evict_fake(layer_caches, block_table, seq_lens, scores, positions, num_t
 @torch.library.custom_op(f"{_NS}::window_attn", mutates_args=("out", "lse"))
 def window_attn(q: Tensor, k: Tensor, v: Tensor, window: int, sinks: int, seq_lens: Optional[Tensor], scale: float,
                 out: Tensor, lse: Optional[Tensor]) -> None:
-    """abkv_window_attn: attention of whole prompts under a sliding window with sinks, q [B, S, 32, 128]."""
+    """abkv_window_attn: attention of whole prompts under a sliding window with sinks, q [B, S, 32, 128]. A forward whose
+    gradients will be taken: window_attn_low."""
     _ops.window_attention(q, k, v, window, sinks, seq_lens=seq_lens, scale=scale, out=out, lse=lse)
 
 
@@ -329,16 +330,33 @@ def _window_attn_fake(q, k, v, window, sinks, seq_lens, scale, out, lse):
     _need(tuple(out.shape) == tuple(q.shape), "out must be [B, S, 32, 128]")
 
 
+@torch.library.custom_op(f"{_NS}::window_attn_low", mutates_args=("out", "lse", "out_low"))
+def window_attn_low(q: Tensor, k: Tensor, v: Tensor, window: int, sinks: int, seq_lens: Optional[Tensor], scale: float,
+                    out: Tensor, lse: Tensor, out_low: Tensor) -> None:
+    """abkv_window_attn as a training step takes it: out_low [B, S, 32, 128] float8_e5m2 gets what out's rounding left off, for
+    window_attn_bwd."""
+    _ops.window_attention(q, k, v, window, sinks, seq_lens=seq_lens, scale=scale, out=out, lse=lse, out_low=out_low)
+
+
+@window_attn_low.register_fake
+def _window_attn_low_fake(q, k, v, window, sinks, seq_lens, scale, out, lse, out_low):
+    _need(tuple(out.shape) == tuple(q.shape) == tuple(out_low.shape), "out and out_low must be [B, S, 32, 128]")
+
+
 @torch.library.custom_op(f"{_NS}::window_attn_bwd", mutates_args=())
 def window_attn_bwd(q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor, dout: Tensor, window: int, sinks: int,
-                    seq_lens: Optional[Tensor], scale: float) -> tuple[Tensor, Tensor, Tensor]:
-    """abkv_window_attn_bwd: (dq, dk, dv) of sum(dout * out) under the same window (new tensors)."""
-    return _ops.window_attention_backward(q, k, v, out, lse, dout, window, sinks, seq_lens=seq_lens, scale=scale)
+                    seq_lens: Optional[Tensor], scale: float,
+                    out_low: Optional[Tensor] = None) -> tuple[Tensor, Tensor, Tensor]:
+    """abkv_window_attn_bwd: (dq, dk, dv) of sum(dout * out) under the same window (new tensors). Without the ``out_low`` of
+    window_attn_low dq and dk are less exact over few keys."""
+    return _ops.window_attention_backward(q, k, v, out, lse, dout, window, sinks, seq_lens=seq_lens, scale=scale,
+                                          out_low=out_low)
 
 
 @window_attn_bwd.register_fake
-def _window_attn_bwd_fake(q, k, v, out, lse, dout, window, sinks, seq_lens, scale):
+def _window_attn_bwd_fake(q, k, v, out, lse, dout, window, sinks, seq_lens, scale, out_low=None):
     return (q.new_empty(q.shape), k.new_empty(k.shape), k.new_empty(k.shape))
 
 
 BOUNDED_OPS = ("decode_attn_window", "decode_attn_scored", "kv_evict", "window_attn", "window_attn_bwd")
+TRAINING_OPS = ("window_attn_low",)                          # window_attn with what window_attn_bwd takes beside out and lse
