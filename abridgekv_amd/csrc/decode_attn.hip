@@ -731,10 +731,12 @@ inline bool share_splits(int max_splits, int num_seqs) {
 template <int kMode>
 inline void launch_decode(const DecodeArgs& a, int max_splits, int num_seqs, hipStream_t stream) {
   // Sequences of one split: eight waves share it (the windows' short ones; see _step_split_pages)
-  if (kMode != kPlain && max_splits == 1) {
-    hipLaunchKernelGGL((decode_attn_kernel<1, 2 * kGroup, kMode>), dim3(kHeadsKV, num_seqs), dim3(128 * kGroup), 0, stream,
-                       a);
-    return;
+  if constexpr (kMode != kPlain) {
+    if (max_splits == 1) {
+      hipLaunchKernelGGL((decode_attn_kernel<1, 2 * kGroup, kMode>), dim3(kHeadsKV, num_seqs), dim3(128 * kGroup), 0,
+                         stream, a);
+      return;
+    }
   }
   if (share_splits(max_splits, num_seqs)) {
     hipLaunchKernelGGL((decode_attn_kernel<1, kGroup, kMode>), dim3(max_splits * kHeadsKV, num_seqs), dim3(64 * kGroup), 0,
