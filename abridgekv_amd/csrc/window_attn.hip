@@ -14,6 +14,8 @@
 // buffers each, us a call of two sequences of 4096 rows under windows of 64 / 128 / 512 / 1024: 58 / 66 / 105 / 156 -> 48 / 57 /
 // 99 / 147 (copies of the query rows and outputs alone: 27). Outputs in whole 64-byte runs (store_acc_rows) before it 66 / 73 /
 // 112 / 160 -> 58 / 66 / 105 / 156. Bound by issue within a tile (as the masked prefill) and the edge tiles under long windows.
+#include <algorithm>
+
 #include "window_tile.h"
 
 namespace abkv {
@@ -199,7 +201,7 @@ int abkv_paged_prefill_attn_window(const void* q, long q_stride_tok, long q_stri
       out == nullptr || num_pages <= 0 || table_width <= 0 || window <= 0 || sinks < 0 || !softmax_scale_ok(scale) ||
       !row_strides_ok(q_stride_tok))
     return (int)hipErrorInvalidValue;
-  const long slots = (long)table_width * kPage;
+  const long slots = std::min((long)table_width * kPage, 1L << 30);              // (positions and their counts: 32 bits)
   for (int r = 0; r < num_requests; ++r)
     if (q_start[0] < 0 || q_start[r + 1] < q_start[r] || kv_start[r] < 0 ||
         (long)kv_start[r] + q_start[r + 1] - q_start[r] > slots)

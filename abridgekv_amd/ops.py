@@ -1143,8 +1143,8 @@ def _check_chunks(q, block_table, q_start, kv_start):
              "q_start [R + 1] and kv_start [R] must be flat sequences, R at most the table's rows")
     nq = qs[1:] - qs[:-1]
     _require(qs[0] == 0 and (ks.size == 0 or nq.min() >= 0) and qs[-1] <= q.shape[0], "q_start must be a prefix sum <= T")
-    _require(ks.size == 0 or (ks.min() >= 0 and (ks + nq).max() <= block_table.shape[1] * PAGE),
-             "the chunks' rows must lie in [0, block_table width * 16)")
+    _require(ks.size == 0 or (ks.min() >= 0 and (ks + nq).max() <= min(block_table.shape[1] * PAGE, 1 << 30)),
+             "the chunks' rows must lie in [0, block_table width * 16), at most 2^30")
     return qs, ks, nq
 
 
