@@ -77,3 +77,24 @@ def test_backend_layer_with_pages_given_back():
     want = step(cache, table)
     got = step(*_hide(cache, table, window, sinks, float("nan"), 1 << 30, past))
     assert torch.isfinite(want).all() and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (40, 4), (63, 17), (100, 32), (300, 130), (700, 5)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("split_pages", [None, 2])
+def test_hidden_rows_of_a_decode_step(window, sinks, value, split_pages):
+    """Those on the edge pages of the sinks and of the window, and the rows past the sequence, among them."""
+    past = [0, 40, 299, 640, 1000]
+    q, cache, table = _batch(window, [1] * 5, past)
+    bad, ids_table = _hide(cache, table, window, sinks, value, 1 << 30, past)
+    for r, p in enumerate(past):                             # (the rest of the last page)
+        bad[int(table[r, p // 16]), :, p % 16 + 1:] = value
+    lens = torch.tensor([p + 1 for p in past], dtype=torch.int32, device="cuda")
+    got = []
+    for c, t in ((cache, table), (bad, ids_table)):
+        lse = torch.empty((5, 32), device="cuda")
+        out, _ = ops.decode_attention_window(q.cuda(), c.cuda(), torch.from_numpy(t).cuda(), lens, window, sinks, lse=lse,
+                                             split_pages=split_pages)
+        assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+        got.append((out, lse))
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
