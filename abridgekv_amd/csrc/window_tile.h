@@ -155,7 +155,11 @@ __device__ __forceinline__ void attend_sinks(const __bf16* buf, int sinks, const
     for (int u = 0; u < H; ++u) o[t][u] = mfma16x16x32(vop, pop[u], o[t][u]);
   }
 #pragma unroll
-  for (int u = 0; u < H; ++u) l[u] = mfma16x16x32(ones, pop[u], floatx4{0.f, 0.f, 0.f, 0.f})[0];
+  for (int u = 0; u < H; ++u) {
+    // every entry is the sum; their mean, or the compiler holds all four over the walk, in scratch
+    const floatx4 sum = mfma16x16x32(ones, pop[u], floatx4{0.f, 0.f, 0.f, 0.f});
+    l[u] = 0.5f * (sum[0] + sum[1]);
+  }
 }
 
 // The first DMAs of a walk of at least one tile: K and V of tile 0, K of tile 1 (the first again where there is none).
