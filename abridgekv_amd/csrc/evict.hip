@@ -15,12 +15,13 @@ namespace abkv {
 // are the KV head's four query heads by four groups of 32 keys (kTiles = 2), or by two groups at alternate steps (kTiles = 1,
 // where the longest workgroup would bound the launch). 32 query rows of the four heads at a time come into triple-buffered LDS
 // by DMA. One owner per score: no atomics, the same bits every time.
-// Bound by issue: a 16 x 64 step costs 419 cycles of MFMA, FMA, exponential and addition (measured alone, overlapped), here 640
-// with the operands' reads and the barriers. 1500 rows and 2048 behind 2048: 94 us a call, 650 TFLOP/s of visible pairs. Tried:
-// query rows straight into operand registers 166 us (64 bytes of each of 16 rows an instruction; without those loads 88); 64
-// keys a wave at two waves a SIMD, its three stages interleaved by hand, 95, with a step a barrier more 99.
-// The requests and the tiles' order go with the launch's arguments (uploaded before it, two prompts 88 us a call and 64 queries
-// behind 4000 rows 41, this 83 and 21).
+// 1500 rows and 2048 behind 2048: 76 us a call among others, 800 TFLOP/s of visible pairs. Matrix units 30 % of the SIMDs'
+// cycles, other vector work 43 %, 10 % both at once; the waves wait for rows and barriers 45 % of their time. A 16 x 64 step of
+// MFMA, FMA, exponential and addition alone costs 419 cycles, here 640. Tried, against 94 us of this form at that time: query rows
+// straight into operand registers 166 (64 bytes of each of 16 rows an instruction; without those loads 88); 64 keys a wave at
+// two waves a SIMD, its three stages interleaved by hand, 95, with a step a barrier more 99.
+// The requests and the tiles' order go with the launch's arguments (before, by an upload: two prompts 88 us a call, 64 queries
+// behind 4000 rows 41; with it 83 and 21).
 constexpr int kScoreRequests = 64, kScoreTiles = 640;        // of a launch (3.3 KiB of arguments)
 struct PromptScoreArgs {
   const __bf16* q;  long q_st, q_sh;           // [T, 32, 128]

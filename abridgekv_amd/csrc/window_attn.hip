@@ -13,7 +13,9 @@
 // that one's loads and stores run beside the other's products. Against one workgroup of 8 waves for all four heads, three
 // buffers each, us a call of two sequences of 4096 rows under windows of 64 / 128 / 512 / 1024: 58 / 66 / 105 / 156 -> 48 / 57 /
 // 99 / 147 (copies of the query rows and outputs alone: 27). Outputs in whole 64-byte runs (store_acc_rows) before it 66 / 73 /
-// 112 / 160 -> 58 / 66 / 105 / 156. Bound by issue within a tile (as the masked prefill) and the edge tiles under long windows.
+// 112 / 160 -> 58 / 66 / 105 / 156. Long windows (8192 and 5000 rows, window
+// 1024): matrix units 41 % of the SIMDs' cycles, other vector work 35 %, 10 % both at once; the waves are ready but not issued
+// 37 % of their time and wait 26 %.
 #include <algorithm>
 
 #include "window_tile.h"
@@ -36,9 +38,9 @@ struct DenseArgs {
 };
 
 // kLse: the call wants lse. The output is divided by the sum of its rounded weights, but lse takes the unrounded ones, up to 2^8
-// under the running maximum's headroom: rounded, a few heavy keys would leave it up to 2^-8 off however many rows are visible (600 rows, one key 6 log2 units
-// above the others: 2.3e-3, this 2e-6). The additions cost 4 % (two sequences of 8192 and 5000 rows, window 1024: 244 -> 253 us),
-// so calls without lse leave them out.
+// under the running maximum's headroom: rounded, a few heavy keys would leave it up to 2^-8 off however many rows are visible
+// (600 rows, one key 6 log2 units above the others: 2.3e-3, this 2e-6). The additions cost 4 % (two sequences of 8192 and 5000
+// rows, window 1024: 244 -> 253 us), so calls without lse leave them out.
 template <class Chunks, bool kLse>
 __global__ __launch_bounds__(256, 2) void window_attn_kernel(WindowArgs a, Chunks c) {
   constexpr bool kPaged = Chunks::kPaged;

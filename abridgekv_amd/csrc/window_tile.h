@@ -65,15 +65,16 @@ struct PagedWindowRows : PagedRows {
   }
 };
 
-// Up to 32 sinks before a query tile's windows take half a tile of their own, outside the walk (a whole one costs a tenth
-// of a query tile under a window of 512; 4 sinks: windows of 128 / 512 / 1024 81 / 121 / 269 -> 74 / 114 / 262 us): 32 K
-// rows and 32 V rows in one LDS tile. Sinks that the windows reach, or more of them, stay with the walk.
+// Up to 32 sinks before a query tile's windows take half a tile of their own, outside the walk: 32 K rows and 32 V rows in one
+// LDS tile. Sinks that the windows reach, or more of them, stay with the walk. (us of two sequences of 4096 rows with 4 sinks in
+// the walk's whole tile / in this, windows of 64 52.9 / 51.2, 128 65.3 / 63.4, 512 106.6 / 103, 1024 149.4 / 146.)
 constexpr int kShortSinks = 32;
 __device__ __forceinline__ bool short_sinks(int q0, int window, int sinks) {
   return sinks > 0 && sinks <= kShortSinks && q0 + 1 - window >= kBN;
 }
 
-// DMA of the sinks' rows (keys 0 .. 31, fewer than n_keys >= 64; rows decides what stands for those past the sinks): K in rows 0 .. 31 of buf, V in rows 32 .. 63, by 4 waves.
+// DMA of the sinks' rows (keys 0 .. 31, fewer than n_keys >= 64; `rows` decides what stands for those past the sinks): K in rows
+// 0 .. 31 of buf, V in rows 32 .. 63, by 4 waves.
 template <class Rows>
 __device__ __forceinline__ void issue_sinks(const Rows& rows, int n_keys, __bf16* buf, int w, int lane) {
   const auto src = rows.template src<4>(0, w & 1, n_keys);   // waves 2 and 3: the V rows of the same keys
@@ -233,7 +234,8 @@ __device__ __forceinline__ void attend_pair(const Rows& rows, Walk& walk, int n_
 // D = sum_d dO O takes it: with O rounded, D is off by about 2^-9 of a sum of 128 products, and over few keys, where dP and D
 // nearly cancel, that is more than the rounding of dS: relative errors of dQ and dK (their own rounding gives 1.7e-3) of 2 rows
 // 3.9e-3, of 8 2.9e-3, of 777 under a window of 129 2.5e-3; with it 2.4e-3 each. e5m2 keeps all but an eighth of it down to
-// bf16's smallest values (beyond 57344 it saturates). Two of 4096 rows, window 512: 460 -> 477 us a forward and backward.
+// bf16's smallest values (beyond 57344 it saturates). Two of 4096 rows, window 512: 460 -> 477 us a forward and
+// backward.
 template <int H>
 __device__ __forceinline__ void store_low(uint8_t* dst, const floatx4 (&o)[8][H], int u, int j, float inv) {
   const bool odd = j & 1;

@@ -1183,9 +1183,11 @@ def paged_prefill_attention_window(q: torch.Tensor, kv_cache: torch.Tensor, bloc
 
 def _step_split_pages(num_seqs: int, pages: int) -> int:
     """Pages per split of a step's launch over ``num_seqs`` sequences of up to ``pages`` pages: by all pages of the batch, then
-    evened over the splits that takes. Short splits end a small launch sooner, long ones write fewer partials. us a step of
-    8 / 16 / 32 / 64 pages a split: one sequence of 1024 window rows 8.5 / 9.1 / 10.3 / 12.0, of 2100 scored rows 8.0 / 9.3 /
-    11.5 / 14.4; 32 of 1024 33.3 / 34.4 / 30.6 / 31.1; 64 of 4096 211 / 192 / 191 / 176, of 2100 scored 126 / 130 / 121 / 120."""
+    evened over the splits that takes. Short splits end a small launch sooner, long ones write fewer partials, even ones end
+    together. us a step, pages a split: us (the choice in brackets), windows of 1024 rows (66 pages): one sequence [8: 8.4] 16: 9.4
+    32: 11.4; 8 sequences 8: 13.5 [12: 13.2] 32: 15.4; 32 sequences 8: 31.8 16: 35.2 [22: 30.3] 40: 33.2; 256 8: 221 22: 188 [34:
+    186] 64: 277. Of 4096 rows: 64 sequences 8: 207 32: 198 [52: 176] 64: 177; 256 8: 847 32: 734 [52: 697] 64: 721. Scored, one of
+    2100 rows 8: 7.9 [12: 8.7] 32: 12.0; 16 of them 12: 33.7 [22: 34.0] 32: 41.7; 256 of 5000 8: 1168 32: 1141 [64: 1135]."""
     total = num_seqs * pages
     most = 8 if total < 128 else 12 if total < 1500 else 24 if total < 3000 else 40 if total < 12000 else 64
     splits = -(-pages // most)
@@ -1328,8 +1330,8 @@ def decode_attention_scored(q: torch.Tensor, kv_cache: torch.Tensor, block_table
 def _score_tile_keys(ks: np.ndarray, nq: np.ndarray, num_cus: int) -> int:
     """Keys of a workgroup of the prompt scores, 64 or 128, from requests of nq queries behind ks rows. By the longest
     workgroup (as many queries as a request has) and the sum over all, a workgroup a CU: a query row takes 21 ns against 64 keys
-    and 33 against 128, a workgroup 5 us beside. us a call with 64 / 128: one prompt of 512 rows 22 / 28, of 2048 57 / 81, of
-    4096 120 / 149; 64 queries behind 4000 rows 18 / 15; 2048 behind 2048 beside 1500 118 / 94; four of 512 behind 512 38 / 31."""
+    and 33 against 128, a workgroup 5 us beside. us a call with 64 / 128: one prompt of 512 rows 15 / 22, of 2048 51 / 76, of
+    4096 119 / 153; 64 queries behind 4000 rows 10 / 7; 2048 behind 2048 beside 1500 110 / 88; four of 512 behind 512 32 / 26."""
     longest, total = int(nq.max()), int((nq * (2 * ks + nq)).sum()) / 128
     groups = HEADS_KV * int((ks + nq).sum()) / 64 / num_cus
     per = HEADS_KV * total / num_cus
@@ -1342,7 +1344,8 @@ def paged_prefill_scores(q: torch.Tensor, kv_cache: torch.Tensor, block_table: t
     see row j, and KV head h's four query heads, of exp(scale q.k - lse).
 
     Queries as :func:`paged_prefill_attention` takes causal chunks (q [T, 32, 128] bf16, host q_start [R + 1] and kv_start
-    [R]); ``lse`` [T, 32] fp32: what that call left for them (rows with -inf add nothing, whatever they hold). To weigh by a
+    [R]); ``lse`` [T, 32] fp32: what that call left for them (rows with -inf add nothing, whatever they hold); its sums are of
+    bf16-rounded weights, so a query's weights are all off by one factor, up to 2^-8. To weigh by a
     prompt's last queries only, pass those alone with their kv_start. ``scores`` [R, 8, rows] fp32 is updated in place, one
     owner a score. The starts go with the launch (a captured one keeps them).
     """
