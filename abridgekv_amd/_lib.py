@@ -129,6 +129,27 @@ SIGNATURES = {
     "abkv_kv_evict_workspace_size": (C.c_size_t, [C.c_int] * 3),
     "abkv_kv_evict": (C.c_int, [C.POINTER(_vp), C.c_int, C.c_int, _vp, C.c_long, _vp, C.c_int, C.c_int, _vp, _vp,
                                 C.c_long, _vp, C.c_int, C.c_int, C.c_int, _vp, _vp, C.c_size_t, _vp]),
+    "abkv_qk_norm_rope_append": (C.c_int, [_vp, C.c_long, C.c_long] * 3
+                                 + [_vp, C.c_int, _vp, _vp, C.c_int, C.c_float, C.c_int, C.c_int, C.c_int, _vp, C.c_long,
+                                    _vp, _vp, C.c_int, C.c_int, _vp, C.c_long, C.c_long, _vp]),
+    "abkv_qk_norm_rope": (C.c_int, [C.c_int] + [_vp, C.c_long, C.c_long, C.c_long] * 2
+                          + [C.c_int, C.c_int, _vp, _vp, C.c_int, C.c_float, _vp, _vp, C.c_long, C.c_long, C.c_int, _vp, _vp,
+                             _vp]),
+    "abkv_qk_norm_rope_bwd_workspace_size": (C.c_size_t, [C.c_int, C.c_int]),
+    "abkv_qk_norm_rope_bwd": (C.c_int, [C.c_int] + [_vp, C.c_long, C.c_long, C.c_long] * 4
+                              + [C.c_int, C.c_int, _vp, _vp, C.c_int, C.c_float, _vp, _vp, C.c_long, C.c_long, C.c_int, _vp,
+                                 _vp, _vp, _vp, _vp, C.c_size_t, _vp]),
+    "abkv_kv_append_int4": (C.c_int, [_vp, C.c_long, C.c_long] * 2 + [_vp, C.c_int, _vp, C.c_int, _vp]),
+    "abkv_kv_read_int4": (C.c_int, [_vp, C.c_int, _vp, C.c_int, C.c_int, _vp, _vp, _vp]),
+    "abkv_decode_int4_workspace_size": (C.c_size_t, [C.c_int] * 3),
+    "abkv_decode_attn_int4": (C.c_int, [_vp, C.c_long, C.c_long, _vp, C.c_int, _vp, C.c_long, _vp, C.c_int, C.c_int, C.c_int,
+                                        C.c_float, _vp, C.c_long, C.c_long, _vp, _vp, C.c_size_t, _vp]),
+    "abkv_kv_widen_int4": (C.c_int, [_vp, C.c_int, _vp, C.c_long, _vp, C.c_int, C.c_int, _vp, _vp, C.c_int, _vp]),
+    "abkv_token_logprobs_workspace_size": (C.c_size_t, [C.c_int] * 4),
+    "abkv_token_logprobs": (C.c_int, [C.c_int, _vp, C.c_long, C.c_int, C.c_int, _vp, C.c_float, C.c_int, _vp, _vp, _vp, _vp,
+                                      _vp, _vp, C.c_size_t, _vp]),
+    "abkv_token_logprobs_bwd": (C.c_int, [C.c_int, _vp, C.c_long, C.c_int, C.c_int, _vp, C.c_float, _vp, _vp, _vp, _vp,
+                                          C.c_long, _vp]),
 }
 
 _LIB = None

@@ -16,7 +16,8 @@ PROBE_LIB = PKG / "libabridgekv_probes.so"      # measurement probes, loaded by 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 DEVICE_SOURCES = ["decode_attn.hip", "kv_cache.hip", "prefill_attn.hip", "prefill_bwd.hip", "paged_prefill.hip",
-                  "attn_f32.hip", "window_attn.hip", "window_bwd.hip", "evict.hip"]
+                  "attn_f32.hip", "window_attn.hip", "window_bwd.hip", "evict.hip", "norm_rope.hip", "kv_int4.hip",
+                  "logprobs.hip"]
 HOST_SOURCES = ["planner.cpp", "paged_plan.cpp"]
 PROBE_SOURCES = ["probes.hip"]
 

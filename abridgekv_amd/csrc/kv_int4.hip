@@ -1,0 +1,484 @@
+// The paged cache in 4 bits (int4.h): rows written and read back, single-token attention over it, and its pages widened for the
+// multi-query kernel (gfx950).
+#include "abridgekv_amd.h"
+#include "int4.h"
+
+namespace abkv {
+
+__device__ __forceinline__ u32x4 ld16b(const char* p) { return *reinterpret_cast<const u32x4*>(p); }
+
+// -- rows in and out ----------------------------------------------------------------------------------------------------
+struct Append4Args {
+  const __bf16* k; long k_st, k_sh;            // [T, 8, 128]
+  const __bf16* v; long v_st, v_sh;
+  const int64_t* slot_mapping;                 // [T]; < 0 or past the cache = skip
+  char* cache; long num_pages;
+};
+
+// Workgroup per token; thread: 8 dims of a head of K (the first 128 threads) or V.
+__global__ __launch_bounds__(256) void kv_append4_kernel(Append4Args a) {
+  const long t = blockIdx.x;
+  const long slot = a.slot_mapping[t];
+  if (slot < 0 || slot >= a.num_pages * kPage) return;       // (uniform)
+  const int half = threadIdx.x >> 7, h = (threadIdx.x >> 4) & 7, b = threadIdx.x & 15;
+  const __bf16* row = half ? a.v + t * a.v_st + h * a.v_sh : a.k + t * a.k_st + h * a.k_sh;
+  const u32x4 w = *reinterpret_cast<const u32x4*>(row + 8 * b);
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = bf16_lo(w[i]);
+    x[2 * i + 1] = bf16_hi(w[i]);
+  }
+  uint32_t pair;
+  const uint32_t word = quantise8(x, pair);
+  char* to = a.cache + slot / kPage * kPage4 + half * kHalf4 + slot % kPage * kSlot4;
+  reinterpret_cast<uint32_t*>(to + h * kHeadCodes4)[code_word(b)] = word;
+  if ((b & 3) == 0) reinterpret_cast<uint32_t*>(to + kParams4 + h * 16)[b >> 2] = pair;
+}
+
+// The eight values of a word and its group's pair.
+__device__ __forceinline__ void values8(uint32_t word, uint32_t pair, float (&x)[8]) {
+  const float s = bf16_lo(pair), m = bf16_hi(pair);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = fmaf(s, (float)((word >> (2 * i + ((i & 1) ? 14 : 0))) & 15), m);
+}
+
+// Rows by slot, as fp32 or bf16 [T, 8, 128]; a slot outside the cache reads as zeros. Threads as in kv_append4_kernel.
+template <class T>
+__global__ __launch_bounds__(256) void kv_read4_kernel(const char* cache, long num_pages, const int64_t* slot_mapping, T* k,
+                                                       T* v) {
+  const long t = blockIdx.x;
+  const long slot = slot_mapping[t];
+  const int half = threadIdx.x >> 7, h = (threadIdx.x >> 4) & 7, b = threadIdx.x & 15;
+  float x[8] = {};
+  if (slot >= 0 && slot < num_pages * kPage) {
+    const char* from = cache + slot / kPage * kPage4 + half * kHalf4 + slot % kPage * kSlot4;
+    values8(reinterpret_cast<const uint32_t*>(from + h * kHeadCodes4)[code_word(b)],
+            reinterpret_cast<const uint32_t*>(from + kParams4 + h * 16)[b >> 2], x);
+  }
+  T* to = (half ? v : k) + (t * kHeadsKV + h) * kHeadDim + 8 * b;
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<floatx4*>(to) = floatx4{x[0], x[1], x[2], x[3]};
+    *reinterpret_cast<floatx4*>(to + 4) = floatx4{x[4], x[5], x[6], x[7]};
+  } else {
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+    *reinterpret_cast<u32x4*>(to) = w;
+  }
+}
+
+// -- one token per sequence ---------------------------------------------------------------------------------------------
+struct Decode4Args {
+  const __bf16* q; long q_sb, q_sh;            // [B, 32, 128]
+  const char* kv; int num_pages;
+  const int32_t* block_table; long bt_stride;
+  const int32_t* seq_lens;                     // [B]
+  int split_pages, max_splits, max_pages;
+  float scale_log2;
+  __bf16* out; long o_sb, o_sh;                // [B, 32, 128]
+  float* lse;                                  // [B, 32] or nullptr
+  _Float16* part_o;                            // [B, max_splits, 32, 128]: split output / (l * scale)
+  float* part_ml;                              // [B, max_splits, 32, 4]: m (log2 units), l, scale, unused
+};
+
+__device__ __forceinline__ int rows_of(const Decode4Args& a, int b) {
+  return max(min(a.seq_lens[b], a.max_pages * kPage), 0);
+}
+__device__ __forceinline__ int splits_of(const Decode4Args& a, int rows) {
+  return max(1, ((rows + kPage - 1) / kPage + a.split_pages - 1) / a.split_pages);
+}
+
+// Codes of two neighbouring dims (nibbles n and n + 4 of a word) as the bf16 pair 128 + c: c lies in the low bits of the
+// mantissa, so every code is exact, and the 128s leave with the sums.
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, int n) { return ((w >> (4 * n)) & 0x000f000fu) | 0x43004300u; }
+
+// Workgroup (split, sequence), a wave per KV head: the heads' rows lie next to each other, so the workgroup streams whole pages
+// (a wave's 64 bytes of a slot are half a cache line). A wave walks its split 32 slots (two pages) at a time.
+//
+// Scores: the four groups of 32 dims have their own steps and minima, so a score is the sum of four products:
+//   x_j = sum_g (s_jg a_jg + m_jg Q_g),  a_jg = sum_{d in g} q_d c_jd,  Q_g = sum_{d in g} q_d.
+// One MFMA tile has 16 columns where a KV head has 4 query heads: column 4 h + g holds query head h with the dims of group g
+// alone (zero elsewhere), so that the four MFMAs of a tile leave a_jg in one accumulator and the sum over g is two DPP steps.
+// Values: out_d = sum_j (p_j s_jg) (c_jd - 8) + sum_j p_j (m_jg + 8 s_jg): column 4 h + g of P^T carries p_j s_jg, and of the four
+// accumulator rows 4 j + r of an output tile (words of the value rows, word % 4 its group) a lane keeps r = g: 8 dims in a row.
+// The codes enter as 128 + c (code_pair): the score accumulator starts at -128 Q_g, and a row of -136s among the V tiles takes
+// them, and the codes' middle, out of the output. p_j s_jg is rounded to bf16 (2^-8 of a weight), which errs by that part of
+// s |c - 8|, no more than values of that size would (by s c, from the minimum, it was 2.5 times as much); everything else is
+// exact or fp32.
+//
+// A lane's V operand is one word of 8 slots while a wide load brings four words of one, and its parameters likewise: both
+// are exchanged through LDS, in a part of its own for each wave (no barrier).
+__device__ __forceinline__ void wave_exchange() {              // LDS is in order within a wave; this keeps the compiler so too
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+constexpr int kVRow = 16, kPRow = 80;                        // dwords: a slot's codes; a tile's pairs [4 groups][16 slots], padded
+__global__ __launch_bounds__(64 * kHeadsKV, 4) void decode4_kernel(Decode4Args a) {
+  const int b = blockIdx.y, split = blockIdx.x;
+  const int kvh = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, m16 = lane & 15, j = lane >> 4;
+  const int h = m16 >> 2, g = m16 & 3;
+  const int row_end = rows_of(a, b);
+  const int n_splits = splits_of(a, row_end);
+  if (split >= n_splits) return;
+  const int pg_begin = split * a.split_pages;
+  const int pg_end = min((row_end + kPage - 1) / kPage, pg_begin + a.split_pages);
+  __shared__ __attribute__((aligned(16))) uint32_t vbuf[kHeadsKV][32 * kVRow], pbuf[kHeadsKV][4 * kPRow];
+  uint32_t* const vl = vbuf[kvh];
+  uint32_t* const pl = pbuf[kvh];
+
+  // Page ids of the split, lane l page pg_begin + l (split_pages <= 64)
+  const int32_t* bt = a.block_table + (long)b * a.bt_stride;
+  int pid_l = 0;
+  if (lane < pg_end - pg_begin) pid_l = min(max(bt[pg_begin + lane], 0), a.num_pages - 1);
+
+  // Q^T: dims 32 g + 8 j .. + 7 of head h, for the MFMA of group g
+  bf16x8 qop[4];
+  float qsum = 0.f;
+  {
+    const u32x4 w = *reinterpret_cast<const u32x4*>(a.q + (long)b * a.q_sb + (long)(kvh * kGroup + h) * a.q_sh + 32 * g + 8 * j);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      qop[i] = __builtin_bit_cast(bf16x8, g == i ? w : u32x4{0, 0, 0, 0});
+      qsum += bf16_lo(w[i]) + bf16_hi(w[i]);
+    }
+    qsum = sum_xor32(sum_xor16(qsum));                       // Q_g
+  }
+  const float q128 = -128.f * qsum;
+  typedef short s8 __attribute__((ext_vector_type(8)));
+  const short n136 = (short)0xc308;                          // bf16 -136
+  const bf16x8 minus = __builtin_bit_cast(bf16x8, s8{n136, n136, n136, n136, n136, n136, n136, n136});
+
+  floatx4 o[8], off = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+  float m_run = -INFINITY, l_run = 0.f, om = 0.f;            // om: sum of p_j (m_jg + 8 s_jg) over this lane's slots
+
+  // This lane's pieces: K words 4 j .. + 3 of slot m16; V words 4 (lane & 3) .. of the slot whose LDS row is lane >> 2; and the
+  // pairs of slot m16, of K (j 0, 1) or V (j 2, 3), page j & 1. LDS row 4 e + j holds slot 4 j + e: the reads below then take
+  // all banks.
+  const int vrow = lane >> 2, vslot = 4 * (vrow & 3) + (vrow >> 2);
+  const long k_at = m16 * kSlot4 + kvh * kHeadCodes4 + 16 * j;
+  const long v_at = kHalf4 + vslot * kSlot4 + kvh * kHeadCodes4 + 16 * (lane & 3);
+  const long p_at = (j >> 1) * kHalf4 + m16 * kSlot4 + kParams4 + kvh * 16;
+  struct Tile {
+    u32x4 k[2], v[2], p;
+  };
+  auto load = [&](int pg) {
+    const int at = pg - pg_begin;
+    const char* p0 = a.kv + (long)__builtin_amdgcn_readlane(pid_l, at) * kPage4;
+    const char* p1 = a.kv + (long)__builtin_amdgcn_readlane(pid_l, min(at + 1, pg_end - 1 - pg_begin)) * kPage4;
+    Tile t;
+    t.k[0] = ld16b(p0 + k_at);
+    t.k[1] = ld16b(p1 + k_at);
+    t.v[0] = ld16b(p0 + v_at);
+    t.v[1] = ld16b(p1 + v_at);
+    t.p = ld16b((j & 1 ? p1 : p0) + p_at);
+    return t;
+  };
+  Tile cur;
+  if (pg_begin < pg_end) cur = load(pg_begin);
+  for (int pg = pg_begin; pg < pg_end; pg += 2) {
+    Tile nxt;
+    const bool more = pg + 2 < pg_end;
+    if (more) nxt = load(pg + 2);
+
+    floatx4 s[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      s[t] = floatx4{q128, q128, q128, q128};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t w = cur.k[t][i];
+        const u32x4 codes = {code_pair(w, 0), code_pair(w, 1), code_pair(w, 2), code_pair(w, 3)};
+        s[t] = mfma16x16x32(__builtin_bit_cast(bf16x8, codes), qop[i], s[t]);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) *reinterpret_cast<u32x4*>(vl + (16 * t + vrow) * kVRow + 4 * (lane & 3)) = cur.v[t];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pl[j * kPRow + 16 * i + m16] = cur.p[i];
+    wave_exchange();
+    u32x4 kp[2], vp[2];                                      // pairs of group g of slots 4 j .. + 3 of the two pages
+    uint32_t vw[8];                                          // word m16 of slots 4 j + e of page 0, then of page 1
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      kp[t] = *reinterpret_cast<const u32x4*>(pl + t * kPRow + 16 * g + 4 * j);
+      vp[t] = *reinterpret_cast<const u32x4*>(pl + (2 + t) * kPRow + 16 * g + 4 * j);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) vw[4 * t + e] = vl[(16 * t + 4 * e + j) * kVRow + m16];
+    }
+    wave_exchange();
+
+    const bool tail = (pg + 2) * kPage > row_end;
+    float sv[8];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float x = fmaf(bf16_lo(kp[t][r]), s[t][r], bf16_hi(kp[t][r]) * qsum);
+        x += dpp<kDppXor1>(x);
+        x += dpp<kDppXor2>(x);
+        x *= a.scale_log2;
+        if (tail) {                                          // rows past the end: whatever their slots hold
+          const bool in = pg * kPage + 16 * t + 4 * j + r < row_end;
+          x = in ? x : -INFINITY;
+          vp[t][r] = in ? vp[t][r] : 0u;
+        }
+        sv[4 * t + r] = x;
+      }
+    float mx = sv[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) mx = fmaxf(mx, sv[e]);
+    // The maximum moves only when some row passes it by more than 8 (weights stay below 2^8)
+    if (__any(mx > m_run + 8.f)) {
+      const float m_new = fmaxf(m_run, max_xor32(max_xor16(mx)));
+      const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_new);
+      m_run = m_new;
+      l_run *= alpha;
+      om *= alpha;
+      off *= alpha;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] *= alpha;
+    }
+    const float m_ref = m_run == -INFINITY ? 0.f : m_run;
+    u32x4 pw;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const float p0 = fast_exp2(sv[e] - m_ref), p1 = fast_exp2(sv[e + 1] - m_ref);
+      const uint32_t w0 = vp[e >> 2][e & 3], w1 = vp[e >> 2][(e & 3) + 1];
+      l_run += p0 + p1;
+      const float s0 = bf16_lo(w0), s1 = bf16_lo(w1);
+      om = fmaf(p0, fmaf(8.f, s0, bf16_hi(w0)), om);
+      om = fmaf(p1, fmaf(8.f, s1, bf16_hi(w1)), om);
+      pw[e / 2] = pack_bf16x2(p0 * s0, p1 * s1);
+    }
+    const bf16x8 pop = __builtin_bit_cast(bf16x8, pw);
+    off = mfma16x16x32(minus, pop, off);
+    uint32_t lo[4], hi[4];                                   // nibbles 0 .. 3 and 4 .. 7 of two slots
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      lo[k] = __builtin_amdgcn_perm(vw[2 * k + 1], vw[2 * k], 0x05040100u);
+      hi[k] = __builtin_amdgcn_perm(vw[2 * k + 1], vw[2 * k], 0x07060302u);
+    }
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const u32x4 even = {code_pair(lo[0], n), code_pair(lo[1], n), code_pair(lo[2], n), code_pair(lo[3], n)};
+      const u32x4 odd = {code_pair(hi[0], n), code_pair(hi[1], n), code_pair(hi[2], n), code_pair(hi[3], n)};
+      o[2 * n] = mfma16x16x32(__builtin_bit_cast(bf16x8, even), pop, o[2 * n]);
+      o[2 * n + 1] = mfma16x16x32(__builtin_bit_cast(bf16x8, odd), pop, o[2 * n + 1]);
+    }
+    cur = nxt;
+  }
+
+  // This lane's 8 dims 32 g + 8 j .. + 7 of head h
+  const float l = sum_xor32(sum_xor16(l_run));
+  om = sum_xor32(sum_xor16(om));
+  const float inv = l > 0.f ? 1.f / l : l;                   // (a NaN stays one; no row: 0)
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float v = g == 0 ? o[i][0] : g == 1 ? o[i][1] : g == 2 ? o[i][2] : o[i][3];
+    x[i] = (v + off[0] + om) * inv;
+  }
+  const int head = kvh * kGroup + h, dim = 32 * g + 8 * j;
+  if (n_splits == 1) {
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+    *reinterpret_cast<u32x4*>(a.out + (long)b * a.o_sb + (long)head * a.o_sh + dim) = w;
+    if (a.lse != nullptr && g == 0 && j == 0)
+      a.lse[(long)b * kHeadsQ + head] = l > 0.f ? (m_run + __log2f(l)) * 0.69314718055994531f : l == 0.f ? -INFINITY : l;
+    return;
+  }
+  // Partials as the bf16 decode's: fp16 of the split's output, over a power of two that fits its largest value (F16Range)
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i]));
+  amax = fmaxf(amax, dpp<kDppXor1>(amax));
+  amax = fmaxf(amax, dpp<kDppXor2>(amax));
+  amax = max_xor32(max_xor16(amax));
+  const F16Range range(amax);
+  typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+  f16x8 w;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = (_Float16)(x[i] * range.inv);
+  const long at = ((long)b * a.max_splits + split) * kHeadsQ + head;
+  *reinterpret_cast<f16x8*>(a.part_o + at * kHeadDim + dim) = w;
+  if (g == 0 && j == 0) *reinterpret_cast<floatx4*>(a.part_ml + at * 4) = floatx4{m_run, l, range.scale, 0.f};
+}
+
+// Joins the splits of a sequence: workgroup (head, sequence), 16 groups of 16 lanes take the splits k = i, i + 16, ..., a lane 8
+// dims; their sums meet in LDS.
+__global__ __launch_bounds__(256) void decode4_merge_kernel(Decode4Args a) {
+  const int head = blockIdx.x, b = blockIdx.y;
+  const int n = splits_of(a, rows_of(a, b));
+  if (n == 1) return;
+  const int grp = threadIdx.x >> 4, c = threadIdx.x & 15;
+  typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+  const long at = (long)b * a.max_splits * kHeadsQ + head;
+  float M = -INFINITY, L = 0.f, acc[8] = {};
+#pragma unroll 4
+  for (int k = grp; k < n; k += 16) {
+    const floatx4 rec = *reinterpret_cast<const floatx4*>(a.part_ml + (at + (long)k * kHeadsQ) * 4);
+    const f16x8 v = *reinterpret_cast<const f16x8*>(a.part_o + (at + (long)k * kHeadsQ) * kHeadDim + 8 * c);
+    const float mn = fmaxf(M, rec[0]);
+    const float alpha = mn == -INFINITY ? 1.f : fast_exp2(M - mn);
+    const float w = mn == -INFINITY ? rec[1] : fast_exp2(rec[0] - mn) * rec[1];
+    L = L * alpha + w;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] = acc[i] * alpha + (float)v[i] * (w * rec[2]);
+    M = mn;
+  }
+  __shared__ float sm[16], sl[16], so[16][kHeadDim + 4];
+  if (c == 0) {
+    sm[grp] = M;
+    sl[grp] = L;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) so[grp][8 * c + i] = acc[i];
+  __syncthreads();
+  if (threadIdx.x >= kHeadDim) return;
+  M = -INFINITY;
+  L = 0.f;
+  float x = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) M = fmaxf(M, sm[i]);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float f = sm[i] == M ? 1.f : fast_exp2(sm[i] - M);
+    L += sl[i] * f;
+    x += so[i][threadIdx.x] * f;
+  }
+  a.out[(long)b * a.o_sb + (long)head * a.o_sh + threadIdx.x] = (__bf16)(L == 0.f ? 0.f : x / L);
+  if (a.lse != nullptr && threadIdx.x == 0)
+    a.lse[(long)b * kHeadsQ + head] = L > 0.f ? (M + __log2f(L)) * 0.69314718055994531f : L == 0.f ? -INFINITY : L;
+}
+
+// -- pages widened for the multi-query kernel -----------------------------------------------------------------------------
+// Workgroup per page of a request: the page in bf16 ([2][16][8][128]), and its place in the requests' table of such pages.
+// starts [R + 1]: first widened page of each request. A value m + s c is rounded to bf16 (2^-8 of it), as the multi-query
+// kernel's tiles hold them.
+__global__ __launch_bounds__(512) void widen4_kernel(const char* cache, int num_pages, const int32_t* block_table, long bt_stride,
+                                                     const int32_t* starts, int num_requests, __bf16* pages, int32_t* table,
+                                                     int table_width) {
+  const int p = blockIdx.x;
+  int r = 0;
+  while (r + 1 < num_requests && p >= starts[r + 1]) ++r;
+  const int i = p - starts[r];
+  if (threadIdx.x == 0) table[(long)r * table_width + i] = p;
+  const char* from = cache + (long)min(max(block_table[(long)r * bt_stride + i], 0), num_pages - 1) * kPage4;
+  __bf16* to = pages + (long)p * kPageElems;
+  // thread: 8 dims of a head, of every fourth slot
+  const int b = threadIdx.x & 15, h = (threadIdx.x >> 4) & 7;
+#pragma unroll
+  for (int n = 0; n < 8; ++n) {
+    const int row = 4 * n + (threadIdx.x >> 7), half = row >> 4, slot = row & 15;      // of the page's 32
+    const char* s = from + half * kHalf4 + slot * kSlot4;
+    float x[8];
+    values8(reinterpret_cast<const uint32_t*>(s + h * kHeadCodes4)[code_word(b)],
+            reinterpret_cast<const uint32_t*>(s + kParams4 + h * 16)[b >> 2], x);
+    u32x4 w;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = pack_bf16x2(x[2 * k], x[2 * k + 1]);
+    *reinterpret_cast<u32x4*>(to + half * kHalfElems + slot * kSlotElems + h * kHeadDim + 8 * b) = w;
+  }
+}
+
+}  // namespace abkv
+
+using namespace abkv;
+
+static bool rows16_ok(const void* p, long st, long sh) {
+  return p != nullptr && ((uintptr_t)p & 15) == 0 && ((st | sh) & 7) == 0;
+}
+
+extern "C" {
+
+int abkv_kv_append_int4(const void* key, long key_stride_t, long key_stride_h, const void* value, long value_stride_t,
+                        long value_stride_h, const int64_t* slot_mapping, int num_tokens, void* kv_cache, int num_pages,
+                        hipStream_t stream) {
+  if (num_tokens <= 0) return 0;
+  if (!rows16_ok(key, key_stride_t, key_stride_h) || !rows16_ok(value, value_stride_t, value_stride_h) ||
+      slot_mapping == nullptr || !rows16_ok(kv_cache, 0, 0) || num_pages <= 0)
+    return (int)hipErrorInvalidValue;
+  const Append4Args a = {static_cast<const __bf16*>(key), key_stride_t, key_stride_h, static_cast<const __bf16*>(value),
+                         value_stride_t, value_stride_h, slot_mapping, static_cast<char*>(kv_cache), num_pages};
+  hipLaunchKernelGGL(kv_append4_kernel, dim3(num_tokens), dim3(256), 0, stream, a);
+  return (int)hipGetLastError();
+}
+
+int abkv_kv_read_int4(const void* kv_cache, int num_pages, const int64_t* slot_mapping, int num_tokens, int f32, void* key,
+                      void* value, hipStream_t stream) {
+  if (num_tokens <= 0) return 0;
+  if (!rows16_ok(kv_cache, 0, 0) || num_pages <= 0 || slot_mapping == nullptr || !rows16_ok(key, 0, 0) || !rows16_ok(value, 0, 0))
+    return (int)hipErrorInvalidValue;
+  const char* cache = static_cast<const char*>(kv_cache);
+  if (f32)
+    hipLaunchKernelGGL(kv_read4_kernel<float>, dim3(num_tokens), dim3(256), 0, stream, cache, num_pages, slot_mapping,
+                       static_cast<float*>(key), static_cast<float*>(value));
+  else
+    hipLaunchKernelGGL(kv_read4_kernel<__bf16>, dim3(num_tokens), dim3(256), 0, stream, cache, num_pages, slot_mapping,
+                       static_cast<__bf16*>(key), static_cast<__bf16*>(value));
+  return (int)hipGetLastError();
+}
+
+size_t abkv_decode_int4_workspace_size(int num_seqs, int max_pages_per_seq, int split_pages) {
+  if (num_seqs <= 0 || max_pages_per_seq <= 0 || split_pages <= 0) return 0;
+  const int splits = (max_pages_per_seq + split_pages - 1) / split_pages;
+  return splits > 1 ? (size_t)num_seqs * splits * kHeadsQ * (kHeadDim * sizeof(_Float16) + 4 * sizeof(float)) : 0;
+}
+
+int abkv_decode_attn_int4(const void* q, long q_stride_seq, long q_stride_head, const void* kv_cache, int num_pages,
+                          const int32_t* block_table, long block_table_stride, const int32_t* seq_lens, int num_seqs,
+                          int max_pages_per_seq, int split_pages, float scale, void* out, long out_stride_seq,
+                          long out_stride_head, float* lse, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  if (num_seqs <= 0) return 0;
+  if (split_pages <= 0 || (split_pages & 1) || split_pages > 64 || max_pages_per_seq <= 0 || max_pages_per_seq > (1 << 26) ||
+      num_pages <= 0 || block_table_stride < max_pages_per_seq || num_seqs > 65535 || !softmax_scale_ok(scale) ||
+      !rows16_ok(q, q_stride_seq, q_stride_head) || !rows16_ok(kv_cache, 0, 0) || block_table == nullptr ||
+      seq_lens == nullptr || !rows16_ok(out, out_stride_seq, out_stride_head))
+    return (int)hipErrorInvalidValue;
+  const size_t need = abkv_decode_int4_workspace_size(num_seqs, max_pages_per_seq, split_pages);
+  if (need > 0 && (!rows16_ok(workspace, 0, 0) || workspace_bytes < need)) return (int)hipErrorInvalidValue;
+  Decode4Args a;
+  a.q = static_cast<const __bf16*>(q);
+  a.q_sb = q_stride_seq;
+  a.q_sh = q_stride_head;
+  a.kv = static_cast<const char*>(kv_cache);
+  a.num_pages = num_pages;
+  a.block_table = block_table;
+  a.bt_stride = block_table_stride;
+  a.seq_lens = seq_lens;
+  a.split_pages = split_pages;
+  a.max_splits = (max_pages_per_seq + split_pages - 1) / split_pages;
+  a.max_pages = max_pages_per_seq;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.out = static_cast<__bf16*>(out);
+  a.o_sb = out_stride_seq;
+  a.o_sh = out_stride_head;
+  a.lse = lse;
+  a.part_o = static_cast<_Float16*>(workspace);
+  a.part_ml = reinterpret_cast<float*>(a.part_o + (size_t)num_seqs * a.max_splits * kHeadsQ * kHeadDim);
+  hipLaunchKernelGGL(decode4_kernel, dim3(a.max_splits, num_seqs), dim3(64 * kHeadsKV), 0, stream, a);
+  const hipError_t err = hipGetLastError();
+  if (err != hipSuccess || a.max_splits == 1) return (int)err;
+  hipLaunchKernelGGL(decode4_merge_kernel, dim3(kHeadsQ, num_seqs), dim3(256), 0, stream, a);
+  return (int)hipGetLastError();
+}
+
+int abkv_kv_widen_int4(const void* kv_cache, int num_pages, const int32_t* block_table, long block_table_stride,
+                       const int32_t* page_starts, int num_requests, int total_pages, void* pages, int32_t* table,
+                       int table_width, hipStream_t stream) {
+  if (num_requests <= 0 || total_pages <= 0) return 0;
+  if (!rows16_ok(kv_cache, 0, 0) || num_pages <= 0 || block_table == nullptr || page_starts == nullptr || !rows16_ok(pages, 0, 0) ||
+      table == nullptr || table_width <= 0 || total_pages > 0x007fffff)
+    return (int)hipErrorInvalidValue;
+  hipLaunchKernelGGL(widen4_kernel, dim3(total_pages), dim3(512), 0, stream, static_cast<const char*>(kv_cache), num_pages,
+                     block_table, block_table_stride, page_starts, num_requests, static_cast<__bf16*>(pages), table, table_width);
+  return (int)hipGetLastError();
+}
+
+}  // extern "C"

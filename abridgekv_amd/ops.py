@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+from typing import NamedTuple
 
 import numpy as np
 import torch
@@ -227,10 +228,25 @@ def _decode_attention_f32(q, kv_cache, block_table, seq_lens, scale, max_pages, 
     return out, lse
 
 
+_BF16_ROWS = (PAGE, PAGE_BYTES, HALF_BYTES, SLOT_BYTES)
+
+
+def _row_geometry(layer_caches):
+    """(slots, page, half and slot bytes) of the caches that a move's rows lie in: bf16 or 4 bits, all alike."""
+    if not any(is_int4_cache(c) for c in layer_caches):
+        return _BF16_ROWS
+    _require(all(is_int4_cache(c) for c in layer_caches), "rows move among caches of one kind")
+    return (PAGE, 2 * PAGE * SLOT4_BYTES, PAGE * SLOT4_BYTES, SLOT4_BYTES)
+
+
 def _layer_ptrs(layer_caches):
     _require(0 < len(layer_caches) <= 16, "between 1 and 16 layer caches per launch")
     for c in layer_caches:
-        _check_cache(c)
+        if is_int4_cache(c):
+            _check_cache4(c)
+            _require(c.is_cuda, "kv_cache must be on the GPU")
+        else:
+            _check_cache(c)
     _require(len({c.shape[0] for c in layer_caches}) == 1, "layer caches of one launch must have equal page counts")
     arr = (C.c_void_p * len(layer_caches))(*[c.data_ptr() for c in layer_caches])
     return arr, layer_caches[0].shape[0]
@@ -247,7 +263,7 @@ def kv_move_segments(layer_caches, ops: torch.Tensor, seg_offsets: torch.Tensor)
     if n_seg <= 0 or ops.shape[0] == 0:
         return
     arr, num_pages = _layer_ptrs(layer_caches)
-    rc = lib().abkv_kv_move_segments(arr, len(layer_caches), num_pages, PAGE, PAGE_BYTES, HALF_BYTES, SLOT_BYTES, _ptr(ops),
+    rc = lib().abkv_kv_move_segments(arr, len(layer_caches), num_pages, *_row_geometry(layer_caches), _ptr(ops),
                                      _ptr(seg_offsets), n_seg, _stream())
     check(rc, "abkv_kv_move_segments")
 
@@ -262,7 +278,7 @@ class _MoveGroup(C.Structure):
 def kv_move_groups(groups) -> None:
     """abkv_kv_move_groups: the moves of several KV-cache groups in one launch (per 8 groups). ``groups``: a list of
     (layer caches, ops, seg_offsets, free_ops) as :func:`kv_move_mixed` takes them. Groups that share layer caches must
-    not touch each other's slots (a planner step's groups own disjoint pages)."""
+    not touch each other's slots (a planner step's groups own disjoint pages). The caches are all bf16 or all in 4 bits."""
     table = (_MoveGroup * len(groups))()
     n, arrays = 0, []
     for layer_caches, ops, seg_offsets, free_ops in groups:
@@ -283,7 +299,8 @@ def kv_move_groups(groups) -> None:
         n += 1
     if n == 0:
         return
-    rc = lib().abkv_kv_move_groups(C.byref(table), n, PAGE, PAGE_BYTES, HALF_BYTES, SLOT_BYTES, _stream())
+    geometry = _row_geometry([c for group in groups for c in group[0]])
+    rc = lib().abkv_kv_move_groups(C.byref(table), n, *geometry, _stream())
     check(rc, "abkv_kv_move_groups")
 
 
@@ -302,13 +319,13 @@ def kv_copy_staged(layer_caches, ops: torch.Tensor, stage: torch.Tensor | None =
     if n == 0:
         return
     arr, num_pages = _layer_ptrs(layer_caches)
-    need = lib().abkv_kv_stage_bytes(len(layer_caches), n, SLOT_BYTES)
+    geometry = _row_geometry(layer_caches)
+    need = lib().abkv_kv_stage_bytes(len(layer_caches), n, geometry[3])
     if stage is None:
         stage = torch.empty(need, dtype=torch.uint8, device=ops.device)
     nbytes = stage.numel() * stage.element_size()
     _require(nbytes >= need, "stage buffer too small")
-    rc = lib().abkv_kv_copy_staged(arr, len(layer_caches), num_pages, PAGE, PAGE_BYTES, HALF_BYTES, SLOT_BYTES, _ptr(ops), n,
-                                   _ptr(stage), nbytes, _stream())
+    rc = lib().abkv_kv_copy_staged(arr, len(layer_caches), num_pages, *geometry, _ptr(ops), n, _ptr(stage), nbytes, _stream())
     check(rc, "abkv_kv_copy_staged")
 
 
@@ -1122,14 +1139,15 @@ def window_backward(q, k, v, out, lse, dout, window, sinks, seq_lens, scale, out
     return dq, dk, dv
 
 
-def _check_paged(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor) -> tuple[int, int, int]:
+def _check_paged(q: torch.Tensor, kv_cache: torch.Tensor | None, block_table: torch.Tensor) -> tuple[int, int, int]:
     """bf16 query rows [T, 32, 128], a layer cache and its page table; (T, the table's rows and width)."""
     T = q.shape[0] if q.dim() else 0
     _check_rows("q", q, torch.bfloat16, (T, HEADS_Q, HEAD_DIM))
-    shape = kv_cache.shape
-    if (kv_cache.dtype is not torch.bfloat16 or len(shape) != 5 or shape[1:] != _PAGE_SHAPE or shape[0] == 0
-            or not kv_cache.is_contiguous()):
-        raise ValueError(f"kv_cache must be contiguous bf16 [P, 2, {PAGE}, {HEADS_KV}, {HEAD_DIM}]")
+    if kv_cache is not None:
+        shape = kv_cache.shape
+        if (kv_cache.dtype is not torch.bfloat16 or len(shape) != 5 or shape[1:] != _PAGE_SHAPE or shape[0] == 0
+                or not kv_cache.is_contiguous()):
+            raise ValueError(f"kv_cache must be contiguous bf16 [P, 2, {PAGE}, {HEADS_KV}, {HEAD_DIM}]")
     shape = block_table.shape
     if block_table.dtype is not torch.int32 or len(shape) != 2 or shape[1] == 0 or block_table.stride(1) != 1:
         raise ValueError("block_table must be int32 [B, W] with contiguous rows")
@@ -1208,7 +1226,8 @@ def window_split_pages(num_seqs: int, max_pages: int, window: int, sinks: int) -
 
 
 def _check_step(q, kv_cache, block_table, seq_lens, max_pages, split_pages, out, lse):
-    """Checks of a decode step's arguments but their device; (sequences, bound on their pages)."""
+    """Checks of a decode step's arguments but their device (``kv_cache`` None: checked by the caller); (sequences, bound on
+    their pages)."""
     B, rows, W = _check_paged(q, kv_cache, block_table)
     if rows < B or B > 65535:
         raise ValueError("block_table must have a row per sequence (at most 65535)")
@@ -1433,6 +1452,340 @@ def kv_evict(layer_caches, block_table: torch.Tensor, seq_lens: torch.Tensor, sc
                              _ptr(scores), _ptr(positions), scores.shape[3], _ptr(num_tokens), budget, sinks, recent,
                              _ptr(out), _ptr(workspace), ws_bytes, _stream())
     check(rc, "abkv_kv_evict")
+    return out
+
+
+# -- a cache in 4 bits -------------------------------------------------------------------------------------------------------
+SLOT4_BYTES = HEADS_KV * 80                    # one slot of K (or V) of one layer: 8 x 64 bytes of codes, 8 x 4 bf16 pairs
+_PAGE4_SHAPE = (2, PAGE, SLOT4_BYTES)
+
+
+def kv_cache_int4_shape(num_pages: int) -> tuple[int, ...]:
+    """Layer cache shape [num_pages, 2, 16, 640] uint8 of a cache in 4 bits: per (slot, head) and 32 dims a bf16 step and minimum
+    and 32 codes, 80 bytes a head row (bf16: 256)."""
+    return (num_pages, *_PAGE4_SHAPE)
+
+
+def is_int4_cache(kv_cache: torch.Tensor) -> bool:
+    return kv_cache.dtype == torch.uint8
+
+
+def _check_cache4(kv_cache: torch.Tensor) -> None:
+    shape = kv_cache.shape
+    if (kv_cache.dtype is not torch.uint8 or len(shape) != 4 or shape[1:] != _PAGE4_SHAPE or shape[0] == 0
+            or not kv_cache.is_contiguous() or kv_cache.data_ptr() % 16):
+        raise ValueError(f"kv_cache must be contiguous, 16-byte aligned uint8 [P, 2, {PAGE}, {SLOT4_BYTES}]")
+
+
+def _check_slots(slot_mapping: torch.Tensor, T: int) -> None:
+    _require(slot_mapping.dtype == torch.int64 and slot_mapping.shape == (T,) and slot_mapping.is_contiguous(),
+             f"slot_mapping must be contiguous int64 [{T}]")
+
+
+def kv_append_int4(key: torch.Tensor, value: torch.Tensor, slot_mapping: torch.Tensor, kv_cache: torch.Tensor) -> None:
+    """:func:`kv_append` into a cache in 4 bits: key/value [T, 8, 128] bf16 rows (contiguous, 16-byte aligned dims) are quantised
+    and written at slot_mapping [T] int64 (negative = skip; no slot twice). Per 32 dims the minimum is kept (in bf16, exactly),
+    the step is (max - min) / 15 rounded to bf16, and a code is the nearest of 16; a group of 32 with a value that is not finite
+    reads as NaN."""
+    T = slot_mapping.numel()
+    for name, t in (("key", key), ("value", value)):
+        _check_rows(name, t, torch.bfloat16, (T, HEADS_KV, HEAD_DIM))
+    _check_slots(slot_mapping, T)
+    _check_cache4(kv_cache)
+    _check_device(key, value, slot_mapping, kv_cache)
+    if T == 0:
+        return
+    rc = lib().abkv_kv_append_int4(key.data_ptr(), *key.stride()[:2], value.data_ptr(), *value.stride()[:2],
+                                   slot_mapping.data_ptr(), T, kv_cache.data_ptr(), kv_cache.shape[0], _stream())
+    check(rc, "abkv_kv_append_int4")
+
+
+def kv_read_int4(kv_cache: torch.Tensor, slot_mapping: torch.Tensor,
+                 dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
+    """The values (key, value) [T, 8, 128] that slots [T] int64 of a cache in 4 bits stand for, fp32 or bf16; zeros for a slot
+    outside the cache."""
+    _require(dtype in (torch.float32, torch.bfloat16), "rows are read as float32 or bfloat16")
+    T = slot_mapping.numel()
+    _check_slots(slot_mapping, T)
+    _check_cache4(kv_cache)
+    _check_device(slot_mapping, kv_cache)
+    key, value = (torch.empty((T, HEADS_KV, HEAD_DIM), dtype=dtype, device=kv_cache.device) for _ in range(2))
+    if T:
+        rc = lib().abkv_kv_read_int4(kv_cache.data_ptr(), kv_cache.shape[0], slot_mapping.data_ptr(), T,
+                                     int(dtype == torch.float32), key.data_ptr(), value.data_ptr(), _stream())
+        check(rc, "abkv_kv_read_int4")
+    return key, value
+
+
+def int4_split_pages(num_seqs: int, max_pages: int) -> int:
+    """Pages per split of a decode over a cache in 4 bits."""
+    total = num_seqs * max_pages
+    most = min(64, max(4, -(-total // 1024) * 2))
+    splits = -(-max_pages // most)
+    return -(-max_pages // (2 * splits)) * 2
+
+
+def decode_int4_bytes(num_seqs: int, max_pages: int, split_pages: int) -> int:
+    """Workspace bytes that :func:`decode_attention_int4` takes with ``split_pages`` pages a split."""
+    return lib().abkv_decode_int4_workspace_size(num_seqs, max_pages, split_pages)
+
+
+def decode_int4_workspace(num_seqs: int, max_pages: int, split_pages: int | None = None, device=None) -> torch.Tensor | None:
+    """Workspace for :func:`decode_attention_int4` of the same sizes (None when no sequence can need a second split)."""
+    n = decode_int4_bytes(num_seqs, max_pages, split_pages or int4_split_pages(num_seqs, max_pages))
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+
+
+def decode_attention_int4(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                          scale: float | None = None, max_pages: int | None = None, out: torch.Tensor | None = None,
+                          lse: torch.Tensor | None = None, split_pages: int | None = None,
+                          workspace: torch.Tensor | None = None):
+    """:func:`decode_attention` over a cache in 4 bits (:func:`kv_cache_int4_shape`): q [B, 32, 128] bf16; returns
+    (out [B, 32, 128] bf16, lse [B, 32] fp32 or None). The codes enter the products exactly; a weight times its row's step is
+    rounded to bf16. Slots behind a sequence's rows may hold anything. ``split_pages`` None: chosen by the sizes."""
+    scale = _softmax_scale(scale)
+    _check_cache4(kv_cache)
+    B, max_pages = _check_step(q, None, block_table, seq_lens, max_pages, split_pages, out, lse)
+    _check_device(q, kv_cache, block_table, seq_lens, out, lse)
+    if out is None:
+        out = q.new_empty((B, HEADS_Q, HEAD_DIM))
+    split_pages = split_pages or int4_split_pages(B, max_pages)
+    need = lib().abkv_decode_int4_workspace_size(B, max_pages, split_pages)
+    workspace, ws_bytes = _take_workspace(workspace, need, q.device)
+    rc = lib().abkv_decode_attn_int4(_ptr(q), q.stride(0), q.stride(1), _ptr(kv_cache), kv_cache.shape[0], _ptr(block_table),
+                                     _row_stride(block_table), _ptr(seq_lens), B, max_pages, split_pages, scale, _ptr(out),
+                                     out.stride(0), out.stride(1), _ptr(lse), _ptr(workspace), ws_bytes, _stream())
+    check(rc, "abkv_decode_attn_int4")
+    return out, lse
+
+
+def paged_prefill_attention_int4(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, q_start, kv_start,
+                                 kv_limit, causal, scale: float | None = None, out: torch.Tensor | None = None,
+                                 lse: torch.Tensor | None = None, excluded=None):
+    """:func:`paged_prefill_attention` (prompt chunks and code steps; bf16 queries) over a cache in 4 bits, whose values the
+    tiles hold in bf16. Returns (out [T, 32, 128] bf16, lse [T, 32] fp32 or None)."""
+    _check_cache4(kv_cache)
+    _check_rows("q", q, torch.bfloat16, (q.shape[0] if q.dim() else 0, HEADS_Q, HEAD_DIM))
+    _require(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[1] > 0
+             and block_table.stride(1) == 1, "block_table must be int32 [B, W] with contiguous rows")
+    scale = _softmax_scale(scale)
+    qs, kl = np.asarray(q_start, dtype=np.int64), np.asarray(kv_limit, dtype=np.int64)
+    R, W = kl.size, block_table.shape[1]
+    _require(kl.ndim == 1 and R <= block_table.shape[0] and (R == 0 or (kl.min() >= 0 and kl.max() <= W * PAGE)),
+             "kv_limit must lie in [0, block_table width * 16], one for each of at most the table's rows")
+    _check_device(q, kv_cache, block_table, out, lse)
+    starts = np.concatenate([[0], np.cumsum(-(-kl // PAGE))])
+    total, width = int(starts[-1]), max(1, int((-(-kl // PAGE)).max(initial=0)))
+    pages = torch.empty((max(1, total), *_PAGE_SHAPE), dtype=torch.bfloat16, device=q.device)
+    table = torch.empty((max(1, R), width), dtype=torch.int32, device=q.device)
+    if total:
+        meta = _upload([starts], q.device)
+        rc = lib().abkv_kv_widen_int4(kv_cache.data_ptr(), kv_cache.shape[0], block_table.data_ptr(), _row_stride(block_table),
+                                      meta.data_ptr(), R, total, pages.data_ptr(), table.data_ptr(), width, _stream())
+        check(rc, "abkv_kv_widen_int4")
+    return paged_prefill_attention(q, pages, table, qs, kv_start, kl, causal, scale, out=out, lse=lse, excluded=excluded)
+
+
+# -- per-head norms and the rotation in one pass ---------------------------------------------------------------------------------
+def _check_weights(q_weight, k_weight, dtype) -> int:
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        _require(w.dtype in (dtype, torch.float32) and w.shape == (HEAD_DIM,) and w.is_contiguous() and w.data_ptr() % 16 == 0,
+                 f"{name} must be contiguous [128], {dtype} or float32")
+    _require(q_weight.dtype == k_weight.dtype, "the norms' weights must have one type")
+    return int(q_weight.dtype == torch.float32)
+
+
+def _check_eps(eps) -> float:
+    eps = float(eps)
+    _require(0 <= eps < math.inf, "eps must be finite and not negative")
+    return eps
+
+
+def qk_norm_rope_append(q: torch.Tensor, key: torch.Tensor, value: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor,
+                        slot_mapping: torch.Tensor, kv_cache: torch.Tensor, q_weight: torch.Tensor | None = None,
+                        k_weight: torch.Tensor | None = None, eps: float = 1e-6, block_c: int = 0, codes_k: int = 0,
+                        max_position: int | None = None, code_span: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """A serving step's RMS norms of queries and keys for each head, rotation and append in one pass: returns the rotated
+    queries [T, 32, 128]; the rotated keys and the values go to slot_mapping [T] int64 (negative = skip; no slot twice) of
+    ``kv_cache``, bf16 or in 4 bits (:func:`kv_cache_int4_shape`; the row that the bf16 cache would hold, quantised).
+
+    q [T, 32, 128], key/value [T, 8, 128] bf16 (any strides with contiguous, 16-byte aligned dims) stay as they are; ``out`` may
+    be q. q_weight / k_weight [128]: bf16 or fp32, or None for both: no norms. A row is rounded to bf16 once, after the rotation
+    (the modules one after the other round after the norm, after its weight and after the rotation). positions, cos_sin,
+    block_c, codes_k, code_span and max_position as in :func:`rope_kv_append`."""
+    T = positions.numel()
+    _check_rows("q", q, torch.bfloat16, (T, HEADS_Q, HEAD_DIM))
+    for name, t in (("key", key), ("value", value)):
+        _check_rows(name, t, torch.bfloat16, (T, HEADS_KV, HEAD_DIM))
+    _require(positions.dtype == torch.int64 and positions.is_contiguous(), "positions must be contiguous int64 [T]")
+    _require(cos_sin.dtype == torch.float32 and cos_sin.dim() == 2 and cos_sin.shape[1] == HEAD_DIM and cos_sin.shape[0] > 0
+             and cos_sin.is_contiguous() and cos_sin.data_ptr() % 16 == 0, "cos_sin must be contiguous fp32 [P, 128]")
+    _check_slots(slot_mapping, T)
+    int4 = is_int4_cache(kv_cache)
+    if int4:
+        _check_cache4(kv_cache)
+    else:
+        _check_cache(kv_cache)
+        _require(kv_cache.shape[0] > 0, "kv_cache must have pages")
+    _require((q_weight is None) == (k_weight is None), "norm weights are given for queries and keys, or for neither")
+    wf32 = 0 if q_weight is None else _check_weights(q_weight, k_weight, torch.bfloat16)
+    eps = _check_eps(eps)
+    if block_c:
+        _require(block_c > 0 and codes_k > 0 and codes_k & (codes_k - 1) == 0 and codes_k <= block_c,
+                 "codes_k must be a power of two <= block_c")
+        _require(code_span == 0 or codes_k <= code_span <= block_c, "code_span must be 0 or in [codes_k, block_c]")
+    if out is None:
+        out = torch.empty((T, HEADS_Q, HEAD_DIM), dtype=torch.bfloat16, device=q.device)
+    else:
+        _check_out(out, torch.bfloat16, (T, HEADS_Q, HEAD_DIM))
+    _check_device(q, key, value, positions, cos_sin, slot_mapping, kv_cache, q_weight, k_weight, out)
+    if T == 0:
+        return out
+    bound = rope_bound(int(positions.max()) if max_position is None else max_position, block_c, codes_k)
+    if bound >= cos_sin.shape[0]:
+        raise ValueError(f"RoPE positions up to {bound} exceed the cos/sin table ({cos_sin.shape[0]} rows)")
+    rc = lib().abkv_qk_norm_rope_append(q.data_ptr(), *q.stride()[:2], key.data_ptr(), *key.stride()[:2], value.data_ptr(),
+                                        *value.stride()[:2], positions.data_ptr(), T, _ptr(q_weight), _ptr(k_weight), wf32, eps,
+                                        int(block_c), int(codes_k), int(code_span), cos_sin.data_ptr(), cos_sin.shape[0],
+                                        slot_mapping.data_ptr(), kv_cache.data_ptr(), kv_cache.shape[0], int(int4),
+                                        out.data_ptr(), *out.stride()[:2], _stream())
+    check(rc, "abkv_qk_norm_rope_append")
+    return out
+
+
+def _norm_rope_args(q, k, cos, sin, q_weight, k_weight, eps):
+    """Checks of a training step's arguments; the entries' common ones before the outputs."""
+    _require(q.dim() == 4 and q.dtype in (torch.bfloat16, torch.float32), "q must be bf16 or fp32 [B, S, 32, 128]")
+    B, S = q.shape[:2]
+    _check_rows("q", q, q.dtype, (B, S, HEADS_Q, HEAD_DIM))
+    _check_rows("k", k, q.dtype, (B, S, HEADS_KV, HEAD_DIM))
+    wf32 = _check_weights(q_weight, k_weight, q.dtype)
+    n = cos.shape[0] if cos.dim() == 3 else 0
+    for name, t in (("cos", cos), ("sin", sin)):
+        st = t.stride()
+        _require(t.dtype in (torch.bfloat16, torch.float32) and t.dtype == cos.dtype and n in (1, B)
+                 and t.shape == (n, S, HEAD_DIM) and st == cos.stride() and st[2] == 1
+                 and (st[0] | st[1]) * t.element_size() % 16 == 0 and t.data_ptr() % 16 == 0,
+                 f"{name} must be bf16 or fp32 [1 or B, S, 128], both alike, with contiguous, 16-byte aligned rows")
+    st = cos.stride()
+    return (int(q.dtype == torch.float32), q, k, (B, S, q_weight.data_ptr(), k_weight.data_ptr(), wf32, _check_eps(eps),
+                                                  cos.data_ptr(), sin.data_ptr(), st[0] if n > 1 else 0, st[1],
+                                                  int(cos.dtype == torch.float32)))
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, q_weight: torch.Tensor,
+                 k_weight: torch.Tensor, eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
+    """RMS norms of queries and keys for each head and their rotation (NeoX halves) in one pass, as a training step takes them:
+    q [B, S, 32, 128], k [B, S, 8, 128] bf16 or fp32 (any strides with contiguous, 16-byte aligned dims), cos/sin
+    [1 or B, S, 128] as the models' rotary embedding returns them (two equal halves; bf16 or fp32), weights [128] of q's type or
+    fp32. Returns new dense (q, k) of the same type, rounded once. With gradients: :func:`abridgekv_amd.fused.qk_norm_rope`."""
+    f32, q, k, args = _norm_rope_args(q, k, cos, sin, q_weight, k_weight, eps)
+    _check_device(q, k, cos, sin, q_weight, k_weight)
+    q_out, k_out = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
+    rc = lib().abkv_qk_norm_rope(f32, q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], *args, q_out.data_ptr(),
+                                 k_out.data_ptr(), _stream())
+    check(rc, "abkv_qk_norm_rope")
+    return q_out, k_out
+
+
+def qk_norm_rope_backward(q: torch.Tensor, k: torch.Tensor, dq_out: torch.Tensor, dk_out: torch.Tensor, cos: torch.Tensor,
+                          sin: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, eps: float = 1e-6):
+    """Gradients (dq, dk, dq_weight, dk_weight) of sum(dq_out * q_out + dk_out * k_out) for :func:`qk_norm_rope`, of the inputs'
+    types. The weights' sums are fp32, in a fixed order."""
+    f32, q, k, args = _norm_rope_args(q, k, cos, sin, q_weight, k_weight, eps)
+    _check_rows("dq_out", dq_out, q.dtype, q.shape)
+    _check_rows("dk_out", dk_out, q.dtype, k.shape)
+    _check_device(q, k, dq_out, dk_out, cos, sin, q_weight, k_weight)
+    dq, dk = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
+    dwq, dwk = torch.empty_like(q_weight), torch.empty_like(k_weight)
+    if q.numel() == 0:
+        return dq, dk, dwq.zero_(), dwk.zero_()
+    n = lib().abkv_qk_norm_rope_bwd_workspace_size(*q.shape[:2])
+    ws = torch.empty(n, dtype=torch.uint8, device=q.device)
+    rc = lib().abkv_qk_norm_rope_bwd(f32, q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], dq_out.data_ptr(),
+                                     *dq_out.stride()[:3], dk_out.data_ptr(), *dk_out.stride()[:3], *args, dq.data_ptr(),
+                                     dk.data_ptr(), dwq.data_ptr(), dwk.data_ptr(), ws.data_ptr(), n, _stream())
+    check(rc, "abkv_qk_norm_rope_bwd")
+    return dq, dk, dwq, dwk
+
+
+# -- log probabilities of given tokens -------------------------------------------------------------------------------------------
+class TokenLogprobs(NamedTuple):
+    """What :func:`token_logprobs` returns: logprob and entropy [T] fp32 (entropy None where it was not asked for), the
+    alternatives' ids [T, top] int64 and log probabilities [T, top] fp32, and what the backward needs ([T, 3] fp32, or None)."""
+    logprob: torch.Tensor
+    entropy: torch.Tensor | None
+    top_ids: torch.Tensor
+    top_logprobs: torch.Tensor
+    stats: torch.Tensor | None
+
+
+TOP_MAX = 32
+
+
+def _check_logits(logits, targets, temperature) -> float:
+    _require(logits.dim() == 2 and logits.dtype in (torch.bfloat16, torch.float32) and logits.shape[1] > 0
+             and logits.stride(1) == 1 and (logits.shape[0] <= 1 or logits.stride(0) >= logits.shape[1]),
+             "logits must be bf16 or fp32 [T, V] with contiguous rows that do not overlap")
+    _require(targets.dtype == torch.int64 and targets.shape == logits.shape[:1] and targets.is_contiguous(),
+             "targets must be contiguous int64 [T]")
+    temperature = float(temperature)
+    _require(0 < temperature < math.inf, "temperature must be positive and finite")
+    return temperature
+
+
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, temperature: float = 1.0, top: int = 0, entropy: bool = True,
+                   stats: bool = False) -> TokenLogprobs:
+    """Log probabilities of given tokens under softmax(logits / temperature), in one read of the logits, with the
+    distribution's entropy and its ``top`` (0 .. 32) most likely tokens.
+
+    logits [T, V] bf16 or fp32 (rows of any alignment); targets [T] int64: outside [0, V) a row has no target and log probability
+    0. Alternatives in descending order (ties: the lowest id). Logits below -1e25 (-inf, a type's lowest value) have probability
+    0; a row without another, or with a NaN or +inf, is NaN. ``stats``: also what :func:`token_logprobs_backward` takes. fp32 sums; equal calls give equal
+    bits. With gradients: :func:`abridgekv_amd.fused.token_logprobs`."""
+    temperature = _check_logits(logits, targets, temperature)
+    T, V = logits.shape
+    top = int(top)
+    _require(0 <= top <= min(TOP_MAX, V), f"top must be in [0, {min(TOP_MAX, V)}]")
+    _check_device(logits, targets)
+    f32 = int(logits.dtype == torch.float32)
+    dev = logits.device
+    logprob = torch.empty(T, dtype=torch.float32, device=dev)
+    ent = torch.empty(T, dtype=torch.float32, device=dev) if entropy else None
+    st = torch.empty((T, 3), dtype=torch.float32, device=dev) if stats else None
+    ids = torch.empty((T, top), dtype=torch.int64, device=dev)
+    tops = torch.empty((T, top), dtype=torch.float32, device=dev)
+    if T:
+        n = lib().abkv_token_logprobs_workspace_size(T, V, f32, top)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+        rc = lib().abkv_token_logprobs(f32, logits.data_ptr(), logits.stride(0), T, V, targets.data_ptr(), temperature, top,
+                                       logprob.data_ptr(), _ptr(ent), _ptr(st), ids.data_ptr(), tops.data_ptr(), _ptr(ws), n,
+                                       _stream())
+        check(rc, "abkv_token_logprobs")
+    return TokenLogprobs(logprob, ent, ids, tops, st)
+
+
+def token_logprobs_backward(logits: torch.Tensor, targets: torch.Tensor, stats: torch.Tensor,
+                            dlogprob: torch.Tensor | None, dentropy: torch.Tensor | None = None, temperature: float = 1.0,
+                            out: torch.Tensor | None = None) -> torch.Tensor:
+    """Gradient [T, V] (of the logits' type) of sum(dlogprob * logprob + dentropy * entropy) for :func:`token_logprobs` with its
+    ``stats``; dlogprob, dentropy [T] fp32 or None. ``out`` may be the logits themselves."""
+    temperature = _check_logits(logits, targets, temperature)
+    T, V = logits.shape
+    _require(stats.dtype == torch.float32 and stats.shape == (T, 3) and stats.is_contiguous(), "stats must be contiguous fp32 [T, 3]")
+    for name, t in (("dlogprob", dlogprob), ("dentropy", dentropy)):
+        _require(t is None or (t.dtype == torch.float32 and t.shape == (T,) and t.is_contiguous()),
+                 f"{name} must be contiguous fp32 [T]")
+    if out is None:
+        out = torch.empty((T, V), dtype=logits.dtype, device=logits.device)
+    _require(out.dtype == logits.dtype and out.shape == (T, V) and out.stride(1) == 1 and (T <= 1 or out.stride(0) >= V),
+             "out must be [T, V] of the logits' type with contiguous rows that do not overlap")
+    _check_device(logits, targets, stats, dlogprob, dentropy, out)
+    if T:
+        rc = lib().abkv_token_logprobs_bwd(int(logits.dtype == torch.float32), logits.data_ptr(), logits.stride(0), T, V,
+                                           targets.data_ptr(), temperature, stats.data_ptr(), _ptr(dlogprob), _ptr(dentropy),
+                                           out.data_ptr(), out.stride(0), _stream())
+        check(rc, "abkv_token_logprobs_bwd")
     return out
 
 

@@ -525,6 +525,85 @@ int abkv_kv_evict(void* const* layer_caches, int num_layers, int num_pages, cons
                   int32_t* positions, long rows_stride, const int32_t* num_tokens, int budget, int sinks, int recent,
                   int32_t* out_lens, void* workspace, size_t workspace_bytes, abkv_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------------------------------
+ * Per-head RMS norms of queries and keys with the position rotation in the same pass. A head row x [128] of a token becomes
+ * the rotation (NeoX halves, as abkv_rope_kv_append) of weight * x / sqrt(mean(x^2) + eps); fp32 inside, one rounding at the
+ * end. The reference's models normalise with the layer's q_norm and k_norm modules and rotate in a call of its own.
+ * Weights [128] are bf16, or fp32 with weight_f32; every row is 16-byte aligned (strides in elements), every dense tensor too.
+ *
+ * Serving: q [T, 32, 128], key and value [T, 8, 128] bf16. Rotated queries go to q_out [T, 32, 128] (which may be q), the
+ * rotated keys and the values to the cache rows slot_mapping[t] (negative or past the cache: not written; no two the same),
+ * in bf16, or with int4 != 0 in 4 bits as abkv_kv_append_int4 would write them. Without weights (both NULL) the rows are only
+ * rotated. Positions and the layout's arguments as in abkv_rope_kv_append (positions past cos_sin are clamped to its last row). */
+int abkv_qk_norm_rope_append(const void* q, long q_stride_t, long q_stride_h, const void* key, long key_stride_t,
+                             long key_stride_h, const void* value, long value_stride_t, long value_stride_h,
+                             const int64_t* positions, int num_tokens, const void* q_weight, const void* k_weight,
+                             int weight_f32, float eps, int block_c, int codes_k, int code_span, const float* cos_sin,
+                             long max_pos, const int64_t* slot_mapping, void* kv_cache, int num_pages, int int4, void* q_out,
+                             long out_stride_t, long out_stride_h, abkv_stream_t stream);
+/* Training: q [batch, seq_len, 32, 128], k [batch, seq_len, 8, 128], bf16 or (f32 != 0) fp32; cos and sin [batch, seq_len, 128]
+ * (angle_stride_b 0: one for the batch; fp32 with angle_f32, else bf16), of whose rows the first 64 are read. q_out, k_out dense,
+ * of the inputs' type. */
+int abkv_qk_norm_rope(int f32, const void* q, long q_stride_b, long q_stride_s, long q_stride_h, const void* k,
+                      long k_stride_b, long k_stride_s, long k_stride_h, int batch, int seq_len, const void* q_weight,
+                      const void* k_weight, int weight_f32, float eps, const void* cos, const void* sin, long angle_stride_b,
+                      long angle_stride_s, int angle_f32, void* q_out, void* k_out, abkv_stream_t stream);
+/* Gradients of sum(dq_out * q_out + dk_out * k_out): dq, dk dense, of the inputs' type; dq_weight, dk_weight [128] of the
+ * weights' type (sums in a fixed order). workspace: abkv_qk_norm_rope_bwd_workspace_size bytes. */
+size_t abkv_qk_norm_rope_bwd_workspace_size(int batch, int seq_len);
+int abkv_qk_norm_rope_bwd(int f32, const void* q, long q_stride_b, long q_stride_s, long q_stride_h, const void* k,
+                          long k_stride_b, long k_stride_s, long k_stride_h, const void* dq_out, long dqo_stride_b,
+                          long dqo_stride_s, long dqo_stride_h, const void* dk_out, long dko_stride_b, long dko_stride_s,
+                          long dko_stride_h, int batch, int seq_len, const void* q_weight, const void* k_weight,
+                          int weight_f32, float eps, const void* cos, const void* sin, long angle_stride_b,
+                          long angle_stride_s, int angle_f32, void* dq, void* dk, void* dq_weight, void* dk_weight,
+                          void* workspace, size_t workspace_bytes, abkv_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------------------------
+ * A cache in 4 bits: [num_pages, 2 (K, V), 16 slots, 640 bytes], 16-byte aligned. A slot's row of K (or V) is 8 heads x 64 bytes
+ * of codes, then 8 heads x 4 pairs (step s, minimum m; bf16, step first), a pair for each 32 dims; a value is m + s code.
+ * Word 4 (b % 4) + b / 4 of a head's 16 holds dims 8 b .. + 7, dim d at bits 4 (d % 8 / 2) + 16 (d % 2).
+ * Rows move as any others: abkv_kv_move_groups and abkv_kv_copy_staged with page, half and slot bytes 20480, 10240 and 640.
+ *
+ * abkv_kv_append_int4: key / value rows [T, 8, 128] bf16 at slot_mapping (as abkv_kv_append; no two slots the same). m is the
+ * group's minimum, s = bf16((max - m) / 15), a code the nearest. A group with a value that is not finite reads as NaN. */
+int abkv_kv_append_int4(const void* key, long key_stride_t, long key_stride_h, const void* value, long value_stride_t,
+                        long value_stride_h, const int64_t* slot_mapping, int num_tokens, void* kv_cache, int num_pages,
+                        abkv_stream_t stream);
+/* Rows by slot as values [T, 8, 128], fp32 (f32 != 0) or bf16, dense; a slot outside the cache reads as zeros. */
+int abkv_kv_read_int4(const void* kv_cache, int num_pages, const int64_t* slot_mapping, int num_tokens, int f32, void* key,
+                      void* value, abkv_stream_t stream);
+/* abkv_decode_attn over a cache in 4 bits. workspace: abkv_decode_int4_workspace_size bytes, 16-byte aligned (0: none needed).
+ * num_seqs <= 65535. */
+size_t abkv_decode_int4_workspace_size(int num_seqs, int max_pages_per_seq, int split_pages);
+int abkv_decode_attn_int4(const void* q, long q_stride_seq, long q_stride_head, const void* kv_cache, int num_pages,
+                          const int32_t* block_table, long block_table_stride, const int32_t* seq_lens, int num_seqs,
+                          int max_pages_per_seq, int split_pages, float scale, void* out, long out_stride_seq,
+                          long out_stride_head, float* lse, void* workspace, size_t workspace_bytes, abkv_stream_t stream);
+/* Pages of a batch's requests in bf16: page i of request r (the first page_starts[r + 1] - page_starts[r] of its table row) goes
+ * to page page_starts[r] + i of `pages` [total_pages, 2, 16, 8, 128], and that number to table[r][i]: the cache and the page
+ * table that abkv_paged_prefill_attn_items then takes. page_starts [num_requests + 1] on the device, page_starts[0] = 0. */
+int abkv_kv_widen_int4(const void* kv_cache, int num_pages, const int32_t* block_table, long block_table_stride,
+                       const int32_t* page_starts, int num_requests, int total_pages, void* pages, int32_t* table,
+                       int table_width, abkv_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------------------------
+ * Log probabilities of given tokens: logits [num_tokens, vocab] bf16 or (f32 != 0) fp32, rows `stride` elements apart, of any
+ * alignment. With x = logits / temperature: logprob[t] = x[target] - logsumexp(x) (0 for a target outside [0, vocab)); entropy[t]
+ * (or NULL); the `top` (0 .. 32) highest logits' ids and log probabilities [num_tokens, top], ties by the lower id, NaN below
+ * every number; stats [num_tokens, 3] (or NULL): what the gradient needs. Logits below -1e25 (-inf, a type's lowest value) have
+ * probability 0; a row without another, or with a NaN or +inf, is NaN. workspace: abkv_token_logprobs_workspace_size bytes, 8-byte aligned (0: none).
+ * The reference takes its losses and scores from torch's cross entropy (abridgekv/compress_forward.py:957-1042). */
+size_t abkv_token_logprobs_workspace_size(int num_tokens, int vocab, int f32, int top);
+int abkv_token_logprobs(int f32, const void* logits, long stride, int num_tokens, int vocab, const int64_t* targets,
+                        float temperature, int top, float* logprob, float* entropy, float* stats, int64_t* top_ids,
+                        float* top_logprobs, void* workspace, size_t workspace_bytes, abkv_stream_t stream);
+/* dlogits = the gradient of sum(dlogprob * logprob + dentropy * entropy) (either NULL: zeros), rows grad_stride elements apart,
+ * of the logits' type; it may be the logits themselves. */
+int abkv_token_logprobs_bwd(int f32, const void* logits, long stride, int num_tokens, int vocab, const int64_t* targets,
+                            float temperature, const float* stats, const float* dlogprob, const float* dentropy, void* dlogits,
+                            long grad_stride, abkv_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
