@@ -19,7 +19,8 @@ reorder FlashInfer applies with decode threshold 1) and then multi-token request
   a retained tail the block's own tail rows hidden as a per-request excluded range (:2086-2094).
 
 New K/V rows are written by ``abkv_kv_append`` (``torch.ops.abridgekv.kv_append``) before attention
-(``reshape_and_cache`` semantics: slot < 0 skips).
+(``reshape_and_cache`` semantics: slot < 0 skips). A layer whose cache holds its rows in 4 bits (``kv_cache_dtype="int4"``)
+takes the same metadata through ``abkv_kv_append_int4``, ``abkv_decode_attn_int4`` and the multi-query form of them.
 """
 from __future__ import annotations
 
@@ -32,6 +33,12 @@ from . import ops
 from . import torch_ops  # noqa: F401  (torch.ops.abridgekv.*)
 
 NOT_CODE = -1
+
+
+def _int4_cache(kv_cache_dtype: str) -> bool:
+    if kv_cache_dtype not in ("auto", "bfloat16", "int4"):
+        raise NotImplementedError(f"kv cache dtype must be bf16 or int4, got {kv_cache_dtype!r}")
+    return kv_cache_dtype == "int4"
 
 
 @dataclass
@@ -190,10 +197,15 @@ class AbridgeMetadataBuilder:
     max_pages: int
     device: torch.device | str = "cuda"
     split_pages: int | None = None          # None: per step, ops.auto_split_pages of the decode requests' rows
+    kv_cache_dtype: str = "auto"            # "int4": the workspace holds every batch's splits of a decode over 4 bits
     _workspace: torch.Tensor | None = field(default=None, init=False, repr=False)
 
     def workspace(self) -> torch.Tensor:
-        if self._workspace is None:
+        if self._workspace is None and self.kv_cache_dtype == "int4":
+            n = max(ops.decode_int4_bytes(b, self.max_pages, ops.int4_split_pages(b, self.max_pages))
+                    for b in range(1, self.max_num_seqs + 1))
+            self._workspace = torch.empty(max(n, 16), dtype=torch.uint8, device=self.device)
+        elif self._workspace is None:
             sp = min(self.split_pages or ops.DEFAULT_SPLIT_PAGES, ops.DEFAULT_SPLIT_PAGES)
             self._workspace = ops.decode_workspace(self.max_num_seqs, self.max_pages, sp, device=self.device)
         return self._workspace
@@ -266,7 +278,8 @@ class AbridgeAttentionImpl:
     """Backend implementation for one attention layer (32 query heads, 8 KV heads, head size 128, bf16).
 
     ``sliding_window`` W: a token sees the W rows up to its own and the first ``sinks`` rows of its sequence; decodes then
-    read only the window's and the sinks' pages. Code steps see their whole context, so a windowed layer refuses them."""
+    read only the window's and the sinks' pages. Code steps see their whole context, so a windowed layer refuses them.
+    ``kv_cache_dtype`` "int4": the layer's cache holds its rows in 4 bits (``ops.kv_cache_int4_shape``)."""
 
     def __init__(self, num_heads: int = ops.HEADS_Q, head_size: int = ops.HEAD_DIM, scale: float | None = None,
                  num_kv_heads: int = ops.HEADS_KV, kv_cache_dtype: str = "auto", sliding_window: int | None = None,
@@ -274,8 +287,9 @@ class AbridgeAttentionImpl:
         if (num_heads, head_size, num_kv_heads) != (ops.HEADS_Q, ops.HEAD_DIM, ops.HEADS_KV):
             raise NotImplementedError(f"kernels are built for {ops.HEADS_Q} q heads, {ops.HEADS_KV} KV heads, "
                                       f"head size {ops.HEAD_DIM}")
-        if kv_cache_dtype not in ("auto", "bfloat16"):
-            raise NotImplementedError("kv cache dtype must be bf16")
+        self.int4 = _int4_cache(kv_cache_dtype)
+        if self.int4 and sliding_window is not None:
+            raise NotImplementedError("a sliding window runs over a bf16 cache")
         if sliding_window is None and sinks:
             raise ValueError("sinks need a sliding_window")
         if sliding_window is not None and (sliding_window < 1 or sinks < 0):
@@ -298,9 +312,9 @@ class AbridgeAttentionImpl:
         md = attn_metadata
         if key is not None:
             n = md.num_actual_tokens
-            torch.ops.abridgekv.kv_append(key.view(-1, self.num_kv_heads, self.head_size)[:n],
-                                          value.view(-1, self.num_kv_heads, self.head_size)[:n], md.slot_mapping[:n],
-                                          kv_cache)
+            append = torch.ops.abridgekv.kv_append_int4 if self.int4 else torch.ops.abridgekv.kv_append
+            append(key.view(-1, self.num_kv_heads, self.head_size)[:n],
+                   value.view(-1, self.num_kv_heads, self.head_size)[:n], md.slot_mapping[:n], kv_cache)
         self.attend(q, kv_cache, md, output.view(T, self.num_heads, self.head_size), output_lse)
         return output
 
@@ -310,7 +324,16 @@ class AbridgeAttentionImpl:
         if self.sliding_window is not None:
             return self._attend_window(q, kv_cache, md, out, lse)
         nd, nd_tok, n_tok = md.num_decodes, md.num_decode_tokens, md.num_actual_tokens
-        if nd:
+        if nd and self.int4:
+            # a builder of the bf16 cache holds splits of 32 pages; shorter ones where they fit too
+            pages, held = md.max_decode_pages, md.workspace.numel() if md.workspace is not None else 0
+            split = ops.int4_split_pages(nd, pages)
+            if ops.decode_int4_bytes(nd, pages, split) > held:
+                split = max(split, ops.DEFAULT_SPLIT_PAGES)
+            torch.ops.abridgekv.decode_attn_int4(q[:nd_tok], kv_cache, md.block_table[:nd], md.seq_lens_dev[:nd], self.scale,
+                                                 pages, split, out[:nd_tok], None if lse is None else lse[:nd_tok],
+                                                 md.workspace)
+        elif nd:
             torch.ops.abridgekv.decode_attn(q[:nd_tok], kv_cache, md.block_table[:nd], md.seq_lens_dev[:nd],
                                             self.scale, md.max_decode_pages, md.split_pages, out[:nd_tok],
                                             None if lse is None else lse[:nd_tok], md.workspace)
@@ -325,10 +348,9 @@ class AbridgeAttentionImpl:
             causal = md.causal & ~code
             if md.code_causal is not None:
                 causal = causal | (code & md.code_causal[nd:])
-            ops.paged_prefill_attention(q[nd_tok:n_tok], kv_cache, md.block_table[nd:], qsl, sl - qlen,
-                                        np.where(code, lim, sl), causal, self.scale,
-                                        out=out[nd_tok:n_tok], lse=None if lse is None else lse[nd_tok:n_tok],
-                                        excluded=ex)
+            attend = ops.paged_prefill_attention_int4 if self.int4 else ops.paged_prefill_attention
+            attend(q[nd_tok:n_tok], kv_cache, md.block_table[nd:], qsl, sl - qlen, np.where(code, lim, sl), causal, self.scale,
+                   out=out[nd_tok:n_tok], lse=None if lse is None else lse[nd_tok:n_tok], excluded=ex)
 
     def _attend_window(self, q, kv_cache, md: AbridgeAttentionMetadata, out, lse) -> None:
         """:meth:`attend` of a layer with a sliding window."""
@@ -369,13 +391,13 @@ class AbridgeAttentionBackend:
 
     @staticmethod
     def get_kv_cache_shape(num_blocks: int, block_size: int = ops.PAGE, num_kv_heads: int = ops.HEADS_KV,
-                           head_size: int = ops.HEAD_DIM) -> tuple[int, ...]:
+                           head_size: int = ops.HEAD_DIM, kv_cache_dtype: str = "auto") -> tuple[int, ...]:
         """[num_blocks, 2, block_size, num_kv_heads, head_size] (NHD), the layout the worker allocates once per
-        shared layer tensor (gpu_model_runner.py:1215-1217)."""
+        shared layer tensor (gpu_model_runner.py:1215-1217); "int4": [num_blocks, 2, block_size, 640] bytes."""
         if (block_size, num_kv_heads, head_size) != (ops.PAGE, ops.HEADS_KV, ops.HEAD_DIM):
             raise NotImplementedError(f"kernels are built for page {ops.PAGE}, {ops.HEADS_KV} KV heads, "
                                       f"head size {ops.HEAD_DIM}")
-        return ops.kv_cache_shape(num_blocks)
+        return ops.kv_cache_int4_shape(num_blocks) if _int4_cache(kv_cache_dtype) else ops.kv_cache_shape(num_blocks)
 
     @staticmethod
     def get_supported_head_sizes() -> list[int]:

@@ -28,16 +28,21 @@ content row i of the next block sees the block's last W - i content rows (the ro
 and the block's codes see their whole block.
 Gradients flow through the attention by the kernel's HIP backward (dq, dk, dv under the same mask), so the module
 trains.
+
+``CompressLM(fused_norms=True)`` runs the layers' per-head norms and their rotation as one kernel each way (one rounding for
+three; :func:`fuse_norms`), ``fused_ce=True`` takes the cross entropies from the logits as they are, without a float32 copy of them
+(``fused.token_logprobs``). Both are choices of the caller: without them the model's own modules run as before.
 """
 from __future__ import annotations
 
+import types
 from dataclasses import dataclass
 
 import torch
 import torch.nn.functional as F
 from torch import nn
 
-from . import ops
+from . import fused, ops
 from .config import bitrev_offsets
 
 ATTN_IMPLEMENTATION = "abridgekv_hip"
@@ -188,6 +193,32 @@ def register_attention() -> None:
     """Register ``"abridgekv_hip"`` with transformers' attention interface (idempotent)."""
     from transformers import AttentionInterface
     AttentionInterface.register(ATTN_IMPLEMENTATION, masked_attention_forward)
+
+
+def _fused_attention_forward(attn, hidden_states, position_embeddings, attention_mask=None, **kwargs):
+    """Forward of a decoder layer's attention with the norms and the rotation in one pass (:func:`fuse_norms`)."""
+    if kwargs.get("past_key_values") is not None or kwargs.get("past_key_value") is not None:
+        raise NotImplementedError("fused norms run without a key-value cache of the model's own")
+    B, S = hidden_states.shape[:2]
+    q, k, v = (proj(hidden_states).view(B, S, -1, attn.head_dim) for proj in (attn.q_proj, attn.k_proj, attn.v_proj))
+    cos, sin = position_embeddings
+    wq, wk, eps = fused.head_norms(attn)
+    q, k = fused.qk_norm_rope(q, k, cos, sin, wq, wk, eps)
+    dropout = getattr(attn, "attention_dropout", 0.0) if attn.training else 0.0
+    out, _ = masked_attention_forward(attn, q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), attention_mask,
+                                      scaling=attn.scaling, dropout=dropout,
+                                      sliding_window=getattr(attn, "sliding_window", None))
+    return attn.o_proj(out.reshape(B, S, -1)), None
+
+
+def fuse_norms(model) -> None:
+    """Let the attention of every decoder layer run its per-head norms with the rotation (``fused.qk_norm_rope``) and the
+    attention of this module. Models whose layers have RMS norms of queries and keys over a head's 128 dims."""
+    for layer in model.model.layers:
+        if fused.head_norms(layer.self_attn)[0] is None:
+            raise NotImplementedError("fused norms need layers with q_norm and k_norm")
+    for layer in model.model.layers:
+        layer.self_attn.forward = types.MethodType(_fused_attention_forward, layer.self_attn)
 
 
 def roles(C: int, N: int, K: int, device=None, L: int = 1, R: int = 0):
@@ -341,13 +372,14 @@ class CompressLM(nn.Module):
 
     ``base_model`` is a HuggingFace causal LM with 32 query heads, 8 KV heads and head size 128 in bf16 (e.g.
     Qwen3-4B or a random model of that attention shape); its attention implementation is switched to
-    ``"abridgekv_hip"``.
+    ``"abridgekv_hip"``. ``fused_norms``, ``fused_ce``: the norms with the rotation, and the cross entropies, as one kernel.
     """
 
     def __init__(self, base_model, C, N, K, L=1, pause_xattn="full", pool_init=False, query_residual=False,
                  code_q_heads=False, code_kv_heads=False, seg_pool=False, gated_seg_pool=False, raw_tail=0,
                  replay_tail=0, code_exclude_replay_tail=False, retain_tail_kv=0, retain_tail_policy="rolling",
-                 head_code_quotas=None, active_code_rows=None, code_positions="appended"):
+                 head_code_quotas=None, active_code_rows=None, code_positions="appended", *, fused_norms=False,
+                 fused_ce=False):
         super().__init__()
         if int(L) != L or L < 1:
             raise ValueError(f"L must be a positive integer, got {L}")
@@ -429,6 +461,9 @@ class CompressLM(nn.Module):
             if code_kv_heads:
                 attn.k_proj = _QProjCode(attn.k_proj, self._code_rows)
                 attn.v_proj = _QProjCode(attn.v_proj, self._code_rows)
+        self.fused_norms, self.fused_ce = bool(fused_norms), bool(fused_ce)
+        if fused_norms:
+            fuse_norms(base_model)
         self._set_layout(self.N)
         self.set_head_code_quotas(head_code_quotas)
 
@@ -501,7 +536,15 @@ class CompressLM(nn.Module):
                             self.raw_tail or self.retain_tail_kv, policy, self.pause_xattn, self.L,
                             copy_rows, self.replay_tail, self.code_exclude_replay_tail)
 
+    def _ce_rows(self, hid, tgt):
+        """Cross entropy of every row."""
+        if self.fused_ce:
+            return -fused.token_logprobs(self.model.lm_head(hid), tgt)[0]
+        return F.cross_entropy(self.model.lm_head(hid).float(), tgt, reduction="none")
+
     def _lm_ce(self, hid, tgt, chunk):
+        if self.fused_ce:
+            return self._per_token_lm_ce(hid, tgt, chunk).mean()
         if chunk <= 0:
             return F.cross_entropy(self.model.lm_head(hid).float(), tgt)
         tot = hid.new_zeros((), dtype=torch.float32)
@@ -512,15 +555,14 @@ class CompressLM(nn.Module):
 
     def _per_token_lm_ce(self, hid, tgt, chunk):
         step = hid.size(0) if chunk <= 0 else chunk
-        return torch.cat([F.cross_entropy(self.model.lm_head(hid[i:i + step]).float(), tgt[i:i + step],
-                                          reduction="none") for i in range(0, hid.size(0), step)])
+        return torch.cat([self._ce_rows(hid[i:i + step], tgt[i:i + step]) for i in range(0, hid.size(0), step)])
 
     def _masked_lm_ce(self, hid, tgt, mask, chunk):
         den = mask.sum().clamp_min(1.0)
         return (self._per_token_lm_ce(hid, tgt, chunk) * mask).sum() / den
 
     def _perblock_ce(self, hid, tgt, blk_idx, nblk, reps):
-        ce = F.cross_entropy(self.model.lm_head(hid).float(), tgt, reduction="none")
+        ce = self._ce_rows(hid, tgt)
         blk = blk_idx.repeat(reps)
         s = ce.new_zeros(nblk).scatter_add_(0, blk, ce)
         c = ce.new_zeros(nblk).scatter_add_(0, blk, torch.ones_like(ce))
@@ -754,3 +796,14 @@ class CompressLM(nn.Module):
         out = self.hidden_states(content_ids, prompt_len)
         hid = out[:, self.loss_pos, :].reshape(-1, out.size(-1))
         return self.model.lm_head(hid).float()
+
+    @torch.no_grad()
+    def token_logprobs(self, content_ids, prompt_len=None, temperature=1.0, top=0, chunk=4096) -> ops.TokenLogprobs:
+        """Log probabilities of the content tokens at the loss positions (block-major, as :meth:`loss_logits` orders them), with
+        the distributions' entropies and ``top`` alternatives, ``chunk`` rows of logits at a time."""
+        hid = self.hidden_states(content_ids, prompt_len)[:, self.loss_pos, :].reshape(-1, self.model.config.hidden_size)
+        B, N, C = content_ids.shape
+        tgt = content_ids.reshape(B, N * C)[:, self.predict_flat + 1].reshape(-1)
+        parts = [ops.token_logprobs(self.model.lm_head(hid[i:i + chunk]), tgt[i:i + chunk], temperature, top=top)
+                 for i in range(0, hid.size(0), chunk)]
+        return ops.TokenLogprobs(*(torch.cat(x) for x in list(zip(*parts))[:4]), None)

@@ -56,6 +56,19 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch
     return _QKNormRope.apply(q, k, cos, sin, q_weight, k_weight, float(eps))
 
 
+def head_norms(attn):
+    """(q weight, k weight, eps) of an attention layer's per-head RMS norms, (None, None, 0.0) of a layer without any; norms of
+    another kind are refused."""
+    qn, kn = getattr(attn, "q_norm", None), getattr(attn, "k_norm", None)
+    if qn is None and kn is None:
+        return None, None, 0.0
+    eps = [getattr(n, "variance_epsilon", None) for n in (qn, kn)]
+    weights = [getattr(n, "weight", None) for n in (qn, kn)]
+    if None in eps or eps[0] != eps[1] or any(w is None or w.shape != (ops.HEAD_DIM,) for w in weights):
+        raise NotImplementedError("the fused norms take RMS norms of queries and keys over a head's 128 dims")
+    return weights[0], weights[1], float(eps[0])
+
+
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, temperature):

@@ -50,6 +50,11 @@ serving sidecar (compresslm_packed_kv.py): one KV-cache group; the code step hid
 head (``abkv_paged_prefill_attn_packed``); ``compress`` then copies the block's code rows into one packed page per
 layer (``abkv_packed_capture``) and removes the response content and all K codes as one span; content steps attend
 over the packed pages plus the paged rows (``abkv_decode_attn_packed`` / ``abkv_paged_prefill_attn_packed``).
+
+``kv_cache_dtype="int4"`` holds every row in 4 bits (a third of the bytes, beside what the code rows save): the same pages and
+moves, with the 4-bit append, decode and multi-query kernels. ``fused_norms`` (always so over 4 bits) runs a layer's q_norm and
+k_norm with the rotation and the append, in one pass and one rounding (``abkv_qk_norm_rope_append``). ``score`` gives the log
+probabilities of a given answer, by which the caches are compared.
 """
 from __future__ import annotations
 
@@ -58,7 +63,7 @@ import torch
 import torch.nn.functional as F
 
 from . import backend as bk
-from . import ops
+from . import fused, ops
 from .compress_forward import _QProjCode, _QProjQRes, code_seeds
 from .config import CompressLMConfig, bitrev_offsets
 from .packed_kv import PackedKVLayout, PackedKVSidecar
@@ -110,7 +115,8 @@ class CompressGen:
     page pool must hold."""
 
     def __init__(self, clm, device, raw_prompt_len=0, head_code_quotas=None, code_attend_current_content=True,
-                 code_init_override=None, raw_tail_override=None, max_tokens: int = 1 << 15, **options):
+                 code_init_override=None, raw_tail_override=None, max_tokens: int = 1 << 15, kv_cache_dtype: str = "auto",
+                 fused_norms: bool = False, **options):
         bad = sorted(name for name in options if name not in _UNSUPPORTED)
         if bad:
             raise TypeError(f"unexpected CompressGen options {bad}")
@@ -178,6 +184,15 @@ class CompressGen:
         if self.packed and self.xattn != "full":
             raise NotImplementedError("per-head packed pages serve bidirectional code steps (pause_xattn='full')")
 
+        self.impl = bk.AbridgeAttentionImpl(scale=getattr(self.layers[0].self_attn, "scaling", None),
+                                            kv_cache_dtype=kv_cache_dtype)
+        if self.impl.int4 and self.packed:
+            raise NotImplementedError("per-head packed pages hold bf16 rows")
+        self.fused_norms = bool(fused_norms) or self.impl.int4
+        if self.fused_norms:
+            for layer in self.layers:                        # (refused here rather than in the first step)
+                fused.head_norms(layer.self_attn)
+
         # KV-cache groups: layers of equal quota, in order of first appearance; tensor i = i-th layer of each group
         distinct = list(dict.fromkeys(self.quotas))
         self.group_quotas = distinct
@@ -187,7 +202,8 @@ class CompressGen:
         G = len(distinct)
         pages_per_group = -(-int(max_tokens) // ops.PAGE) + 2
         self.num_pages = G * pages_per_group + 1
-        self.caches = [torch.zeros(ops.kv_cache_shape(self.num_pages), dtype=torch.bfloat16, device=self.device)
+        shape = bk.AbridgeAttentionBackend.get_kv_cache_shape(self.num_pages, kv_cache_dtype=kv_cache_dtype)
+        self.caches = [torch.zeros(shape, dtype=torch.uint8 if self.impl.int4 else torch.bfloat16, device=self.device)
                        for _ in range(n_tensors)]
         self.caches_by_group = [[self.caches[self.tensor_of[li]] for li in range(self.num_layers)
                                  if self.group_of[li] == g] for g in range(G)]
@@ -205,8 +221,8 @@ class CompressGen:
         self.proc = CompressLMProcessor(pcfg)
         if not self.packed:
             self.proc.set_group_quotas(self.group_quotas)
-        self.impl = bk.AbridgeAttentionImpl(scale=getattr(self.layers[0].self_attn, "scaling", None))
-        self.builder = bk.AbridgeMetadataBuilder(max_num_seqs=1, max_pages=pages_per_group, device=self.device)
+        self.builder = bk.AbridgeMetadataBuilder(max_num_seqs=1, max_pages=pages_per_group, device=self.device,
+                                                 kv_cache_dtype=kv_cache_dtype)
         self.sidecar = None
         if self.packed:
             layout = PackedKVLayout.from_schedule(self.head_code_quotas.tolist(), num_layers=self.num_layers,
@@ -280,15 +296,21 @@ class CompressGen:
             normed = layer.input_layernorm(hidden)
             q = _project(attn.q_proj, normed, code_step).view(1, n, -1, attn.head_dim)
             k = _project(attn.k_proj, normed, code_step).view(1, n, -1, attn.head_dim)
-            if getattr(attn, "q_norm", None) is not None:
-                q = attn.q_norm(q)
-            if getattr(attn, "k_norm", None) is not None:
-                k = attn.k_norm(k)
-            q = q[0].to(self.dtype).contiguous()
-            k = k[0].to(self.dtype).contiguous()
             v = _project(attn.v_proj, normed, code_step).view(n, -1, attn.head_dim).contiguous()
-            ops.rope_kv_append(q, k, v, logical, self._cos_sin, slot_mapping=md.slot_mapping, kv_cache=cache,
-                               block_c=bc, codes_k=bk, max_position=last, code_span=bc - self.X if bc else 0)
+            if self.fused_norms:
+                wq, wk, eps = fused.head_norms(attn)
+                q = ops.qk_norm_rope_append(q[0], k[0], v, logical, self._cos_sin, md.slot_mapping, cache, q_weight=wq,
+                                            k_weight=wk, eps=eps, block_c=bc, codes_k=bk, max_position=last,
+                                            code_span=bc - self.X if bc else 0)
+            else:
+                if getattr(attn, "q_norm", None) is not None:
+                    q = attn.q_norm(q)
+                if getattr(attn, "k_norm", None) is not None:
+                    k = attn.k_norm(k)
+                q = q[0].to(self.dtype).contiguous()
+                k = k[0].to(self.dtype).contiguous()
+                ops.rope_kv_append(q, k, v, logical, self._cos_sin, slot_mapping=md.slot_mapping, kv_cache=cache,
+                                   block_c=bc, codes_k=bk, max_position=last, code_span=bc - self.X if bc else 0)
             o = torch.empty((n, ops.HEADS_Q, ops.HEAD_DIM), dtype=self.dtype, device=self.device)
             if self.sidecar is not None:
                 # paged rows + this layer's per-head packed pages; a code step's paged keys stop at the block's
@@ -427,6 +449,28 @@ class CompressGen:
             if self.f == self.C:
                 self.compress()
         return last
+
+    @torch.no_grad()
+    def score(self, prompt_ids, answer_ids, temperature=1.0, top=0) -> ops.TokenLogprobs:
+        """Log probabilities of the answer's tokens behind the prompt under this cache (with the distributions' entropies and
+        ``top`` alternatives), as the cache stands when each is predicted: fed in chunks, blocks compressed as they fill. The
+        answer's last token is not fed."""
+        ids = [int(t) for t in prompt_ids] + [int(t) for t in answer_ids]
+        first, n = len(prompt_ids), len(ids)
+        if first == 0 or n == first:
+            raise ValueError("score needs a prompt and an answer")
+        parts, i = [], 0
+        while i < n - 1:
+            take = min(self.C - self.f, n - 1 - i)
+            h = self.feed_content(ids[i:i + take])
+            skip = max(first - 1 - i, 0)                     # row j predicts token i + j + 1
+            if skip < take:
+                targets = torch.tensor(ids[i + skip + 1:i + take + 1], device=self.device)
+                parts.append(ops.token_logprobs(self.lm_head(h[skip:]), targets, temperature, top=top))
+            i += take
+            if self.f == self.C:
+                self.compress()
+        return ops.TokenLogprobs(*(torch.cat(x) for x in list(zip(*parts))[:4]), None)
 
     @torch.no_grad()
     def generate(self, prompt_ids, max_new_tokens, eos_id=None, temperature=0.0, top_p=1.0, top_k=0, gen=None):

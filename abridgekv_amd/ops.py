@@ -1139,15 +1139,19 @@ def window_backward(q, k, v, out, lse, dout, window, sinks, seq_lens, scale, out
     return dq, dk, dv
 
 
+def _check_paged_cache(kv_cache: torch.Tensor) -> None:
+    shape = kv_cache.shape
+    if (kv_cache.dtype is not torch.bfloat16 or len(shape) != 5 or shape[1:] != _PAGE_SHAPE or shape[0] == 0
+            or not kv_cache.is_contiguous()):
+        raise ValueError(f"kv_cache must be contiguous bf16 [P, 2, {PAGE}, {HEADS_KV}, {HEAD_DIM}]")
+
+
 def _check_paged(q: torch.Tensor, kv_cache: torch.Tensor | None, block_table: torch.Tensor) -> tuple[int, int, int]:
     """bf16 query rows [T, 32, 128], a layer cache and its page table; (T, the table's rows and width)."""
     T = q.shape[0] if q.dim() else 0
     _check_rows("q", q, torch.bfloat16, (T, HEADS_Q, HEAD_DIM))
     if kv_cache is not None:
-        shape = kv_cache.shape
-        if (kv_cache.dtype is not torch.bfloat16 or len(shape) != 5 or shape[1:] != _PAGE_SHAPE or shape[0] == 0
-                or not kv_cache.is_contiguous()):
-            raise ValueError(f"kv_cache must be contiguous bf16 [P, 2, {PAGE}, {HEADS_KV}, {HEAD_DIM}]")
+        _check_paged_cache(kv_cache)
     shape = block_table.shape
     if block_table.dtype is not torch.int32 or len(shape) != 2 or shape[1] == 0 or block_table.stride(1) != 1:
         raise ValueError("block_table must be int32 [B, W] with contiguous rows")
@@ -1625,8 +1629,7 @@ def qk_norm_rope_append(q: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     if int4:
         _check_cache4(kv_cache)
     else:
-        _check_cache(kv_cache)
-        _require(kv_cache.shape[0] > 0, "kv_cache must have pages")
+        _check_paged_cache(kv_cache)
     _require((q_weight is None) == (k_weight is None), "norm weights are given for queries and keys, or for neither")
     wf32 = 0 if q_weight is None else _check_weights(q_weight, k_weight, torch.bfloat16)
     eps = _check_eps(eps)

@@ -360,3 +360,103 @@ def _window_attn_bwd_fake(q, k, v, out, lse, dout, window, sinks, seq_lens, scal
 
 BOUNDED_OPS = ("decode_attn_window", "decode_attn_scored", "kv_evict", "window_attn", "window_attn_bwd")
 TRAINING_OPS = ("window_attn_low",)                          # window_attn with what window_attn_bwd takes beside out and lse
+
+
+# -- a step over a cache in 4 bits: norms with rotation, append, decode, log probabilities -----------------------------
+@torch.library.custom_op(f"{_NS}::kv_append_int4", mutates_args=("kv_cache",))
+def kv_append_int4(key: Tensor, value: Tensor, slot_mapping: Tensor, kv_cache: Tensor) -> None:
+    """abkv_kv_append_int4: key / value rows [T, 8, 128] quantised into a cache in 4 bits at slot_mapping."""
+    _ops.kv_append_int4(key, value, slot_mapping, kv_cache)
+
+
+@kv_append_int4.register_fake
+def _kv_append_int4_fake(key, value, slot_mapping, kv_cache):
+    _need(key.shape == value.shape and key.shape[0] == slot_mapping.shape[0], "one slot per key and value row")
+
+
+@torch.library.custom_op(f"{_NS}::decode_attn_int4", mutates_args=("out", "lse", "workspace"))
+def decode_attn_int4(q: Tensor, kv_cache: Tensor, block_table: Tensor, seq_lens: Tensor, scale: float, max_pages: int,
+                     split_pages: int, out: Tensor, lse: Optional[Tensor], workspace: Optional[Tensor]) -> None:
+    """abkv_decode_attn_int4: decode over a cache in 4 bits. A batch that needs more than one split must bring ``workspace``
+    (ops.decode_int4_workspace): the op never allocates."""
+    if lib().abkv_decode_int4_workspace_size(q.shape[0], max_pages, split_pages):
+        _need(workspace is not None, "decode_attn_int4: the batch needs a workspace (ops.decode_int4_workspace)")
+    _ops.decode_attention_int4(q, kv_cache, block_table, seq_lens, scale, max_pages=max_pages, out=out, lse=lse,
+                               split_pages=split_pages, workspace=workspace)
+
+
+@decode_attn_int4.register_fake
+def _decode_attn_int4_fake(q, kv_cache, block_table, seq_lens, scale, max_pages, split_pages, out, lse, workspace):
+    _need(q.dim() == 3 and tuple(q.shape[1:]) == (_ops.HEADS_Q, _ops.HEAD_DIM), "q must be [B, 32, 128]")
+    _need(tuple(out.shape) == tuple(q.shape), "out must be [B, 32, 128]")
+    _need(kv_cache.dim() == 4, "kv_cache must be [P, 2, 16, 640]")
+
+
+@torch.library.custom_op(f"{_NS}::qk_norm_rope_append", mutates_args=("kv_cache", "out"))
+def qk_norm_rope_append(q: Tensor, key: Tensor, value: Tensor, positions: Tensor, cos_sin: Tensor, slot_mapping: Tensor,
+                        kv_cache: Tensor, q_weight: Optional[Tensor], k_weight: Optional[Tensor], eps: float, block_c: int,
+                        codes_k: int, max_position: int, code_span: int, out: Tensor) -> None:
+    """abkv_qk_norm_rope_append: per-head norms (or none) and rotation, queries to ``out`` (not q itself: a custom op's
+    outputs are their own), keys and values to the bf16 or 4-bit cache. ``max_position``: host bound on the positions."""
+    _ops.qk_norm_rope_append(q, key, value, positions, cos_sin, slot_mapping, kv_cache, q_weight=q_weight, k_weight=k_weight,
+                             eps=eps, block_c=block_c, codes_k=codes_k, max_position=max_position, code_span=code_span, out=out)
+
+
+@qk_norm_rope_append.register_fake
+def _qk_norm_rope_append_fake(q, key, value, positions, cos_sin, slot_mapping, kv_cache, q_weight, k_weight, eps, block_c,
+                              codes_k, max_position, code_span, out):
+    _need(tuple(out.shape) == tuple(q.shape) and positions.shape == slot_mapping.shape, "out [T, 32, 128], one slot per position")
+
+
+@torch.library.custom_op(f"{_NS}::qk_norm_rope", mutates_args=())
+def qk_norm_rope(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, q_weight: Tensor, k_weight: Tensor,
+                 eps: float) -> tuple[Tensor, Tensor]:
+    """abkv_qk_norm_rope: a training step's norms and rotation, q [B, S, 32, 128] (new tensors)."""
+    return _ops.qk_norm_rope(q, k, cos, sin, q_weight, k_weight, eps)
+
+
+@qk_norm_rope.register_fake
+def _qk_norm_rope_fake(q, k, cos, sin, q_weight, k_weight, eps):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+@torch.library.custom_op(f"{_NS}::qk_norm_rope_bwd", mutates_args=())
+def qk_norm_rope_bwd(q: Tensor, k: Tensor, dq_out: Tensor, dk_out: Tensor, cos: Tensor, sin: Tensor, q_weight: Tensor,
+                     k_weight: Tensor, eps: float) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    """abkv_qk_norm_rope_bwd: (dq, dk, dq_weight, dk_weight)."""
+    return _ops.qk_norm_rope_backward(q, k, dq_out, dk_out, cos, sin, q_weight, k_weight, eps)
+
+
+@qk_norm_rope_bwd.register_fake
+def _qk_norm_rope_bwd_fake(q, k, dq_out, dk_out, cos, sin, q_weight, k_weight, eps):
+    return q.new_empty(q.shape), k.new_empty(k.shape), torch.empty_like(q_weight), torch.empty_like(k_weight)
+
+
+@torch.library.custom_op(f"{_NS}::token_logprobs", mutates_args=())
+def token_logprobs(logits: Tensor, targets: Tensor, temperature: float,
+                   top: int) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """abkv_token_logprobs: (logprob [T], entropy [T], ids [T, top], their log probabilities, stats [T, 3])."""
+    return tuple(_ops.token_logprobs(logits, targets, temperature, top=top, stats=True))
+
+
+@token_logprobs.register_fake
+def _token_logprobs_fake(logits, targets, temperature, top):
+    T = logits.shape[0]
+    f32 = [logits.new_empty(shape, dtype=torch.float32) for shape in ((T,), (T,), (T, top), (T, 3))]
+    return f32[0], f32[1], logits.new_empty((T, top), dtype=torch.int64), f32[2], f32[3]
+
+
+@torch.library.custom_op(f"{_NS}::token_logprobs_bwd", mutates_args=())
+def token_logprobs_bwd(logits: Tensor, targets: Tensor, stats: Tensor, dlogprob: Optional[Tensor], dentropy: Optional[Tensor],
+                       temperature: float) -> Tensor:
+    """abkv_token_logprobs_bwd: the gradient of the logits (a new tensor)."""
+    return _ops.token_logprobs_backward(logits, targets, stats, dlogprob, dentropy, temperature)
+
+
+@token_logprobs_bwd.register_fake
+def _token_logprobs_bwd_fake(logits, targets, stats, dlogprob, dentropy, temperature):
+    return logits.new_empty(logits.shape)
+
+
+STEP_OPS = ("kv_append_int4", "decode_attn_int4", "qk_norm_rope_append", "qk_norm_rope", "qk_norm_rope_bwd", "token_logprobs",
+            "token_logprobs_bwd")
