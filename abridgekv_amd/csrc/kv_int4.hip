@@ -3,6 +3,8 @@
 #include "abridgekv_amd.h"
 #include "int4.h"
 
+#define ABKV_LDS(p) ((__attribute__((address_space(3))) void*)(p))
+
 namespace abkv {
 
 __device__ __forceinline__ u32x4 ld16b(const char* p) { return *reinterpret_cast<const u32x4*>(p); }
@@ -68,6 +70,15 @@ __global__ __launch_bounds__(256) void kv_read4_kernel(const char* cache, long n
   }
 }
 
+// (Values: a conditional of two array elements would be their place, and the array in memory.)
+__device__ __forceinline__ float pick(bool c, float a, float b) { return c ? a : b; }
+
+// The middle of a group's values, m + 8 s.
+__device__ __forceinline__ float middle(uint32_t pair) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), bf16x2{(__bf16)8.f, (__bf16)1.f}, 0.f, false);
+}
+
 // -- one token per sequence ---------------------------------------------------------------------------------------------
 struct Decode4Args {
   const __bf16* q; long q_sb, q_sh;            // [B, 32, 128]
@@ -91,10 +102,11 @@ __device__ __forceinline__ int splits_of(const Decode4Args& a, int rows) {
 
 // Codes of two neighbouring dims (nibbles n and n + 4 of a word) as the bf16 pair 128 + c: c lies in the low bits of the
 // mantissa, so every code is exact, and the 128s leave with the sums.
-__device__ __forceinline__ uint32_t code_pair(uint32_t w, int n) { return ((w >> (4 * n)) & 0x000f000fu) | 0x43004300u; }
+// (mask in a vector register: with both constants literal the and and the or are instructions of their own)
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, int n, uint32_t mask) { return ((w >> (4 * n)) & mask) | 0x43004300u; }
 
-// Workgroup (split, sequence), a wave per KV head: the heads' rows lie next to each other, so the workgroup streams whole pages
-// (a wave's 64 bytes of a slot are half a cache line). A wave walks its split 32 slots (two pages) at a time.
+// Workgroup (split, sequence), a wave per KV head. A wave walks its split 32 slots (two pages) at a time, the next step's rows
+// on the way meanwhile.
 //
 // Scores: the four groups of 32 dims have their own steps and minima, so a score is the sum of four products:
 //   x_j = sum_g (s_jg a_jg + m_jg Q_g),  a_jg = sum_{d in g} q_d c_jd,  Q_g = sum_{d in g} q_d.
@@ -107,16 +119,26 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t w, int n) { return ((w >>
 // s |c - 8|, no more than values of that size would (by s c, from the minimum, it was 2.5 times as much); everything else is
 // exact or fp32.
 //
-// A lane's V operand is one word of 8 slots while a wide load brings four words of one, and its parameters likewise: both
-// are exchanged through LDS, in a part of its own for each wave (no barrier).
-__device__ __forceinline__ void wave_exchange() {              // LDS is in order within a wave; this keeps the compiler so too
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+// What bounds the reads is the number of cache lines that a CU asks for (about one in six cycles), so a line should bring what it
+// holds: a head's codes are half of one, its pairs an eighth. The workgroup's waves therefore fetch whole rows together, straight
+// into LDS (a wave 5 of the step's 40 KB), one barrier a step. (64 sequences of 500 to 9500 rows, every wave its own pieces: 118
+// us, of which 59 went with the pairs alone; the pairs shared, 93.)
+constexpr int kPairs4 = 16 * 4 * kHeadsKV, kCodes4 = 16 * kHeadsKV * 16;     // dwords of a page's pairs and codes (of K or V)
+template <class T>
+__device__ __forceinline__ const T& at4(const uint32_t* base, uint32_t bytes) {
+  return *reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + bytes);
 }
-constexpr int kVRow = 16, kPRow = 80;                        // dwords: a slot's codes; a tile's pairs [4 groups][16 slots], padded
+// LDS of a step: parts K0 K1 V0 V1 (pages 0 and 1). Codes in rows of 32 16-byte chunks, slot by slot, chunk 4 head + word / 4 at
+// place (chunk ^ slot): both kinds of reads below then take all banks. Pairs in rows of 8 chunks, a chunk a head: row 4 r + j is
+// slot 4 j + r, its chunks at place (head ^ (j >> 1)).
+struct Step4 {
+  uint32_t codes[4][kCodes4];
+  uint32_t pairs[4][kPairs4];
+};
 __global__ __launch_bounds__(64 * kHeadsKV, 4) void decode4_kernel(Decode4Args a) {
-  const int b = blockIdx.y, split = blockIdx.x;
+  // Linear grid, sequence by sequence; a sequence's splits start one further each time: workgroups go to the 8 XCDs round-robin,
+  // and sequences end at different splits.
+  const int b = blockIdx.x / a.max_splits, split = (blockIdx.x + b) % a.max_splits;
   const int kvh = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, m16 = lane & 15, j = lane >> 4;
   const int h = m16 >> 2, g = m16 & 3;
@@ -125,9 +147,7 @@ __global__ __launch_bounds__(64 * kHeadsKV, 4) void decode4_kernel(Decode4Args a
   if (split >= n_splits) return;
   const int pg_begin = split * a.split_pages;
   const int pg_end = min((row_end + kPage - 1) / kPage, pg_begin + a.split_pages);
-  __shared__ __attribute__((aligned(16))) uint32_t vbuf[kHeadsKV][32 * kVRow], pbuf[kHeadsKV][4 * kPRow];
-  uint32_t* const vl = vbuf[kvh];
-  uint32_t* const pl = pbuf[kvh];
+  __shared__ __attribute__((aligned(16))) Step4 lds0, lds1;
 
   // Page ids of the split, lane l page pg_begin + l (split_pages <= 64)
   const int32_t* bt = a.block_table + (long)b * a.bt_stride;
@@ -146,95 +166,129 @@ __global__ __launch_bounds__(64 * kHeadsKV, 4) void decode4_kernel(Decode4Args a
     }
     qsum = sum_xor32(sum_xor16(qsum));                       // Q_g
   }
+  // Q_g in three bf16 parts (lane groups j = 0 .. 2), against a slot's pairs as they lie in the row: (s_0, m_0), .. (s_3, m_3).
+  // One MFMA then leaves sum_g m_g Q_g, in the columns of g = 0.
+  bf16x8 qmin;
+  {
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float v = __shfl(qsum, (lane & 48) + 4 * h + i, 64);   // Q_i of this head
+      const float v0 = bf16_hi(__float_as_uint(v)), v1 = bf16_hi(__float_as_uint(v - v0));
+      const float x = j == 0 ? v0 : j == 1 ? v1 : v - v0 - v1;
+      w[i] = g == 0 && j < 3 ? __float_as_uint(x) & 0xffff0000u : 0u;
+    }
+    qmin = __builtin_bit_cast(bf16x8, w);
+  }
   const float q128 = -128.f * qsum;
   typedef short s8 __attribute__((ext_vector_type(8)));
   const short n136 = (short)0xc308;                          // bf16 -136
   const bf16x8 minus = __builtin_bit_cast(bf16x8, s8{n136, n136, n136, n136, n136, n136, n136, n136});
+  uint32_t mask = 0x000f000fu;
+  __asm__("" : "+v"(mask));
 
   floatx4 o[8], off = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < 8; ++i) o[i] = floatx4{0.f, 0.f, 0.f, 0.f};
   float m_run = -INFINITY, l_run = 0.f, om = 0.f;            // om: sum of p_j (m_jg + 8 s_jg) over this lane's slots
 
-  // This lane's pieces: K words 4 j .. + 3 of slot m16; V words 4 (lane & 3) .. of the slot whose LDS row is lane >> 2; and the
-  // pairs of slot m16, of K (j 0, 1) or V (j 2, 3), page j & 1. LDS row 4 e + j holds slot 4 j + e: the reads below then take
-  // all banks.
-  const int vrow = lane >> 2, vslot = 4 * (vrow & 3) + (vrow >> 2);
-  const long k_at = m16 * kSlot4 + kvh * kHeadCodes4 + 16 * j;
-  const long v_at = kHalf4 + vslot * kSlot4 + kvh * kHeadCodes4 + 16 * (lane & 3);
-  const long p_at = (j >> 1) * kHalf4 + m16 * kSlot4 + kParams4 + kvh * 16;
-  struct Tile {
-    u32x4 k[2], v[2], p;
+  // What this wave fetches, of part wave / 2 (of K or V: part / 2; of page part % 2): slots 8 (wave % 2) .. + 7, two a load, and
+  // rows 8 (wave % 2) .. + 7 of the pairs.
+  const int part = kvh >> 1, rows8 = 8 * (kvh & 1);
+  const int p_row = rows8 + (lane >> 3);
+  uint32_t code_from = 16 * ((lane & 31) ^ (rows8 + (lane >> 5)));
+  uint32_t pair_from = (4 * (p_row & 3) + (p_row >> 2)) * kSlot4 + kParams4 + 16 * ((lane & 7) ^ (p_row >> 1 & 1));
+  const uint32_t slot_from = (lane >> 5) * kSlot4;
+  const int last = pg_end - 1 - pg_begin;
+  // Offsets as the instructions take them: 32 bits in a register beside a uniform base. (Pinned: made into 64-bit addresses
+  // ahead of the loop they spill.)
+  auto fetch = [&](Step4& to, int pg) {                      // (past the end: the last page again)
+    const int at = min(pg + (part & 1) - pg_begin, last);
+    const char* from = a.kv + (long)__builtin_amdgcn_readlane(pid_l, at) * kPage4 + (part >> 1) * kHalf4;
+    __asm__("" : "+v"(pair_from), "+v"(code_from));
+    __builtin_amdgcn_global_load_lds((const void*)(from + pair_from), ABKV_LDS(&to.pairs[part][32 * rows8]), 16, 0, 0);
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const uint32_t off = (code_from ^ 32 * n) + slot_from;
+      __builtin_amdgcn_global_load_lds((const void*)(from + (rows8 + 2 * n) * kSlot4 + off),
+                                       ABKV_LDS(&to.codes[part][128 * (rows8 + 2 * n)]), 16, 0, 0);
+    }
   };
-  auto load = [&](int pg) {
-    const int at = pg - pg_begin;
-    const char* p0 = a.kv + (long)__builtin_amdgcn_readlane(pid_l, at) * kPage4;
-    const char* p1 = a.kv + (long)__builtin_amdgcn_readlane(pid_l, min(at + 1, pg_end - 1 - pg_begin)) * kPage4;
-    Tile t;
-    t.k[0] = ld16b(p0 + k_at);
-    t.k[1] = ld16b(p1 + k_at);
-    t.v[0] = ld16b(p0 + v_at);
-    t.v[1] = ld16b(p1 + v_at);
-    t.p = ld16b((j & 1 ? p1 : p0) + p_at);
-    return t;
-  };
-  Tile cur;
-  if (pg_begin < pg_end) cur = load(pg_begin);
-  for (int pg = pg_begin; pg < pg_end; pg += 2) {
-    Tile nxt;
-    const bool more = pg + 2 < pg_end;
-    if (more) nxt = load(pg + 2);
-
+  // What it reads of a step, in bytes: K words 4 j .. + 3 of slot m16; word m16 of the V slots 4 j + e; group g's pairs of slots
+  // 4 j + r; slot m16's pairs
+  uint32_t k_at = 512 * m16 + 16 * ((4 * kvh + j) ^ m16);
+  uint32_t v_at = 512 * 4 * j + 16 * ((4 * kvh + (m16 >> 2)) ^ (4 * j)) + 4 * (m16 & 3);           // (e: 512 e, the place ^ e)
+  uint32_t pair_at = ((j * kHeadsKV + (kvh ^ (j >> 1))) * 4 + g) * 4;
+  uint32_t row_at = ((4 * (m16 & 3) + (m16 >> 2)) * kHeadsKV + (kvh ^ (m16 >> 3))) * 16;
+  // One step over the 32 slots from page pg on, which `cur` holds; the next step's rows go to nxt.
+  auto step = [&](const Step4& cur, Step4& nxt, int pg) {
+    __asm__ volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070);                      // (vmcnt(0) lgkmcnt(0), as a builtin: the compiler counts on from it)
+    __builtin_amdgcn_s_barrier();                            // cur is whole, and nobody reads nxt any more
+    __asm__ volatile("" ::: "memory");
+    if (pg + 2 < pg_end) fetch(nxt, pg + 2);
+    __asm__("" : "+v"(k_at), "+v"(v_at), "+v"(pair_at), "+v"(row_at));
     floatx4 s[2];
+    u32x4 k[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) k[t] = at4<u32x4>(cur.codes[t], k_at);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       s[t] = floatx4{q128, q128, q128, q128};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t w = cur.k[t][i];
-        const u32x4 codes = {code_pair(w, 0), code_pair(w, 1), code_pair(w, 2), code_pair(w, 3)};
+        const uint32_t w = k[t][i];
+        const u32x4 codes = {code_pair(w, 0, mask), code_pair(w, 1, mask), code_pair(w, 2, mask), code_pair(w, 3, mask)};
         s[t] = mfma16x16x32(__builtin_bit_cast(bf16x8, codes), qop[i], s[t]);
       }
     }
-#pragma unroll
-    for (int t = 0; t < 2; ++t) *reinterpret_cast<u32x4*>(vl + (16 * t + vrow) * kVRow + 4 * (lane & 3)) = cur.v[t];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) pl[j * kPRow + 16 * i + m16] = cur.p[i];
-    wave_exchange();
-    u32x4 kp[2], vp[2];                                      // pairs of group g of slots 4 j .. + 3 of the two pages
-    uint32_t vw[8];                                          // word m16 of slots 4 j + e of page 0, then of page 1
+    floatx4 mq[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      kp[t] = *reinterpret_cast<const u32x4*>(pl + t * kPRow + 16 * g + 4 * j);
-      vp[t] = *reinterpret_cast<const u32x4*>(pl + (2 + t) * kPRow + 16 * g + 4 * j);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) vw[4 * t + e] = vl[(16 * t + 4 * e + j) * kVRow + m16];
+      const u32x4 row = at4<u32x4>(cur.pairs[t], row_at);
+      mq[t] = mfma16x16x32(__builtin_bit_cast(bf16x8, row), qmin, floatx4{0.f, 0.f, 0.f, 0.f});
     }
-    wave_exchange();
-
-    const bool tail = (pg + 2) * kPage > row_end;
-    float sv[8];
+    uint32_t kp[2][4], vp[2][4];                             // pairs of group g of slots 4 j .. + 3 of the two pages
+    uint32_t vw[8];                                          // word m16 of slots 4 j + e of page 0, then of page 1
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        float x = fmaf(bf16_lo(kp[t][r]), s[t][r], bf16_hi(kp[t][r]) * qsum);
-        x += dpp<kDppXor1>(x);
-        x += dpp<kDppXor2>(x);
-        x *= a.scale_log2;
-        if (tail) {                                          // rows past the end: whatever their slots hold
-          const bool in = pg * kPage + 16 * t + 4 * j + r < row_end;
-          x = in ? x : -INFINITY;
-          vp[t][r] = in ? vp[t][r] : 0u;
-        }
-        sv[4 * t + r] = x;
+        kp[t][r] = at4<uint32_t>(cur.pairs[t] + r * 16 * kHeadsKV, pair_at);
+        vp[t][r] = at4<uint32_t>(cur.pairs[2 + t] + r * 16 * kHeadsKV, pair_at);
+        vw[4 * t + r] = at4<uint32_t>(cur.codes[2 + t] + 128 * r, v_at ^ 16 * r);
       }
-    float mx = sv[0];
+
+    // Scores summed over the groups, i.e. the lanes of a quad, of which lane g keeps the slots e = 2 g, 2 g + 1 (of the order of
+    // vw; page e / 4, slot 4 j + e % 4)
+    float x[8], y[4], sv[2];
 #pragma unroll
-    for (int e = 1; e < 8; ++e) mx = fmaxf(mx, sv[e]);
+    for (int e = 0; e < 8; ++e) x[e] = fmaf(bf16_lo(kp[e >> 2][e & 3]), s[e >> 2][e & 3], mq[e >> 2][e & 3]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] += dpp<kDppXor2>(x[e]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      y[e] = pick(g & 2, x[4 + e], x[e]);
+      y[e] += dpp<kDppXor1>(y[e]);
+    }
+    sv[0] = pick(g & 1, y[2], y[0]);
+    sv[1] = pick(g & 1, y[3], y[1]);
+    if ((pg + 2) * kPage > row_end) {                        // rows past the end: whatever their slots hold
+      __asm__ volatile("" ::: "memory");                     // (a branch: the last step's work, not every step's)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (pg * kPage + 8 * (g & 2) + 4 * j + 2 * (g & 1) + i >= row_end) sv[i] = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (pg * kPage + 16 * (e >> 2) + 4 * j + (e & 3) >= row_end) vp[e >> 2][e & 3] = 0u;
+    }
+    const float mx = fmaxf(sv[0], sv[1]);
     // The maximum moves only when some row passes it by more than 8 (weights stay below 2^8)
-    if (__any(mx > m_run + 8.f)) {
-      const float m_new = fmaxf(m_run, max_xor32(max_xor16(mx)));
+    if (__any(mx * a.scale_log2 > m_run + 8.f)) {
+      __asm__ volatile("" ::: "memory");
+      float m_new = max_xor32(max_xor16(mx));
+      m_new = fmaxf(m_new, dpp<kDppXor1>(m_new));
+      m_new = fmaxf(m_run, fmaxf(m_new, dpp<kDppXor2>(m_new)) * a.scale_log2);
       const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_new);
       m_run = m_new;
       l_run *= alpha;
@@ -243,45 +297,63 @@ __global__ __launch_bounds__(64 * kHeadsKV, 4) void decode4_kernel(Decode4Args a
 #pragma unroll
       for (int i = 0; i < 8; ++i) o[i] *= alpha;
     }
-    const float m_ref = m_run == -INFINITY ? 0.f : m_run;
+    const float m_ref = m_run == -INFINITY ? 0.f : -m_run;
+    const float pe[2] = {fast_exp2(fmaf(sv[0], a.scale_log2, m_ref)), fast_exp2(fmaf(sv[1], a.scale_log2, m_ref))};
+    l_run += pe[0] + pe[1];
+    float p[8];                                              // of all eight slots: lane e / 2 of the quad has it
+    p[0] = dpp<0x00>(pe[0]);
+    p[1] = dpp<0x00>(pe[1]);
+    p[2] = dpp<0x55>(pe[0]);
+    p[3] = dpp<0x55>(pe[1]);
+    p[4] = dpp<0xaa>(pe[0]);
+    p[5] = dpp<0xaa>(pe[1]);
+    p[6] = dpp<0xff>(pe[0]);
+    p[7] = dpp<0xff>(pe[1]);
     u32x4 pw;
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
-      const float p0 = fast_exp2(sv[e] - m_ref), p1 = fast_exp2(sv[e + 1] - m_ref);
       const uint32_t w0 = vp[e >> 2][e & 3], w1 = vp[e >> 2][(e & 3) + 1];
-      l_run += p0 + p1;
-      const float s0 = bf16_lo(w0), s1 = bf16_lo(w1);
-      om = fmaf(p0, fmaf(8.f, s0, bf16_hi(w0)), om);
-      om = fmaf(p1, fmaf(8.f, s1, bf16_hi(w1)), om);
-      pw[e / 2] = pack_bf16x2(p0 * s0, p1 * s1);
+      om = fmaf(p[e], middle(w0), om);
+      om = fmaf(p[e + 1], middle(w1), om);
+      pw[e / 2] = pack_bf16x2(p[e] * bf16_lo(w0), p[e + 1] * bf16_lo(w1));
     }
     const bf16x8 pop = __builtin_bit_cast(bf16x8, pw);
     off = mfma16x16x32(minus, pop, off);
     uint32_t lo[4], hi[4];                                   // nibbles 0 .. 3 and 4 .. 7 of two slots
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      lo[k] = __builtin_amdgcn_perm(vw[2 * k + 1], vw[2 * k], 0x05040100u);
-      hi[k] = __builtin_amdgcn_perm(vw[2 * k + 1], vw[2 * k], 0x07060302u);
+    for (int n = 0; n < 4; ++n) {
+      lo[n] = __builtin_amdgcn_perm(vw[2 * n + 1], vw[2 * n], 0x05040100u);
+      hi[n] = __builtin_amdgcn_perm(vw[2 * n + 1], vw[2 * n], 0x07060302u);
     }
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
-      const u32x4 even = {code_pair(lo[0], n), code_pair(lo[1], n), code_pair(lo[2], n), code_pair(lo[3], n)};
-      const u32x4 odd = {code_pair(hi[0], n), code_pair(hi[1], n), code_pair(hi[2], n), code_pair(hi[3], n)};
+      const u32x4 even = {code_pair(lo[0], n, mask), code_pair(lo[1], n, mask), code_pair(lo[2], n, mask), code_pair(lo[3], n, mask)};
+      const u32x4 odd = {code_pair(hi[0], n, mask), code_pair(hi[1], n, mask), code_pair(hi[2], n, mask), code_pair(hi[3], n, mask)};
       o[2 * n] = mfma16x16x32(__builtin_bit_cast(bf16x8, even), pop, o[2 * n]);
       o[2 * n + 1] = mfma16x16x32(__builtin_bit_cast(bf16x8, odd), pop, o[2 * n + 1]);
     }
-    cur = nxt;
+  };
+  if (pg_begin < pg_end) {
+    fetch(lds0, pg_begin);
+    for (int pg = pg_begin;;) {
+      step(lds0, lds1, pg);
+      if ((pg += 2) >= pg_end) break;
+      step(lds1, lds0, pg);
+      if ((pg += 2) >= pg_end) break;
+    }
   }
 
   // This lane's 8 dims 32 g + 8 j .. + 7 of head h
-  const float l = sum_xor32(sum_xor16(l_run));
+  float l = sum_xor32(sum_xor16(l_run));
+  l += dpp<kDppXor1>(l);
+  l += dpp<kDppXor2>(l);
   om = sum_xor32(sum_xor16(om));
   const float inv = l > 0.f ? 1.f / l : l;                   // (a NaN stays one; no row: 0)
   float x[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float v = g == 0 ? o[i][0] : g == 1 ? o[i][1] : g == 2 ? o[i][2] : o[i][3];
-    x[i] = (v + off[0] + om) * inv;
+    const float even = g & 2 ? o[i][2] : o[i][0], odd = g & 2 ? o[i][3] : o[i][1];
+    x[i] = ((g & 1 ? odd : even) + off[0] + om) * inv;
   }
   const int head = kvh * kGroup + h, dim = 32 * g + 8 * j;
   if (n_splits == 1) {
@@ -462,7 +534,9 @@ int abkv_decode_attn_int4(const void* q, long q_stride_seq, long q_stride_head, 
   a.lse = lse;
   a.part_o = static_cast<_Float16*>(workspace);
   a.part_ml = reinterpret_cast<float*>(a.part_o + (size_t)num_seqs * a.max_splits * kHeadsQ * kHeadDim);
-  hipLaunchKernelGGL(decode4_kernel, dim3(a.max_splits, num_seqs), dim3(64 * kHeadsKV), 0, stream, a);
+  const long groups = (long)num_seqs * a.max_splits;
+  if (groups * 64 * kHeadsKV > 0xFFFFFFFFL) return (int)hipErrorInvalidValue;
+  hipLaunchKernelGGL(decode4_kernel, dim3((unsigned)groups), dim3(64 * kHeadsKV), 0, stream, a);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess || a.max_splits == 1) return (int)err;
   hipLaunchKernelGGL(decode4_merge_kernel, dim3(kHeadsQ, num_seqs), dim3(256), 0, stream, a);
