@@ -325,11 +325,11 @@ class AbridgeAttentionImpl:
             return self._attend_window(q, kv_cache, md, out, lse)
         nd, nd_tok, n_tok = md.num_decodes, md.num_decode_tokens, md.num_actual_tokens
         if nd and self.int4:
-            # a builder of the bf16 cache holds splits of 32 pages; shorter ones where they fit too
+            # the workspace holds the splits of the longest tables, 64 pages or shorter: those of any step, if not all as short
             pages, held = md.max_decode_pages, md.workspace.numel() if md.workspace is not None else 0
             split = ops.int4_split_pages(nd, pages)
-            if ops.decode_int4_bytes(nd, pages, split) > held:
-                split = max(split, ops.DEFAULT_SPLIT_PAGES)
+            while split < 64 and ops.decode_int4_bytes(nd, pages, split) > held:
+                split += 2
             torch.ops.abridgekv.decode_attn_int4(q[:nd_tok], kv_cache, md.block_table[:nd], md.seq_lens_dev[:nd], self.scale,
                                                  pages, split, out[:nd_tok], None if lse is None else lse[:nd_tok],
                                                  md.workspace)

@@ -77,4 +77,16 @@ __device__ __forceinline__ float sum_xor32(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// Another lane's value within 16 lanes, by the DPP control kCtrl.
+template <int kCtrl>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kCtrl, 0xf, 0xf, true);
+}
+template <int kCtrl>
+__device__ __forceinline__ float dpp(float v) {
+  return __uint_as_float(dpp<kCtrl>(__float_as_uint(v)));
+}
+constexpr int kDppXor1 = 0xB1, kDppXor2 = 0x4E;              // quad_perm [1 0 3 2], [2 3 0 1]
+constexpr int kDppHalfMirror = 0x141, kDppMirror = 0x140;    // lane i of 8 <-> 7 - i, of 16 <-> 15 - i
+
 }  // namespace abkv

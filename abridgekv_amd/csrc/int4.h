@@ -17,13 +17,6 @@ constexpr int kSlot4 = kParams4 + kHeadsKV * 16;             // 640
 constexpr int kHalf4 = kPage * kSlot4;                       // V half of a page
 constexpr int kPage4 = 2 * kHalf4;
 
-template <int kCtrl>
-__device__ __forceinline__ float dpp(float v) {
-  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), kCtrl, 0xf, 0xf, true));
-}
-constexpr int kDppXor1 = 0xB1, kDppXor2 = 0x4E;              // quad_perm [1 0 3 2], [2 3 0 1]
-constexpr int kDppHalfMirror = 0x141;                        // lane i of 8 <-> 7 - i
-
 __device__ __forceinline__ int code_word(int b) { return 4 * (b & 3) + (b >> 2); }      // word of dims 8 b .. + 7
 
 // Quantises 32 dims that the four lanes of a quad hold, eight each: this lane's word of codes and the group's pair. x are bf16

@@ -382,9 +382,11 @@ __global__ __launch_bounds__(64 * kHeadsKV, 4) void decode4_kernel(Decode4Args a
   if (g == 0 && j == 0) *reinterpret_cast<floatx4*>(a.part_ml + at * 4) = floatx4{m_run, l, range.scale, 0.f};
 }
 
-// Joins the splits of a sequence: workgroup (head, sequence), 16 groups of 16 lanes take the splits k = i, i + 16, ..., a lane 8
-// dims; their sums meet in LDS.
-__global__ __launch_bounds__(256) void decode4_merge_kernel(Decode4Args a) {
+// Joins the splits of a sequence: workgroup (head, sequence), kGroups groups of 16 lanes take the splits k = i, i + kGroups, ...,
+// four at a time, a lane 8 dims; their sums meet in LDS. A pass is a trip to another XCD's memory, so long sequences take more
+// groups.
+template <int kGroups>
+__global__ __launch_bounds__(16 * kGroups) void decode4_merge_kernel(Decode4Args a) {
   const int head = blockIdx.x, b = blockIdx.y;
   const int n = splits_of(a, rows_of(a, b));
   if (n == 1) return;
@@ -392,19 +394,33 @@ __global__ __launch_bounds__(256) void decode4_merge_kernel(Decode4Args a) {
   typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
   const long at = (long)b * a.max_splits * kHeadsQ + head;
   float M = -INFINITY, L = 0.f, acc[8] = {};
-#pragma unroll 4
-  for (int k = grp; k < n; k += 16) {
-    const floatx4 rec = *reinterpret_cast<const floatx4*>(a.part_ml + (at + (long)k * kHeadsQ) * 4);
-    const f16x8 v = *reinterpret_cast<const f16x8*>(a.part_o + (at + (long)k * kHeadsQ) * kHeadDim + 8 * c);
-    const float mn = fmaxf(M, rec[0]);
-    const float alpha = mn == -INFINITY ? 1.f : fast_exp2(M - mn);
-    const float w = mn == -INFINITY ? rec[1] : fast_exp2(rec[0] - mn) * rec[1];
-    L = L * alpha + w;
+  for (int k0 = grp; k0 < n; k0 += 4 * kGroups) {
+    floatx4 rec[4];
+    f16x8 v[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] = acc[i] * alpha + (float)v[i] * (w * rec[2]);
+    for (int u = 0; u < 4; ++u) {                            // (past the end: the last split again, without weight)
+      const long from = at + (long)min(k0 + u * kGroups, n - 1) * kHeadsQ;
+      rec[u] = *reinterpret_cast<const floatx4*>(a.part_ml + from * 4);
+      v[u] = *reinterpret_cast<const f16x8*>(a.part_o + from * kHeadDim + 8 * c);
+    }
+    float mn = M;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) mn = fmaxf(mn, rec[u][0]);
+    const float alpha = mn == -INFINITY ? 1.f : fast_exp2(M - mn);
     M = mn;
+    L *= alpha;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] *= alpha;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (k0 + u * kGroups >= n) break;
+      const float w = mn == -INFINITY ? rec[u][1] : fast_exp2(rec[u][0] - mn) * rec[u][1];
+      L += w;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] += (float)v[u][i] * (w * rec[u][2]);
+    }
   }
-  __shared__ float sm[16], sl[16], so[16][kHeadDim + 4];
+  __shared__ float sm[kGroups], sl[kGroups], so[kGroups][kHeadDim + 4];
   if (c == 0) {
     sm[grp] = M;
     sl[grp] = L;
@@ -417,9 +433,9 @@ __global__ __launch_bounds__(256) void decode4_merge_kernel(Decode4Args a) {
   L = 0.f;
   float x = 0.f;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) M = fmaxf(M, sm[i]);
+  for (int i = 0; i < kGroups; ++i) M = fmaxf(M, sm[i]);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
+  for (int i = 0; i < kGroups; ++i) {
     const float f = sm[i] == M ? 1.f : fast_exp2(sm[i] - M);
     L += sl[i] * f;
     x += so[i][threadIdx.x] * f;
@@ -539,7 +555,8 @@ int abkv_decode_attn_int4(const void* q, long q_stride_seq, long q_stride_head, 
   hipLaunchKernelGGL(decode4_kernel, dim3((unsigned)groups), dim3(64 * kHeadsKV), 0, stream, a);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess || a.max_splits == 1) return (int)err;
-  hipLaunchKernelGGL(decode4_merge_kernel, dim3(kHeadsQ, num_seqs), dim3(256), 0, stream, a);
+  if (a.max_splits > 64) hipLaunchKernelGGL(decode4_merge_kernel<64>, dim3(kHeadsQ, num_seqs), dim3(1024), 0, stream, a);
+  else hipLaunchKernelGGL(decode4_merge_kernel<16>, dim3(kHeadsQ, num_seqs), dim3(256), 0, stream, a);
   return (int)hipGetLastError();
 }
 

@@ -8,10 +8,10 @@
 // second launch joins the splits. Logits below -1e25 (banned tokens: -inf, or the type's lowest value) weigh nothing; a NaN or
 // +inf makes its row NaN.
 //
-// Alternatives: the n-th largest of the threads' maxima bounds the n-th largest logit from below, so only the threads whose
-// maximum reaches it read their part again, collect what reaches it in LDS, and every candidate counts how many come before it
-// (higher, or equal at a lower index). More candidates than the list holds (rows of many equal logits) are found one after the
-// other instead.
+// Alternatives: the n-th largest of a wave's thread maxima bounds the n-th largest logit from below, and so does the largest of
+// the waves' bounds. Only the threads whose maximum reaches it read their part again and collect what reaches it in LDS; every
+// candidate counts how many come before it (higher, or equal at a lower index). More candidates than the list holds (rows of many
+// equal logits) are found one after the other instead.
 //
 // Bound by memory: 2 (bf16) or 4 bytes a logit, beside one exponential and ten other operations.
 #include "abridgekv_amd.h"
@@ -104,6 +104,29 @@ __device__ __forceinline__ Running joined(const Running& a, const Running& b, fl
   r.e = fa * (a.e + da * a.l) + fb * (b.e + db * b.l);
   return r;
 }
+__device__ __forceinline__ float wave_max(float v) {
+  v = fmaxf(v, dpp<kDppXor1>(v));
+  v = fmaxf(v, dpp<kDppXor2>(v));
+  v = fmaxf(v, dpp<kDppHalfMirror>(v));
+  v = fmaxf(v, dpp<kDppMirror>(v));
+  return max_xor32(max_xor16(v));
+}
+__device__ __forceinline__ float wave_sum(float v) {
+  v += dpp<kDppXor1>(v);
+  v += dpp<kDppXor2>(v);
+  v += dpp<kDppHalfMirror>(v);
+  v += dpp<kDppMirror>(v);
+  return sum_xor32(sum_xor16(v));
+}
+// The lanes' sums in one, in every lane.
+__device__ __forceinline__ Running wave_joined(const Running& a, float c) {
+  Running r;
+  r.m = wave_max(a.m);
+  const float d = a.m - r.m, f = fast_exp2(d * c);
+  r.l = wave_sum(a.l * f);
+  r.e = wave_sum(f * (a.e + d * a.l));
+  return r;
+}
 template <int N, bool kEntropy>
 __device__ __forceinline__ void take(Running& st, const float (&raw)[N], float c) {
   float x[N], mx = st.m;
@@ -147,6 +170,14 @@ __device__ __forceinline__ void store_top(const LogprobArgs& a, long t, int rank
   a.top_logprobs[t * a.top + rank] = (order_value((uint32_t)(key >> 32)) - m) * a.inv_t - log_l;
 }
 
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+  v = max(v, dpp<kDppXor1>(v));
+  v = max(v, dpp<kDppXor2>(v));
+  v = max(v, dpp<kDppHalfMirror>(v));
+  v = max(v, dpp<kDppMirror>(v));
+  v = max(v, (uint32_t)__shfl_xor((int)v, 16, 64));
+  return max(v, (uint32_t)__shfl_xor((int)v, 32, 64));
+}
 __device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
 #pragma unroll
   for (int k = 1; k < 64; k <<= 1) {
@@ -185,9 +216,7 @@ __global__ __launch_bounds__(kRowThreads) void logprob_kernel(LogprobArgs a) {
     take<1, kEntropy>(st, x, c);
   }
   const float mine = st.m;                                   // this thread's largest (kLowest for -inf and none)
-#pragma unroll
-  for (int k = 1; k < 64; k <<= 1)
-    st = joined(st, Running{__shfl_xor(st.m, k, 64), __shfl_xor(st.l, k, 64), __shfl_xor(st.e, k, 64)}, c);
+  st = wave_joined(st, c);
   __shared__ Running wave_st[kWaves];
   __shared__ float row_m, row_log_l;
   if (lane == 0) wave_st[wave] = st;
@@ -207,24 +236,21 @@ __global__ __launch_bounds__(kRowThreads) void logprob_kernel(LogprobArgs a) {
   }
   if (a.top == 0) return;
 
-  // the top-th largest of the threads' maxima: each counts those before its own
-  __shared__ float maxima[kRowThreads];
   __shared__ uint64_t list[kListMax];
   __shared__ uint64_t wave_best[kWaves];
-  __shared__ float bound;
+  __shared__ float bounds[kWaves];
   __shared__ int count;
-  maxima[tid] = mine;
+  float bound = mine;                                        // the top-th largest of this wave's maxima, then of all waves' ones
+  float left = mine;
+  for (int k = 0; k < a.top; ++k) {
+    bound = wave_max(left);
+    if (lane == __ffsll(__ballot(left == bound)) - 1) left = -INFINITY;
+  }
+  if (lane == 0) bounds[wave] = bound;
   if (tid == 0) count = 0;
   __syncthreads();
-  int before = 0;
-#pragma unroll 4
-  for (int i = 0; i < kRowThreads; i += 4) {
-    const floatx4 m4 = *reinterpret_cast<const floatx4*>(&maxima[i]);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) before += m4[k] > mine || (m4[k] == mine && i + k < tid);
-  }
-  if (before == a.top - 1) bound = mine;
-  __syncthreads();
+  for (int w = 0; w < kWaves; ++w) bound = fmaxf(bound, bounds[w]);
   const float lowest = bound > kLowest ? bound : -INFINITY;  // (kLowest: fewer threads than `top` hold a finite logit)
   auto each = [&](auto&& f) {                                // every element of this thread
     for (int v = v0 + tid; v < v1; v += kRowThreads) {
@@ -285,31 +311,31 @@ __global__ __launch_bounds__(256) void logprob_join_kernel(LogprobArgs a) {
   const int tid = threadIdx.x, lane = tid & 63;
   const T* row = static_cast<const T*>(a.logits) + t * a.stride;
   const float c = a.inv_t * kLog2e;
-  __shared__ float row_m, row_log_l;
   __shared__ uint64_t list[kMergeMax];
   const int n = a.splits * a.top;                            // at most kMergeMax (the host's choice of splits)
   for (int i = tid; i < n; i += 256) list[i] = a.part_top[t * n + i];
-  if (tid < 64) {
-    Running st{kLowest, 0.f, 0.f};
-    for (int s = lane; s < a.splits; s += 64) {
-      const float* p = a.part + (t * a.splits + s) * 3;
-      st = joined(st, Running{p[0], p[1], p[2]}, c);
-    }
-#pragma unroll
-    for (int k = 1; k < 64; k <<= 1)
-      st = joined(st, Running{__shfl_xor(st.m, k, 64), __shfl_xor(st.l, k, 64), __shfl_xor(st.e, k, 64)}, c);
-    if (lane == 0) {
-      row_m = st.m;
-      row_log_l = finish_row(a, t, row, st);
-    }
+  Running st{kLowest, 0.f, 0.f};
+  if (tid < a.splits) {                                      // (at most 64 splits)
+    const float* p = a.part + (t * a.splits + tid) * 3;
+    st = Running{p[0], p[1], p[2]};
   }
   __syncthreads();
-  for (int i = tid; i < n; i += 256) {
-    const uint64_t key = list[i];
-    if (key == 0) continue;
-    int rank = 0;
-    for (int k = 0; k < n; ++k) rank += list[k] > key;
-    if (rank < a.top) store_top(a, t, rank, key, row_m, row_log_l);
+  if (tid >= 64) return;
+  st = wave_joined(st, c);
+  float log_l = 0.f;
+  if (lane == 0) log_l = finish_row(a, t, row, st);
+  log_l = __shfl(log_l, 0, 64);
+  // Every split's candidates lie in order, and a split's come before the next one's: the largest of the splits' first ones, at the
+  // first split that has it, again and again.
+  const uint64_t* next = list + (lane < a.splits ? lane * a.top : 0);
+  int left = lane < a.splits ? a.top : 0;
+  for (int rank = 0; rank < a.top; ++rank) {
+    const uint64_t key = left > 0 ? *next : 0;
+    const uint32_t best = wave_max_u32((uint32_t)(key >> 32));
+    if (lane != __ffsll(__ballot((uint32_t)(key >> 32) == best)) - 1) continue;
+    store_top(a, t, rank, key, st.m, log_l);
+    ++next;
+    --left;
   }
 }
 
@@ -332,7 +358,8 @@ struct Grad {
   float m, c, a, b, log2_l;
   // p (-g - h (ln p + H)) / temperature, with ln p = y ln 2, y = (x - m) c - log2 l
   __device__ __forceinline__ float operator()(float x) const {
-    const float y = ((x < kLowest ? kLowest : x) - m) * c - log2_l;
+    float y = ((x < kLowest ? kLowest : x) - m) * c - log2_l;
+    y = y < -1000.f ? -1000.f : y;                           // (weighs nothing; its product with b stays finite)
     return fast_exp2(y) * (a + b * y);
   }
 };

@@ -1522,11 +1522,21 @@ def kv_read_int4(kv_cache: torch.Tensor, slot_mapping: torch.Tensor,
 
 
 def int4_split_pages(num_seqs: int, max_pages: int) -> int:
-    """Pages per split of a decode over a cache in 4 bits."""
+    """Pages per split of a decode over a cache in 4 bits, an even number of at most 64, for tables of ``max_pages``.
+
+    A compute unit holds two workgroups, and what has no full round of them waits for its slowest, so a split is as long as
+    leaves one workgroup on each of the 256 units (one sequence of 131000 rows: 32 pages 32.8 us, 16 pages 38.1; 32000 rows:
+    8 pages 16.8 us, 4 pages 20.4, 16 pages 19.7), or two where that would take more than 32 pages (32 sequences of 9500 rows:
+    40 pages 77 us, 64 pages 86, 20 pages 82). More than two rounds of 64 pages run in splits of 20, whose uneven ends weigh
+    little (256 sequences of 500 to 3000 rows: 134 us, in 48 pages 138, in 64 pages 145, in 8 pages 142)."""
     total = num_seqs * max_pages
-    most = min(64, max(4, -(-total // 1024) * 2))
+    most = -(-total // 256)
+    if most > 32:
+        most = -(-total // 512)
+        most = 20 if most > 64 else max(most, 20)
+    most = max(2, most)
     splits = -(-max_pages // most)
-    return -(-max_pages // (2 * splits)) * 2
+    return min(64, -(-max_pages // (2 * splits)) * 2)
 
 
 def decode_int4_bytes(num_seqs: int, max_pages: int, split_pages: int) -> int:

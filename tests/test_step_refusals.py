@@ -229,3 +229,14 @@ def test_c_entries_return_errors():
     assert L.abkv_qk_norm_rope_bwd_workspace_size(0, 5) == 0 and L.abkv_qk_norm_rope_bwd_workspace_size(2, 5) > 0
     assert L.abkv_decode_int4_workspace_size(2, 4, 4) == 0
     assert L.abkv_decode_int4_workspace_size(2, 4, 2) == 2 * 2 * 32 * (256 + 16)
+
+
+def test_int4_splits_fit_any_step():
+    """A split is an even number of pages up to 64, and 64 a split take no more than any longer table's own splits."""
+    for B in (1, 2, 7, 64, 300):
+        for longest in (1, 3, 63, 64, 65, 512, 513, 2048, 8191, 8193, 40000):
+            own = ops.int4_split_pages(B, longest)
+            assert own % 2 == 0 and 2 <= own <= 64
+            held = ops.decode_int4_bytes(B, longest, own)
+            for pages in {1, longest // 3 + 1, longest - 1 or 1, longest}:
+                assert ops.decode_int4_bytes(B, pages, 64) <= held
