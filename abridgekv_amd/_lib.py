@@ -144,7 +144,9 @@ SIGNATURES = {
     "abkv_decode_int4_workspace_size": (C.c_size_t, [C.c_int] * 3),
     "abkv_decode_attn_int4": (C.c_int, [_vp, C.c_long, C.c_long, _vp, C.c_int, _vp, C.c_long, _vp, C.c_int, C.c_int, C.c_int,
                                         C.c_float, _vp, C.c_long, C.c_long, _vp, _vp, C.c_size_t, _vp]),
-    "abkv_kv_widen_int4": (C.c_int, [_vp, C.c_int, _vp, C.c_long, _vp, C.c_int, C.c_int, _vp, _vp, C.c_int, _vp]),
+    "abkv_paged_prefill_attn_items_int4": (C.c_int, [_vp, C.c_long, C.c_long, _vp, C.c_int, _vp, C.c_long, C.c_int, _vp,
+                                                _vp, _vp, _vp, _vp, _vp, C.c_int, _vp, C.c_int, C.c_int, C.c_float,
+                                                _vp, C.c_long, C.c_long, _vp, _vp, C.c_size_t, _vp]),
     "abkv_token_logprobs_workspace_size": (C.c_size_t, [C.c_int] * 4),
     "abkv_token_logprobs": (C.c_int, [C.c_int, _vp, C.c_long, C.c_int, C.c_int, _vp, C.c_float, C.c_int, _vp, _vp, _vp, _vp,
                                       _vp, _vp, C.c_size_t, _vp]),

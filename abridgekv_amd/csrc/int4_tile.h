@@ -1,0 +1,273 @@
+// Attention tiles over a paged cache in 4 bits (int4.h), for the multi-query kernel (gfx950).
+//
+// The waves unpack a 64-key tile of codes into K and V tiles of fp16 in LDS, laid out as attn_tile.h's, and attend to them with
+// v_mfma_f32_16x16x32_f16. fp16 keeps a value m + s c to 2^-12 of itself where bf16 (the type that the cache is written from)
+// would round it a second time, to 2^-9; the weights gain as much. Its range is made up for by powers of two, which are exact:
+//   K: 2^eK for each page, multiplied back into the page's scores;
+//   Q: 2^eQ for each query row and head, likewise;
+//   V: 2^eV for all of a walk, the largest need of its tiles so far; the output's sums are rescaled when it grows.
+// An exponent is a multiple of 8 (it hardly ever moves), and leaves the largest value in [2^7, 2^15).
+//
+// Wave w unpacks page w % 4 of K (waves 0 .. 3) or V (4 .. 7): 20 bytes a slot and head in place of 256, so that a tile costs each
+// lane two 16-byte loads and about 80 VALU operations, beside 200 for its part of the softmax.
+#pragma once
+#include "attn_tile.h"
+#include "int4.h"
+
+namespace abkv {
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ floatx4 mfma16x16x32(const f16x8 a, const f16x8 b, floatx4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// One sequence in the cache.
+struct Int4Rows {
+  const char* kv;
+  int kvh;
+  const int32_t* table;    // the sequence's page-table row
+  int width;               // entries in the row
+  int num_pages;
+};
+
+// A lane's part of a page: words 4 (lane % 4) .. + 3 of slot lane / 4, and the slot's four pairs.
+struct Int4Part {
+  u32x4 codes, pairs;
+};
+__device__ __forceinline__ Int4Part load_part(const Int4Rows& rows, int page, bool v, int lane) {
+  const __attribute__((address_space(4))) int32_t* table = (const __attribute__((address_space(4))) int32_t*)rows.table;
+  const int id = min(max(table[min(page, rows.width - 1)], 0), rows.num_pages - 1);
+  const char* slot = rows.kv + (long)id * kPage4 + (v ? kHalf4 : 0) + (lane >> 2) * kSlot4;
+  Int4Part p;
+  p.codes = *reinterpret_cast<const u32x4*>(slot + rows.kvh * kHeadCodes4 + 16 * (lane & 3));
+  p.pairs = *reinterpret_cast<const u32x4*>(slot + kParams4 + 16 * rows.kvh);
+  return p;
+}
+
+// The exponent that values up to `bound` take; at least `lowest` (a multiple of 8).
+__device__ __forceinline__ int range_exp(float bound, int lowest) {
+  const int e = (int)(__float_as_uint(bound) >> 23) - 127 - 14;
+  return max((e + 7) & ~7, lowest);
+}
+__device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+// K and Q: no lower than 2^-40, so that their product with the softmax's scale stays a number; V: as low as its reciprocal goes.
+constexpr int kLowestQK = -40, kLowestV = -104;
+
+// The largest |value| of a page, in every lane.
+__device__ __forceinline__ float page_bound(const Int4Part& p) {
+  float x = 0.f;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const float s = bf16_lo(p.pairs[g]), m = bf16_hi(p.pairs[g]);
+    x = fmaxf(x, fmaxf(fabsf(m), fabsf(fmaf(15.f, s, m))));
+  }
+  x = fmaxf(x, dpp<kDppHalfMirror>(x));                      // (the lanes of a quad have the same pairs)
+  x = fmaxf(x, dpp<kDppMirror>(x));
+  return max_xor32(max_xor16(x));
+}
+
+// A lane's part as fp16 values over 2^e, to slot `row` of a tile.
+__device__ __forceinline__ void unpack_part(const Int4Part& p, int e, __bf16* tile, int row, int lane) {
+  const float f = exp2i(-e);
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {                              // word 4 (lane % 4) + g: dims 32 g + 8 (lane % 4) .. + 7
+    const _Float16 s = (_Float16)(bf16_lo(p.pairs[g]) * f), m = (_Float16)(bf16_hi(p.pairs[g]) * f);
+    u32x4 x;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {                            // 1024 + c, c, m + s c: one rounding, of the last
+      const uint32_t c = ((p.codes[g] >> (4 * n)) & 0x000f000fu) | 0x64006400u;
+      const f16x2 code = __builtin_bit_cast(f16x2, c) - f16x2{(_Float16)1024.f, (_Float16)1024.f};
+      x[n] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(code, f16x2{s, s}, f16x2{m, m}));
+    }
+    *reinterpret_cast<u32x4*>(tile + row * kHeadDim + 8 * ((4 * g + (lane & 3)) ^ (row & 15))) = x;
+  }
+}
+
+// attend_tiles over rows in 4 bits: same walk (contiguous tiles), masks, lanes and results. Iteration n attends to tile n and unpacks K of tile
+// n + 2 (whose scores iteration n + 1 takes) and V of tile n + 1, from what the iteration before loaded; one barrier each.
+template <int H, int kWaves, class Walk, class Lane>
+__device__ __forceinline__ void attend_tiles_int4(const Int4Rows& rows, Walk& walk, int n_keys,
+                                                  __bf16* const (&K)[kStages], __bf16* const (&V)[kStages],
+                                                  const bf16x8 (&qop)[H][4], floatx4 (&o)[8][H], float (&m_run)[H],
+                                                  float (&l_run)[H], const Lane& lane_mask, float scale_log2, int w, int lane) {
+  static_assert(kWaves == 8 && kBN == 4 * kPage, "a wave a page of K or V");
+  const int m16 = lane & 15, j = lane >> 4;
+  const bool is_v = w >= 4;
+  const int page = w & 3, row = 16 * page + (lane >> 2);
+  const int tiles = walk.kt_end - walk.kt_begin;
+  if (tiles <= 0) return;
+  __shared__ __attribute__((aligned(16))) float k_scale[4][4]; // [tile % 4][page]: 2^eK
+  __shared__ int v_need[2][4];                               // [tile % 2][page]
+
+  f16x8 q[H][4];
+  float scale[H];
+#pragma unroll
+  for (int u = 0; u < H; ++u) {
+    float x = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int d = 0; d < 8; ++d) x = fmaxf(x, fabsf((float)qop[u][i][d]));
+    const int e = range_exp(max_xor32(max_xor16(x)), kLowestQK);
+    const float f = exp2i(-e);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int d = 0; d < 8; ++d) q[u][i][d] = (_Float16)((float)qop[u][i][d] * f);
+    scale[u] = scale_log2 * exp2i(e);
+  }
+
+  // This wave's part of tile i of the walk; slots past the last key read as zeros (their weights are 0)
+  auto load = [&](int i) {
+    const int k0 = (walk.kt_begin + i) * kBN;
+    Int4Part p = load_part(rows, (k0 >> 4) + page, is_v, lane);
+    if (k0 + row >= n_keys) p.pairs = u32x4{0, 0, 0, 0};
+    return p;
+  };
+  auto unpack_k = [&](const Int4Part& p, float bound, int i) {
+    const int e = range_exp(bound, kLowestQK);
+    if (lane == 0) k_scale[i & 3][page] = exp2i(e);
+    unpack_part(p, e, i & 1 ? K[1] : K[0], row, lane);
+  };
+  auto needed = [&](int i) { return max(max(v_need[i & 1][0], v_need[i & 1][1]), max(v_need[i & 1][2], v_need[i & 1][3])); };
+  int v_exp;
+  Int4Part next = load(0);
+  {
+    const float bound = page_bound(next);
+    if (is_v) {
+      if (lane == 0) v_need[0][page] = range_exp(bound, kLowestV);
+    } else {
+      unpack_k(next, bound, 0);
+      next = load(1);
+      unpack_k(next, page_bound(next), 1);
+    }
+    __syncthreads();
+    v_exp = needed(0);
+    if (is_v) unpack_part(next, v_exp, V[0], row, lane);
+    next = load(is_v ? 1 : 2);
+  }
+  __syncthreads();
+  floatx4 lsum[H];
+#pragma unroll
+  for (int u = 0; u < H; ++u) lsum[u] = floatx4{0.f, 0.f, 0.f, 0.f};
+  const f16x2 one2 = {(_Float16)1.f, (_Float16)1.f};
+  const f16x8 ones = {one2[0], one2[0], one2[0], one2[0], one2[0], one2[0], one2[0], one2[0]};
+
+  auto scores = [&](const __bf16* buf, floatx4 (&s)[2][2][H]) {
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int u = 0; u < H; ++u) s[kk][t][u] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const f16x8 kop = __builtin_bit_cast(f16x8, lds16(buf, 32 * kk + 16 * t + m16, 4 * i + j));
+#pragma unroll
+          for (int u = 0; u < H; ++u) s[kk][t][u] = mfma16x16x32(kop, q[u][i], s[kk][t][u]);
+        }
+  };
+  floatx4 sa[2][2][H], sb[2][2][H];
+  scores(K[0], sa);
+
+  int k0 = 0;
+  TileMask tm;
+  auto step = [&](floatx4 (&s)[2][2][H], floatx4 (&s_next)[2][2][H], auto slot_c, int n) {
+    constexpr int slot = decltype(slot_c)::value;
+    const Int4Part part = next;
+    next = load(n + (is_v ? 2 : 3));
+    const float bound = page_bound(part);
+    if (is_v && lane == 0) v_need[slot ^ 1][page] = range_exp(bound, kLowestV);
+    __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    __asm__ volatile("" ::: "memory");
+    const int v_next = max(v_exp, needed(n + 1));
+    const floatx4 kf = *reinterpret_cast<const floatx4*>(k_scale[n & 3]);
+    walk.next(k0, tm, n == 0);
+    tile_mask<H, Walk>(s, k0, tm, lane_mask, j);
+    // online softmax, as tile_softmax: the log2 scores relative to the running maximum, which moves when a score passes it by
+    // more than 8
+    float neg_m[H];
+    bool need = false;
+#pragma unroll
+    for (int u = 0; u < H; ++u) {
+      neg_m[u] = m_run[u] == -INFINITY ? 0.f : -m_run[u];
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const float f = scale[u] * kf[2 * kk + t];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[kk][t][u][r] = fmaf(s[kk][t][u][r], f, neg_m[u]);
+        }
+      need |= lane_max(s, u) > (m_run[u] == -INFINITY ? -INFINITY : 8.f);
+    }
+    if (__any(need)) {
+#pragma unroll
+      for (int u = 0; u < H; ++u) {
+        const float tmax = max_xor32(max_xor16(lane_max(s, u)));
+        const float m_new = fmaxf(m_run[u], tmax - neg_m[u]);
+        const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run[u] - m_new);
+        const float d = m_new == -INFINITY ? 0.f : m_new + neg_m[u];
+        m_run[u] = m_new;
+        lsum[u] *= alpha;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i][u] *= alpha;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) s[kk][t][u] -= d;
+      }
+    }
+    f16x8 pop[2][H];
+#pragma unroll
+    for (int u = 0; u < H; ++u)
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) pop[kk][u][e] = (_Float16)fast_exp2(s[kk][e >> 2][u][e & 3]);
+    scores(K[slot ^ 1], s_next);                             // (past the last tile: zeros, discarded)
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        const f16x8 vop = __builtin_bit_cast(f16x8, vt_operand(V[slot], 32 * kk, t, lane));
+#pragma unroll
+        for (int u = 0; u < H; ++u) o[t][u] = mfma16x16x32(vop, pop[kk][u], o[t][u]);
+      }
+#pragma unroll
+      for (int u = 0; u < H; ++u) lsum[u] = mfma16x16x32(ones, pop[kk][u], lsum[u]);
+    }
+    if (is_v) unpack_part(part, v_next, V[slot ^ 1], row, lane);
+    else unpack_k(part, bound, n + 2);
+    if (v_next != v_exp) {
+      const float f = exp2i(max(v_exp - v_next, -126));
+#pragma unroll
+      for (int u = 0; u < H; ++u)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i][u] *= f;
+      v_exp = v_next;
+    }
+  };
+  for (int n = 0;;) {
+    step(sa, sb, Slot<0>{}, n);
+    if (++n >= tiles) break;
+    step(sb, sa, Slot<1>{}, n);
+    if (++n >= tiles) break;
+  }
+  const float f = exp2i(v_exp);
+#pragma unroll
+  for (int u = 0; u < H; ++u) {
+    l_run[u] = lsum[u][0];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i][u] *= f;
+  }
+}
+
+}  // namespace abkv

@@ -1,5 +1,4 @@
-// The paged cache in 4 bits (int4.h): rows written and read back, single-token attention over it, and its pages widened for the
-// multi-query kernel (gfx950).
+// The paged cache in 4 bits (int4.h): rows written and read back, and single-token attention over it (gfx950).
 #include "abridgekv_amd.h"
 #include "int4.h"
 
@@ -445,36 +444,6 @@ __global__ __launch_bounds__(16 * kGroups) void decode4_merge_kernel(Decode4Args
     a.lse[(long)b * kHeadsQ + head] = L > 0.f ? (M + __log2f(L)) * 0.69314718055994531f : L == 0.f ? -INFINITY : L;
 }
 
-// -- pages widened for the multi-query kernel -----------------------------------------------------------------------------
-// Workgroup per page of a request: the page in bf16 ([2][16][8][128]), and its place in the requests' table of such pages.
-// starts [R + 1]: first widened page of each request. A value m + s c is rounded to bf16 (2^-8 of it), as the multi-query
-// kernel's tiles hold them.
-__global__ __launch_bounds__(512) void widen4_kernel(const char* cache, int num_pages, const int32_t* block_table, long bt_stride,
-                                                     const int32_t* starts, int num_requests, __bf16* pages, int32_t* table,
-                                                     int table_width) {
-  const int p = blockIdx.x;
-  int r = 0;
-  while (r + 1 < num_requests && p >= starts[r + 1]) ++r;
-  const int i = p - starts[r];
-  if (threadIdx.x == 0) table[(long)r * table_width + i] = p;
-  const char* from = cache + (long)min(max(block_table[(long)r * bt_stride + i], 0), num_pages - 1) * kPage4;
-  __bf16* to = pages + (long)p * kPageElems;
-  // thread: 8 dims of a head, of every fourth slot
-  const int b = threadIdx.x & 15, h = (threadIdx.x >> 4) & 7;
-#pragma unroll
-  for (int n = 0; n < 8; ++n) {
-    const int row = 4 * n + (threadIdx.x >> 7), half = row >> 4, slot = row & 15;      // of the page's 32
-    const char* s = from + half * kHalf4 + slot * kSlot4;
-    float x[8];
-    values8(reinterpret_cast<const uint32_t*>(s + h * kHeadCodes4)[code_word(b)],
-            reinterpret_cast<const uint32_t*>(s + kParams4 + h * 16)[b >> 2], x);
-    u32x4 w;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) w[k] = pack_bf16x2(x[2 * k], x[2 * k + 1]);
-    *reinterpret_cast<u32x4*>(to + half * kHalfElems + slot * kSlotElems + h * kHeadDim + 8 * b) = w;
-  }
-}
-
 }  // namespace abkv
 
 using namespace abkv;
@@ -557,18 +526,6 @@ int abkv_decode_attn_int4(const void* q, long q_stride_seq, long q_stride_head, 
   if (err != hipSuccess || a.max_splits == 1) return (int)err;
   if (a.max_splits > 64) hipLaunchKernelGGL(decode4_merge_kernel<64>, dim3(kHeadsQ, num_seqs), dim3(1024), 0, stream, a);
   else hipLaunchKernelGGL(decode4_merge_kernel<16>, dim3(kHeadsQ, num_seqs), dim3(256), 0, stream, a);
-  return (int)hipGetLastError();
-}
-
-int abkv_kv_widen_int4(const void* kv_cache, int num_pages, const int32_t* block_table, long block_table_stride,
-                       const int32_t* page_starts, int num_requests, int total_pages, void* pages, int32_t* table,
-                       int table_width, hipStream_t stream) {
-  if (num_requests <= 0 || total_pages <= 0) return 0;
-  if (!rows16_ok(kv_cache, 0, 0) || num_pages <= 0 || block_table == nullptr || page_starts == nullptr || !rows16_ok(pages, 0, 0) ||
-      table == nullptr || table_width <= 0 || total_pages > 0x007fffff)
-    return (int)hipErrorInvalidValue;
-  hipLaunchKernelGGL(widen4_kernel, dim3(total_pages), dim3(512), 0, stream, static_cast<const char*>(kv_cache), num_pages,
-                     block_table, block_table_stride, page_starts, num_requests, static_cast<__bf16*>(pages), table, table_width);
   return (int)hipGetLastError();
 }
 

@@ -10,7 +10,8 @@
 // Prompt chunks are the causal case with kv_limit = seq_len. Same tile machinery as the masked-prefill kernel
 // (attn_tile.h): 8 waves x (16 rows x 2 heads), 64-key tiles DMA'd from the page table into double-buffered LDS. A mixed
 // batch runs the work items of a host plan (paged_plan.cpp), in which only long key ranges are split.
-#include "attn_tile.h"
+#include "abridgekv_amd.h"
+#include "int4_tile.h"
 
 namespace abkv {
 
@@ -109,10 +110,12 @@ struct RangeWalk {
   }
 };
 
-// kSide = false: the paged rows of the request; true: its side rows (all visible to every query).
-template <bool kSide>
+// kRows: the paged rows of the request; its side rows (all visible to every query); its rows in a cache of 4 bits.
+constexpr int kPagedRows = 0, kSideRows = 1, kInt4Rows = 2;
+template <int kRows>
 __global__ __launch_bounds__(512, 1) void paged_prefill_kernel(PagedPrefillArgs a) {
   constexpr int H = 2, kWaves = 8;
+  constexpr bool kSide = kRows == kSideRows;
   __shared__ __attribute__((aligned(16))) __bf16 K0[kTileElems], K1[kTileElems], K2[kTileElems];
   __shared__ __attribute__((aligned(16))) __bf16 V0[kTileElems], V1[kTileElems], V2[kTileElems];
   __bf16* const Kbuf[kStages] = {K0, K1, K2};
@@ -212,6 +215,11 @@ __global__ __launch_bounds__(512, 1) void paged_prefill_kernel(PagedPrefillArgs 
                           2L * a.side_rows * kHeadDim, (long)a.side_rows * kHeadDim};
     attend_tiles<H, kWaves>(rows, walk, k_end, Kbuf, Vbuf, qop, o, m_run, l_run, CausalLane{lane_limit}, a.scale_log2,
                             w, lane);
+  } else if constexpr (kRows == kInt4Rows) {
+    const Int4Rows rows{reinterpret_cast<const char*>(a.kv), kvh, a.block_table + (long)r * a.bt_stride, a.bt_width,
+                        a.num_pages};
+    attend_tiles_int4<H, kWaves>(rows, walk, k_end, Kbuf, Vbuf, qop, o, m_run, l_run, CausalLane{lane_limit}, a.scale_log2,
+                                 w, lane);
   } else {
     const PagedRows rows{a.kv + kvh * kHeadDim, a.block_table + (long)r * a.bt_stride, a.bt_width, a.num_pages};
     attend_tiles<H, kWaves>(rows, walk, k_end, Kbuf, Vbuf, qop, o, m_run, l_run, CausalLane{lane_limit}, a.scale_log2,
@@ -367,6 +375,65 @@ unsigned paged_grid(int num_tiles, int splits) {
 }
 }  // namespace
 
+using namespace abkv;
+
+static int prefill_items(bool int4, const void* q, long q_stride_t, long q_stride_h, const void* kv_cache, int num_pages,
+                         const int32_t* block_table, long block_table_stride, int block_table_width,
+                         const int32_t* q_start, const int32_t* kv_start, const int32_t* kv_limit,
+                         const int32_t* kv_excluded, const int32_t* causal, const int32_t* items, int n_items,
+                         const int32_t* merges, int n_merges, int part_rows, float scale, void* out,
+                         long out_stride_t, long out_stride_h, float* lse, void* workspace,
+                         size_t workspace_bytes, hipStream_t stream) {
+  if (n_items <= 0) return 0;
+  if (q == nullptr || kv_cache == nullptr || block_table == nullptr || q_start == nullptr || kv_start == nullptr ||
+      kv_limit == nullptr || causal == nullptr || items == nullptr || out == nullptr || num_pages <= 0 ||
+      block_table_width <= 0 || n_merges < 0 || part_rows < 0 || (n_merges > 0 && merges == nullptr) ||
+      (part_rows > 0 && (workspace == nullptr || workspace_bytes < abkv_paged_prefill_items_workspace_size(part_rows))) ||
+      part_rows % kBM != 0 || (long)n_merges * 8 * kHeadsKV * 256 > 0xFFFFFFFFL)
+    return (int)hipErrorInvalidValue;
+  PagedPrefillArgs a;
+  a.q = static_cast<const __bf16*>(q);
+  a.q_st = q_stride_t;
+  a.q_sh = q_stride_h;
+  a.kv = static_cast<const __bf16*>(kv_cache);
+  a.num_pages = num_pages;
+  a.block_table = block_table;
+  a.bt_stride = block_table_stride;
+  a.bt_width = block_table_width;
+  a.q_start = q_start;
+  a.kv_start = kv_start;
+  a.kv_limit = kv_limit;
+  a.kv_excluded = kv_excluded;
+  a.tile_req = a.tile_q0 = nullptr;
+  a.causal = causal;
+  a.causal_default = 1;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.out = static_cast<__bf16*>(out);
+  a.o_st = out_stride_t;
+  a.o_sh = out_stride_h;
+  a.lse = lse;
+  a.items = items;
+  a.merges = merges;
+  a.num_tiles = 0;
+  a.split_tiles = 0;
+  a.num_tokens = 0;
+  a.part_o = nullptr;
+  a.part_ml = nullptr;
+  a.item_o = static_cast<float*>(workspace);
+  a.item_ml = a.item_o + (size_t)part_rows * kHeadsQ * kHeadDim;
+  a.split_base = 0;
+  a.head_quota = nullptr;
+  a.side_count = nullptr;
+  const unsigned grid = paged_grid(n_items, 1);
+  if (grid == 0) return (int)hipErrorInvalidValue;
+  if (int4) hipLaunchKernelGGL(paged_prefill_kernel<kInt4Rows>, dim3(grid), dim3(512), 0, stream, a);
+  else hipLaunchKernelGGL(paged_prefill_kernel<kPagedRows>, dim3(grid), dim3(512), 0, stream, a);
+  hipError_t err = hipGetLastError();
+  if (err != hipSuccess || n_merges == 0) return (int)err;
+  hipLaunchKernelGGL(paged_merge_items_kernel, dim3((unsigned)n_merges * 8 * kHeadsKV), dim3(256), 0, stream, a);
+  return (int)hipGetLastError();
+}
+
 extern "C" {
 
 size_t abkv_paged_prefill_workspace_size(int num_tokens, int num_splits) {
@@ -435,7 +502,7 @@ int abkv_paged_prefill_attn(const void* q, long q_stride_t, long q_stride_h, con
   const unsigned grid = paged_grid(num_tiles, num_splits > 1 ? num_splits : 1);
   if (grid == 0) return (int)hipErrorInvalidValue;
   a.num_tiles = num_tiles;
-  hipLaunchKernelGGL(paged_prefill_kernel<false>, dim3(grid), dim3(512), 0, stream, a);
+  hipLaunchKernelGGL(paged_prefill_kernel<kPagedRows>, dim3(grid), dim3(512), 0, stream, a);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess || num_splits <= 1) return (int)err;
   hipLaunchKernelGGL(paged_merge_kernel, dim3(num_tokens, kHeadsQ / 8), dim3(256), 0, stream, a, num_splits);
@@ -449,54 +516,24 @@ int abkv_paged_prefill_attn_items(const void* q, long q_stride_t, long q_stride_
                                   const int32_t* merges, int n_merges, int part_rows, float scale, void* out,
                                   long out_stride_t, long out_stride_h, float* lse, void* workspace,
                                   size_t workspace_bytes, hipStream_t stream) {
-  using namespace abkv;
-  if (n_items <= 0) return 0;
-  if (q == nullptr || kv_cache == nullptr || block_table == nullptr || q_start == nullptr || kv_start == nullptr ||
-      kv_limit == nullptr || causal == nullptr || items == nullptr || out == nullptr || num_pages <= 0 ||
-      block_table_width <= 0 || n_merges < 0 || part_rows < 0 || (n_merges > 0 && merges == nullptr) ||
-      (part_rows > 0 && (workspace == nullptr || workspace_bytes < abkv_paged_prefill_items_workspace_size(part_rows))) ||
-      part_rows % kBM != 0 || (long)n_merges * 8 * kHeadsKV * 256 > 0xFFFFFFFFL)
-    return (int)hipErrorInvalidValue;
-  PagedPrefillArgs a;
-  a.q = static_cast<const __bf16*>(q);
-  a.q_st = q_stride_t;
-  a.q_sh = q_stride_h;
-  a.kv = static_cast<const __bf16*>(kv_cache);
-  a.num_pages = num_pages;
-  a.block_table = block_table;
-  a.bt_stride = block_table_stride;
-  a.bt_width = block_table_width;
-  a.q_start = q_start;
-  a.kv_start = kv_start;
-  a.kv_limit = kv_limit;
-  a.kv_excluded = kv_excluded;
-  a.tile_req = a.tile_q0 = nullptr;
-  a.causal = causal;
-  a.causal_default = 1;
-  a.scale_log2 = scale * 1.4426950408889634f;
-  a.out = static_cast<__bf16*>(out);
-  a.o_st = out_stride_t;
-  a.o_sh = out_stride_h;
-  a.lse = lse;
-  a.items = items;
-  a.merges = merges;
-  a.num_tiles = 0;
-  a.split_tiles = 0;
-  a.num_tokens = 0;
-  a.part_o = nullptr;
-  a.part_ml = nullptr;
-  a.item_o = static_cast<float*>(workspace);
-  a.item_ml = a.item_o + (size_t)part_rows * kHeadsQ * kHeadDim;
-  a.split_base = 0;
-  a.head_quota = nullptr;
-  a.side_count = nullptr;
-  const unsigned grid = paged_grid(n_items, 1);
-  if (grid == 0) return (int)hipErrorInvalidValue;
-  hipLaunchKernelGGL(paged_prefill_kernel<false>, dim3(grid), dim3(512), 0, stream, a);
-  hipError_t err = hipGetLastError();
-  if (err != hipSuccess || n_merges == 0) return (int)err;
-  hipLaunchKernelGGL(paged_merge_items_kernel, dim3((unsigned)n_merges * 8 * kHeadsKV), dim3(256), 0, stream, a);
-  return (int)hipGetLastError();
+  return prefill_items(false, q, q_stride_t, q_stride_h, kv_cache, num_pages, block_table, block_table_stride, block_table_width, q_start, kv_start,
+                       kv_limit, kv_excluded, causal, items, n_items, merges, n_merges, part_rows, scale, out, out_stride_t,
+                       out_stride_h, lse, workspace, workspace_bytes, stream);
+}
+
+int abkv_paged_prefill_attn_items_int4(const void* q, long q_stride_t, long q_stride_h, const void* kv_cache, int num_pages,
+                                       const int32_t* block_table, long block_table_stride, int block_table_width,
+                                       const int32_t* q_start, const int32_t* kv_start, const int32_t* kv_limit,
+                                       const int32_t* kv_excluded, const int32_t* causal, const int32_t* items, int n_items,
+                                       const int32_t* merges, int n_merges, int part_rows, float scale, void* out,
+                                       long out_stride_t, long out_stride_h, float* lse, void* workspace,
+                                       size_t workspace_bytes, hipStream_t stream) {
+  if ((((uintptr_t)q | (uintptr_t)kv_cache | (uintptr_t)out) & 15) || ((q_stride_t | q_stride_h | out_stride_t | out_stride_h) & 7) ||
+      !softmax_scale_ok(scale))
+    return n_items <= 0 ? 0 : (int)hipErrorInvalidValue;
+  return prefill_items(true, q, q_stride_t, q_stride_h, kv_cache, num_pages, block_table, block_table_stride, block_table_width, q_start, kv_start,
+                       kv_limit, kv_excluded, causal, items, n_items, merges, n_merges, part_rows, scale, out, out_stride_t,
+                       out_stride_h, lse, workspace, workspace_bytes, stream);
 }
 
 int abkv_paged_prefill_attn_packed(const void* q, long q_stride_t, long q_stride_h, const void* kv_cache,
@@ -575,12 +612,12 @@ int abkv_paged_prefill_attn_packed(const void* q, long q_stride_t, long q_stride
   const unsigned grid_main = paged_grid(num_tiles, num_splits), grid_side = paged_grid(num_tiles, side_splits);
   if (grid_main == 0 || grid_side == 0) return (int)hipErrorInvalidValue;
   a.num_tiles = num_tiles;
-  hipLaunchKernelGGL(paged_prefill_kernel<false>, dim3(grid_main), dim3(512), 0, stream, a);
+  hipLaunchKernelGGL(paged_prefill_kernel<kPagedRows>, dim3(grid_main), dim3(512), 0, stream, a);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return (int)err;
   a.split_tiles = side_split_tiles;
   a.split_base = num_splits;
-  hipLaunchKernelGGL(paged_prefill_kernel<true>, dim3(grid_side), dim3(512), 0, stream, a);
+  hipLaunchKernelGGL(paged_prefill_kernel<kSideRows>, dim3(grid_side), dim3(512), 0, stream, a);
   err = hipGetLastError();
   if (err != hipSuccess) return (int)err;
   hipLaunchKernelGGL(paged_merge_kernel, dim3(num_tokens, kHeadsQ / 8), dim3(256), 0, stream, a, total);

@@ -697,6 +697,55 @@ def _excluded_pairs(excluded, B):
     return pairs if pairs[:, 1].max(initial=0) > 0 else None
 
 
+def _check_batch(q, dt, block_table, q_start, kv_start, kv_limit, causal, out, lse, excluded):
+    """(the requests' numbers as the plan takes them, B, rows, excluded pairs or None, out) of a multi-query call."""
+    qs = np.asarray(q_start, dtype=np.int64)
+    ks = np.asarray(kv_start, dtype=np.int64)
+    kl = np.asarray(kv_limit, dtype=np.int64)
+    B = ks.size
+    W = block_table.shape[1]
+    _require(qs.size == B + 1 and kl.size == B and B <= block_table.shape[0], "q_start [B+1], kv_start/kv_limit [B]")
+    _require(qs.ndim == ks.ndim == kl.ndim == 1 and np.ndim(causal) <= 1, "lengths and flags must be flat sequences")
+    T, total = q.shape[0], int(qs[-1])
+    _require(qs[0] == 0 and total <= T and (B == 0 or (qs[1:] >= qs[:-1]).all()), "q_start must be a prefix sum <= T")
+    _require(B == 0 or (kl.min() >= 0 and kl.max() <= W * PAGE), "kv_limit must lie in [0, block_table width * 16]")
+    _require(B == 0 or ks.min() >= 0, "kv_start must be non-negative")
+    if out is None:
+        out = torch.empty((T, HEADS_Q, HEAD_DIM), dtype=dt, device=q.device)
+    _require(out.dtype == dt and out.shape == (T, HEADS_Q, HEAD_DIM) and out.stride(2) == 1,
+             "out must be [T, 32, 128] (dtype of q) with contiguous dims")
+    if lse is not None:
+        _require(lse.dtype == torch.float32 and lse.is_contiguous() and tuple(lse.shape) == (T, HEADS_Q),
+                 "lse must be contiguous fp32 [T, 32]")
+    exd = _excluded_pairs(excluded, B)
+    if total == 0:
+        return None, B, total, exd, out
+    host = np.empty(4 * B + 1, np.int64)                     # q_start | kv_start | kv_limit | causal
+    host[: B + 1], host[B + 1: 2 * B + 1], host[2 * B + 1: 3 * B + 1], host[3 * B + 1:] = qs, ks, kl, causal
+    return host, B, total, exd, out
+
+
+def _prefill_items(name, q, kv_cache, block_table, host, B, exd, scale, out, lse):
+    """The work items of a batch's plan, through the entry ``name``."""
+    dev = q.device
+    ex = [] if exd is None else [exd.reshape(-1)]
+    o1, o2, o3, o4 = B + 1, 2 * B + 1, 3 * B + 1, 4 * B + 1
+    o5 = o4 + 2 * B * len(ex)                                # end of the excluded ranges
+    items, merges, part_rows = _paged_plan_from(host, B, _num_cus())
+    meta = _upload([host, *ex, items, merges], dev)
+    at = meta.data_ptr()
+    ws, ws_bytes = None, 0
+    if part_rows:
+        ws_bytes = lib().abkv_paged_prefill_items_workspace_size(part_rows)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    rc = getattr(lib(), name)(_ptr(q), q.stride(0), q.stride(1), _ptr(kv_cache), kv_cache.shape[0], _ptr(block_table),
+                              _row_stride(block_table), block_table.shape[1], at, at + 4 * o1, at + 4 * o2,
+                              at + 4 * o4 if ex else None, at + 4 * o3, at + 4 * o5, items.size // 5, at + 4 * (o5 + items.size),
+                              merges.size // 4, part_rows, scale, _ptr(out), out.stride(0), out.stride(1), _ptr(lse),
+                              _ptr(ws), ws_bytes, _stream())
+    check(rc, name)
+
+
 def paged_prefill_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, q_start, kv_start,
                             kv_limit, causal, scale: float | None = None, out: torch.Tensor | None = None,
                             lse: torch.Tensor | None = None, split: int | None = None, excluded=None):
@@ -719,31 +768,15 @@ def paged_prefill_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table
              and q.stride(2) == 1, "q must be cuda [T, 32, 128] with contiguous dims")
     _require(block_table.is_cuda and block_table.dtype == torch.int32 and block_table.dim() == 2
              and block_table.stride(1) == 1, "block_table must be cuda int32 [B, W]")
-    qs = np.asarray(q_start, dtype=np.int64)
-    ks = np.asarray(kv_start, dtype=np.int64)
-    kl = np.asarray(kv_limit, dtype=np.int64)
-    B = ks.size
-    W = block_table.shape[1]
-    _require(qs.size == B + 1 and kl.size == B and B <= block_table.shape[0], "q_start [B+1], kv_start/kv_limit [B]")
-    _require(qs.ndim == ks.ndim == kl.ndim == 1 and np.ndim(causal) <= 1, "lengths and flags must be flat sequences")
-    T, total = q.shape[0], int(qs[-1])
-    _require(qs[0] == 0 and total <= T and (B == 0 or (qs[1:] >= qs[:-1]).all()), "q_start must be a prefix sum <= T")
-    _require(B == 0 or (kl.min() >= 0 and kl.max() <= W * PAGE), "kv_limit must lie in [0, block_table width * 16]")
-    _require(B == 0 or ks.min() >= 0, "kv_start must be non-negative")
-    if out is None:
-        out = torch.empty((T, HEADS_Q, HEAD_DIM), dtype=dt, device=q.device)
-    _require(out.dtype == dt and out.shape == (T, HEADS_Q, HEAD_DIM) and out.stride(2) == 1,
-             "out must be [T, 32, 128] (dtype of q) with contiguous dims")
-    if lse is not None:
-        _require(lse.dtype == torch.float32 and lse.is_contiguous() and tuple(lse.shape) == (T, HEADS_Q),
-                 "lse must be contiguous fp32 [T, 32]")
-    exd = _excluded_pairs(excluded, B)
+    host, B, total, exd, out = _check_batch(q, dt, block_table, q_start, kv_start, kv_limit, causal, out, lse, excluded)
     if total == 0:
         return out, lse
     dev = q.device
     scale = default_scale() if scale is None else float(scale)
-    host = np.empty(4 * B + 1, np.int64)                     # q_start | kv_start | kv_limit | causal
-    host[: B + 1], host[B + 1: 2 * B + 1], host[2 * B + 1: 3 * B + 1], host[3 * B + 1:] = qs, ks, kl, causal
+    if split is None and not f32:
+        _prefill_items("abkv_paged_prefill_attn_items", q, kv_cache, block_table, host, B, exd, scale, out, lse)
+        return out, lse
+    qs, kl, W = host[: B + 1], host[2 * B + 1: 3 * B + 1], block_table.shape[1]
     o1, o2, o3, o4 = B + 1, 2 * B + 1, 3 * B + 1, 4 * B + 1
     ex = [] if exd is None else [exd.reshape(-1)]
     o5 = o4 + 2 * B * len(ex)                                # end of the excluded ranges
@@ -756,22 +789,6 @@ def paged_prefill_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table
                                                at + 4 * o3, 1, scale, _ptr(out), out.stride(0), out.stride(1),
                                                _ptr(lse), _stream())
         check(rc, "abkv_paged_prefill_attn_f32")
-        return out, lse
-    if split is None:
-        items, merges, part_rows = _paged_plan_from(host, B, _num_cus())
-        meta = _upload([host, *ex, items, merges], dev)
-        at = meta.data_ptr()
-        ws, ws_bytes = None, 0
-        if part_rows:
-            ws_bytes = lib().abkv_paged_prefill_items_workspace_size(part_rows)
-            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-        rc = lib().abkv_paged_prefill_attn_items(_ptr(q), q.stride(0), q.stride(1), _ptr(kv_cache), kv_cache.shape[0],
-                                                 _ptr(block_table), _row_stride(block_table), W, at, at + 4 * o1,
-                                                 at + 4 * o2, at + 4 * o4 if ex else None, at + 4 * o3, at + 4 * o5,
-                                                 items.size // 5, at + 4 * (o5 + items.size), merges.size // 4,
-                                                 part_rows, scale, _ptr(out), out.stride(0), out.stride(1), _ptr(lse),
-                                                 _ptr(ws), ws_bytes, _stream())
-        check(rc, "abkv_paged_prefill_attn_items")
         return out, lse
     nq = np.diff(qs)
     tr = np.asarray([(r, q0) for r in range(B) for q0 in range(0, int(nq[r]), 64)], dtype=np.int32)
@@ -1576,28 +1593,20 @@ def decode_attention_int4(q: torch.Tensor, kv_cache: torch.Tensor, block_table: 
 def paged_prefill_attention_int4(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, q_start, kv_start,
                                  kv_limit, causal, scale: float | None = None, out: torch.Tensor | None = None,
                                  lse: torch.Tensor | None = None, excluded=None):
-    """:func:`paged_prefill_attention` (prompt chunks and code steps; bf16 queries) over a cache in 4 bits, whose values the
-    tiles hold in bf16. Returns (out [T, 32, 128] bf16, lse [T, 32] fp32 or None)."""
+    """:func:`paged_prefill_attention` (prompt chunks and code steps; bf16 queries) over a cache in 4 bits, whose values and
+    weights the products take in fp16. Returns (out [T, 32, 128] bf16, lse [T, 32] fp32 or None)."""
     _check_cache4(kv_cache)
     _check_rows("q", q, torch.bfloat16, (q.shape[0] if q.dim() else 0, HEADS_Q, HEAD_DIM))
     _require(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[1] > 0
              and block_table.stride(1) == 1, "block_table must be int32 [B, W] with contiguous rows")
     scale = _softmax_scale(scale)
-    qs, kl = np.asarray(q_start, dtype=np.int64), np.asarray(kv_limit, dtype=np.int64)
-    R, W = kl.size, block_table.shape[1]
-    _require(kl.ndim == 1 and R <= block_table.shape[0] and (R == 0 or (kl.min() >= 0 and kl.max() <= W * PAGE)),
-             "kv_limit must lie in [0, block_table width * 16], one for each of at most the table's rows")
+    if out is not None:
+        _check_out(out, torch.bfloat16, (q.shape[0], HEADS_Q, HEAD_DIM))
+    host, B, total, exd, out = _check_batch(q, torch.bfloat16, block_table, q_start, kv_start, kv_limit, causal, out, lse, excluded)
     _check_device(q, kv_cache, block_table, out, lse)
-    starts = np.concatenate([[0], np.cumsum(-(-kl // PAGE))])
-    total, width = int(starts[-1]), max(1, int((-(-kl // PAGE)).max(initial=0)))
-    pages = torch.empty((max(1, total), *_PAGE_SHAPE), dtype=torch.bfloat16, device=q.device)
-    table = torch.empty((max(1, R), width), dtype=torch.int32, device=q.device)
     if total:
-        meta = _upload([starts], q.device)
-        rc = lib().abkv_kv_widen_int4(kv_cache.data_ptr(), kv_cache.shape[0], block_table.data_ptr(), _row_stride(block_table),
-                                      meta.data_ptr(), R, total, pages.data_ptr(), table.data_ptr(), width, _stream())
-        check(rc, "abkv_kv_widen_int4")
-    return paged_prefill_attention(q, pages, table, qs, kv_start, kl, causal, scale, out=out, lse=lse, excluded=excluded)
+        _prefill_items("abkv_paged_prefill_attn_items_int4", q, kv_cache, block_table, host, B, exd, scale, out, lse)
+    return out, lse
 
 
 # -- per-head norms and the rotation in one pass ---------------------------------------------------------------------------------

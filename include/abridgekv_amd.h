@@ -580,12 +580,15 @@ int abkv_decode_attn_int4(const void* q, long q_stride_seq, long q_stride_head, 
                           const int32_t* block_table, long block_table_stride, const int32_t* seq_lens, int num_seqs,
                           int max_pages_per_seq, int split_pages, float scale, void* out, long out_stride_seq,
                           long out_stride_head, float* lse, void* workspace, size_t workspace_bytes, abkv_stream_t stream);
-/* Pages of a batch's requests in bf16: page i of request r (the first page_starts[r + 1] - page_starts[r] of its table row) goes
- * to page page_starts[r] + i of `pages` [total_pages, 2, 16, 8, 128], and that number to table[r][i]: the cache and the page
- * table that abkv_paged_prefill_attn_items then takes. page_starts [num_requests + 1] on the device, page_starts[0] = 0. */
-int abkv_kv_widen_int4(const void* kv_cache, int num_pages, const int32_t* block_table, long block_table_stride,
-                       const int32_t* page_starts, int num_requests, int total_pages, void* pages, int32_t* table,
-                       int table_width, abkv_stream_t stream);
+/* abkv_paged_prefill_attn_items over a cache in 4 bits, whose values and weights the tiles hold in fp16 over powers of two (a
+ * value to 2^-12 of the largest of its row's page, or of its head's V so far). */
+int abkv_paged_prefill_attn_items_int4(const void* q, long q_stride_t, long q_stride_h, const void* kv_cache, int num_pages,
+                                       const int32_t* block_table, long block_table_stride, int block_table_width,
+                                       const int32_t* q_start, const int32_t* kv_start, const int32_t* kv_limit,
+                                       const int32_t* kv_excluded, const int32_t* causal, const int32_t* items, int n_items,
+                                       const int32_t* merges, int n_merges, int part_rows, float scale, void* out,
+                                       long out_stride_t, long out_stride_h, float* lse, void* workspace,
+                                       size_t workspace_bytes, abkv_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------------------------------
  * Log probabilities of given tokens: logits [num_tokens, vocab] bf16 or (f32 != 0) fp32, rows `stride` elements apart, of any

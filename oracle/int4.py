@@ -3,8 +3,9 @@
 Rows are quantised and read in numpy from the format's definition, dim by dim; attention is float64 over the values that the rows
 stand for. ``bounds`` derives how far a kernel may be off: it takes a weight times its row's step, rounded to bf16 (half a step,
 2^-8 of it), against a code less 8, and the weight in fp32 against the group's middle, and rounds the output; split partials are
-fp16 (2^-11 of the split's largest output, itself at most the largest value). ``wide``: the multi-query kernel instead holds
-every value rounded to bf16, and rounds the weights.
+fp16 (2^-11 of the split's largest output, itself at most the largest value). ``wide``: the multi-query kernel instead takes
+values and weights in fp16 (half a step, 2^-11 of each; its powers of two keep them, and what is 2^-21 of its row's or page's largest,
+in the type's normal range), and its partials are fp32.
 """
 from __future__ import annotations
 
@@ -12,6 +13,7 @@ import numpy as np
 
 HEADS, DIM, GROUP = 8, 128, 32
 EPS = 2.0 ** -8
+HALF = 2.0 ** -11              # of fp16
 SLACK = 1.02
 
 
@@ -89,9 +91,9 @@ def attend(q, k_rows, v_rows, vis, scale: float, wide: bool = False):
         if s.size == 0:
             continue
         # Scores in fp32: sums of up to 40 products (8 a lane, 4 lanes, the start of -128 sum q) of |q| (128 + c) s, beside the
-        # minimum's part; wide: of values rounded to bf16
+        # minimum's part; wide: of values rounded to fp16, in sums of 128
         size = np.abs(q[some, h]) @ (np.abs(k[:, u]) + (0 if wide else 136 * np.repeat(ks[:, u], GROUP, -1))).T
-        ds = scale * size * (40 * 2.0 ** -24 + (EPS if wide else 0)) + 2.0 ** -22 * np.abs(np.where(vis[some], s, 0))
+        ds = scale * size * (128 * 2.0 ** -24 + HALF if wide else 40 * 2.0 ** -24) + 2.0 ** -22 * np.abs(np.where(vis[some], s, 0))
         ds = np.where(vis[some], ds, 0)
         m = s.max(1, keepdims=True)
         p = np.exp(s - m)
@@ -102,7 +104,7 @@ def attend(q, k_rows, v_rows, vis, scale: float, wide: bool = False):
         out[some, h] = o
         # a score off by ds moves the output by w ds (v - out), twice that for the sum's own
         moved = (w * ds) @ np.abs(v[:, u]) + (w * ds).sum(1, keepdims=True) * np.abs(o)
-        err = EPS * (w @ (2 * np.abs(v[:, u]))) if wide else EPS * (w @ part[:, u]) + 2.0 ** -22 * (w @ (part + mid)[:, u])
-        tol[some, h] = SLACK * (err + moved + EPS * np.abs(o)) + 2.0 ** -11 * np.abs(v[:, u]).max(initial=0)
-        ltol[some, h] = ds.max(1) + (EPS if wide else 0) + 1e-5
+        err = HALF * (w @ (2 * np.abs(v[:, u]))) if wide else EPS * (w @ part[:, u]) + 2.0 ** -22 * (w @ (part + mid)[:, u])
+        tol[some, h] = SLACK * (err + moved + EPS * np.abs(o)) + (2.0 ** -20 if wide else 2.0 ** -11) * np.abs(v[:, u]).max(initial=0)
+        ltol[some, h] = ds.max(1) + (HALF if wide else 0) + 1e-5
     return out, lse, tol, ltol

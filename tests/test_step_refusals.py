@@ -211,7 +211,10 @@ def test_c_entries_return_errors():
     dec = [a, 4096, 128, a, 1, a, 4, a, 1, 4, 2, 0.1, a, 4096, 128, None, a, 1 << 20, None]
     for i, bad in ((0, None), (3, None), (4, 0), (6, 3), (10, 3), (10, 66), (11, -1.0), (16, None), (17, 100), (8, 70000), (0, a + 2)):
         assert L.abkv_decode_attn_int4(*dec[:i], bad, *dec[i + 1:]) != 0, i
-    assert L.abkv_kv_widen_int4(a, 1, a, 1, None, 1, 1, a, a, 1, None) != 0
+    pre = [a, 4096, 128, a, 1, a, 4, 4, a, a, a, None, a, a, 1, a, 0, 0, 0.1, a, 4096, 128, None, a, 1 << 20, None]
+    for i, bad in ((0, None), (0, a + 2), (1, 4097), (3, None), (3, a + 8), (4, 0), (5, None), (7, 0), (12, None), (16, -1), (17, 64),
+                   (18, -1.0), (18, float("inf")), (19, a + 8), (20, 4100)):
+        assert L.abkv_paged_prefill_attn_items_int4(*pre[:i], bad, *pre[i + 1:]) != 0, i
     app = [a, 4096, 128, a, 1024, 128, a, 1024, 128, a, 1, a, a, 0, 1e-6, 0, 0, 0, a, 9, a, a, 1, 0, a, 4096, 128, None]
     for i, bad in ((0, None), (0, a + 4), (4, 1020), (9, None), (11, None), (14, -1.0), (15, -1), (19, 0), (20, None), (22, 0),
                    (24, None)):
