@@ -68,21 +68,21 @@ __device__ __forceinline__ float page_bound(const Int4Part& p) {
   return max_xor32(max_xor16(x));
 }
 
-// A lane's part as fp16 values over 2^e, to slot `row` of a tile.
-__device__ __forceinline__ void unpack_part(const Int4Part& p, int e, __bf16* tile, int row, int lane) {
-  const float f = exp2i(-e);
+// Word 4 (lane % 4) + g of a lane's part, dims 32 g + 8 (lane % 4) .. + 7, as fp16 values times f to slot `row` of a tile.
+__device__ __forceinline__ void unpack_word(const Int4Part& p, int g, float f, uint32_t mask, __bf16* tile, int row, int lane) {
+  const _Float16 s = (_Float16)(bf16_lo(p.pairs[g]) * f), m = (_Float16)(bf16_hi(p.pairs[g]) * f);
+  u32x4 x;
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {                              // word 4 (lane % 4) + g: dims 32 g + 8 (lane % 4) .. + 7
-    const _Float16 s = (_Float16)(bf16_lo(p.pairs[g]) * f), m = (_Float16)(bf16_hi(p.pairs[g]) * f);
-    u32x4 x;
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {                            // 1024 + c, c, m + s c: one rounding, of the last
-      const uint32_t c = ((p.codes[g] >> (4 * n)) & 0x000f000fu) | 0x64006400u;
-      const f16x2 code = __builtin_bit_cast(f16x2, c) - f16x2{(_Float16)1024.f, (_Float16)1024.f};
-      x[n] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(code, f16x2{s, s}, f16x2{m, m}));
-    }
-    *reinterpret_cast<u32x4*>(tile + row * kHeadDim + 8 * ((4 * g + (lane & 3)) ^ (row & 15))) = x;
+  for (int n = 0; n < 4; ++n) {                              // 1024 + c, c, m + s c: one rounding, of the last
+    const uint32_t c = ((p.codes[g] >> (4 * n)) & mask) | 0x64006400u;
+    const f16x2 code = __builtin_bit_cast(f16x2, c) - f16x2{(_Float16)1024.f, (_Float16)1024.f};
+    x[n] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(code, f16x2{s, s}, f16x2{m, m}));
   }
+  *reinterpret_cast<u32x4*>(tile + row * kHeadDim + 8 * ((4 * g + (lane & 3)) ^ (row & 15))) = x;
+}
+__device__ __forceinline__ void unpack_part(const Int4Part& p, int e, uint32_t mask, __bf16* tile, int row, int lane) {
+#pragma unroll
+  for (int g = 0; g < 4; ++g) unpack_word(p, g, exp2i(-e), mask, tile, row, lane);
 }
 
 // attend_tiles over rows in 4 bits: same walk (contiguous tiles), masks, lanes and results. Iteration n attends to tile n and unpacks K of tile
@@ -126,10 +126,12 @@ __device__ __forceinline__ void attend_tiles_int4(const Int4Rows& rows, Walk& wa
     if (k0 + row >= n_keys) p.pairs = u32x4{0, 0, 0, 0};
     return p;
   };
-  auto unpack_k = [&](const Int4Part& p, float bound, int i) {
+  uint32_t mask = 0x000f000fu;                               // (in a register: and and or in one instruction)
+  __asm__("" : "+v"(mask));
+  auto k_exp = [&](float bound, int i) {
     const int e = range_exp(bound, kLowestQK);
     if (lane == 0) k_scale[i & 3][page] = exp2i(e);
-    unpack_part(p, e, i & 1 ? K[1] : K[0], row, lane);
+    return e;
   };
   auto needed = [&](int i) { return max(max(v_need[i & 1][0], v_need[i & 1][1]), max(v_need[i & 1][2], v_need[i & 1][3])); };
   int v_exp;
@@ -139,13 +141,13 @@ __device__ __forceinline__ void attend_tiles_int4(const Int4Rows& rows, Walk& wa
     if (is_v) {
       if (lane == 0) v_need[0][page] = range_exp(bound, kLowestV);
     } else {
-      unpack_k(next, bound, 0);
+      unpack_part(next, k_exp(bound, 0), mask, K[0], row, lane);
       next = load(1);
-      unpack_k(next, page_bound(next), 1);
+      unpack_part(next, k_exp(page_bound(next), 1), mask, K[1], row, lane);
     }
     __syncthreads();
     v_exp = needed(0);
-    if (is_v) unpack_part(next, v_exp, V[0], row, lane);
+    if (is_v) unpack_part(next, v_exp, mask, V[0], row, lane);
     next = load(is_v ? 1 : 2);
   }
   __syncthreads();
@@ -189,6 +191,11 @@ __device__ __forceinline__ void attend_tiles_int4(const Int4Rows& rows, Walk& wa
     __asm__ volatile("" ::: "memory");
     const int v_next = max(v_exp, needed(n + 1));
     const floatx4 kf = *reinterpret_cast<const floatx4*>(k_scale[n & 3]);
+    // (the unpacking amid the products of the values, which leave the vector unit idle)
+    const float f_part = exp2i(-(is_v ? v_next : k_exp(bound, n + 2)));
+    __bf16* const to = is_v ? V[slot ^ 1] : K[slot];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) unpack_word(part, g, f_part, mask, to, row, lane);
     walk.next(k0, tm, n == 0);
     tile_mask<H, Walk>(s, k0, tm, lane_mask, j);
     // online softmax, as tile_softmax: the log2 scores relative to the running maximum, which moves when a score passes it by
@@ -244,8 +251,6 @@ __device__ __forceinline__ void attend_tiles_int4(const Int4Rows& rows, Walk& wa
 #pragma unroll
       for (int u = 0; u < H; ++u) lsum[u] = mfma16x16x32(ones, pop[kk][u], lsum[u]);
     }
-    if (is_v) unpack_part(part, v_next, V[slot ^ 1], row, lane);
-    else unpack_k(part, bound, n + 2);
     if (v_next != v_exp) {
       const float f = exp2i(max(v_exp - v_next, -126));
 #pragma unroll

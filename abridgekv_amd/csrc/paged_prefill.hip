@@ -287,44 +287,44 @@ __global__ __launch_bounds__(512, 1) void paged_prefill_kernel(PagedPrefillArgs 
   }
 }
 
-// Combine the parts of a merged tile: workgroup (tile, KV head, wave w of the attention kernel), its waves (head u of the
-// two, accumulator tiles 4 * half .. + 3) in the attention kernel's lane order, so every load is a whole 1 KiB run.
-__global__ __launch_bounds__(256) void paged_merge_items_kernel(PagedPrefillArgs a) {
+// Combine the parts of a merged tile: workgroup (tile, KV head, wave w of the attention kernel, two of its accumulator tiles), its
+// waves (head u of the two) in the attention kernel's lane order, so every load is a whole 1 KiB run. (Two accumulator tiles, not
+// eight, so that one merged query tile, of up to 32 parts of 1 MiB, is work for all 256 compute units: 19 -> 11 us; many
+// merged tiles take what they took.)
+__global__ __launch_bounds__(128) void paged_merge_items_kernel(PagedPrefillArgs a) {
   constexpr int H = 2, kWaves = 8, kLaneRuns = kItemFloats / kHeadsKV / kWaves;
-  const int w = blockIdx.x % kWaves, kvh = blockIdx.x / kWaves % kHeadsKV;
-  const int32_t* mt = a.merges + 4 * (blockIdx.x / (kWaves * kHeadsKV));
+  const int p = blockIdx.x % 4, w = blockIdx.x / 4 % kWaves, kvh = blockIdx.x / (4 * kWaves) % kHeadsKV;
+  const int32_t* mt = a.merges + 4 * (blockIdx.x / (4 * kWaves * kHeadsKV));
   const int parts = mt[3];
   const int lane = threadIdx.x & 63, m16 = lane & 15, j = lane >> 4;
-  const int u = (threadIdx.x >> 6) & 1, half = threadIdx.x >> 7;
+  const int u = threadIdx.x >> 6;
   const int row = 16 * (w >> 1) + m16;                       // within the tile
   const long first = (mt[2] / kBM * (long)kHeadsKV + kvh) * kWaves + w;
   constexpr long kStep = kHeadsKV * kWaves;                  // between the parts
   const float2* ml = reinterpret_cast<const float2*>(a.item_ml) + (first * H + u) * 16 + m16;
-  const float* po = a.item_o + first * kLaneRuns + 256 * (8 * u + 4 * half) + 4 * lane;
+  const float* po = a.item_o + first * kLaneRuns + 256 * (8 * u + 2 * p) + 4 * lane;
   float M = -INFINITY;
 #pragma unroll 8
   for (int s = 0; s < parts; ++s) M = fmaxf(M, ml[s * kStep * H * 16].x);
   float L = 0.f;
-  floatx4 acc[4];
+  floatx4 acc[2];
 #pragma unroll
-  for (int t = 0; t < 4; ++t) acc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
+  for (int t = 0; t < 2; ++t) acc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
   for (int s = 0; s < parts; ++s) {
     const float2 rec = ml[s * kStep * H * 16];               // m, l
     const float f = rec.x == M ? 1.f : fast_exp2(rec.x - M); // (m and M are both -inf without a finite score: sums of 0,
     L += f * rec.y;                                          // or of NaN scores, which go through)
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int t = 0; t < 2; ++t)
       acc[t] += *reinterpret_cast<const floatx4*>(po + s * kStep * kLaneRuns + 256 * t) * f;
   }
   if (row >= mt[1]) return;
   const float inv = L > 0.f ? 1.f / L : 0.f;
   const long tok = (long)mt[0] + row;
   const int head = kvh * kGroup + H * (w & 1) + u;
-  __bf16* oh = a.out + tok * a.o_st + (long)head * a.o_sh + 32 * j + 16 * half;
-#pragma unroll
-  for (int p = 0; p < 2; ++p) store_acc_bf16x8(oh + 8 * p, acc[2 * p], acc[2 * p + 1], j, inv);
-  if (a.lse != nullptr && j == 0 && half == 0)
+  store_acc_bf16x8(a.out + tok * a.o_st + (long)head * a.o_sh + 32 * j + 8 * p, acc[0], acc[1], j, inv);
+  if (a.lse != nullptr && j == 0 && p == 0)
     a.lse[tok * kHeadsQ + head] = L > 0.f ? (M + __log2f(L)) * 0.69314718055994531f : -INFINITY;
 }
 
@@ -389,7 +389,7 @@ static int prefill_items(bool int4, const void* q, long q_stride_t, long q_strid
       kv_limit == nullptr || causal == nullptr || items == nullptr || out == nullptr || num_pages <= 0 ||
       block_table_width <= 0 || n_merges < 0 || part_rows < 0 || (n_merges > 0 && merges == nullptr) ||
       (part_rows > 0 && (workspace == nullptr || workspace_bytes < abkv_paged_prefill_items_workspace_size(part_rows))) ||
-      part_rows % kBM != 0 || (long)n_merges * 8 * kHeadsKV * 256 > 0xFFFFFFFFL)
+      part_rows % kBM != 0 || (long)n_merges * 4 * 8 * kHeadsKV * 128 > 0xFFFFFFFFL)
     return (int)hipErrorInvalidValue;
   PagedPrefillArgs a;
   a.q = static_cast<const __bf16*>(q);
@@ -430,7 +430,7 @@ static int prefill_items(bool int4, const void* q, long q_stride_t, long q_strid
   else hipLaunchKernelGGL(paged_prefill_kernel<kPagedRows>, dim3(grid), dim3(512), 0, stream, a);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess || n_merges == 0) return (int)err;
-  hipLaunchKernelGGL(paged_merge_items_kernel, dim3((unsigned)n_merges * 8 * kHeadsKV), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL(paged_merge_items_kernel, dim3((unsigned)n_merges * 4 * 8 * kHeadsKV), dim3(128), 0, stream, a);
   return (int)hipGetLastError();
 }
 

@@ -1675,6 +1675,10 @@ def qk_norm_rope_append(q: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     return out
 
 
+def _dense_like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _norm_rope_args(q, k, cos, sin, q_weight, k_weight, eps):
     """Checks of a training step's arguments; the entries' common ones before the outputs."""
     _require(q.dim() == 4 and q.dtype in (torch.bfloat16, torch.float32), "q must be bf16 or fp32 [B, S, 32, 128]")
@@ -1682,14 +1686,12 @@ def _norm_rope_args(q, k, cos, sin, q_weight, k_weight, eps):
     _check_rows("q", q, q.dtype, (B, S, HEADS_Q, HEAD_DIM))
     _check_rows("k", k, q.dtype, (B, S, HEADS_KV, HEAD_DIM))
     wf32 = _check_weights(q_weight, k_weight, q.dtype)
-    n = cos.shape[0] if cos.dim() == 3 else 0
+    n, st, dt = cos.shape[0] if cos.dim() == 3 else 0, cos.stride(), cos.dtype
     for name, t in (("cos", cos), ("sin", sin)):
-        st = t.stride()
-        _require(t.dtype in (torch.bfloat16, torch.float32) and t.dtype == cos.dtype and n in (1, B)
-                 and t.shape == (n, S, HEAD_DIM) and st == cos.stride() and st[2] == 1
-                 and (st[0] | st[1]) * t.element_size() % 16 == 0 and t.data_ptr() % 16 == 0,
-                 f"{name} must be bf16 or fp32 [1 or B, S, 128], both alike, with contiguous, 16-byte aligned rows")
-    st = cos.stride()
+        if not (t.shape == (n, S, HEAD_DIM) and n in (1, B) and t.dtype == dt and t.stride() == st and st[2] == 1
+                and dt in (torch.bfloat16, torch.float32) and (st[0] | st[1]) * t.element_size() % 16 == 0
+                and t.data_ptr() % 16 == 0):
+            raise ValueError(f"{name} must be bf16 or fp32 [1 or B, S, 128], both alike, with contiguous, 16-byte aligned rows")
     return (int(q.dtype == torch.float32), q, k, (B, S, q_weight.data_ptr(), k_weight.data_ptr(), wf32, _check_eps(eps),
                                                   cos.data_ptr(), sin.data_ptr(), st[0] if n > 1 else 0, st[1],
                                                   int(cos.dtype == torch.float32)))
@@ -1703,8 +1705,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch
     fp32. Returns new dense (q, k) of the same type, rounded once. With gradients: :func:`abridgekv_amd.fused.qk_norm_rope`."""
     f32, q, k, args = _norm_rope_args(q, k, cos, sin, q_weight, k_weight, eps)
     _check_device(q, k, cos, sin, q_weight, k_weight)
-    q_out, k_out = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
-    rc = lib().abkv_qk_norm_rope(f32, q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], *args, q_out.data_ptr(),
+    q_out, k_out = _dense_like(q), _dense_like(k)
+    (qb, qs, qh, _), (kb, ks, kh, _) = q.stride(), k.stride()
+    rc = lib().abkv_qk_norm_rope(f32, q.data_ptr(), qb, qs, qh, k.data_ptr(), kb, ks, kh, *args, q_out.data_ptr(),
                                  k_out.data_ptr(), _stream())
     check(rc, "abkv_qk_norm_rope")
     return q_out, k_out
@@ -1718,15 +1721,16 @@ def qk_norm_rope_backward(q: torch.Tensor, k: torch.Tensor, dq_out: torch.Tensor
     _check_rows("dq_out", dq_out, q.dtype, q.shape)
     _check_rows("dk_out", dk_out, q.dtype, k.shape)
     _check_device(q, k, dq_out, dk_out, cos, sin, q_weight, k_weight)
-    dq, dk = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
-    dwq, dwk = torch.empty_like(q_weight), torch.empty_like(k_weight)
+    dq, dk, dwq, dwk = _dense_like(q), _dense_like(k), torch.empty_like(q_weight), torch.empty_like(k_weight)
     if q.numel() == 0:
         return dq, dk, dwq.zero_(), dwk.zero_()
-    n = lib().abkv_qk_norm_rope_bwd_workspace_size(*q.shape[:2])
+    L = lib()
+    n = L.abkv_qk_norm_rope_bwd_workspace_size(args[0], args[1])
     ws = torch.empty(n, dtype=torch.uint8, device=q.device)
-    rc = lib().abkv_qk_norm_rope_bwd(f32, q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], dq_out.data_ptr(),
-                                     *dq_out.stride()[:3], dk_out.data_ptr(), *dk_out.stride()[:3], *args, dq.data_ptr(),
-                                     dk.data_ptr(), dwq.data_ptr(), dwk.data_ptr(), ws.data_ptr(), n, _stream())
+    (qb, qs, qh, _), (kb, ks, kh, _), (db, ds, dh, _), (eb, es, eh, _) = (t.stride() for t in (q, k, dq_out, dk_out))
+    rc = L.abkv_qk_norm_rope_bwd(f32, q.data_ptr(), qb, qs, qh, k.data_ptr(), kb, ks, kh, dq_out.data_ptr(), db, ds, dh,
+                                 dk_out.data_ptr(), eb, es, eh, *args, dq.data_ptr(), dk.data_ptr(), dwq.data_ptr(),
+                                 dwk.data_ptr(), ws.data_ptr(), n, _stream())
     check(rc, "abkv_qk_norm_rope_bwd")
     return dq, dk, dwq, dwk
 
