@@ -10,6 +10,11 @@
 //
 // Wave w unpacks page w % 4 of K (waves 0 .. 3) or V (4 .. 7): 20 bytes a slot and head in place of 256, so that a tile costs each
 // lane two 16-byte loads and about 80 VALU operations, beside 200 for its part of the softmax.
+//
+// A SIMD has one wave of either kind, and a tile is two phases of each: the vector unit's (softmax, unpacking) and the matrix
+// unit's (products). The V waves are a phase behind, so that one wave's vector work runs beside the other's products; in step,
+// they took turns at both units: 1.4 us a tile at the vector unit and 0.9 at the matrix unit came to 2.5 us, and are now 2.1
+// (three chunks of 300 to 441 queries behind up to 8000 rows: 180 -> 160 us; with the two kinds on different SIMDs, 193).
 #pragma once
 #include "attn_tile.h"
 #include "int4.h"
@@ -48,24 +53,31 @@ __device__ __forceinline__ Int4Part load_part(const Int4Rows& rows, int page, bo
 
 // The exponent that values up to `bound` take; at least `lowest` (a multiple of 8).
 __device__ __forceinline__ int range_exp(float bound, int lowest) {
-  const int e = (int)(__float_as_uint(bound) >> 23) - 127 - 14;
+  const int e = (int)(__float_as_uint(bound) >> 23) - 127 - 14;           // (bound >= 0; infinity: 114)
   return max((e + 7) & ~7, lowest);
 }
 __device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 // K and Q: no lower than 2^-40, so that their product with the softmax's scale stays a number; V: as low as its reciprocal goes.
 constexpr int kLowestQK = -40, kLowestV = -104;
 
-// The largest |value| of a page, in every lane.
+// The larger number; a NaN counts for nothing. (The instruction itself: fmaxf takes another one to quiet each operand.)
+__device__ __forceinline__ float max_num(float a, float b) {
+  float r;
+  __asm__("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
+// What no |value| of a page exceeds, in every lane: |m| + 15 |s|, at most three times the largest.
 __device__ __forceinline__ float page_bound(const Int4Part& p) {
-  float x = 0.f;
+  float x[4];
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    const float s = bf16_lo(p.pairs[g]), m = bf16_hi(p.pairs[g]);
-    x = fmaxf(x, fmaxf(fabsf(m), fabsf(fmaf(15.f, s, m))));
-  }
-  x = fmaxf(x, dpp<kDppHalfMirror>(x));                      // (the lanes of a quad have the same pairs)
-  x = fmaxf(x, dpp<kDppMirror>(x));
-  return max_xor32(max_xor16(x));
+  for (int g = 0; g < 4; ++g) x[g] = fmaf(15.f, fabsf(bf16_lo(p.pairs[g])), fabsf(bf16_hi(p.pairs[g])));
+  float b = max_num(max_num(x[0], x[1]), max_num(x[2], x[3]));
+  b = max_num(b, dpp<kDppHalfMirror>(b));                    // (the lanes of a quad have the same pairs)
+  b = max_num(b, dpp<kDppMirror>(b));
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(b), __float_as_uint(b), false, false);
+  b = max_num(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  const auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(b), __float_as_uint(b), false, false);
+  return max_num(max_num(__uint_as_float(q[0]), __uint_as_float(q[1])), 0.f);
 }
 
 // Word 4 (lane % 4) + g of a lane's part, dims 32 g + 8 (lane % 4) .. + 7, as fp16 values times f to slot `row` of a tile.
@@ -80,13 +92,12 @@ __device__ __forceinline__ void unpack_word(const Int4Part& p, int g, float f, u
   }
   *reinterpret_cast<u32x4*>(tile + row * kHeadDim + 8 * ((4 * g + (lane & 3)) ^ (row & 15))) = x;
 }
-__device__ __forceinline__ void unpack_part(const Int4Part& p, int e, uint32_t mask, __bf16* tile, int row, int lane) {
-#pragma unroll
-  for (int g = 0; g < 4; ++g) unpack_word(p, g, exp2i(-e), mask, tile, row, lane);
-}
 
-// attend_tiles over rows in 4 bits: same walk (contiguous tiles), masks, lanes and results. Iteration n attends to tile n and unpacks K of tile
-// n + 2 (whose scores iteration n + 1 takes) and V of tile n + 1, from what the iteration before loaded; one barrier each.
+// attend_tiles over rows in 4 bits: same walk (contiguous tiles), masks, lanes and results. Phase A of tile n unpacks this wave's
+// page of tile n + 1 and turns the scores of tile n into weights; phase B is O += V . P of tile n and the scores of tile n + 1. A
+// barrier ends each. K waves take A(n) in phase 2 n, V waves in 2 n + 1, so what a buffer held is read for the last time:
+//   K tile n - 1 by B(n - 2), in phases 2 n - 3 and 2 n - 2; the K waves put tile n + 1 in its place in phase 2 n;
+//   V tile n - 1 by B(n - 1), in phases 2 n - 1 and 2 n; the V waves put tile n + 1 in its place in phase 2 n + 1.
 template <int H, int kWaves, class Walk, class Lane>
 __device__ __forceinline__ void attend_tiles_int4(const Int4Rows& rows, Walk& walk, int n_keys,
                                                   __bf16* const (&K)[kStages], __bf16* const (&V)[kStages],
@@ -128,36 +139,25 @@ __device__ __forceinline__ void attend_tiles_int4(const Int4Rows& rows, Walk& wa
   };
   uint32_t mask = 0x000f000fu;                               // (in a register: and and or in one instruction)
   __asm__("" : "+v"(mask));
-  auto k_exp = [&](float bound, int i) {
-    const int e = range_exp(bound, kLowestQK);
-    if (lane == 0) k_scale[i & 3][page] = exp2i(e);
-    return e;
-  };
   auto needed = [&](int i) { return max(max(v_need[i & 1][0], v_need[i & 1][1]), max(v_need[i & 1][2], v_need[i & 1][3])); };
-  int v_exp;
-  Int4Part next = load(0);
-  {
-    const float bound = page_bound(next);
-    if (is_v) {
-      if (lane == 0) v_need[0][page] = range_exp(bound, kLowestV);
-    } else {
-      unpack_part(next, k_exp(bound, 0), mask, K[0], row, lane);
-      next = load(1);
-      unpack_part(next, k_exp(page_bound(next), 1), mask, K[1], row, lane);
+  auto unpack = [&](const Int4Part& p, int v_exp, int i, __bf16* k_to, __bf16* v_to) {
+    int e = v_exp;
+    if (!is_v) {
+      e = range_exp(page_bound(p), kLowestQK);
+      if (lane == 0) k_scale[i & 3][page] = exp2i(e);
     }
-    __syncthreads();
-    v_exp = needed(0);
-    if (is_v) unpack_part(next, v_exp, mask, V[0], row, lane);
-    next = load(is_v ? 1 : 2);
-  }
-  __syncthreads();
-  floatx4 lsum[H];
+    const float f = exp2i(-e);
+    __bf16* const to = is_v ? v_to : k_to;
 #pragma unroll
-  for (int u = 0; u < H; ++u) lsum[u] = floatx4{0.f, 0.f, 0.f, 0.f};
-  const f16x2 one2 = {(_Float16)1.f, (_Float16)1.f};
-  const f16x8 ones = {one2[0], one2[0], one2[0], one2[0], one2[0], one2[0], one2[0], one2[0]};
-
-  auto scores = [&](const __bf16* buf, floatx4 (&s)[2][2][H]) {
+    for (int g = 0; g < 4; ++g) unpack_word(p, g, f, mask, to, row, lane);
+  };
+  auto announce = [&](const Int4Part& p, int i) {            // what a V wave's page of tile i needs
+    if (!is_v) return;
+    const int e = range_exp(page_bound(p), kLowestV);
+    if (lane == 0) v_need[i & 1][page] = e;
+  };
+  floatx4 s[2][2][H];
+  auto scores = [&](const __bf16* buf) {
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
@@ -175,27 +175,45 @@ __device__ __forceinline__ void attend_tiles_int4(const Int4Rows& rows, Walk& wa
           for (int u = 0; u < H; ++u) s[kk][t][u] = mfma16x16x32(kop, q[u][i], s[kk][t][u]);
         }
   };
-  floatx4 sa[2][2][H], sb[2][2][H];
-  scores(K[0], sa);
-
-  int k0 = 0;
-  TileMask tm;
-  auto step = [&](floatx4 (&s)[2][2][H], floatx4 (&s_next)[2][2][H], auto slot_c, int n) {
-    constexpr int slot = decltype(slot_c)::value;
-    const Int4Part part = next;
-    next = load(n + (is_v ? 2 : 3));
-    const float bound = page_bound(part);
-    if (is_v && lane == 0) v_need[slot ^ 1][page] = range_exp(bound, kLowestV);
+  // Ends a phase: this wave's LDS reads and writes are done (loads from memory stay in flight)
+  auto end_phase = [] {
     __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     __asm__ volatile("" ::: "memory");
-    const int v_next = max(v_exp, needed(n + 1));
-    const floatx4 kf = *reinterpret_cast<const floatx4*>(k_scale[n & 3]);
-    // (the unpacking amid the products of the values, which leave the vector unit idle)
-    const float f_part = exp2i(-(is_v ? v_next : k_exp(bound, n + 2)));
-    __bf16* const to = is_v ? V[slot ^ 1] : K[slot];
+  };
+
+  Int4Part part = load(0);
+  announce(part, 0);
+  __syncthreads();
+  int v_exp = needed(0);
+  unpack(part, v_exp, 0, K[0], V[0]);
+  part = load(1);
+  announce(part, 1);
+  __syncthreads();
+  scores(K[0]);
+  floatx4 lsum[H];
 #pragma unroll
-    for (int g = 0; g < 4; ++g) unpack_word(part, g, f_part, mask, to, row, lane);
+  for (int u = 0; u < H; ++u) lsum[u] = floatx4{0.f, 0.f, 0.f, 0.f};
+  const _Float16 one = (_Float16)1.f;
+  const f16x8 ones = {one, one, one, one, one, one, one, one};
+
+  int k0 = 0;
+  TileMask tm;
+  auto tile = [&](auto slot_c, int n) {
+    constexpr int slot = decltype(slot_c)::value;
+    // -- phase A
+    const int v_now = max(v_exp, needed(n));
+    if (v_now != v_exp) {
+      const float f = exp2i(max(v_exp - v_now, -126));
+#pragma unroll
+      for (int u = 0; u < H; ++u)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i][u] *= f;
+      v_exp = v_now;
+    }
+    const floatx4 kf = *reinterpret_cast<const floatx4*>(k_scale[n & 3]);
+    unpack(part, is_v ? max(v_exp, needed(n + 1)) : 0, n + 1, K[slot ^ 1], V[slot ^ 1]);
+    part = load(n + 2);
     walk.next(k0, tm, n == 0);
     tile_mask<H, Walk>(s, k0, tm, lane_mask, j);
     // online softmax, as tile_softmax: the log2 scores relative to the running maximum, which moves when a score passes it by
@@ -236,10 +254,12 @@ __device__ __forceinline__ void attend_tiles_int4(const Int4Rows& rows, Walk& wa
 #pragma unroll
     for (int u = 0; u < H; ++u)
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk)
+      for (int kk = 0; kk < 2; ++kk) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) pop[kk][u][e] = (_Float16)fast_exp2(s[kk][e >> 2][u][e & 3]);
-    scores(K[slot ^ 1], s_next);                             // (past the last tile: zeros, discarded)
+      }
+    end_phase();
+    // -- phase B
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
 #pragma unroll
@@ -251,21 +271,18 @@ __device__ __forceinline__ void attend_tiles_int4(const Int4Rows& rows, Walk& wa
 #pragma unroll
       for (int u = 0; u < H; ++u) lsum[u] = mfma16x16x32(ones, pop[kk][u], lsum[u]);
     }
-    if (v_next != v_exp) {
-      const float f = exp2i(max(v_exp - v_next, -126));
-#pragma unroll
-      for (int u = 0; u < H; ++u)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i][u] *= f;
-      v_exp = v_next;
-    }
+    scores(K[slot ^ 1]);                                     // (past the last tile: of zeros, or of another part's, discarded)
+    announce(part, n + 2);
+    end_phase();
   };
+  if (is_v) end_phase();
   for (int n = 0;;) {
-    step(sa, sb, Slot<0>{}, n);
+    tile(Slot<0>{}, n);
     if (++n >= tiles) break;
-    step(sb, sa, Slot<1>{}, n);
+    tile(Slot<1>{}, n);
     if (++n >= tiles) break;
   }
+  if (!is_v) end_phase();
   const float f = exp2i(v_exp);
 #pragma unroll
   for (int u = 0; u < H; ++u) {
