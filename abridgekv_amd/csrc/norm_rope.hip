@@ -320,10 +320,12 @@ __global__ __launch_bounds__(256) void norm_weights_kernel(const float* parts, i
   else static_cast<__bf16*>(to)[dim % kHeadDim] = (__bf16)v;
 }
 
-// Workgroups of the backward: two a CU, fewer where tokens are few.
+// Workgroups of the backward: three a CU, what its registers let a CU hold (two sequences of 4096 tokens in bf16, with the
+// weights' launch: 47 us; 1024 workgroups, a third of them in a second round: 54, 512: 48; eight of 8192: 385, 504 and 482 us);
+// fewer where tokens are few.
 inline int bwd_groups(long tokens) {
   const long n = (tokens + kTokenWaves - 1) / kTokenWaves;
-  return n < 1024 ? (int)n : 1024;
+  return n < 768 ? (int)n : 768;
 }
 
 }  // namespace abkv
