@@ -1,8 +1,8 @@
 // Attention tiles over a paged cache in 4 bits (int4.h), for the multi-query kernel (gfx950).
 //
 // The waves unpack a 64-key tile of codes into K and V tiles of fp16 in LDS, laid out as attn_tile.h's, and attend to them with
-// v_mfma_f32_16x16x32_f16. fp16 keeps a value m + s c to 2^-12 of itself where bf16 (the type that the cache is written from)
-// would round it a second time, to 2^-9; the weights gain as much. Its range is made up for by powers of two, which are exact:
+// v_mfma_f32_16x16x32_f16. fp16 keeps a value m + s c to 2^-11 of itself where bf16 (the type that the cache is written from)
+// would round it a second time, to 2^-8; the weights gain as much. Its range is made up for by powers of two, which are exact:
 //   K: 2^eK for each page, multiplied back into the page's scores;
 //   Q: 2^eQ for each query row and head, likewise;
 //   V: 2^eV for all of a walk, the largest need of its tiles so far; the output's sums are rescaled when it grows.
