@@ -6,7 +6,7 @@
 //   K: 2^eK for each page, multiplied back into the page's scores;
 //   Q: 2^eQ for each query row and head, likewise;
 //   V: 2^eV for all of a walk, the largest need of its tiles so far; the output's sums are rescaled when it grows.
-// An exponent is a multiple of 8 (it hardly ever moves), and leaves the largest value in [2^7, 2^15).
+// An exponent is a multiple of 8 (it hardly ever moves), and leaves the largest value between 2^5 and 2^15.
 //
 // Wave w unpacks page w % 4 of K (waves 0 .. 3) or V (4 .. 7): 20 bytes a slot and head in place of 256, so that a tile costs each
 // lane two 16-byte loads and about 80 VALU operations, beside 200 for its part of the softmax.
@@ -51,14 +51,17 @@ __device__ __forceinline__ Int4Part load_part(const Int4Rows& rows, int page, bo
   return p;
 }
 
-// The exponent that values up to `bound` take; at least `lowest` (a multiple of 8).
-__device__ __forceinline__ int range_exp(float bound, int lowest) {
+constexpr int kLowestExp = -104;                             // (2^104 is still a float)
+// The exponent that values up to `bound` take.
+__device__ __forceinline__ int range_exp(float bound) {
   const int e = (int)(__float_as_uint(bound) >> 23) - 127 - 14;           // (bound >= 0; infinity: 114)
-  return max((e + 7) & ~7, lowest);
+  return max((e + 7) & ~7, kLowestExp);
 }
 __device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
-// K and Q: no lower than 2^-40, so that their product with the softmax's scale stays a number; V: as low as its reciprocal goes.
-constexpr int kLowestQK = -40, kLowestV = -104;
+// A float's bits times 2^e for e << 23, from 2^-100 (so that -inf stays that, and no score that counts is as small) to 2^127.
+__device__ __forceinline__ float scaled_bits(int bits, int e23) {
+  return __int_as_float(min(max(__builtin_elementwise_add_sat(bits, e23), 27 << 23), 254 << 23));
+}
 
 // The larger number; a NaN counts for nothing. (The instruction itself: fmaxf takes another one to quiet each operand.)
 __device__ __forceinline__ float max_num(float a, float b) {
@@ -109,11 +112,11 @@ __device__ __forceinline__ void attend_tiles_int4(const Int4Rows& rows, Walk& wa
   const int page = w & 3, row = 16 * page + (lane >> 2);
   const int tiles = walk.kt_end - walk.kt_begin;
   if (tiles <= 0) return;
-  __shared__ __attribute__((aligned(16))) float k_scale[4][4]; // [tile % 4][page]: 2^eK
+  __shared__ __attribute__((aligned(16))) int k_exp[4][4];   // [tile % 4][page]: eK << 23
   __shared__ int v_need[2][4];                               // [tile % 2][page]
 
   f16x8 q[H][4];
-  float scale[H];
+  int scale[H];                                              // the scale's bits, times 2^eQ
 #pragma unroll
   for (int u = 0; u < H; ++u) {
     float x = 0.f;
@@ -121,13 +124,13 @@ __device__ __forceinline__ void attend_tiles_int4(const Int4Rows& rows, Walk& wa
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int d = 0; d < 8; ++d) x = fmaxf(x, fabsf((float)qop[u][i][d]));
-    const int e = range_exp(max_xor32(max_xor16(x)), kLowestQK);
+    const int e = range_exp(max_xor32(max_xor16(x)));
     const float f = exp2i(-e);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int d = 0; d < 8; ++d) q[u][i][d] = (_Float16)((float)qop[u][i][d] * f);
-    scale[u] = scale_log2 * exp2i(e);
+    scale[u] = __float_as_int(scaled_bits(__float_as_int(scale_log2), e * (1 << 23)));
   }
 
   // This wave's part of tile i of the walk; slots past the last key read as zeros (their weights are 0)
@@ -143,8 +146,8 @@ __device__ __forceinline__ void attend_tiles_int4(const Int4Rows& rows, Walk& wa
   auto unpack = [&](const Int4Part& p, int v_exp, int i, __bf16* k_to, __bf16* v_to) {
     int e = v_exp;
     if (!is_v) {
-      e = range_exp(page_bound(p), kLowestQK);
-      if (lane == 0) k_scale[i & 3][page] = exp2i(e);
+      e = range_exp(page_bound(p));
+      if (lane == 0) k_exp[i & 3][page] = e * (1 << 23);
     }
     const float f = exp2i(-e);
     __bf16* const to = is_v ? v_to : k_to;
@@ -153,7 +156,7 @@ __device__ __forceinline__ void attend_tiles_int4(const Int4Rows& rows, Walk& wa
   };
   auto announce = [&](const Int4Part& p, int i) {            // what a V wave's page of tile i needs
     if (!is_v) return;
-    const int e = range_exp(page_bound(p), kLowestV);
+    const int e = range_exp(page_bound(p));
     if (lane == 0) v_need[i & 1][page] = e;
   };
   floatx4 s[2][2][H];
@@ -211,7 +214,8 @@ __device__ __forceinline__ void attend_tiles_int4(const Int4Rows& rows, Walk& wa
         for (int i = 0; i < 8; ++i) o[i][u] *= f;
       v_exp = v_now;
     }
-    const floatx4 kf = *reinterpret_cast<const floatx4*>(k_scale[n & 3]);
+    typedef int i4 __attribute__((ext_vector_type(4)));
+    const i4 ke = *reinterpret_cast<const i4*>(k_exp[n & 3]);
     unpack(part, is_v ? max(v_exp, needed(n + 1)) : 0, n + 1, K[slot ^ 1], V[slot ^ 1]);
     part = load(n + 2);
     walk.next(k0, tm, n == 0);
@@ -227,7 +231,7 @@ __device__ __forceinline__ void attend_tiles_int4(const Int4Rows& rows, Walk& wa
       for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const float f = scale[u] * kf[2 * kk + t];
+          const float f = scaled_bits(scale[u], ke[2 * kk + t]);
 #pragma unroll
           for (int r = 0; r < 4; ++r) s[kk][t][u][r] = fmaf(s[kk][t][u][r], f, neg_m[u]);
         }

@@ -236,6 +236,61 @@ def test_chunks(name):
         _close(out[sl], lse[sl], q[sl], k[r], v[r], vis, wide=True)
 
 
+RANGES = {                                                   # powers of two of page p's keys and values, of the queries
+    "values grow": (lambda p: 0, lambda p: 4 * p, 0),
+    "values shrink": (lambda p: 0, lambda p: 60 - 5 * p, 0),
+    "values huge and tiny": (lambda p: 0, lambda p: (100, -100)[p % 2], 0),
+    "all tiny": (lambda p: -30, lambda p: -60, 30),
+    "keys differ by page": (lambda p: (0, -12, -24)[p % 3], lambda p: 0, 0),
+    "queries tiny": (lambda p: 24, lambda p: 3, -24),
+    "queries huge": (lambda p: -70, lambda p: 0, 70),
+}
+
+
+@pytest.mark.parametrize("name", RANGES)
+def test_any_range(name):
+    """Magnitudes far outside fp16's, alike in a sequence and changing from page to page: chunks, and single tokens."""
+    from abridgekv_amd import ops
+    of_k, of_v, of_q = RANGES[name]
+    n, nq = 400, 70
+    rows = []
+    for seed, of in ((31, of_k), (32, of_v)):
+        x = _bf(seed, (n, 8, 128)).float()
+        x *= torch.tensor([2.0 ** of(i // 16) for i in range(n)])[:, None, None]
+        rows.append(oi.quantise(oi.bf16(x.numpy())))
+    q = (_bf(33, (nq, 32, 128)).float() * 2.0 ** of_q).to(torch.bfloat16)
+    pages = -(-n // 16)
+    cache = np.zeros((pages, 2, 16, 640), np.uint8)
+    at = np.arange(n)
+    for half in (0, 1):
+        cache[at // 16, half, at % 16] = rows[half]
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+    lse = torch.empty((nq, 32), device="cuda")
+    out, _ = ops.paged_prefill_attention_int4(q.cuda(), torch.from_numpy(cache).cuda(), table, [0, nq], [n - nq], [n], True, lse=lse)
+    vis = np.arange(n)[None] <= n - nq + np.arange(nq)[:, None]
+    _close(out, lse, q, *rows, vis, wide=True)
+    sl = torch.tensor([n], dtype=torch.int32, device="cuda")
+    for split in (2, 64):
+        one, _ = ops.decode_attention_int4(q[-1:].cuda(), torch.from_numpy(cache).cuda(), table, sl, lse=lse[:1], split_pages=split)
+        _close(one, lse[:1], q[-1:], *rows, np.ones((1, n), bool))
+
+
+def test_chunk_row_that_is_not_finite():
+    """A NaN group of values reaches the queries that see it, in its dims and KV head, and nothing else of its page."""
+    from abridgekv_amd import ops
+    _, _, _, cache, table, _ = _paged([300], 34)
+    q = _bf(35, (40, 32, 128)).cuda()
+    args = (table, [0, 40], [260], [300], True)
+    good, _ = ops.paged_prefill_attention_int4(q, cache, *args)
+    pairs = cache[int(table[0, 1]), 1, 3, 512 + 16 * 2: 512 + 16 * 2 + 2]        # value row 19, head 2, group 0
+    pairs.copy_(torch.tensor([0xC0, 0x7F], dtype=torch.uint8))
+    out, _ = ops.paged_prefill_attention_int4(q, cache, *args)
+    assert torch.isnan(out[:, 8:12, :32]).all()
+    rest = torch.ones_like(out, dtype=torch.bool)
+    rest[:, 8:12, :32] = False
+    assert torch.equal(out[rest], good[rest])
+
+
 def test_row_moves():
     """Compaction moves of a 4-bit cache: whole rows of bytes, ordered and independent, one launch and several groups, and the
     staged form."""
