@@ -1530,7 +1530,8 @@ def kv_read_int4(kv_cache: torch.Tensor, slot_mapping: torch.Tensor,
     _check_slots(slot_mapping, T)
     _check_cache4(kv_cache)
     _check_device(slot_mapping, kv_cache)
-    key, value = (torch.empty((T, HEADS_KV, HEAD_DIM), dtype=dtype, device=kv_cache.device) for _ in range(2))
+    key = kv_cache.new_empty((T, HEADS_KV, HEAD_DIM), dtype=dtype)
+    value = torch.empty_like(key)
     if T:
         rc = lib().abkv_kv_read_int4(kv_cache.data_ptr(), kv_cache.shape[0], slot_mapping.data_ptr(), T,
                                      int(dtype == torch.float32), key.data_ptr(), value.data_ptr(), _stream())
@@ -1657,7 +1658,7 @@ def qk_norm_rope_append(q: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
                  "codes_k must be a power of two <= block_c")
         _require(code_span == 0 or codes_k <= code_span <= block_c, "code_span must be 0 or in [codes_k, block_c]")
     if out is None:
-        out = torch.empty((T, HEADS_Q, HEAD_DIM), dtype=torch.bfloat16, device=q.device)
+        out = q.new_empty((T, HEADS_Q, HEAD_DIM))
     else:
         _check_out(out, torch.bfloat16, (T, HEADS_Q, HEAD_DIM))
     _check_device(q, key, value, positions, cos_sin, slot_mapping, kv_cache, q_weight, k_weight, out)
@@ -1767,24 +1768,23 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, temperature: flo
 
     logits [T, V] bf16 or fp32 (rows of any alignment); targets [T] int64: outside [0, V) a row has no target and log probability
     0. Alternatives in descending order (ties: the lowest id). Logits below -1e25 (-inf, a type's lowest value) have probability
-    0; a row without another, or with a NaN or +inf, is NaN. ``stats``: also what :func:`token_logprobs_backward` takes. fp32 sums; equal calls give equal
-    bits. With gradients: :func:`abridgekv_amd.fused.token_logprobs`."""
+    0; a row without another, or with a NaN or +inf, is NaN. ``stats``: also what :func:`token_logprobs_backward` takes. fp32 sums;
+    equal calls give equal bits. With gradients: :func:`abridgekv_amd.fused.token_logprobs`."""
     temperature = _check_logits(logits, targets, temperature)
     T, V = logits.shape
     top = int(top)
     _require(0 <= top <= min(TOP_MAX, V), f"top must be in [0, {min(TOP_MAX, V)}]")
     _check_device(logits, targets)
     f32 = int(logits.dtype == torch.float32)
-    dev = logits.device
-    logprob = torch.empty(T, dtype=torch.float32, device=dev)
-    ent = torch.empty(T, dtype=torch.float32, device=dev) if entropy else None
-    st = torch.empty((T, 3), dtype=torch.float32, device=dev) if stats else None
-    ids = torch.empty((T, top), dtype=torch.int64, device=dev)
-    tops = torch.empty((T, top), dtype=torch.float32, device=dev)
+    logprob = logits.new_empty((T,), dtype=torch.float32)
+    ent = torch.empty_like(logprob) if entropy else None
+    st = logprob.new_empty((T, 3)) if stats else None
+    ids, tops = targets.new_empty((T, top)), logprob.new_empty((T, top))
     if T:
-        n = lib().abkv_token_logprobs_workspace_size(T, V, f32, top)
-        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-        rc = lib().abkv_token_logprobs(f32, logits.data_ptr(), logits.stride(0), T, V, targets.data_ptr(), temperature, top,
+        L = lib()
+        n = L.abkv_token_logprobs_workspace_size(T, V, f32, top)
+        ws = logprob.new_empty(((n + 3) // 4,)) if n else None
+        rc = L.abkv_token_logprobs(f32, logits.data_ptr(), logits.stride(0), T, V, targets.data_ptr(), temperature, top,
                                        logprob.data_ptr(), _ptr(ent), _ptr(st), ids.data_ptr(), tops.data_ptr(), _ptr(ws), n,
                                        _stream())
         check(rc, "abkv_token_logprobs")
