@@ -16,7 +16,8 @@ struct Append4Args {
   char* cache; long num_pages;
 };
 
-// Workgroup per token; thread: 8 dims of a head of K (the first 128 threads) or V.
+// Workgroup per token; thread: 8 dims of a head of K (the first 128 threads) or V. (1501 tokens: 4.8 us to write, 5.7 to read in
+// fp32, the copy rate and a launch.)
 __global__ __launch_bounds__(256) void kv_append4_kernel(Append4Args a) {
   const long t = blockIdx.x;
   const long slot = a.slot_mapping[t];
@@ -121,12 +122,16 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t w, int n, uint32_t mask) 
 // What bounds the reads is the number of cache lines that a CU asks for (about one in six cycles), so a line should bring what it
 // holds: a head's codes are half of one, its pairs an eighth. The workgroup's waves therefore fetch whole rows together, straight
 // into LDS (a wave 5 of the step's 40 KB), one barrier a step. (64 sequences of 500 to 9500 rows, every wave its own pieces: 118
-// us, of which 59 went with the pairs alone; the pairs shared, 93.)
+// us, of which 59 went with the pairs alone; the pairs shared, 99; whole rows, 94, of which 62 are vector work: 410 MB at 4.7 TB/s.
+// Three stages of LDS leave one workgroup a CU: 104.)
 constexpr int kPairs4 = 16 * 4 * kHeadsKV, kCodes4 = 16 * kHeadsKV * 16;     // dwords of a page's pairs and codes (of K or V)
 template <class T>
 __device__ __forceinline__ const T& at4(const uint32_t* base, uint32_t bytes) {
   return *reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + bytes);
 }
+// The loads' cache policy: nontemporal, as every row is read once (64 sequences of 500 to 9500 rows: 98 -> 89 us, 256 of 500 to
+// 3000: 136 -> 126).
+constexpr int kOnce = 2;
 // LDS of a step: parts K0 K1 V0 V1 (pages 0 and 1). Codes in rows of 32 16-byte chunks, slot by slot, chunk 4 head + word / 4 at
 // place (chunk ^ slot): both kinds of reads below then take all banks. Pairs in rows of 8 chunks, a chunk a head: row 4 r + j is
 // slot 4 j + r, its chunks at place (head ^ (j >> 1)).
@@ -205,12 +210,12 @@ __global__ __launch_bounds__(64 * kHeadsKV, 4) void decode4_kernel(Decode4Args a
     const int at = min(pg + (part & 1) - pg_begin, last);
     const char* from = a.kv + (long)__builtin_amdgcn_readlane(pid_l, at) * kPage4 + (part >> 1) * kHalf4;
     __asm__("" : "+v"(pair_from), "+v"(code_from));
-    __builtin_amdgcn_global_load_lds((const void*)(from + pair_from), ABKV_LDS(&to.pairs[part][32 * rows8]), 16, 0, 0);
+    __builtin_amdgcn_global_load_lds((const void*)(from + pair_from), ABKV_LDS(&to.pairs[part][32 * rows8]), 16, 0, kOnce);
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
       const uint32_t off = (code_from ^ 32 * n) + slot_from;
       __builtin_amdgcn_global_load_lds((const void*)(from + (rows8 + 2 * n) * kSlot4 + off),
-                                       ABKV_LDS(&to.codes[part][128 * (rows8 + 2 * n)]), 16, 0, 0);
+                                       ABKV_LDS(&to.codes[part][128 * (rows8 + 2 * n)]), 16, 0, kOnce);
     }
   };
   // What it reads of a step, in bytes: K words 4 j .. + 3 of slot m16; word m16 of the V slots 4 j + e; group g's pairs of slots
@@ -448,6 +453,8 @@ __global__ __launch_bounds__(16 * kGroups) void decode4_merge_kernel(Decode4Args
 
 using namespace abkv;
 
+constexpr int kMaxTokens = 0xFFFFFF;           // (256 threads each: work items of a launch fit 32 bits)
+
 static bool rows16_ok(const void* p, long st, long sh) {
   return p != nullptr && ((uintptr_t)p & 15) == 0 && ((st | sh) & 7) == 0;
 }
@@ -458,7 +465,7 @@ int abkv_kv_append_int4(const void* key, long key_stride_t, long key_stride_h, c
                         long value_stride_h, const int64_t* slot_mapping, int num_tokens, void* kv_cache, int num_pages,
                         hipStream_t stream) {
   if (num_tokens <= 0) return 0;
-  if (!rows16_ok(key, key_stride_t, key_stride_h) || !rows16_ok(value, value_stride_t, value_stride_h) ||
+  if (num_tokens > kMaxTokens || !rows16_ok(key, key_stride_t, key_stride_h) || !rows16_ok(value, value_stride_t, value_stride_h) ||
       slot_mapping == nullptr || !rows16_ok(kv_cache, 0, 0) || num_pages <= 0)
     return (int)hipErrorInvalidValue;
   const Append4Args a = {static_cast<const __bf16*>(key), key_stride_t, key_stride_h, static_cast<const __bf16*>(value),
@@ -470,7 +477,8 @@ int abkv_kv_append_int4(const void* key, long key_stride_t, long key_stride_h, c
 int abkv_kv_read_int4(const void* kv_cache, int num_pages, const int64_t* slot_mapping, int num_tokens, int f32, void* key,
                       void* value, hipStream_t stream) {
   if (num_tokens <= 0) return 0;
-  if (!rows16_ok(kv_cache, 0, 0) || num_pages <= 0 || slot_mapping == nullptr || !rows16_ok(key, 0, 0) || !rows16_ok(value, 0, 0))
+  if (num_tokens > kMaxTokens || !rows16_ok(kv_cache, 0, 0) || num_pages <= 0 || slot_mapping == nullptr || !rows16_ok(key, 0, 0) ||
+      !rows16_ok(value, 0, 0))
     return (int)hipErrorInvalidValue;
   const char* cache = static_cast<const char*>(kv_cache);
   if (f32)

@@ -14,6 +14,8 @@
 // equal logits) are found one after the other instead.
 //
 // Bound by memory: 2 (bf16) or 4 bytes a logit, beside one exponential and ten other operations.
+// Measured: 2048 rows of 131072 logits in bf16, forward 85 to 98 us (537 MB, 5.5 to 6.3 TB/s), gradient 172 to 180 (1.07 GB, 6 TB/s);
+// one row in fp32 with 5 alternatives 5.2 + 3.4 us over 64 workgroups.
 #include "abridgekv_amd.h"
 #include "common.h"
 
@@ -187,8 +189,8 @@ __device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
   return v;
 }
 
-// Workgroup (row, split), splits next to each other. The elements of a thread: pieces v0 + tid, v0 + tid + 512, ...; the head's with the first split, the
-// tail's with the last.
+// Workgroup (row, split), splits next to each other. The elements of a thread: pieces v0 + tid, v0 + tid + 512, ...; the head's
+// with the first split, the tail's with the last.
 template <class T, bool kEntropy>
 __global__ __launch_bounds__(kRowThreads) void logprob_kernel(LogprobArgs a) {
   constexpr int N = Vec<T>::n, kWaves = kRowThreads / 64;

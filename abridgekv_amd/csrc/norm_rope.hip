@@ -10,6 +10,8 @@
 // Bound by memory: a row is read once and written once. A row lies in 8 lanes, lane i with dims 8 i .. + 7 and 64 + 8 i .. + 7,
 // both members of its rotation pairs, so a wave holds 8 rows, its loads are whole 16-byte pieces and the sums over a row are
 // three DPP steps.
+// Measured: 2048 tokens appended 10.8 us (4.8 TB/s, what a copy reaches); training, two sequences of 4096 in bf16: forward 33 us
+// (168 MB, 5.1 TB/s), backward 55 (252 MB, 4.6 TB/s).
 #include "abridgekv_amd.h"
 #include "int4.h"
 #include "rope.h"
