@@ -325,7 +325,8 @@ class AbridgeAttentionImpl:
             return self._attend_window(q, kv_cache, md, out, lse)
         nd, nd_tok, n_tok = md.num_decodes, md.num_decode_tokens, md.num_actual_tokens
         if nd and self.int4:
-            # the workspace holds the splits of the longest tables, 64 pages or shorter: those of any step, if not all as short
+            # the workspace holds the parts of any batch of the longest tables, and with them those of a step's shares or of splits
+            # of 64 pages, if not of splits as short as would be best (so does a builder's of the bf16 cache, but for shares)
             pages, held = md.max_decode_pages, md.workspace.numel() if md.workspace is not None else 0
             split = ops.int4_split_pages(nd, pages)
             while split < 64 and ops.decode_int4_bytes(nd, pages, split) > held:

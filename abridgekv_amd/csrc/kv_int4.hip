@@ -85,13 +85,15 @@ struct Decode4Args {
   const char* kv; int num_pages;
   const int32_t* block_table; long bt_stride;
   const int32_t* seq_lens;                     // [B]
-  int split_pages, max_splits, max_pages;
+  int split_pages, max_splits, max_pages;      // split_pages 0: shares
+  int num_seqs, num_shares;
+  int* prefix;                                 // shares: [B + 1] steps before each sequence, written by the first workgroup
   float scale_log2;
   __bf16* out; long o_sb, o_sh;                // [B, 32, 128]
   float* lse;                                  // [B, 32] or nullptr
-  _Float16* part_o;                            // [B, max_splits, 32, 128]: split output / (l * scale)
-  float* part_ml;                              // [B, max_splits, 32, 4]: m (log2 units), l, scale, unused
-};
+  _Float16* part_o;                            // [parts, 32, 128]: a part's output / (l * scale)
+  float* part_ml;                              // [parts, 32, 4]: m (log2 units), l, scale, unused
+};                                             // parts: B x max_splits, or two for each share
 
 __device__ __forceinline__ int rows_of(const Decode4Args& a, int b) {
   return max(min(a.seq_lens[b], a.max_pages * kPage), 0);
@@ -99,6 +101,7 @@ __device__ __forceinline__ int rows_of(const Decode4Args& a, int b) {
 __device__ __forceinline__ int splits_of(const Decode4Args& a, int rows) {
   return max(1, ((rows + kPage - 1) / kPage + a.split_pages - 1) / a.split_pages);
 }
+__device__ __forceinline__ int steps_of(int rows) { return max(1, (rows + 2 * kPage - 1) / (2 * kPage)); }
 
 // Codes of two neighbouring dims (nibbles n and n + 4 of a word) as the bf16 pair 128 + c: c lies in the low bits of the
 // mantissa, so every code is exact, and the 128s leave with the sums.
@@ -139,24 +142,23 @@ struct Step4 {
   uint32_t codes[4][kCodes4];
   uint32_t pairs[4][kPairs4];
 };
-__global__ __launch_bounds__(64 * kHeadsKV, 4) void decode4_kernel(Decode4Args a) {
-  // Linear grid, sequence by sequence; a sequence's splits start one further each time: workgroups go to the 8 XCDs round-robin,
-  // and sequences end at different splits.
-  const int b = blockIdx.x / a.max_splits, split = (blockIdx.x + b) % a.max_splits;
-  const int kvh = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63, m16 = lane & 15, j = lane >> 4;
-  const int h = m16 >> 2, g = m16 & 3;
-  const int row_end = rows_of(a, b);
-  const int n_splits = splits_of(a, row_end);
-  if (split >= n_splits) return;
-  const int pg_begin = split * a.split_pages;
-  const int pg_end = min((row_end + kPage - 1) / kPage, pg_begin + a.split_pages);
-  __shared__ __attribute__((aligned(16))) Step4 lds0, lds1;
+constexpr int kShareSteps = 64;                // steps of a share at most
+constexpr int kShareSeqs = 64 * kHeadsKV;      // sequences of a launch in shares
 
-  // Page ids of the split, lane l page pg_begin + l (split_pages <= 64)
-  const int32_t* bt = a.block_table + (long)b * a.bt_stride;
-  int pid_l = 0;
-  if (lane < pg_end - pg_begin) pid_l = min(max(bt[pg_begin + lane], 0), a.num_pages - 1);
+// Pages [pg_begin, pg_end) of sequence b, at most 2 kShareSteps: its output (part < 0: that is all of the sequence) or a part.
+__device__ __forceinline__ void decode4_piece(const Decode4Args& a, Step4& lds0, Step4& lds1, int b, int row_end, int pg_begin,
+                                              int pg_end, long part_at) {
+  const int kvh = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int lane = threadIdx.x & 63;
+  __asm__("" : "+v"(lane));                                  // (what depends on it is not carried from piece to piece)
+  const int m16 = lane & 15, j = lane >> 4;
+  const int h = m16 >> 2, g = m16 & 3;
+
+  // Page ids, lane l pages pg_begin + l and pg_begin + 64 + l
+  const int32_t* bt = a.block_table + (long)b * a.bt_stride + pg_begin;
+  int pid_l = 0, pid_h = 0;
+  if (lane < pg_end - pg_begin) pid_l = min(max(bt[lane], 0), a.num_pages - 1);
+  if (lane + 64 < pg_end - pg_begin) pid_h = min(max(bt[lane + 64], 0), a.num_pages - 1);
 
   // Q^T: dims 32 g + 8 j .. + 7 of head h, for the MFMA of group g
   bf16x8 qop[4];
@@ -208,7 +210,8 @@ __global__ __launch_bounds__(64 * kHeadsKV, 4) void decode4_kernel(Decode4Args a
   // ahead of the loop they spill.)
   auto fetch = [&](Step4& to, int pg) {                      // (past the end: the last page again)
     const int at = min(pg + (part & 1) - pg_begin, last);
-    const char* from = a.kv + (long)__builtin_amdgcn_readlane(pid_l, at) * kPage4 + (part >> 1) * kHalf4;
+    const int id = at < 64 ? __builtin_amdgcn_readlane(pid_l, at) : __builtin_amdgcn_readlane(pid_h, at - 64);
+    const char* from = a.kv + (long)id * kPage4 + (part >> 1) * kHalf4;
     __asm__("" : "+v"(pair_from), "+v"(code_from));
     __builtin_amdgcn_global_load_lds((const void*)(from + pair_from), ABKV_LDS(&to.pairs[part][32 * rows8]), 16, 0, kOnce);
 #pragma unroll
@@ -360,7 +363,7 @@ __global__ __launch_bounds__(64 * kHeadsKV, 4) void decode4_kernel(Decode4Args a
     x[i] = ((g & 1 ? odd : even) + off[0] + om) * inv;
   }
   const int head = kvh * kGroup + h, dim = 32 * g + 8 * j;
-  if (n_splits == 1) {
+  if (part_at < 0) {
     u32x4 w;
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
@@ -381,29 +384,108 @@ __global__ __launch_bounds__(64 * kHeadsKV, 4) void decode4_kernel(Decode4Args a
   f16x8 w;
 #pragma unroll
   for (int i = 0; i < 8; ++i) w[i] = (_Float16)(x[i] * range.inv);
-  const long at = ((long)b * a.max_splits + split) * kHeadsQ + head;
+  const long at = part_at * kHeadsQ + head;
   *reinterpret_cast<f16x8*>(a.part_o + at * kHeadDim + dim) = w;
   if (g == 0 && j == 0) *reinterpret_cast<floatx4*>(a.part_ml + at * 4) = floatx4{m_run, l, range.scale, 0.f};
 }
 
-// Joins the splits of a sequence: workgroup (head, sequence), kGroups groups of 16 lanes take the splits k = i, i + kGroups, ...,
-// four at a time, a lane 8 dims; their sums meet in LDS. A pass is a trip to another XCD's memory, so long sequences take more
+// Work goes out in one of two ways. Splits: workgroup (sequence, split) of split_pages pages. Shares: the steps of all sequences in
+// a row, cut into num_shares equal parts, one a workgroup, which may end one sequence and begin others; at most its first and
+// its last piece are parts of a sequence. The lengths are on the device, so each workgroup sums them itself.
+template <bool kShares>
+__global__ __launch_bounds__(64 * kHeadsKV, 4) void decode4_kernel(Decode4Args a) {
+  __shared__ __attribute__((aligned(16))) Step4 lds0, lds1;
+  if constexpr (!kShares) {
+    // Linear grid, sequence by sequence; a sequence's splits start one further each time: workgroups go to the 8 XCDs
+    // round-robin, and sequences end at different splits.
+    const int b = blockIdx.x / a.max_splits, split = (blockIdx.x + b) % a.max_splits;
+    const int row_end = rows_of(a, b);
+    const int n_splits = splits_of(a, row_end);
+    if (split >= n_splits) return;
+    const int pg_begin = split * a.split_pages;
+    decode4_piece(a, lds0, lds1, b, row_end, pg_begin, min((row_end + kPage - 1) / kPage, pg_begin + a.split_pages),
+                  n_splits == 1 ? -1 : (long)b * a.max_splits + split);
+  } else {
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    // steps up to and with sequence t
+    int* const sums = reinterpret_cast<int*>(&lds0);          // [8] of the waves, then the sequence and its first step
+    const int mine = t < a.num_seqs ? steps_of(rows_of(a, t)) : 0;
+    int upto = mine;
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) {
+      const int v = __shfl_up(upto, k, 64);
+      if (lane >= k) upto += v;
+    }
+    if (lane == 63) sums[wave] = upto;
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int k = 0; k < kHeadsKV; ++k) {
+      if (k < wave) upto += sums[k];
+      total += sums[k];
+    }
+    total = __builtin_amdgcn_readfirstlane(total);
+    const int share = (total + a.num_shares - 1) / a.num_shares;
+    const int begin = blockIdx.x * share, end = min(begin + share, total);
+    if (blockIdx.x == 0) {
+      if (t < a.num_seqs) a.prefix[t] = upto - mine;
+      if (t == 0) a.prefix[a.num_seqs] = total;
+    }
+    if (begin >= end) return;
+    if (upto - mine <= begin && begin < upto) {
+      sums[kHeadsKV] = t;
+      sums[kHeadsKV + 1] = upto - mine;
+    }
+    __syncthreads();
+    int b = __builtin_amdgcn_readfirstlane(sums[kHeadsKV]);
+    int before = __builtin_amdgcn_readfirstlane(sums[kHeadsKV + 1]);
+    for (int at = begin; at < end; ++b) {
+      __syncthreads();                                       // (LDS is free again)
+      const int rows = rows_of(a, b), steps = steps_of(rows);
+      const int to = min(before + steps, end);
+      const bool whole = at == before && to == before + steps;
+      decode4_piece(a, lds0, lds1, b, rows, 2 * (at - before), min((rows + kPage - 1) / kPage, 2 * (to - before)),
+                    whole ? -1 : 2l * blockIdx.x + (at != begin));
+      at = to;
+      before += steps;
+    }
+  }
+}
+
+// Joins the parts of a sequence: workgroup (head, sequence), kGroups groups of 16 lanes take the parts k = i, i + kGroups, ...,
+// four at a time, a lane 8 dims; their sums meet in LDS. A pass is a trip to another XCD's memory, so many parts take more
 // groups.
 template <int kGroups>
 __global__ __launch_bounds__(16 * kGroups) void decode4_merge_kernel(Decode4Args a) {
   const int head = blockIdx.x, b = blockIdx.y;
-  const int n = splits_of(a, rows_of(a, b));
+  long first;                                                // part 0; the others follow `second`, `apart` from each other
+  long second, apart;
+  int n;
+  if (a.split_pages > 0) {
+    n = splits_of(a, rows_of(a, b));
+    first = (long)b * a.max_splits;
+    second = first + 1;
+    apart = 1;
+  } else {
+    const int total = a.prefix[a.num_seqs], share = (total + a.num_shares - 1) / a.num_shares;
+    const int from = a.prefix[b], to = a.prefix[b + 1] - 1;
+    const int w0 = from / share;
+    n = to / share - w0 + 1;
+    first = 2l * w0 + (from != w0 * share);
+    second = 2l * w0 + 2;
+    apart = 2;
+  }
   if (n == 1) return;
   const int grp = threadIdx.x >> 4, c = threadIdx.x & 15;
   typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-  const long at = (long)b * a.max_splits * kHeadsQ + head;
   float M = -INFINITY, L = 0.f, acc[8] = {};
   for (int k0 = grp; k0 < n; k0 += 4 * kGroups) {
     floatx4 rec[4];
     f16x8 v[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {                            // (past the end: the last split again, without weight)
-      const long from = at + (long)min(k0 + u * kGroups, n - 1) * kHeadsQ;
+      const int k = min(k0 + u * kGroups, n - 1);
+      const long from = (k == 0 ? first : second + (k - 1) * apart) * kHeadsQ + head;
       rec[u] = *reinterpret_cast<const floatx4*>(a.part_ml + from * 4);
       v[u] = *reinterpret_cast<const f16x8*>(a.part_o + from * kHeadDim + 8 * c);
     }
@@ -455,6 +537,13 @@ using namespace abkv;
 
 constexpr int kMaxTokens = 0xFFFFFF;           // (256 threads each: work items of a launch fit 32 bits)
 
+// Shares of a launch: a workgroup a CU while that takes at most 16 steps, else two, in as many rounds as kShareSteps needs.
+static int decode4_shares(int num_seqs, int max_pages) {
+  const long steps = (long)num_seqs * ((max_pages + 1) / 2);
+  if (steps <= 256 * 16) return steps < 256 ? (int)steps : 256;
+  return 512 * (int)((steps + 512 * kShareSteps - 1) / (512 * kShareSteps));
+}
+
 static bool rows16_ok(const void* p, long st, long sh) {
   return p != nullptr && ((uintptr_t)p & 15) == 0 && ((st | sh) & 7) == 0;
 }
@@ -491,9 +580,12 @@ int abkv_kv_read_int4(const void* kv_cache, int num_pages, const int64_t* slot_m
 }
 
 size_t abkv_decode_int4_workspace_size(int num_seqs, int max_pages_per_seq, int split_pages) {
-  if (num_seqs <= 0 || max_pages_per_seq <= 0 || split_pages <= 0) return 0;
+  if (num_seqs <= 0 || max_pages_per_seq <= 0 || split_pages < 0) return 0;
+  constexpr size_t kPart = kHeadsQ * (kHeadDim * sizeof(_Float16) + 4 * sizeof(float));
+  if (split_pages == 0)
+    return num_seqs > kShareSeqs ? 0 : 2 * (size_t)decode4_shares(num_seqs, max_pages_per_seq) * kPart + (num_seqs + 1) * sizeof(int);
   const int splits = (max_pages_per_seq + split_pages - 1) / split_pages;
-  return splits > 1 ? (size_t)num_seqs * splits * kHeadsQ * (kHeadDim * sizeof(_Float16) + 4 * sizeof(float)) : 0;
+  return splits > 1 ? (size_t)num_seqs * splits * kPart : 0;
 }
 
 int abkv_decode_attn_int4(const void* q, long q_stride_seq, long q_stride_head, const void* kv_cache, int num_pages,
@@ -501,7 +593,7 @@ int abkv_decode_attn_int4(const void* q, long q_stride_seq, long q_stride_head, 
                           int max_pages_per_seq, int split_pages, float scale, void* out, long out_stride_seq,
                           long out_stride_head, float* lse, void* workspace, size_t workspace_bytes, hipStream_t stream) {
   if (num_seqs <= 0) return 0;
-  if (split_pages <= 0 || (split_pages & 1) || split_pages > 64 || max_pages_per_seq <= 0 || max_pages_per_seq > (1 << 26) ||
+  if (split_pages < 0 || (split_pages & 1) || split_pages > 64 || (split_pages == 0 && num_seqs > kShareSeqs) || max_pages_per_seq <= 0 || max_pages_per_seq > (1 << 26) ||
       num_pages <= 0 || block_table_stride < max_pages_per_seq || num_seqs > 65535 || !softmax_scale_ok(scale) ||
       !rows16_ok(q, q_stride_seq, q_stride_head) || !rows16_ok(kv_cache, 0, 0) || block_table == nullptr ||
       seq_lens == nullptr || !rows16_ok(out, out_stride_seq, out_stride_head))
@@ -518,21 +610,27 @@ int abkv_decode_attn_int4(const void* q, long q_stride_seq, long q_stride_head, 
   a.bt_stride = block_table_stride;
   a.seq_lens = seq_lens;
   a.split_pages = split_pages;
-  a.max_splits = (max_pages_per_seq + split_pages - 1) / split_pages;
+  a.max_splits = split_pages ? (max_pages_per_seq + split_pages - 1) / split_pages : 0;
   a.max_pages = max_pages_per_seq;
+  a.num_seqs = num_seqs;
+  a.num_shares = split_pages ? 0 : decode4_shares(num_seqs, max_pages_per_seq);
   a.scale_log2 = scale * 1.4426950408889634f;
   a.out = static_cast<__bf16*>(out);
   a.o_sb = out_stride_seq;
   a.o_sh = out_stride_head;
   a.lse = lse;
+  const size_t parts = split_pages ? (size_t)num_seqs * a.max_splits : 2 * (size_t)a.num_shares;
   a.part_o = static_cast<_Float16*>(workspace);
-  a.part_ml = reinterpret_cast<float*>(a.part_o + (size_t)num_seqs * a.max_splits * kHeadsQ * kHeadDim);
-  const long groups = (long)num_seqs * a.max_splits;
+  a.part_ml = reinterpret_cast<float*>(a.part_o + parts * kHeadsQ * kHeadDim);
+  a.prefix = reinterpret_cast<int*>(a.part_ml + parts * kHeadsQ * 4);
+  const long groups = split_pages ? (long)num_seqs * a.max_splits : a.num_shares;
   if (groups * 64 * kHeadsKV > 0xFFFFFFFFL) return (int)hipErrorInvalidValue;
-  hipLaunchKernelGGL(decode4_kernel, dim3((unsigned)groups), dim3(64 * kHeadsKV), 0, stream, a);
+  if (split_pages) hipLaunchKernelGGL(decode4_kernel<false>, dim3((unsigned)groups), dim3(64 * kHeadsKV), 0, stream, a);
+  else hipLaunchKernelGGL(decode4_kernel<true>, dim3((unsigned)groups), dim3(64 * kHeadsKV), 0, stream, a);
   const hipError_t err = hipGetLastError();
-  if (err != hipSuccess || a.max_splits == 1) return (int)err;
-  if (a.max_splits > 64) hipLaunchKernelGGL(decode4_merge_kernel<64>, dim3(kHeadsQ, num_seqs), dim3(1024), 0, stream, a);
+  if (err != hipSuccess || (split_pages && a.max_splits == 1)) return (int)err;
+  const int most = split_pages ? a.max_splits : (a.num_shares + num_seqs - 1) / num_seqs;     // parts a sequence, about
+  if (most > 64) hipLaunchKernelGGL(decode4_merge_kernel<64>, dim3(kHeadsQ, num_seqs), dim3(1024), 0, stream, a);
   else hipLaunchKernelGGL(decode4_merge_kernel<16>, dim3(kHeadsQ, num_seqs), dim3(256), 0, stream, a);
   return (int)hipGetLastError();
 }

@@ -1539,32 +1539,37 @@ def kv_read_int4(kv_cache: torch.Tensor, slot_mapping: torch.Tensor,
     return key, value
 
 
-def int4_split_pages(num_seqs: int, max_pages: int) -> int:
-    """Pages per split of a decode over a cache in 4 bits, an even number of at most 64, for tables of ``max_pages``.
+INT4_SHARE_SEQS = 512
 
-    A compute unit holds two workgroups, and what has no full round of them waits for its slowest, so a split is as long as
-    leaves one workgroup on each of the 256 units (one sequence of 131000 rows: 32 pages 32.8 us, 16 pages 38.1; 32000 rows:
-    8 pages 16.8 us, 4 pages 20.4, 16 pages 19.7), or two where that would take more than 32 pages (32 sequences of 9500 rows:
-    40 pages 77 us, 64 pages 86, 20 pages 82). More than two rounds of 64 pages run in splits of 20, whose uneven ends weigh
-    little (256 sequences of 500 to 3000 rows: 134 us, in 48 pages 138, in 64 pages 145, in 8 pages 142)."""
+
+def int4_split_pages(num_seqs: int, max_pages: int) -> int:
+    """How a decode over a cache in 4 bits goes out, for tables of ``max_pages``: pages per split, an even number up to 64, or 0:
+    equal shares of all sequences' rows.
+
+    Up to 8192 pages a split is as long as leaves one workgroup on each of the 256 compute units (one sequence of 32000 rows: 8
+    pages 16.6 us, 4 pages 19.9, 16 pages 20.0, shares 18.3; of 131000 rows: 32 pages 37, 16 pages 39, shares 38.5). Beyond, a
+    full round of workgroups reads as fast as memory does, and shares end together (64 sequences of 500 to 9500 rows: 78 us,
+    splits of 12, 20, 32 and 40 pages 94, 91, 88 and 92; 256 of 500 to 3000: 110, splits of 20 129; 32 of 9500: 71, splits of
+    40, which fit them, 68), up to 512 sequences; more of them run in splits of 20, whose uneven ends weigh little."""
     total = num_seqs * max_pages
     most = -(-total // 256)
     if most > 32:
-        most = -(-total // 512)
-        most = 20 if most > 64 else max(most, 20)
+        if num_seqs <= INT4_SHARE_SEQS:
+            return 0
+        most = 20
     most = max(2, most)
     splits = -(-max_pages // most)
     return min(64, -(-max_pages // (2 * splits)) * 2)
 
 
 def decode_int4_bytes(num_seqs: int, max_pages: int, split_pages: int) -> int:
-    """Workspace bytes that :func:`decode_attention_int4` takes with ``split_pages`` pages a split."""
+    """Workspace bytes that :func:`decode_attention_int4` takes with ``split_pages`` pages a split (0: shares)."""
     return lib().abkv_decode_int4_workspace_size(num_seqs, max_pages, split_pages)
 
 
 def decode_int4_workspace(num_seqs: int, max_pages: int, split_pages: int | None = None, device=None) -> torch.Tensor | None:
-    """Workspace for :func:`decode_attention_int4` of the same sizes (None when no sequence can need a second split)."""
-    n = decode_int4_bytes(num_seqs, max_pages, split_pages or int4_split_pages(num_seqs, max_pages))
+    """Workspace for :func:`decode_attention_int4` of the same sizes (None when it needs none)."""
+    n = decode_int4_bytes(num_seqs, max_pages, int4_split_pages(num_seqs, max_pages) if split_pages is None else split_pages)
     return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
 
@@ -1574,14 +1579,18 @@ def decode_attention_int4(q: torch.Tensor, kv_cache: torch.Tensor, block_table: 
                           workspace: torch.Tensor | None = None):
     """:func:`decode_attention` over a cache in 4 bits (:func:`kv_cache_int4_shape`): q [B, 32, 128] bf16; returns
     (out [B, 32, 128] bf16, lse [B, 32] fp32 or None). The codes enter the products exactly; a weight times its row's step is
-    rounded to bf16. Slots behind a sequence's rows may hold anything. ``split_pages`` None: chosen by the sizes."""
+    rounded to bf16. Slots behind a sequence's rows may hold anything. ``split_pages``: pages a workgroup takes of one sequence; 0
+    (up to 512 sequences): workgroups take equal shares of all sequences' rows, whatever their lengths; None: chosen by the sizes
+    (:func:`int4_split_pages`)."""
     scale = _softmax_scale(scale)
     _check_cache4(kv_cache)
-    B, max_pages = _check_step(q, None, block_table, seq_lens, max_pages, split_pages, out, lse)
+    B, max_pages = _check_step(q, None, block_table, seq_lens, max_pages, split_pages or None, out, lse)
+    _require(split_pages != 0 or B <= INT4_SHARE_SEQS, f"split_pages 0 takes up to {INT4_SHARE_SEQS} sequences")
     _check_device(q, kv_cache, block_table, seq_lens, out, lse)
     if out is None:
         out = q.new_empty((B, HEADS_Q, HEAD_DIM))
-    split_pages = split_pages or int4_split_pages(B, max_pages)
+    if split_pages is None:
+        split_pages = int4_split_pages(B, max_pages)
     need = lib().abkv_decode_int4_workspace_size(B, max_pages, split_pages)
     workspace, ws_bytes = _take_workspace(workspace, need, q.device)
     rc = lib().abkv_decode_attn_int4(_ptr(q), q.stride(0), q.stride(1), _ptr(kv_cache), kv_cache.shape[0], _ptr(block_table),

@@ -377,8 +377,8 @@ def _kv_append_int4_fake(key, value, slot_mapping, kv_cache):
 @torch.library.custom_op(f"{_NS}::decode_attn_int4", mutates_args=("out", "lse", "workspace"))
 def decode_attn_int4(q: Tensor, kv_cache: Tensor, block_table: Tensor, seq_lens: Tensor, scale: float, max_pages: int,
                      split_pages: int, out: Tensor, lse: Optional[Tensor], workspace: Optional[Tensor]) -> None:
-    """abkv_decode_attn_int4: decode over a cache in 4 bits. A batch that needs more than one split must bring ``workspace``
-    (ops.decode_int4_workspace): the op never allocates."""
+    """abkv_decode_attn_int4: decode over a cache in 4 bits. ``split_pages`` 0: equal shares. A batch that needs a ``workspace``
+    (ops.decode_int4_workspace) must bring it: the op never allocates."""
     if lib().abkv_decode_int4_workspace_size(q.shape[0], max_pages, split_pages):
         _need(workspace is not None, "decode_attn_int4: the batch needs a workspace (ops.decode_int4_workspace)")
     _ops.decode_attention_int4(q, kv_cache, block_table, seq_lens, scale, max_pages=max_pages, out=out, lse=lse,

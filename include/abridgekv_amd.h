@@ -573,7 +573,8 @@ int abkv_kv_append_int4(const void* key, long key_stride_t, long key_stride_h, c
 /* Rows by slot as values [T, 8, 128], fp32 (f32 != 0) or bf16, dense; a slot outside the cache reads as zeros. */
 int abkv_kv_read_int4(const void* kv_cache, int num_pages, const int64_t* slot_mapping, int num_tokens, int f32, void* key,
                       void* value, abkv_stream_t stream);
-/* abkv_decode_attn over a cache in 4 bits. workspace: abkv_decode_int4_workspace_size bytes, 16-byte aligned (0: none needed).
+/* abkv_decode_attn over a cache in 4 bits. split_pages 0 (num_seqs <= 512): workgroups take equal shares of all sequences' rows
+ * in place of split_pages pages of one sequence. workspace: abkv_decode_int4_workspace_size bytes, 16-byte aligned (0: none needed).
  * num_seqs <= 65535. */
 size_t abkv_decode_int4_workspace_size(int num_seqs, int max_pages_per_seq, int split_pages);
 int abkv_decode_attn_int4(const void* q, long q_stride_seq, long q_stride_head, const void* kv_cache, int num_pages,

@@ -124,7 +124,7 @@ def _close(out, lse, q, k, v, vis, wide=False):
 LENS = [0, 1, 15, 16, 17, 33, 100, 511, 513, 1300]
 
 
-@pytest.mark.parametrize("split_pages", [2, 8, 64, None])
+@pytest.mark.parametrize("split_pages", [0, 2, 8, 64, None])
 def test_decode(split_pages):
     from abridgekv_amd import ops
     q, k, v, cache, table, sl = _paged(LENS, 11)
@@ -133,6 +133,44 @@ def test_decode(split_pages):
     assert got is lse
     for b, n in enumerate(LENS):
         _close(out[b: b + 1], lse[b: b + 1], q[b: b + 1], k[b], v[b], np.ones((1, n), bool))
+
+
+@pytest.mark.parametrize("lens", [[1], [32], [33], [5000], [9000, 1], [0] * 5, [7] * 300, [0, 2100, 0, 0, 31, 4097, 64, 1, 0], "many", "long"])
+def test_decode_in_shares(lens):
+    """Equal shares against splits: shares that end inside sequences, at their ends, that hold many of them, empty ones; few
+    sequences, 512, and enough rows for shares of more than 64 pages."""
+    from abridgekv_amd import ops
+    if lens == "many":
+        lens = np.random.default_rng(5).integers(0, 400, 512).tolist()
+    if lens == "long":
+        lens = [33000 + 1000 * i for i in range(40)]
+    B, W = len(lens), max(1, -(-max(lens) // 16))
+    gen = torch.Generator(device="cuda").manual_seed(B)
+    k, v = (torch.randn((16 * 500, 8, 128), device="cuda", generator=gen).to(torch.bfloat16) for _ in range(2))
+    cache = torch.zeros(ops.kv_cache_int4_shape(500), dtype=torch.uint8, device="cuda")
+    ops.kv_append_int4(k, v, torch.arange(16 * 500, device="cuda"), cache)
+    table = torch.randint(0, 500, (B, W), device="cuda", dtype=torch.int32, generator=gen)
+    sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    q = torch.randn((B, 32, 128), device="cuda", generator=gen).to(torch.bfloat16)
+    la, lb = (torch.full((B, 32), 3.0, device="cuda") for _ in range(2))
+    a, _ = ops.decode_attention_int4(q, cache, table, sl, lse=la, split_pages=0)
+    b, _ = ops.decode_attention_int4(q, cache, table, sl, lse=lb, split_pages=64)
+    some = sl > 0
+    assert not a[~some].any() and (la[~some] == -np.inf).all()
+    # each has a weight times a step rounded to bf16 (2^-8, errors that part ways where the running maxima differ) of values
+    # within 8 steps of the middle, its output rounded (2^-8), parts in fp16 (2^-11 of the largest value): twice their sum
+    step, largest = 0.8, 6.0                                 # of rows of normal numbers: (max - min) / 15, and of any value
+    size = 8 * step + a.float().abs() + largest * 2.0 ** -3
+    assert ((a.float() - b.float()).abs() <= 2 * 2.0 ** -8 * size).all()
+    assert torch.allclose(la[some], lb[some], rtol=1e-5, atol=1e-4)
+    c, _ = ops.decode_attention_int4(q, cache, table, sl, split_pages=0)
+    assert torch.equal(a, c)
+    if B > 40:
+        for i in (0, B // 2, B - 1):
+            n, t = lens[i], table[i].long().cpu().numpy()
+            rows = cache.cpu().numpy()[t[np.arange(n) // 16], :, np.arange(n) % 16] if n else np.zeros((0, 2, 640), np.uint8)
+            _close(a[i: i + 1], la[i: i + 1], q[i: i + 1].cpu(), np.ascontiguousarray(rows[:, 0]), np.ascontiguousarray(rows[:, 1]),
+                   np.ones((1, n), bool))
 
 
 def test_decode_bounds_and_views():

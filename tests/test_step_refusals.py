@@ -235,11 +235,16 @@ def test_c_entries_return_errors():
 
 
 def test_int4_splits_fit_any_step():
-    """A split is an even number of pages up to 64, and 64 a split take no more than any longer table's own splits."""
-    for B in (1, 2, 7, 64, 300):
-        for longest in (1, 3, 63, 64, 65, 512, 513, 2048, 8191, 8193, 40000):
-            own = ops.int4_split_pages(B, longest)
-            assert own % 2 == 0 and 2 <= own <= 64
-            held = ops.decode_int4_bytes(B, longest, own)
-            for pages in {1, longest // 3 + 1, longest - 1 or 1, longest}:
-                assert ops.decode_int4_bytes(B, pages, 64) <= held
+    """Equal shares or an even number of pages up to 64; a step of shorter tables and fewer sequences finds room in what a builder
+    holds for the longest ones: its own splits or shares, or longer splits."""
+    for most in (1, 2, 64, 512, 520):
+        for longest in (1, 3, 65, 129, 512, 513, 8191, 8193, 40000):
+            held = max(ops.decode_int4_bytes(b, longest, ops.int4_split_pages(b, longest)) for b in range(1, most + 1))
+            for b in {1, most // 2 + 1, most}:
+                for pages in {1, longest // 3 + 1, longest - 1 or 1, longest}:
+                    split = ops.int4_split_pages(b, pages)
+                    assert split % 2 == 0 and 0 <= split <= 64 and (split > 0 or (b <= 512 and b * pages > 8192))
+                    need = ops.decode_int4_bytes(b, pages, split)
+                    assert need <= held or (split > 0 and ops.decode_int4_bytes(b, pages, 64) <= held)
+    q, c = torch.zeros((513, 32, 128), dtype=BF), _cache()
+    _bad("512 sequences", ops.decode_attention_int4, q, c, torch.zeros((513, 4), dtype=I32), torch.zeros(513, dtype=I32), split_pages=0)
