@@ -108,8 +108,8 @@ __device__ __forceinline__ int steps_of(int rows) { return max(1, (rows + 2 * kP
 // (mask in a vector register: with both constants literal the and and the or are instructions of their own)
 __device__ __forceinline__ uint32_t code_pair(uint32_t w, int n, uint32_t mask) { return ((w >> (4 * n)) & mask) | 0x43004300u; }
 
-// Workgroup (split, sequence), a wave per KV head. A wave walks its split 32 slots (two pages) at a time, the next step's rows
-// on the way meanwhile.
+// A wave per KV head. A workgroup walks its rows of a sequence 32 slots (two pages) at a time, the next step's rows on the way
+// meanwhile.
 //
 // Scores: the four groups of 32 dims have their own steps and minima, so a score is the sum of four products:
 //   x_j = sum_g (s_jg a_jg + m_jg Q_g),  a_jg = sum_{d in g} q_d c_jd,  Q_g = sum_{d in g} q_d.
@@ -125,8 +125,8 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t w, int n, uint32_t mask) 
 // What bounds the reads is the number of cache lines that a CU asks for (about one in six cycles), so a line should bring what it
 // holds: a head's codes are half of one, its pairs an eighth. The workgroup's waves therefore fetch whole rows together, straight
 // into LDS (a wave 5 of the step's 40 KB), one barrier a step. (64 sequences of 500 to 9500 rows, every wave its own pieces: 118
-// us, of which 59 went with the pairs alone; the pairs shared, 99; whole rows, 94, of which 62 are vector work: 410 MB at 4.7 TB/s.
-// Three stages of LDS leave one workgroup a CU: 104.)
+// us, of which 59 went with the pairs alone; the pairs shared, 99; whole rows, 94, nontemporal, 86, in equal shares, 73 without the
+// merge: 410 MB at 5.6 TB/s; 62 are vector work. Three stages of LDS leave one workgroup a CU: 104 where two took 94.)
 constexpr int kPairs4 = 16 * 4 * kHeadsKV, kCodes4 = 16 * kHeadsKV * 16;     // dwords of a page's pairs and codes (of K or V)
 template <class T>
 __device__ __forceinline__ const T& at4(const uint32_t* base, uint32_t bytes) {
