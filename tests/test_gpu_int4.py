@@ -173,6 +173,36 @@ def test_decode_in_shares(lens):
                    np.ones((1, n), bool))
 
 
+def test_shares_in_a_graph():
+    """A captured decode in shares follows lengths that change between replays, through the custom op and its workspace, beside
+    eager calls with a workspace of their own."""
+    from abridgekv_amd import ops, torch_ops  # noqa: F401
+    B, W = 48, 200
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    cache = torch.zeros(ops.kv_cache_int4_shape(300), dtype=torch.uint8, device="cuda")
+    k, v = (torch.randn((16 * 300, 8, 128), device="cuda", generator=gen).to(torch.bfloat16) for _ in range(2))
+    ops.kv_append_int4(k, v, torch.arange(16 * 300, device="cuda"), cache)
+    table = torch.randint(0, 300, (B, W), device="cuda", dtype=torch.int32, generator=gen)
+    q = torch.randn((B, 32, 128), device="cuda", generator=gen).to(torch.bfloat16)
+    sl = torch.randint(0, 16 * W + 1, (B,), device="cuda", dtype=torch.int32, generator=gen)
+    assert ops.int4_split_pages(B, W) == 0
+    out, lse = torch.empty_like(q), torch.empty((B, 32), device="cuda")
+    ws = ops.decode_int4_workspace(B, W, device="cuda")
+    step = lambda: torch.ops.abridgekv.decode_attn_int4(q, cache, table, sl, SCALE, W, 0, out, lse, ws)      # noqa: E731
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for i in range(4):
+        sl.copy_(torch.randint(0, (16 * W, 40)[i % 2] + 1, (B,), device="cuda", dtype=torch.int32, generator=gen))
+        graph.replay()
+        got, got_lse = out.clone(), lse.clone()
+        want_lse = torch.empty_like(lse)
+        want, _ = ops.decode_attention_int4(q, cache, table, sl, SCALE, lse=want_lse)
+        assert torch.equal(got, want) and torch.equal(got_lse, want_lse)
+
+
 def test_decode_bounds_and_views():
     """Lengths past max_pages are cut, queries and outputs are slices, extra table rows and lengths stay unread."""
     from abridgekv_amd import ops
