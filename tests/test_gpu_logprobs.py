@@ -177,6 +177,20 @@ def test_gradient_of_a_banned_target():
     _check_grad(ops.token_logprobs_backward(x.cuda(), t.cuda(), got.stats, g.cuda(), None), x, t, g, torch.zeros(2), 1.0)
 
 
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+def test_gradient_at_a_low_temperature(dt):
+    """Banned tokens take exactly no gradient, however steep the others' are."""
+    from abridgekv_amd import ops
+    x, t = _logits(3, 700, dt, 5, banned=60)
+    x[1, 3] = torch.finfo(dt).min
+    st = ops.token_logprobs(x.cuda(), t.cuda(), 1e-6, stats=True).stats
+    h = torch.full((3,), 1000.0, device="cuda")
+    grad = ops.token_logprobs_backward(x.cuda(), t.cuda(), st, h, h, 1e-6).cpu()
+    banned = x < -1e25
+    banned[torch.arange(3), t] = False
+    assert torch.isfinite(grad).all() and banned.any() and not grad[banned].any()
+
+
 def test_gradient_over_the_logits():
     from abridgekv_amd import ops
     x, t = _logits(9, 4001, torch.bfloat16, 3)
