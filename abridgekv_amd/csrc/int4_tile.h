@@ -2,7 +2,8 @@
 //
 // The waves unpack a 64-key tile of codes into K and V tiles of fp16 in LDS, laid out as attn_tile.h's, and attend to them with
 // v_mfma_f32_16x16x32_f16. fp16 keeps a value m + s c to 2^-11 of itself where bf16 (the type that the cache is written from)
-// would round it a second time, to 2^-8; the weights gain as much. Its range is made up for by powers of two, which are exact:
+// would round it a second time, to 2^-8; the weights gain as much, down to 2^-25 of the largest (kHeadroom). Its range is made up
+// for by powers of two, which are exact:
 //   K: 2^eK for each page, multiplied back into the page's scores;
 //   Q: 2^eQ for each query row and head, likewise;
 //   V: 2^eV for all of a walk, the largest need of its tiles so far; the output's sums are rescaled when it grows.
@@ -52,6 +53,15 @@ __device__ __forceinline__ Int4Part load_part(const Int4Rows& rows, int page, bo
 }
 
 constexpr int kLowestExp = -104;                             // (2^104 is still a float)
+
+// A row's weights are 2^(score - ref), with ref kHeadroom below the running maximum, which moves when a weight would pass 2^15: so
+// the largest lies between 2^kHeadroom and 2^15, the one at the walk's maximum so far among them. A weight is rounded to 2^-11 of
+// itself down to 2^-25 of the largest; below, where fp16 has no finer steps, by up to 2^-36 of the largest, and the sum, taken of
+// the rounded ones, by at most that for each row. (With weights up to 2^8 alone, a row that took most of the weight cost the
+// others theirs from 2^-14 of it on. Less headroom moves ref less often: three chunks of 300 to 441 queries behind up to 8000
+// rows and a code step take 168.6 us with 7, 169.1 with 11, 175.6 with 13; with scores of four times the spread 176, 185 and 191.)
+constexpr int kHeadroom = 11;
+
 // The exponent that values up to `bound` take.
 __device__ __forceinline__ int range_exp(float bound) {
   const int e = (int)(__float_as_uint(bound) >> 23) - 127 - 14;           // (bound >= 0; infinity: 114)
@@ -159,6 +169,9 @@ __device__ __forceinline__ void attend_tiles_int4(const Int4Rows& rows, Walk& wa
     const int e = range_exp(page_bound(p));
     if (lane == 0) v_need[i & 1][page] = e;
   };
+  float ref[H];                                              // the running maximum less kHeadroom
+#pragma unroll
+  for (int u = 0; u < H; ++u) ref[u] = -INFINITY;
   floatx4 s[2][2][H];
   auto scores = [&](const __bf16* buf) {
 #pragma unroll
@@ -220,13 +233,12 @@ __device__ __forceinline__ void attend_tiles_int4(const Int4Rows& rows, Walk& wa
     part = load(n + 2);
     walk.next(k0, tm, n == 0);
     tile_mask<H, Walk>(s, k0, tm, lane_mask, j);
-    // online softmax, as tile_softmax: the log2 scores relative to the running maximum, which moves when a score passes it by
-    // more than 8
+    // online softmax, as tile_softmax: the log2 scores relative to ref, which moves when a weight would pass 2^15
     float neg_m[H];
     bool need = false;
 #pragma unroll
     for (int u = 0; u < H; ++u) {
-      neg_m[u] = m_run[u] == -INFINITY ? 0.f : -m_run[u];
+      neg_m[u] = ref[u] == -INFINITY ? 0.f : -ref[u];
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
@@ -235,16 +247,16 @@ __device__ __forceinline__ void attend_tiles_int4(const Int4Rows& rows, Walk& wa
 #pragma unroll
           for (int r = 0; r < 4; ++r) s[kk][t][u][r] = fmaf(s[kk][t][u][r], f, neg_m[u]);
         }
-      need |= lane_max(s, u) > (m_run[u] == -INFINITY ? -INFINITY : 8.f);
+      need |= lane_max(s, u) > (ref[u] == -INFINITY ? -INFINITY : 15.f);
     }
     if (__any(need)) {
 #pragma unroll
       for (int u = 0; u < H; ++u) {
         const float tmax = max_xor32(max_xor16(lane_max(s, u)));
-        const float m_new = fmaxf(m_run[u], tmax - neg_m[u]);
-        const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run[u] - m_new);
-        const float d = m_new == -INFINITY ? 0.f : m_new + neg_m[u];
-        m_run[u] = m_new;
+        const float r_new = fmaxf(ref[u], tmax - neg_m[u] - kHeadroom);
+        const float alpha = r_new == -INFINITY ? 1.f : fast_exp2(ref[u] - r_new);
+        const float d = r_new == -INFINITY ? 0.f : r_new + neg_m[u];
+        ref[u] = r_new;
         lsum[u] *= alpha;
 #pragma unroll
         for (int i = 0; i < 8; ++i) o[i][u] *= alpha;
@@ -287,10 +299,11 @@ __device__ __forceinline__ void attend_tiles_int4(const Int4Rows& rows, Walk& wa
     if (++n >= tiles) break;
   }
   if (!is_v) end_phase();
-  const float f = exp2i(v_exp);
+  const float f = exp2i(v_exp - kHeadroom);
 #pragma unroll
   for (int u = 0; u < H; ++u) {
-    l_run[u] = lsum[u][0];
+    m_run[u] = ref[u] + kHeadroom;
+    l_run[u] = lsum[u][0] * exp2i(-kHeadroom);
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[i][u] *= f;
   }

@@ -5,7 +5,8 @@ stand for. ``bounds`` derives how far a kernel may be off: it takes a weight tim
 2^-8 of it), against a code less 8, and the weight in fp32 against the group's middle, and rounds the output; split partials are
 fp16 (2^-11 of the split's largest output, itself at most the largest value). ``wide``: the multi-query kernel instead takes
 values and weights in fp16 (half a step, 2^-11 of each; its powers of two keep them, and what is 2^-19 of its row's or page's largest,
-in the type's normal range), and its partials are fp32.
+in the type's normal range; weights down to 2^-25 of the row's largest, and what lies below is off by up to 2^-36 of that, which is
+not in the bounds), and its partials are fp32.
 """
 from __future__ import annotations
 
