@@ -64,11 +64,13 @@ constexpr int kHeadroom = 11;
 
 // The exponent that values up to `bound` take.
 __device__ __forceinline__ int range_exp(float bound) {
-  const int e = (int)(__float_as_uint(bound) >> 23) - 127 - 14;           // (bound >= 0; infinity: 114)
+  const int e = (int)(__float_as_uint(bound) >> 23) - 127 - 14;           // (bound >= 0; infinity: 114, so 120)
   return max((e + 7) & ~7, kLowestExp);
 }
 __device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
-// A float's bits times 2^e for e << 23, from 2^-100 (so that -inf stays that, and no score that counts is as small) to 2^127.
+// A float's bits times 2^e for e << 23, from 2^-100 (so that -inf stays that, and no score that counts is as small) to 2^127. For the
+// softmax scale times 2^(eQ + eK) it is called once, with both exponents (up to 240 << 23, an int): a part of the product may lie
+// outside that range where the whole does not.
 __device__ __forceinline__ float scaled_bits(int bits, int e23) {
   return __int_as_float(min(max(__builtin_elementwise_add_sat(bits, e23), 27 << 23), 254 << 23));
 }
@@ -126,7 +128,7 @@ __device__ __forceinline__ void attend_tiles_int4(const Int4Rows& rows, Walk& wa
   __shared__ int v_need[2][4];                               // [tile % 2][page]
 
   f16x8 q[H][4];
-  int scale[H];                                              // the scale's bits, times 2^eQ
+  int q_exp[H];                                              // eQ << 23
 #pragma unroll
   for (int u = 0; u < H; ++u) {
     float x = 0.f;
@@ -140,7 +142,7 @@ __device__ __forceinline__ void attend_tiles_int4(const Int4Rows& rows, Walk& wa
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int d = 0; d < 8; ++d) q[u][i][d] = (_Float16)((float)qop[u][i][d] * f);
-    scale[u] = __float_as_int(scaled_bits(__float_as_int(scale_log2), e * (1 << 23)));
+    q_exp[u] = e * (1 << 23);
   }
 
   // This wave's part of tile i of the walk; slots past the last key read as zeros (their weights are 0)
@@ -243,7 +245,7 @@ __device__ __forceinline__ void attend_tiles_int4(const Int4Rows& rows, Walk& wa
       for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const float f = scaled_bits(scale[u], ke[2 * kk + t]);
+          const float f = scaled_bits(__float_as_int(scale_log2), q_exp[u] + ke[2 * kk + t]);
 #pragma unroll
           for (int r = 0; r < 4; ++r) s[kk][t][u][r] = fmaf(s[kk][t][u][r], f, neg_m[u]);
         }

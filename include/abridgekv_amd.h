@@ -582,8 +582,8 @@ int abkv_decode_attn_int4(const void* q, long q_stride_seq, long q_stride_head, 
                           int max_pages_per_seq, int split_pages, float scale, void* out, long out_stride_seq,
                           long out_stride_head, float* lse, void* workspace, size_t workspace_bytes, abkv_stream_t stream);
 /* abkv_paged_prefill_attn_items over a cache in 4 bits, whose values and weights the tiles hold in fp16 over powers of two (a
- * value to 2^-11 of itself, and no finer than 2^-30 of the largest of its row's page, or of its head's V so far; a weight to 2^-11
- * of itself, and no finer than 2^-36 of its row's largest). */
+ * value to 2^-11 of itself, and no finer than 2^-30 of the largest of its row's page, or of its head's V so far, or than 2^-129; a
+ * weight to 2^-11 of itself, and no finer than 2^-36 of its row's largest). */
 int abkv_paged_prefill_attn_items_int4(const void* q, long q_stride_t, long q_stride_h, const void* kv_cache, int num_pages,
                                        const int32_t* block_table, long block_table_stride, int block_table_width,
                                        const int32_t* q_start, const int32_t* kv_start, const int32_t* kv_limit,
