@@ -110,6 +110,13 @@ struct RangeWalk {
   }
 };
 
+// A row's lse from its maximum m (log2 units) and weight sum l: -inf where it sees nothing. Of a row that reads as NaN a 4-bit cache
+// makes a NaN (l is one), as its single-token kernel does; the bf16 kernels all leave -inf there.
+template <bool kInt4>
+__device__ __forceinline__ float row_lse(float m, float l) {
+  return l > 0.f ? (m + __log2f(l)) * 0.69314718055994531f : kInt4 && l != 0.f ? l : -INFINITY;
+}
+
 // kRows: the paged rows of the request; its side rows (all visible to every query); its rows in a cache of 4 bits.
 constexpr int kPagedRows = 0, kSideRows = 1, kInt4Rows = 2;
 template <int kRows>
@@ -283,7 +290,7 @@ __global__ __launch_bounds__(512, 1) void paged_prefill_kernel(PagedPrefillArgs 
 #pragma unroll
     for (int p = 0; p < 4; ++p) store_acc_bf16x8(oh + 8 * p, o[2 * p][u], o[2 * p + 1][u], j, inv);
     if (a.lse != nullptr && j == 0)
-      a.lse[(long)(t0 + qi) * kHeadsQ + head] = l > 0.f ? (m_run[u] + __log2f(l)) * 0.69314718055994531f : -INFINITY;
+      a.lse[(long)(t0 + qi) * kHeadsQ + head] = row_lse<kRows == kInt4Rows>(m_run[u], l);
   }
 }
 
@@ -291,6 +298,7 @@ __global__ __launch_bounds__(512, 1) void paged_prefill_kernel(PagedPrefillArgs 
 // waves (head u of the two) in the attention kernel's lane order, so every load is a whole 1 KiB run. (Two accumulator tiles, not
 // eight, so that one merged query tile, of up to 32 parts of 1 MiB, is work for all 256 compute units: 19 -> 11 us; many
 // merged tiles take what they took.)
+template <bool kInt4>
 __global__ __launch_bounds__(128) void paged_merge_items_kernel(PagedPrefillArgs a) {
   constexpr int H = 2, kWaves = 8, kLaneRuns = kItemFloats / kHeadsKV / kWaves;
   const int p = blockIdx.x % 4, w = blockIdx.x / 4 % kWaves, kvh = blockIdx.x / (4 * kWaves) % kHeadsKV;
@@ -325,7 +333,7 @@ __global__ __launch_bounds__(128) void paged_merge_items_kernel(PagedPrefillArgs
   const int head = kvh * kGroup + H * (w & 1) + u;
   store_acc_bf16x8(a.out + tok * a.o_st + (long)head * a.o_sh + 32 * j + 8 * p, acc[0], acc[1], j, inv);
   if (a.lse != nullptr && j == 0 && p == 0)
-    a.lse[tok * kHeadsQ + head] = L > 0.f ? (M + __log2f(L)) * 0.69314718055994531f : -INFINITY;
+    a.lse[tok * kHeadsQ + head] = row_lse<kInt4>(M, L);
 }
 
 // Combine the key-split partials of a query token (uniform splits): workgroup (token, group of 8 heads); thread t handles
@@ -430,7 +438,9 @@ static int prefill_items(bool int4, const void* q, long q_stride_t, long q_strid
   else hipLaunchKernelGGL(paged_prefill_kernel<kPagedRows>, dim3(grid), dim3(512), 0, stream, a);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess || n_merges == 0) return (int)err;
-  hipLaunchKernelGGL(paged_merge_items_kernel, dim3((unsigned)n_merges * 4 * 8 * kHeadsKV), dim3(128), 0, stream, a);
+  const dim3 merge_grid((unsigned)n_merges * 4 * 8 * kHeadsKV);
+  if (int4) hipLaunchKernelGGL(paged_merge_items_kernel<true>, merge_grid, dim3(128), 0, stream, a);
+  else hipLaunchKernelGGL(paged_merge_items_kernel<false>, merge_grid, dim3(128), 0, stream, a);
   return (int)hipGetLastError();
 }
 

@@ -1604,7 +1604,9 @@ def paged_prefill_attention_int4(q: torch.Tensor, kv_cache: torch.Tensor, block_
                                  kv_limit, causal, scale: float | None = None, out: torch.Tensor | None = None,
                                  lse: torch.Tensor | None = None, excluded=None):
     """:func:`paged_prefill_attention` (prompt chunks and code steps; bf16 queries) over a cache in 4 bits, whose values and
-    weights the products take in fp16. Returns (out [T, 32, 128] bf16, lse [T, 32] fp32 or None)."""
+    weights the products take in fp16. Returns (out [T, 32, 128] bf16, lse [T, 32] fp32 or None). A group of keys that reads as NaN
+    makes out and lse NaN for the queries that see it, in its KV head; a group of values makes out NaN in its dims, for these and for
+    queries of the same 64 from which the row is hidden."""
     _check_cache4(kv_cache)
     _check_rows("q", q, torch.bfloat16, (q.shape[0] if q.dim() else 0, HEADS_Q, HEAD_DIM))
     _require(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[1] > 0
