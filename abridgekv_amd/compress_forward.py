@@ -30,8 +30,9 @@ Gradients flow through the attention by the kernel's HIP backward (dq, dk, dv un
 trains.
 
 ``CompressLM(fused_norms=True)`` runs the layers' per-head norms and their rotation as one kernel each way (one rounding for
-three; :func:`fuse_norms`), ``fused_ce=True`` takes the cross entropies from the logits as they are, without a float32 copy of them
-(``fused.token_logprobs``). Both are choices of the caller: without them the model's own modules run as before.
+three; :func:`fuse_norms`), ``fused_ce=True`` takes every cross entropy from the logits as they are, without a float32 copy of them
+(``fused.token_logprobs``); a distillation's divergence makes one for itself. Both are choices of the caller: without them the
+model's own modules run as before.
 """
 from __future__ import annotations
 
@@ -536,11 +537,20 @@ class CompressLM(nn.Module):
                             self.raw_tail or self.retain_tail_kv, policy, self.pause_xattn, self.L,
                             copy_rows, self.replay_tail, self.code_exclude_replay_tail)
 
+    def _logits(self, hid):
+        """Logits as the cross entropies take them: fused, as the head returns them, else in float32."""
+        logits = self.model.lm_head(hid)
+        return logits if self.fused_ce else logits.float()
+
+    def _ce_of(self, logits, tgt):
+        """Cross entropy of every row of :meth:`_logits`."""
+        if self.fused_ce:
+            return -fused.token_logprobs(logits, tgt)[0]
+        return F.cross_entropy(logits, tgt, reduction="none")
+
     def _ce_rows(self, hid, tgt):
         """Cross entropy of every row."""
-        if self.fused_ce:
-            return -fused.token_logprobs(self.model.lm_head(hid), tgt)[0]
-        return F.cross_entropy(self.model.lm_head(hid).float(), tgt, reduction="none")
+        return self._ce_of(self._logits(hid), tgt)
 
     def _lm_ce(self, hid, tgt, chunk):
         if self.fused_ce:
@@ -668,11 +678,11 @@ class CompressLM(nn.Module):
                              f"{tuple(hid.shape)}")
         den = mask.sum().clamp_min(1.0)
         T = float(temp)
-        lm_head = self.model.lm_head
 
         def part(h, t, m, tr):
-            logits = lm_head(h).float()
-            ce = F.cross_entropy(logits, t, reduction="none")
+            logits = self._logits(h)
+            ce = self._ce_of(logits, t)
+            logits = logits.float()
             with torch.no_grad():
                 tl = teacher_head(tr).float()
                 tp, tlp = F.softmax(tl / T, -1), F.log_softmax(tl / T, -1)
@@ -752,8 +762,8 @@ class CompressLM(nn.Module):
                 return {"ce": ce, "distill": kl}
             if not per_token and teacher_logits is None:
                 return {"ce": self._masked_lm_ce(hid, tgt, tmask, ce_chunk)}
-            logits = self.model.lm_head(hid).float()
-            ce = F.cross_entropy(logits, tgt, reduction="none")
+            logits = self._logits(hid)
+            ce = self._ce_of(logits, tgt)
             if per_token:
                 return {"ce_pt": ce, "tmask": tmask, "blk": self.predict_block.repeat(B),
                         "pos": (self.predict_flat % C).repeat(B)}
@@ -761,13 +771,14 @@ class CompressLM(nn.Module):
             outd = {"ce": (ce * tmask).sum() / den}
             if teacher_logits is not None:
                 T = distill_temp
-                kl = F.kl_div(F.log_softmax(logits / T, -1), F.softmax(teacher_logits.float() / T, -1),
+                kl = F.kl_div(F.log_softmax(logits.float() / T, -1), F.softmax(teacher_logits.float() / T, -1),
                               reduction="none").sum(-1) * (T * T)
                 outd["distill"] = (kl * tmask).sum() / den
             return outd
         if distill_lambda > 0:
-            logits = self.model.lm_head(hid).float()
-            losses = {"ce": F.cross_entropy(logits, tgt)}
+            logits = self._logits(hid)
+            losses = {"ce": self._ce_of(logits, tgt).mean() if self.fused_ce else F.cross_entropy(logits, tgt)}
+            logits = logits.float()
             if teacher_logits is None:                                     # self-teacher: the full-context forward
                 with torch.no_grad():
                     teacher_logits = self.full_ctx_logits(content_ids)[:, pred_flat, :].reshape(-1, logits.size(-1))
