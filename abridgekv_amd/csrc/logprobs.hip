@@ -26,8 +26,10 @@ constexpr int kTopMax = 32;                    // alternatives a row
 constexpr int kListMax = 1024;                 // candidates in LDS
 constexpr int kMergeMax = 2048;                // candidates of a row's splits
 // Stands for -inf and whatever lies below it (a mask of the type's lowest value), so that exp(x - m) (x - m), and that times a
-// count, is 0 and not NaN.
+// count, is 0 and not NaN. Temperatures up to 1e20 leave it no weight, and the reciprocals of those from 1e-30 on are floats, with
+// room for a gradient.
 constexpr float kLowest = -1.0e25f;
+inline bool temperature_ok(float t) { return t >= 1e-30f && t <= 1e20f; }
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 
 struct LogprobArgs {
@@ -465,7 +467,7 @@ int abkv_token_logprobs(int f32, const void* logits, long stride, int num_tokens
   if (num_tokens <= 0) return 0;
   const int elem = f32 ? 4 : 2;
   if (vocab <= 0 || vocab > (1 << 30) || num_tokens > kMaxGroups / kRowThreads / 2 || logits == nullptr || ((uintptr_t)logits & (elem - 1)) ||
-      targets == nullptr || logprob == nullptr || !softmax_scale_ok(temperature) || top < 0 || top > kTopMax || top > vocab ||
+      targets == nullptr || logprob == nullptr || !temperature_ok(temperature) || top < 0 || top > kTopMax || top > vocab ||
       (top > 0 && (top_ids == nullptr || top_logprobs == nullptr)) || (num_tokens > 1 && stride < vocab))
     return (int)hipErrorInvalidValue;
   const size_t need = abkv_token_logprobs_workspace_size(num_tokens, vocab, f32, top);
@@ -502,7 +504,7 @@ int abkv_token_logprobs_bwd(int f32, const void* logits, long stride, int num_to
   const int elem = f32 ? 4 : 2;
   if (vocab <= 0 || vocab > (1 << 30) || logits == nullptr || dlogits == nullptr ||
       (((uintptr_t)logits | (uintptr_t)dlogits) & (elem - 1)) || targets == nullptr || stats == nullptr ||
-      !softmax_scale_ok(temperature) || (num_tokens > 1 && (stride < vocab || grad_stride < vocab)))
+      !temperature_ok(temperature) || (num_tokens > 1 && (stride < vocab || grad_stride < vocab)))
     return (int)hipErrorInvalidValue;
   LogprobBwdArgs a;
   a.logits = logits;

@@ -1759,6 +1759,13 @@ class TokenLogprobs(NamedTuple):
 
 
 TOP_MAX = 32
+TEMPERATURES = (1e-30, 1e20)                   # that token_logprobs takes: their reciprocals are floats, and a banned logit weighs nothing
+
+
+def _check_temperature(temperature) -> float:
+    temperature = float(temperature)
+    _require(TEMPERATURES[0] <= temperature <= TEMPERATURES[1], "temperature must lie in [1e-30, 1e20]")
+    return temperature
 
 
 def _check_logits(logits, targets, temperature) -> float:
@@ -1767,15 +1774,13 @@ def _check_logits(logits, targets, temperature) -> float:
              "logits must be bf16 or fp32 [T, V] with contiguous rows that do not overlap")
     _require(targets.dtype == torch.int64 and targets.shape == logits.shape[:1] and targets.is_contiguous(),
              "targets must be contiguous int64 [T]")
-    temperature = float(temperature)
-    _require(0 < temperature < math.inf, "temperature must be positive and finite")
-    return temperature
+    return _check_temperature(temperature)
 
 
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, temperature: float = 1.0, top: int = 0, entropy: bool = True,
                    stats: bool = False) -> TokenLogprobs:
     """Log probabilities of given tokens under softmax(logits / temperature), in one read of the logits, with the
-    distribution's entropy and its ``top`` (0 .. 32) most likely tokens.
+    distribution's entropy and its ``top`` (0 .. 32) most likely tokens. Temperatures from 1e-30 to 1e20.
 
     logits [T, V] bf16 or fp32 (rows of any alignment); targets [T] int64: outside [0, V) a row has no target and log probability
     0. Alternatives in descending order (ties: the lowest id). Logits below -1e25 (-inf, a type's lowest value) have probability

@@ -594,10 +594,11 @@ int abkv_paged_prefill_attn_items_int4(const void* q, long q_stride_t, long q_st
 
 /* ---------------------------------------------------------------------------------------------------------------
  * Log probabilities of given tokens: logits [num_tokens, vocab] bf16 or (f32 != 0) fp32, rows `stride` elements apart, of any
- * alignment. With x = logits / temperature: logprob[t] = x[target] - logsumexp(x) (0 for a target outside [0, vocab)); entropy[t]
- * (or NULL); the `top` (0 .. 32) highest logits' ids and log probabilities [num_tokens, top], ties by the lower id, NaN below
- * every number; stats [num_tokens, 3] (or NULL): what the gradient needs. Logits below -1e25 (-inf, a type's lowest value) have
- * probability 0; a row without another, or with a NaN or +inf, is NaN. workspace: abkv_token_logprobs_workspace_size bytes, 8-byte aligned (0: none).
+ * alignment. With x = logits / temperature (1e-30 to 1e20): logprob[t] = x[target] - logsumexp(x) (0 for a target outside
+ * [0, vocab)); entropy[t] (or NULL); the `top` (0 .. 32) highest logits' ids and log probabilities [num_tokens, top], ties by the
+ * lower id, NaN below every number; stats [num_tokens, 3] (or NULL): what the gradient needs. Logits below -1e25 (-inf, a type's
+ * lowest value) have probability 0; a row without another, or with a NaN or +inf, is NaN. workspace:
+ * abkv_token_logprobs_workspace_size bytes, 8-byte aligned (0: none).
  * The reference takes its losses and scores from torch's cross entropy (abridgekv/compress_forward.py:957-1042). */
 size_t abkv_token_logprobs_workspace_size(int num_tokens, int vocab, int f32, int top);
 int abkv_token_logprobs(int f32, const void* logits, long stride, int num_tokens, int vocab, const int64_t* targets,
