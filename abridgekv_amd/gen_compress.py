@@ -459,6 +459,7 @@ class CompressGen:
         first, n = len(prompt_ids), len(ids)
         if first == 0 or n == first:
             raise ValueError("score needs a prompt and an answer")
+        ops.check_scores(ids, self.lm_head.weight.shape[0], temperature, top)              # (before anything is fed)
         parts, i = [], 0
         while i < n - 1:
             take = min(self.C - self.f, n - 1 - i)

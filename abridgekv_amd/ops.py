@@ -1768,6 +1768,19 @@ def _check_temperature(temperature) -> float:
     return temperature
 
 
+def _check_top(top, V: int) -> int:
+    top = int(top)
+    _require(0 <= top <= min(TOP_MAX, V), f"top must be in [0, {min(TOP_MAX, V)}]")
+    return top
+
+
+def check_scores(ids, V: int, temperature, top) -> None:
+    """What :func:`token_logprobs` would refuse, for callers that run a model before they get there, and ids outside [0, V)."""
+    _check_temperature(temperature)
+    _check_top(top, V)
+    _require(not len(ids) or 0 <= min(ids) <= max(ids) < V, f"token ids must be in [0, {V})")
+
+
 def _check_logits(logits, targets, temperature) -> float:
     _require(logits.dim() == 2 and logits.dtype in (torch.bfloat16, torch.float32) and logits.shape[1] > 0
              and logits.stride(1) == 1 and (logits.shape[0] <= 1 or logits.stride(0) >= logits.shape[1]),
@@ -1788,8 +1801,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, temperature: flo
     equal calls give equal bits. With gradients: :func:`abridgekv_amd.fused.token_logprobs`."""
     temperature = _check_logits(logits, targets, temperature)
     T, V = logits.shape
-    top = int(top)
-    _require(0 <= top <= min(TOP_MAX, V), f"top must be in [0, {min(TOP_MAX, V)}]")
+    top = _check_top(top, V)
     _check_device(logits, targets)
     f32 = int(logits.dtype == torch.float32)
     logprob = logits.new_empty((T,), dtype=torch.float32)
