@@ -811,10 +811,12 @@ class CompressLM(nn.Module):
     @torch.no_grad()
     def token_logprobs(self, content_ids, prompt_len=None, temperature=1.0, top=0, chunk=4096) -> ops.TokenLogprobs:
         """Log probabilities of the content tokens at the loss positions (block-major, as :meth:`loss_logits` orders them), with
-        the distributions' entropies and ``top`` alternatives, ``chunk`` rows of logits at a time."""
+        the distributions' entropies and ``top`` alternatives, ``chunk`` rows of logits at a time (<= 0: all at once)."""
         hid = self.hidden_states(content_ids, prompt_len)[:, self.loss_pos, :].reshape(-1, self.model.config.hidden_size)
         B, N, C = content_ids.shape
         tgt = content_ids.reshape(B, N * C)[:, self.predict_flat + 1].reshape(-1)
-        parts = [ops.token_logprobs(self.model.lm_head(hid[i:i + chunk]), tgt[i:i + chunk], temperature, top=top)
-                 for i in range(0, hid.size(0), chunk)]
+        rows = max(hid.size(0), 1)                           # (no rows at all: one empty chunk)
+        step = rows if chunk <= 0 else chunk
+        parts = [ops.token_logprobs(self.model.lm_head(hid[i:i + step]), tgt[i:i + step], temperature, top=top)
+                 for i in range(0, rows, step)]
         return ops.TokenLogprobs(*(torch.cat(x) for x in list(zip(*parts))[:4]), None)
