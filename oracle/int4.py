@@ -1,9 +1,9 @@
 """Cache rows in 4 bits and attention over them (oracle; test infrastructure only).
 
 Rows are quantised and read in numpy from the format's definition, dim by dim; attention is float64 over the values that the rows
-stand for. ``bounds`` derives how far a kernel may be off: it takes a weight times its row's step, rounded to bf16 (half a step,
-2^-8 of it), against a code less 8, and the weight in fp32 against the group's middle, and rounds the output; split partials are
-fp16 (2^-11 of the split's largest output, itself at most the largest value). ``wide``: the multi-query kernel instead takes
+stand for. Its bounds say how far a kernel may be off: it takes a weight times its row's step, in two bf16 parts (half a step
+of the second, 2^-16 of it), against 128 + code and -136 in fp32 sums, and the weight in fp32 against the group's middle, and rounds
+the output; split partials are fp16 (2^-11 of the split's largest output, itself at most the largest value; ``whole``: none). ``wide``: the multi-query kernel instead takes
 values and weights in fp16 (half a step, 2^-11 of each; its powers of two keep them, and what is 2^-19 of its row's or page's largest,
 in the type's normal range; weights down to 2^-25 of the row's largest, and what lies below is off by up to 2^-36 of that, which is
 not in the bounds), and its partials are fp32.
@@ -74,7 +74,7 @@ def values(rows: np.ndarray) -> np.ndarray:
     return np.repeat(lo, GROUP, -1) + np.repeat(step, GROUP, -1) * codes
 
 
-def attend(q, k_rows, v_rows, vis, scale: float, wide: bool = False):
+def attend(q, k_rows, v_rows, vis, scale: float, wide: bool = False, whole: bool = False):
     """q [n, 32, 128] float64 over m rows of bytes, vis [n, m]: out [n, 32, 128], lse [n, 32] and the bounds of both (rows that
     see nothing: 0 and -inf)."""
     n = len(q)
@@ -83,6 +83,8 @@ def attend(q, k_rows, v_rows, vis, scale: float, wide: bool = False):
     vs, vlo, vc = split(v_rows)
     part = np.repeat(vs, GROUP, -1) * np.abs(vc - 8)                     # what a rounded weight multiplies
     mid = np.abs(np.repeat(vlo + 8 * vs, GROUP, -1))
+    summed = 143 * np.repeat(vs, GROUP, -1) + mid                        # what the sums hold, 32 rows at a time, a step after another
+    adds = (len(v) / 32 + 40) * 2.0 ** -24
     out, lse = np.zeros((n, 32, DIM)), np.full((n, 32), -np.inf)
     tol, ltol = np.zeros_like(out), np.zeros((n, 32))
     some = vis.any(1)
@@ -105,7 +107,8 @@ def attend(q, k_rows, v_rows, vis, scale: float, wide: bool = False):
         out[some, h] = o
         # a score off by ds moves the output by w ds (v - out), twice that for the sum's own
         moved = (w * ds) @ np.abs(v[:, u]) + (w * ds).sum(1, keepdims=True) * np.abs(o)
-        err = HALF * (w @ (2 * np.abs(v[:, u]))) if wide else EPS * (w @ part[:, u]) + 2.0 ** -22 * (w @ (part + mid)[:, u])
-        tol[some, h] = SLACK * (err + moved + EPS * np.abs(o)) + (2.0 ** -20 if wide else 2.0 ** -11) * np.abs(v[:, u]).max(initial=0)
+        err = HALF * (w @ (2 * np.abs(v[:, u]))) if wide else EPS ** 2 * (w @ part[:, u]) + adds * (w @ summed[:, u])
+        floor = 2.0 ** -20 if wide or whole else 2.0 ** -11
+        tol[some, h] = SLACK * (err + moved + EPS * np.abs(o)) + floor * np.abs(v[:, u]).max(initial=0)
         ltol[some, h] = ds.max(1) + (HALF if wide else 0) + 1e-5
     return out, lse, tol, ltol
