@@ -14,8 +14,9 @@
 //
 // A SIMD has one wave of either kind, and a tile is two phases of each: the vector unit's (softmax, unpacking) and the matrix
 // unit's (products). The V waves are a phase behind, so that one wave's vector work runs beside the other's products; in step,
-// they took turns at both units: 1.4 us a tile at the vector unit and 0.9 at the matrix unit came to 2.5 us, and are now 2.1
-// (three chunks of 300 to 441 queries behind up to 8000 rows: 180 -> 160 us; with the two kinds on different SIMDs, 193).
+// they took turns at both units: 1.4 us a tile at the vector unit and 0.9 at the matrix unit came to 2.5 us, and then to 2.1
+// (three chunks of 300 to 441 queries behind up to 8000 rows and a code step: 180 -> 160 us on one box, 169 now on another; with the
+// two kinds on different SIMDs, 193).
 #pragma once
 #include "attn_tile.h"
 #include "int4.h"

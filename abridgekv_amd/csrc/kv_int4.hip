@@ -127,7 +127,8 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t w, int n, uint32_t mask) 
 // holds: a head's codes are half of one, its pairs an eighth. The workgroup's waves therefore fetch whole rows together, straight
 // into LDS (a wave 5 of the step's 40 KB), one barrier a step. (64 sequences of 500 to 9500 rows, every wave its own pieces: 118
 // us, of which 59 went with the pairs alone; the pairs shared, 99; whole rows, 94, nontemporal, 86, in equal shares, 73 without the
-// merge: 410 MB at 5.6 TB/s; 62 are vector work. Three stages of LDS leave one workgroup a CU: 104 where two took 94.)
+// merge: 410 MB at 5.6 TB/s, then beside 62 of vector work, to whose instructions the second parts have added a tenth. Three stages
+// of LDS leave one workgroup a CU: 104 where two took 94.)
 constexpr int kPairs4 = 16 * 4 * kHeadsKV, kCodes4 = 16 * kHeadsKV * 16;     // dwords of a page's pairs and codes (of K or V)
 template <class T>
 __device__ __forceinline__ const T& at4(const uint32_t* base, uint32_t bytes) {
@@ -590,7 +591,8 @@ size_t abkv_decode_int4_workspace_size(int num_seqs, int max_pages_per_seq, int 
   if (num_seqs <= 0 || max_pages_per_seq <= 0 || split_pages < 0) return 0;
   constexpr size_t kPart = kHeadsQ * (kHeadDim * sizeof(_Float16) + 4 * sizeof(float));
   if (split_pages == 0)
-    return num_seqs > kShareSeqs ? 0 : 2 * (size_t)decode4_shares(num_seqs, max_pages_per_seq) * kPart + (num_seqs + 1) * sizeof(int);
+    return num_seqs > kShareSeqs ? 0
+                                 : 2 * (size_t)decode4_shares(num_seqs, max_pages_per_seq) * kPart + (num_seqs + 1) * sizeof(int);
   const int splits = (max_pages_per_seq + split_pages - 1) / split_pages;
   return splits > 1 ? (size_t)num_seqs * splits * kPart : 0;
 }
@@ -600,10 +602,10 @@ int abkv_decode_attn_int4(const void* q, long q_stride_seq, long q_stride_head, 
                           int max_pages_per_seq, int split_pages, float scale, void* out, long out_stride_seq,
                           long out_stride_head, float* lse, void* workspace, size_t workspace_bytes, hipStream_t stream) {
   if (num_seqs <= 0) return 0;
-  if (split_pages < 0 || (split_pages & 1) || split_pages > 64 || (split_pages == 0 && num_seqs > kShareSeqs) || max_pages_per_seq <= 0 || max_pages_per_seq > (1 << 26) ||
-      num_pages <= 0 || block_table_stride < max_pages_per_seq || num_seqs > 65535 || !softmax_scale_ok(scale) ||
-      !rows16_ok(q, q_stride_seq, q_stride_head) || !rows16_ok(kv_cache, 0, 0) || block_table == nullptr ||
-      seq_lens == nullptr || !rows16_ok(out, out_stride_seq, out_stride_head))
+  if (split_pages < 0 || (split_pages & 1) || split_pages > 64 || (split_pages == 0 && num_seqs > kShareSeqs) ||
+      max_pages_per_seq <= 0 || max_pages_per_seq > (1 << 26) || num_pages <= 0 || block_table_stride < max_pages_per_seq ||
+      num_seqs > 65535 || !softmax_scale_ok(scale) || !rows16_ok(q, q_stride_seq, q_stride_head) || !rows16_ok(kv_cache, 0, 0) ||
+      block_table == nullptr || seq_lens == nullptr || !rows16_ok(out, out_stride_seq, out_stride_head))
     return (int)hipErrorInvalidValue;
   const size_t need = abkv_decode_int4_workspace_size(num_seqs, max_pages_per_seq, split_pages);
   if (need > 0 && (!rows16_ok(workspace, 0, 0) || workspace_bytes < need)) return (int)hipErrorInvalidValue;

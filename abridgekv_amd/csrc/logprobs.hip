@@ -14,7 +14,7 @@
 // equal logits) are found one after the other instead.
 //
 // Bound by memory: 2 (bf16) or 4 bytes a logit, beside one exponential and ten other operations.
-// Measured: 2048 rows of 131072 logits in bf16, forward 85 to 98 us (537 MB, 5.5 to 6.3 TB/s), gradient 172 to 180 (1.07 GB, 6 TB/s);
+// Measured: 2048 rows of 131072 logits in bf16, forward 84 to 104 us (537 MB, 5.2 to 6.4 TB/s), gradient 172 to 181 (1.07 GB, 6 TB/s);
 // one row in fp32 with 5 alternatives 5.2 + 3.4 us over 64 workgroups.
 #include "abridgekv_amd.h"
 #include "common.h"
@@ -466,9 +466,10 @@ int abkv_token_logprobs(int f32, const void* logits, long stride, int num_tokens
                         float* top_logprobs, void* workspace, size_t workspace_bytes, hipStream_t stream) {
   if (num_tokens <= 0) return 0;
   const int elem = f32 ? 4 : 2;
-  if (vocab <= 0 || vocab > (1 << 30) || num_tokens > kMaxGroups / kRowThreads / 2 || logits == nullptr || ((uintptr_t)logits & (elem - 1)) ||
-      targets == nullptr || logprob == nullptr || !temperature_ok(temperature) || top < 0 || top > kTopMax || top > vocab ||
-      (top > 0 && (top_ids == nullptr || top_logprobs == nullptr)) || (num_tokens > 1 && stride < vocab))
+  if (vocab <= 0 || vocab > (1 << 30) || num_tokens > kMaxGroups / kRowThreads / 2 || logits == nullptr ||
+      ((uintptr_t)logits & (elem - 1)) || targets == nullptr || logprob == nullptr || !temperature_ok(temperature) || top < 0 ||
+      top > kTopMax || top > vocab || (top > 0 && (top_ids == nullptr || top_logprobs == nullptr)) ||
+      (num_tokens > 1 && stride < vocab))
     return (int)hipErrorInvalidValue;
   const size_t need = abkv_token_logprobs_workspace_size(num_tokens, vocab, f32, top);
   if (need > 0 && (workspace == nullptr || ((uintptr_t)workspace & 7) || workspace_bytes < need))

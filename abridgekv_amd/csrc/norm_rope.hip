@@ -10,8 +10,8 @@
 // Bound by memory: a row is read once and written once. A row lies in 8 lanes, lane i with dims 8 i .. + 7 and 64 + 8 i .. + 7,
 // both members of its rotation pairs, so a wave holds 8 rows, its loads are whole 16-byte pieces and the sums over a row are
 // three DPP steps.
-// Measured: 2048 tokens appended 10.8 us (4.8 TB/s, what a copy reaches); training, two sequences of 4096 in bf16: forward 33 us
-// (168 MB, 5.1 TB/s), backward 55 (252 MB, 4.6 TB/s).
+// Measured, inputs from memory: 2048 tokens appended 10.6 us (4.8 TB/s, what a copy reaches); training, two sequences of 4096 in
+// bf16: forward 33 us (168 MB, 5.1 TB/s), backward 57 (252 MB, 4.4 TB/s).
 #include "abridgekv_amd.h"
 #include "int4.h"
 #include "rope.h"
@@ -322,9 +322,10 @@ __global__ __launch_bounds__(256) void norm_weights_kernel(const float* parts, i
   else static_cast<__bf16*>(to)[dim % kHeadDim] = (__bf16)v;
 }
 
-// Workgroups of the backward: three a CU, what its registers let a CU hold (two sequences of 4096 tokens in bf16, with the
-// weights' launch: 47 us; 1024 workgroups, a third of them in a second round: 54, 512: 48; eight of 8192: 385, 504 and 482 us);
-// fewer where tokens are few.
+// Workgroups of the backward: three a CU, what its registers let a CU hold; fewer where tokens are few. Calls in a row, with the
+// weights' launch, for 512, 768 and 1024 workgroups (a third of these in a second round): two sequences of 4096 tokens in bf16, eight
+// sets of inputs in turn 66, 57 and 72 us, one set again and again, part of which the last-level cache then holds, 48, 47 and 56;
+// eight of 8192, three sets 494, 399 and 513.
 inline int bwd_groups(long tokens) {
   const long n = (tokens + kTokenWaves - 1) / kTokenWaves;
   return n < 768 ? (int)n : 768;

@@ -526,9 +526,9 @@ int abkv_paged_prefill_attn_items(const void* q, long q_stride_t, long q_stride_
                                   const int32_t* merges, int n_merges, int part_rows, float scale, void* out,
                                   long out_stride_t, long out_stride_h, float* lse, void* workspace,
                                   size_t workspace_bytes, hipStream_t stream) {
-  return prefill_items(false, q, q_stride_t, q_stride_h, kv_cache, num_pages, block_table, block_table_stride, block_table_width, q_start, kv_start,
-                       kv_limit, kv_excluded, causal, items, n_items, merges, n_merges, part_rows, scale, out, out_stride_t,
-                       out_stride_h, lse, workspace, workspace_bytes, stream);
+  return prefill_items(false, q, q_stride_t, q_stride_h, kv_cache, num_pages, block_table, block_table_stride, block_table_width,
+                       q_start, kv_start, kv_limit, kv_excluded, causal, items, n_items, merges, n_merges, part_rows, scale, out,
+                       out_stride_t, out_stride_h, lse, workspace, workspace_bytes, stream);
 }
 
 int abkv_paged_prefill_attn_items_int4(const void* q, long q_stride_t, long q_stride_h, const void* kv_cache, int num_pages,
@@ -541,9 +541,9 @@ int abkv_paged_prefill_attn_items_int4(const void* q, long q_stride_t, long q_st
   if ((((uintptr_t)q | (uintptr_t)kv_cache | (uintptr_t)out) & 15) || ((q_stride_t | q_stride_h | out_stride_t | out_stride_h) & 7) ||
       !softmax_scale_ok(scale))
     return n_items <= 0 ? 0 : (int)hipErrorInvalidValue;
-  return prefill_items(true, q, q_stride_t, q_stride_h, kv_cache, num_pages, block_table, block_table_stride, block_table_width, q_start, kv_start,
-                       kv_limit, kv_excluded, causal, items, n_items, merges, n_merges, part_rows, scale, out, out_stride_t,
-                       out_stride_h, lse, workspace, workspace_bytes, stream);
+  return prefill_items(true, q, q_stride_t, q_stride_h, kv_cache, num_pages, block_table, block_table_stride, block_table_width,
+                       q_start, kv_start, kv_limit, kv_excluded, causal, items, n_items, merges, n_merges, part_rows, scale, out,
+                       out_stride_t, out_stride_h, lse, workspace, workspace_bytes, stream);
 }
 
 int abkv_paged_prefill_attn_packed(const void* q, long q_stride_t, long q_stride_h, const void* kv_cache,

@@ -1578,10 +1578,10 @@ def decode_attention_int4(q: torch.Tensor, kv_cache: torch.Tensor, block_table: 
                           lse: torch.Tensor | None = None, split_pages: int | None = None,
                           workspace: torch.Tensor | None = None):
     """:func:`decode_attention` over a cache in 4 bits (:func:`kv_cache_int4_shape`): q [B, 32, 128] bf16; returns
-    (out [B, 32, 128] bf16, lse [B, 32] fp32 or None). The codes enter the products exactly; a weight times its row's step
-    in two bf16 parts (2^-16 of it). Slots behind a sequence's rows may hold anything. ``split_pages``: pages a workgroup takes of one sequence; 0
-    (up to 512 sequences): workgroups take equal shares of all sequences' rows, whatever their lengths; None: chosen by the sizes
-    (:func:`int4_split_pages`)."""
+    (out [B, 32, 128] bf16, lse [B, 32] fp32 or None). The codes enter the products exactly; a weight times its row's step in two
+    bf16 parts (2^-16 of it). Slots behind a sequence's rows may hold anything. ``split_pages``: pages a workgroup takes of one
+    sequence; 0 (up to 512 sequences): workgroups take equal shares of all sequences' rows, whatever their lengths; None: chosen by
+    the sizes (:func:`int4_split_pages`)."""
     scale = _softmax_scale(scale)
     _check_cache4(kv_cache)
     B, max_pages = _check_step(q, None, block_table, seq_lens, max_pages, split_pages or None, out, lse)
@@ -1759,7 +1759,7 @@ class TokenLogprobs(NamedTuple):
 
 
 TOP_MAX = 32
-TEMPERATURES = (1e-30, 1e20)                   # that token_logprobs takes: their reciprocals are floats, and a banned logit weighs nothing
+TEMPERATURES = (1e-30, 1e20)                   # of token_logprobs: reciprocals are floats, and a banned logit weighs nothing
 
 
 def _check_temperature(temperature) -> float:
