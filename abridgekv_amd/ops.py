@@ -1547,10 +1547,10 @@ def int4_split_pages(num_seqs: int, max_pages: int) -> int:
     equal shares of all sequences' rows.
 
     Up to 8192 pages a split is as long as leaves one workgroup on each of the 256 compute units (one sequence of 32000 rows: 8
-    pages 16.6 us, 4 pages 19.9, 16 pages 20.0, shares 18.3; of 131000 rows: 32 pages 37, 16 pages 39, shares 38.5). Beyond, a
+    pages 16.8 us, 4 pages 19.2, 16 pages 20.9, shares 17.6; of 131000 rows: 32 pages 36.5, 16 pages 37.2, shares 37.3). Beyond, a
     full round of workgroups reads as fast as memory does, and shares end together (64 sequences of 500 to 9500 rows: 78 us,
-    splits of 12, 20, 32 and 40 pages 94, 91, 88 and 92; 256 of 500 to 3000: 110, splits of 20 129; 32 of 9500: 71, splits of
-    40, which fit them, 68), up to 512 sequences; more of them run in splits of 20, whose uneven ends weigh little."""
+    splits of 12, 20, 32 and 40 pages 94, 90, 89 and 100; 256 of 500 to 3000: 111, splits of 20 129; 32 of 9500: 71, splits of
+    40, which fit them, 69), up to 512 sequences; more of them run in splits of 20, whose uneven ends weigh little."""
     total = num_seqs * max_pages
     most = -(-total // 256)
     if most > 32:
