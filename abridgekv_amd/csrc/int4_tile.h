@@ -15,8 +15,8 @@
 // A SIMD has one wave of either kind, and a tile is two phases of each: the vector unit's (softmax, unpacking) and the matrix
 // unit's (products). The V waves are a phase behind, so that one wave's vector work runs beside the other's products; in step,
 // they took turns at both units: 1.4 us a tile at the vector unit and 0.9 at the matrix unit came to 2.5 us, and then to 2.1
-// (three chunks of 300 to 441 queries behind up to 8000 rows and a code step: 180 -> 160 us on one box, 169 now on another; with the
-// two kinds on different SIMDs, 193).
+// (three chunks of 300 to 441 queries behind up to 8000 rows and a code step: 180 -> 160 us then, 169 now; with the two kinds on
+// different SIMDs, 193).
 #pragma once
 #include "attn_tile.h"
 #include "int4.h"
@@ -69,9 +69,9 @@ __device__ __forceinline__ int range_exp(float bound) {
   return max((e + 7) & ~7, kLowestExp);
 }
 __device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
-// A float's bits times 2^e for e << 23, from 2^-100 (so that -inf stays that, and no score that counts is as small) to 2^127. For the
-// softmax scale times 2^(eQ + eK) it is called once, with both exponents (up to 240 << 23, an int): a part of the product may lie
-// outside that range where the whole does not.
+// A float's bits times 2^e for e << 23, from 2^-100 (so that -inf stays that, and no score that counts is as small) to 2^127. For
+// the softmax scale times 2^(eQ + eK) it is called once, with both exponents (up to 240 << 23, an int): a part of the product may
+// lie outside that range where the whole does not.
 __device__ __forceinline__ float scaled_bits(int bits, int e23) {
   return __int_as_float(min(max(__builtin_elementwise_add_sat(bits, e23), 27 << 23), 254 << 23));
 }

@@ -118,10 +118,10 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t w, int n, uint32_t mask) 
 // Values: out_d = sum_j (p_j s_jg) (c_jd - 8) + sum_j p_j (m_jg + 8 s_jg): column 4 h + g of P^T carries p_j s_jg, and of the four
 // accumulator rows 4 j + r of an output tile (words of the value rows, word % 4 its group) a lane keeps r = g: 8 dims in a row.
 // The codes enter as 128 + c (code_pair): the score accumulator starts at -128 Q_g, and a row of -136s among the V tiles takes
-// them, and the codes' middle, out of the output. p_j s_jg enters in two bf16 parts, itself and what its rounding leaves, so that it
-// errs by 2^-16 of itself; everything else is exact or fp32. (One part: an output off by 0.0023 of itself in place of 0.0017, its
-// own rounding to bf16; the second products, of the same codes, take 1.3 of 78 us over 64 sequences of 500 to 9500 rows, and no
-// time over one of 32000.)
+// them, and the codes' middle, out of the output. p_j s_jg enters in two bf16 parts, itself and what its rounding leaves, so that
+// it errs by 2^-16 of itself; everything else is exact or fp32. (One part: an output off by 0.0023 of itself in place of 0.0017,
+// its own rounding to bf16; the second products, of the same codes, take 1.3 of 78 us over 64 sequences of 500 to 9500 rows, and
+// no time over one of 32000.)
 //
 // What bounds the reads is the number of cache lines that a CU asks for (about one in six cycles), so a line should bring what it
 // holds: a head's codes are half of one, its pairs an eighth. The workgroup's waves therefore fetch whole rows together, straight

@@ -14,8 +14,8 @@
 // equal logits) are found one after the other instead.
 //
 // Bound by memory: 2 (bf16) or 4 bytes a logit, beside one exponential and ten other operations.
-// Measured: 2048 rows of 131072 logits in bf16, forward 84 to 104 us (537 MB, 5.2 to 6.4 TB/s), gradient 172 to 181 (1.07 GB, 6 TB/s);
-// one row in fp32 with 5 alternatives 5.2 + 3.4 us over 64 workgroups.
+// Measured: 2048 rows of 131072 logits in bf16, forward 84 to 104 us (537 MB, 5.2 to 6.4 TB/s), gradient 172 to 181 (1.07 GB,
+// 6 TB/s); one row in fp32 with 5 alternatives 5.2 + 3.4 us over 64 workgroups.
 #include "abridgekv_amd.h"
 #include "common.h"
 

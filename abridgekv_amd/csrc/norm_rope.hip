@@ -323,9 +323,9 @@ __global__ __launch_bounds__(256) void norm_weights_kernel(const float* parts, i
 }
 
 // Workgroups of the backward: three a CU, what its registers let a CU hold; fewer where tokens are few. Calls in a row, with the
-// weights' launch, for 512, 768 and 1024 workgroups (a third of these in a second round): two sequences of 4096 tokens in bf16, eight
-// sets of inputs in turn 66, 57 and 72 us, one set again and again, part of which the last-level cache then holds, 48, 47 and 56;
-// eight of 8192, three sets 494, 399 and 513.
+// weights' launch, for 512, 768 and 1024 workgroups (a third of these in a second round): two sequences of 4096 tokens in bf16,
+// eight sets of inputs in turn 66, 57 and 72 us, one set again and again, part of which the last-level cache then holds, 48, 47
+// and 56; eight of 8192, three sets 494, 399 and 513.
 inline int bwd_groups(long tokens) {
   const long n = (tokens + kTokenWaves - 1) / kTokenWaves;
   return n < 768 ? (int)n : 768;

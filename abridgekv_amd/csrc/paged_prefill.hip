@@ -110,8 +110,8 @@ struct RangeWalk {
   }
 };
 
-// A row's lse from its maximum m (log2 units) and weight sum l: -inf where it sees nothing. Of a row that reads as NaN a 4-bit cache
-// makes a NaN (l is one), as its single-token kernel does; the bf16 kernels all leave -inf there.
+// A row's lse from its maximum m (log2 units) and weight sum l: -inf where it sees nothing. Where it sees a row that reads as NaN
+// (l is one then) a 4-bit cache makes it NaN, as its single-token kernel does; the bf16 kernels all leave -inf there.
 template <bool kInt4>
 __device__ __forceinline__ float row_lse(float m, float l) {
   return l > 0.f ? (m + __log2f(l)) * 0.69314718055994531f : kInt4 && l != 0.f ? l : -INFINITY;

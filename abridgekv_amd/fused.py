@@ -1,8 +1,8 @@
 """Fused operators with gradients, and a model's attention layers on them.
 
 ``qk_norm_rope``: RMS norms of queries and keys for each head and their rotation; ``token_logprobs``: log probabilities of given
-tokens and the distribution's entropy. Forward and backward are one kernel each (and a small one for the norms' weights). As with any
-autograd function, a backward pass is captured into a graph only when no eager graph of the same leaves is alive.
+tokens and the distribution's entropy. Forward and backward are one kernel each (and a small one for the norms' weights). As with
+any autograd function, a backward pass is captured into a graph only when no eager graph of the same leaves is alive.
 """
 from __future__ import annotations
 
